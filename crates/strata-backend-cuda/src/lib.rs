@@ -20,6 +20,7 @@
 //! the library's message.
 
 mod ffi;
+mod ffi_sequence;
 
 use std::collections::HashMap;
 use std::ffi::CStr;

@@ -1,0 +1,186 @@
+// short_conv.cu — causal depthwise convolution of a recurrent layer's
+// projected channels, with its state (the step before the gated delta rule;
+// the reference's loop is in crates/strata-core/src/gdn.rs).
+//
+//   y[t][c] = act(bias[c] + sum_j w[c][j] x[t - (K - 1) + j][c])
+//
+// Bound by memory: each x is read and each y written once, 2 K flops between
+// them. A thread owns VEC neighbouring channels (one 16-byte access) and walks
+// a tile of kTile tokens with the last K - 1 inputs in registers, so a tile
+// re-reads only its K - 1 rows of halo (from L2). The rows of a tile are
+// loaded kAhead at a time, so that many independent 16-byte loads are in
+// flight per thread.
+//
+// The state of a sequence is read and replaced by the same thread (the one
+// that has its first tile; the new state is the sequence's last K - 1 inputs,
+// read again from x), so no other block has to be waited for.
+#include <cuda_runtime.h>
+
+#include "sequence.cuh"
+
+namespace strata {
+namespace {
+
+constexpr int kTile = 16;
+constexpr int kAhead = 8;
+constexpr int kThreads = 128;
+
+struct ConvArgs {
+    const void* x;
+    const float* w;
+    const float* bias;
+    float* state;  // of the launch's first sequence
+    void* y;
+    int64_t x_stride, y_stride;
+    int channels, blocks;  // blocks of channels
+    int silu;
+};
+
+// z / (1 + exp(-z)). For bf16 outputs the approximate exponential is far below
+// the rounding; f32 outputs take the accurate one. The quick division is good
+// to 2 ulp, and gives 0 where exp(-z) > 2^126 (the true value is below 1e-36).
+template <typename T>
+__device__ __forceinline__ float silu(float z) {
+    return __fdividef(z, 1.0f + (sizeof(T) == 2 ? __expf(-z) : expf(-z)));
+}
+
+template <typename T, int K, int VEC>
+__global__ void __launch_bounds__(kThreads) conv_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
+    const int block = blockIdx.x / a.blocks;
+    const int c = ((blockIdx.x - block * a.blocks) * kThreads + threadIdx.x) * VEC;
+    if (c >= a.channels) return;
+    int seq, row, len, tile;
+    find_tile(tab, block, seq, row, len, tile);
+    const int t0 = tile * kTile;
+    const int n = len - t0 < kTile ? len - t0 : kTile;
+    const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.x_stride + c;
+    T* y = static_cast<T*>(a.y) + (int64_t)(row + t0) * a.y_stride + c;
+    using P = Pack<T, VEC>;
+
+    float w[K][VEC], past[K][VEC];  // past[0 .. K-2]: the inputs before the tile (one spare row keeps K = 1 legal)
+    float bias[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) w[j][v] = a.w[(int64_t)(c + v) * K + j];
+        bias[v] = a.bias ? a.bias[c + v] : 0.0f;
+    }
+    if (K > 1) {
+        float* st = a.state + (int64_t)seq * (K - 1) * a.channels + c;
+        if (t0 == 0) {
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) past[j][v] = st[(int64_t)j * a.channels + v];
+            // the new state: input len - (K - 1) + j, or where that is before the call, old row len + j
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j) {
+                const int p = len - (K - 1) + j;
+                if (p >= 0) {
+                    const P in = *reinterpret_cast<const P*>(x + (int64_t)p * a.x_stride);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) st[(int64_t)j * a.channels + v] = to_f32(in.v[v]);
+                } else {
+#pragma unroll
+                    for (int m = j + 1; m < K - 1; ++m)
+                        if (m == j + len)
+#pragma unroll
+                            for (int v = 0; v < VEC; ++v) st[(int64_t)j * a.channels + v] = past[m][v];
+                }
+            }
+        } else {  // t0 >= kTile > K - 1: the halo lies inside the sequence
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j) {
+                const P in = *reinterpret_cast<const P*>(x + (int64_t)(t0 - (K - 1) + j) * a.x_stride);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) past[j][v] = to_f32(in.v[v]);
+            }
+        }
+    }
+    x += (int64_t)t0 * a.x_stride;
+    for (int t = 0; t < n; t += kAhead) {
+        P in[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (t + u < n) in[u] = *reinterpret_cast<const P*>(x + (int64_t)(t + u) * a.x_stride);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (t + u >= n) break;
+            P out;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float now = to_f32(in[u].v[v]);
+                float z = bias[v];
+#pragma unroll
+                for (int j = 0; j < K - 1; ++j) z = fmaf(w[j][v], past[j][v], z);
+                z = fmaf(w[K - 1][v], now, z);
+#pragma unroll
+                for (int j = 0; j + 1 < K - 1; ++j) past[j][v] = past[j + 1][v];
+                if (K > 1) past[K >= 2 ? K - 2 : 0][v] = now;
+                from_f32(out.v[v], a.silu ? silu<T>(z) : z);
+            }
+            *reinterpret_cast<P*>(y + (int64_t)(t + u) * a.y_stride) = out;
+        }
+    }
+}
+
+template <typename T, int VEC>
+void launch_conv(int taps, const ConvArgs& a, const SeqTable& t, unsigned grid, cudaStream_t s) {
+    switch (taps) {
+        case 1: conv_kernel<T, 1, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 2: conv_kernel<T, 2, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 3: conv_kernel<T, 3, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 4: conv_kernel<T, 4, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 5: conv_kernel<T, 5, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 6: conv_kernel<T, 6, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 7: conv_kernel<T, 7, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        default: conv_kernel<T, 8, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+    }
+}
+
+// The 16-byte form needs whole packs in every row and 16-byte rows.
+bool packs(const strata_short_conv& d, const void* x, const void* y) {
+    const int64_t vec = 16 / dtype_bytes(d.dtype);
+    return d.channels % vec == 0 && d.x_stride % vec == 0 && d.y_stride % vec == 0 && (uintptr_t)x % 16 == 0 &&
+           (uintptr_t)y % 16 == 0;
+}
+
+}  // namespace
+}  // namespace strata
+
+using namespace strata;
+
+extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_conv* desc, const void* x_dev,
+                                          const float* w_dev, const float* bias_dev, float* state_dev, void* y_dev,
+                                          void* stream) {
+    if (!ctx || !desc) return STRATA_ERR_INVALID;
+    STRATA_CALL_RANGE();
+    std::lock_guard<std::mutex> g(ctx->mu);
+    strata_short_conv d = *desc;
+    Why why;
+    int64_t tokens = 0, longest = 0;
+    int rc = check_short_conv(why, d, &tokens, &longest);
+    if (!rc) rc = check_short_conv_buffers(why, d, tokens, x_dev, w_dev, bias_dev, state_dev, y_dev);
+    if (rc) return fail(ctx, rc, "short_conv: %s", why.text);
+    if (longest == 0) return STRATA_OK;
+    const bool bf16 = d.dtype == STRATA_QUANT_BF16, vec = packs(d, x_dev, y_dev);
+    const int64_t per = (int64_t)kThreads * (vec ? (bf16 ? 8 : 4) : 1);
+    ConvArgs a{x_dev, w_dev, bias_dev, state_dev, y_dev, d.x_stride, d.y_stride, (int)d.channels,
+               (int)((d.channels + per - 1) / per), d.silu};
+    DeviceGuard dev(ctx->device);
+    const cudaStream_t s = pick_stream(ctx, stream);
+    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kTile, [&](const SeqTable& t, int64_t tiles,
+                                                                            int64_t first) {
+        if (tiles * a.blocks > kMaxTokens)
+            return fail(ctx, STRATA_ERR_INVALID, "short_conv: %lld tiles of %d channel blocks", (long long)tiles,
+                        a.blocks);
+        ConvArgs b = a;
+        if (state_dev) b.state = state_dev + first * (d.taps - 1) * d.channels;
+        const unsigned grid = (unsigned)(tiles * a.blocks);
+        if (bf16 && vec) launch_conv<__nv_bfloat16, 8>((int)d.taps, b, t, grid, s);
+        else if (bf16) launch_conv<__nv_bfloat16, 1>((int)d.taps, b, t, grid, s);
+        else if (vec) launch_conv<float, 4>((int)d.taps, b, t, grid, s);
+        else launch_conv<float, 1>((int)d.taps, b, t, grid, s);
+        return check_launch(ctx, "short_conv kernel");
+    });
+}

@@ -130,6 +130,11 @@ def lib() -> C.CDLL:
             "strata_cuda_gemv_sharded_dev": (i32, [vp, vp, vp, vp, i32, vp]),
             "strata_cuda_gemm_sharded_dev": (i32, [vp, vp, vp, vp, i64, vp]),
             "strata_cuda_moe_ffn_ep_dev": (i32, [vp, vp, vp, vp, i64, vp, vp]),
+            "strata_cuda_short_conv_dev": (i32, [vp, C.POINTER(ShortConvDesc), vp, vp, vp, vp, vp, vp]),
+            "strata_cuda_gated_delta_work_bytes": (i32, [C.POINTER(GatedDeltaDesc), C.POINTER(u64)]),
+            "strata_cuda_gated_delta_dev": (i32, [vp, C.POINTER(GatedDeltaDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                                  u64, vp]),
+            "strata_cuda_sample_dev": (i32, [vp, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp]),
         }
         for name, (res, args) in sig.items():
             if not hasattr(L, name):
@@ -172,6 +177,73 @@ class GgufValue(C.Structure):
     """strata_gguf_value (strata_gguf.h)."""
     _fields_ = [("type", C.c_uint32), ("i", C.c_int64), ("u", C.c_uint64), ("f", C.c_double),
                 ("str", C.c_void_p), ("str_len", C.c_uint64), ("elem", C.c_uint32), ("count", C.c_uint64)]
+
+
+class ShortConvDesc(C.Structure):
+    """strata_short_conv (strata_sequence.h)."""
+    _fields_ = [("n_seq", C.c_int64), ("seq_len", C.c_int64), ("seq_offsets", C.POINTER(C.c_int64)),
+                ("channels", C.c_int64), ("taps", C.c_int64), ("x_stride", C.c_int64), ("y_stride", C.c_int64),
+                ("dtype", C.c_uint32), ("silu", C.c_int)]
+
+
+class GatedDeltaDesc(C.Structure):
+    """strata_gated_delta (strata_sequence.h)."""
+    _fields_ = [("n_seq", C.c_int64), ("seq_len", C.c_int64), ("seq_offsets", C.POINTER(C.c_int64))]
+    _fields_ += [(nm, C.c_int64) for nm in ("n_k_head", "n_v_head", "k_dim", "v_dim", "q_stride", "k_stride",
+                                            "v_stride", "o_stride", "gate_stride", "beta_stride")]
+    _fields_ += [("scale", C.c_double), ("l2_eps", C.c_double), ("dtype", C.c_uint32), ("tiled", C.c_int),
+                 ("raw_gates", C.c_int)]
+
+
+def _sequences(desc, n_seq: int, seq_len: int, offsets):
+    """Fills a desc's sequences; returns the host array its pointer needs alive."""
+    desc.n_seq, desc.seq_len = n_seq, seq_len
+    if offsets is None:
+        return None
+    if len(offsets) != n_seq + 1:
+        raise BackendError(ERR_INVALID, f"{len(offsets)} offsets for {n_seq} sequences")
+    rows = (C.c_int64 * (n_seq + 1))(*offsets)
+    desc.seq_offsets = C.cast(rows, C.POINTER(C.c_int64))
+    return rows
+
+
+class ShortConv:
+    """The shape of a short convolution call (strata_short_conv): n_seq sequences of seq_len
+    tokens, or of the rows between `offsets` (n_seq + 1 row numbers); strides of 0 are packed."""
+
+    def __init__(self, n_seq: int, channels: int, taps: int, seq_len: int = 1, offsets=None, dtype: int = F32,
+                 silu: bool = True, x_stride: int = 0, y_stride: int = 0):
+        d = self.desc = ShortConvDesc()
+        self._rows = _sequences(d, n_seq, seq_len, offsets)
+        d.channels, d.taps, d.x_stride, d.y_stride = channels, taps, x_stride, y_stride
+        d.dtype, d.silu = dtype, int(silu)
+
+
+class GatedDelta:
+    """The shape of a gated delta rule call (strata_gated_delta): sequences as in ShortConv,
+    n_k_head query / key heads of k_dim and n_v_head value heads of v_dim; strides of 0 are
+    packed. A negative l2_eps leaves q and k unnormalised; scale None is 1 / sqrt(k_dim)."""
+
+    def __init__(self, n_seq: int, n_k_head: int, n_v_head: int, k_dim: int, v_dim: int, seq_len: int = 1,
+                 offsets=None, dtype: int = F32, scale: float | None = None, l2_eps: float = -1.0,
+                 tiled: bool = False, raw_gates: bool = False, q_stride: int = 0, k_stride: int = 0,
+                 v_stride: int = 0, o_stride: int = 0, gate_stride: int = 0, beta_stride: int = 0):
+        d = self.desc = GatedDeltaDesc()
+        self._rows = _sequences(d, n_seq, seq_len, offsets)
+        d.n_k_head, d.n_v_head, d.k_dim, d.v_dim = n_k_head, n_v_head, k_dim, v_dim
+        d.q_stride, d.k_stride, d.v_stride, d.o_stride = q_stride, k_stride, v_stride, o_stride
+        d.gate_stride, d.beta_stride = gate_stride, beta_stride
+        d.scale = max(k_dim, 1) ** -0.5 if scale is None else scale
+        d.l2_eps, d.dtype, d.tiled, d.raw_gates = l2_eps, dtype, int(tiled), int(raw_gates)
+
+
+def gated_delta_work_bytes(shape: GatedDelta) -> int:
+    """Bytes of device workspace gated_delta_dev needs for this shape (0: none)."""
+    v = C.c_uint64()
+    rc = lib().strata_cuda_gated_delta_work_bytes(C.byref(shape.desc), C.byref(v))
+    if rc != OK:
+        raise BackendError(rc, "gated_delta: bad shape")
+    return v.value
 
 
 def _fptr(a: np.ndarray):
@@ -658,6 +730,30 @@ class Context:
                        stream: int = 0):
         self.check(lib().strata_cuda_moe_ffn_ep_dev(self.h, layer.handle, x_ptr, logits_ptr or None, tokens, out_ptr,
                                                     stream or None))
+
+    # ---- the sequence operators (strata_sequence.h), on device pointers
+
+    def short_conv_dev(self, shape: ShortConv, x_ptr: int, w_ptr: int, bias_ptr: int, state_ptr: int, y_ptr: int,
+                       stream: int = 0):
+        self.check(lib().strata_cuda_short_conv_dev(self.h, C.byref(shape.desc), x_ptr or None, w_ptr or None,
+                                                    bias_ptr or None, state_ptr or None, y_ptr or None,
+                                                    stream or None))
+
+    def gated_delta_dev(self, shape: GatedDelta, q_ptr: int, k_ptr: int, v_ptr: int, gate_ptr: int, beta_ptr: int,
+                        coef_ptr: int, shift_ptr: int, state_ptr: int, o_ptr: int, work_ptr: int = 0,
+                        work_bytes: int = 0, stream: int = 0):
+        self.check(lib().strata_cuda_gated_delta_dev(self.h, C.byref(shape.desc), q_ptr or None, k_ptr or None,
+                                                     v_ptr or None, gate_ptr or None, beta_ptr or None,
+                                                     coef_ptr or None, shift_ptr or None, state_ptr or None,
+                                                     o_ptr or None, work_ptr or None, work_bytes, stream or None))
+
+    def sample_dev(self, logits_ptr: int, rows: int, vocab: int, uniform_ptr: int, ids_ptr: int,
+                   logprobs_ptr: int = 0, temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0,
+                   min_p_ptr: int = 0, stride: int = 0, stream: int = 0):
+        self.check(lib().strata_cuda_sample_dev(self.h, logits_ptr or None, rows, vocab, stride,
+                                                temperature_ptr or None, top_k_ptr or None, top_p_ptr or None,
+                                                min_p_ptr or None, uniform_ptr or None, ids_ptr or None,
+                                                logprobs_ptr or None, stream or None))
 
     def set_gemm_terms(self, terms: int):
         self.check(lib().strata_cuda_set_gemm_terms(self.h, terms))
