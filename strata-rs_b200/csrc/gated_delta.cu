@@ -13,34 +13,10 @@
 // warps. For one token per sequence it is bound by the state's bytes.
 #include <cuda_runtime.h>
 
-#include "sequence.cuh"
+#include "gated_delta.cuh"
 
 namespace strata {
 namespace {
-
-struct DeltaArgs {
-    const void *q, *k, *v;
-    const float *gate, *beta, *coef, *shift;
-    float* state;  // of the launch's first sequence
-    void* o;
-    int64_t q_stride, k_stride, v_stride, o_stride, gate_stride, beta_stride;
-    int k_heads, v_heads, k_dim, v_dim;
-    int col_blocks;
-    int tiled, raw_gates, norm;
-    float scale, eps;
-};
-
-__device__ __forceinline__ int key_head(const DeltaArgs& a, int h) {
-    return a.tiled ? h % a.k_heads : h / (a.v_heads / a.k_heads);
-}
-
-// The log of the decay and the step of value head h from what the call gives.
-__device__ __forceinline__ void gates(const DeltaArgs& a, int h, float& g, float& beta) {
-    if (!a.raw_gates) return;
-    const float z = g + (a.shift ? a.shift[h] : 0.0f);
-    g = a.coef[h] * (fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))));  // softplus without overflow
-    beta = 1.0f / (1.0f + expf(-beta));
-}
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_pack(const T* p, float (&d)[VEC]) {
@@ -50,6 +26,7 @@ __device__ __forceinline__ void load_pack(const T* p, float (&d)[VEC]) {
 }
 
 constexpr int kRows = 32;  // rows of S a thread holds
+constexpr int64_t kChunkFrom = 16;
 
 template <typename T, int WARPS, int VEC>
 __global__ void __launch_bounds__(WARPS * 32, VEC == 4 ? (WARPS == 8 ? 1 : 12 / WARPS) : 1)
@@ -62,12 +39,12 @@ __global__ void __launch_bounds__(WARPS * 32, VEC == 4 ? (WARPS == 8 ? 1 : 12 / 
     const int cb = b % a.col_blocks;
     b /= a.col_blocks;
     const int h = b % a.v_heads;
-    int seq, row, len, tile;
-    find_tile(tab, b / a.v_heads, seq, row, len, tile);
+    const Seq seq = sequence_at(tab, b / a.v_heads);
+    const int row = seq.row, len = seq.len;
     const int hk = key_head(a, h);
     const int c = (cb * 32 + lane) * VEC;
     const bool live = c < a.v_dim;
-    float* S = a.state + ((int64_t)seq * a.v_heads + h) * a.k_dim * a.v_dim + c;
+    float* S = a.state + ((int64_t)seq.slot * a.v_heads + h) * a.k_dim * a.v_dim + c;
     const int r0 = warp * kRows;
 
     float s[kRows][VEC];
@@ -186,7 +163,13 @@ int columns(const strata_gated_delta& d, const void* v, const float* state, cons
     return 1;
 }
 
-uint64_t work_needed(const strata_gated_delta&, int64_t) { return 0; }
+// Whether a call is read in chunks: k_dim as the chunk kernels hold it, and a
+// sequence long enough that chunks beat single tokens.
+bool in_chunks(const strata_gated_delta& d, int64_t longest) { return d.k_dim <= 128 && longest >= kChunkFrom; }
+
+uint64_t work_needed(const strata_gated_delta& d, int64_t longest) {
+    return in_chunks(d, longest) ? delta_chunk_work(d) : 0;
+}
 
 }  // namespace
 }  // namespace strata
@@ -231,22 +214,20 @@ int strata_cuda_gated_delta_dev(strata_ctx* ctx, const strata_gated_delta* desc,
                 (float)d.l2_eps};
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kMaxTokens, [&](const SeqTable& t, int64_t tiles,
-                                                                                 int64_t first) {
-        if (tiles * blocks * d.n_v_head > kMaxTokens)
-            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld sequences of %lld heads", (long long)tiles,
+    if (in_chunks(d, longest)) return delta_chunk_enqueue(ctx, d, a, work_dev, s);
+    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kMaxTokens, [&](const SeqTable& t, int64_t) {
+        if (t.n * blocks * d.n_v_head > kMaxTokens)
+            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %d sequences of %lld heads", t.n,
                         (long long)d.n_v_head);
-        DeltaArgs b = a;
-        b.state = state_dev + first * d.n_v_head * d.k_dim * d.v_dim;
-        const unsigned grid = (unsigned)(tiles * blocks * d.n_v_head);
+        const unsigned grid = (unsigned)(t.n * blocks * d.n_v_head);
         if (d.dtype == STRATA_QUANT_BF16) {
-            if (vec == 4) launch_step<__nv_bfloat16, 4>(b, t, grid, s);
-            else if (vec == 2) launch_step<__nv_bfloat16, 2>(b, t, grid, s);
-            else launch_step<__nv_bfloat16, 1>(b, t, grid, s);
+            if (vec == 4) launch_step<__nv_bfloat16, 4>(a, t, grid, s);
+            else if (vec == 2) launch_step<__nv_bfloat16, 2>(a, t, grid, s);
+            else launch_step<__nv_bfloat16, 1>(a, t, grid, s);
         } else {
-            if (vec == 4) launch_step<float, 4>(b, t, grid, s);
-            else if (vec == 2) launch_step<float, 2>(b, t, grid, s);
-            else launch_step<float, 1>(b, t, grid, s);
+            if (vec == 4) launch_step<float, 4>(a, t, grid, s);
+            else if (vec == 2) launch_step<float, 2>(a, t, grid, s);
+            else launch_step<float, 1>(a, t, grid, s);
         }
         return check_launch(ctx, "gated_delta kernel");
     });

@@ -1,0 +1,668 @@
+// gated_delta_chunk.cu — the gated delta rule over prompts, kChunk tokens at a
+// time, on the tensor cores.
+//
+// With G_i the sum of the log decays of a chunk's tokens up to i, the updates
+// u_i = beta_i (v_i - e^{g_i} S_{i-1}^T k_i) of a chunk that starts at state S
+// solve (I + A) U = X with
+//   A_ij = beta_i e^{G_i - G_j} k_i . k_j  (i > j),
+//   X_i  = beta_i (v_i - e^{G_i} S^T k_i),
+// and then
+//   o_i = scale (e^{G_i} S^T q_i + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) u_j),
+//   S  <- e^{G_C} S + sum_j e^{G_C - G_j} k_j u_j^T.
+// T = (I + A)^-1 and P_ij = e^{G_i - G_j} (q_i . k_j) do not depend on S:
+// delta_prepare_kernel computes them for all chunks at once (and U = T X needs
+// no second product with the keys). delta_scan_kernel then goes through the
+// chunks of a sequence in order with S in registers.
+//
+// Precision. The products run on the tensor cores as f16 limbs: x 2^e = hi + lo
+// with the exponent e taken per row from the row's largest magnitude, so a
+// limb pair carries 22 bits of it, and hi hi + hi lo + lo hi is summed in f32
+// (the two small products in accumulators of their own). That keeps f32-like
+// results at f16 rate; plain tf32 would carry 11 bits. Keys and queries given
+// as bf16 are exact in one limb. The scan adds to S outside the tensor core,
+// where the addition rounds to nearest.
+//
+// Layout of the scan. The columns of S are independent, and products are
+// written transposed: a warp's tile is 16 columns of S as the 16 rows of an
+// m16n8k16 product, S^T K^T, X^T T^T, U^T P^T, U^T K. An accumulator tile is
+// then, split into limbs, the left operand of the next product without leaving
+// the registers, and the right operands (keys, queries, T, P) are the same for
+// all columns: they are staged in shared memory by asynchronous copies one
+// chunk ahead. Two warps share a tile's 16 columns, each with half of k_dim:
+// they exchange their halves of S^T K^T and S^T Q^T through shared memory, and
+// each computes half of the chunk's outputs. A long sequence is bound by one
+// chunk's chain of products and exchanges, a batch by the tensor cores.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "gated_delta.cuh"
+
+namespace strata {
+namespace {
+
+constexpr int kChunk = 32;
+constexpr int kThreads = 128;
+constexpr int kCols = 32;                      // columns of S a scan block holds
+constexpr int kPitchT = kChunk * 2 + 16;       // bytes of a row of T or P: 16-byte steps that no two of 8 rows share
+constexpr int kLimbT = kChunk * kPitchT;
+constexpr int kGates = 4 * kLimbT;             // T hi, T lo, P hi, P lo, then the gate rows
+enum { kBeta, kXk, kOq, kDown, kScaleT, kScaleP, kTotal, kGateRows };
+constexpr int kImageT = kGates + kGateRows * kChunk * 4;
+constexpr uint64_t kMaxWork = uint64_t(256) << 20;
+
+// The image of a chunk's keys and queries: K limbs, then Q limbs, rows of
+// DK halves padded as T's.
+template <int DK, int LIMBS>
+struct Image {
+    static constexpr int kPitch = DK * 2 + 16;
+    static constexpr int kLimb = kChunk * kPitch;
+    static constexpr int kBytes = 2 * LIMBS * kLimb;
+};
+
+// The power of two that brings m to [2^14, 2^15), and its inverse. Both stay normal numbers.
+__device__ __forceinline__ void power_for(float m, float& up, float& down) {
+    int f = 268 - (int)((__float_as_uint(m) >> 23) & 255u);
+    f = f < 2 ? 2 : f > 252 ? 252 : f;
+    up = __uint_as_float((uint32_t)f << 23);
+    down = __uint_as_float((uint32_t)(254 - f) << 23);
+}
+
+// (x, y) as two f16 limbs, packed with x in the low half.
+__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ uint32_t shared_addr(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+
+// ---------------------------------------------------------------- prepare
+
+template <int DK, int LIMBS>
+constexpr int prepare_smem() {
+    return Image<DK, LIMBS>::kBytes + (2 * kChunk * (kChunk + 1) + 2 * kChunk + 4 * kChunk * (kChunk + 4)) * 4;
+}
+
+// One block per chunk and key head: limbs of K and Q, K K^T and Q K^T; then
+// one warp per value head of that key head: T and P.
+template <typename T, int DK, int LIMBS>
+__global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab,
+                                                                 uint8_t* __restrict__ images,
+                                                                 uint8_t* __restrict__ images_t) {
+    using I = Image<DK, LIMBS>;
+    constexpr int PER = DK / 32;  // elements of a row a lane holds
+    extern __shared__ __align__(16) uint8_t smem[];
+    float(*kk)[kChunk + 1] = reinterpret_cast<float(*)[kChunk + 1]>(smem + I::kBytes);
+    float(*qk)[kChunk + 1] = kk + kChunk;
+    float* fk = &qk[kChunk][0];  // what a row of limbs is to be multiplied with
+    float* fq = fk + kChunk;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float(*A)[kChunk + 4] = reinterpret_cast<float(*)[kChunk + 4]>(fq + kChunk) + warp * kChunk;
+    const int tile = blockIdx.x / a.k_heads, hk = blockIdx.x - tile * a.k_heads;
+    const Seq seq = sequence_of_tile(tab, tile);
+    const int t0 = (tile - seq.tile0) * kChunk, n = min(kChunk, seq.len - t0);
+    const int64_t row = (int64_t)seq.row + t0;
+
+    const T* K = static_cast<const T*>(a.k) + row * a.k_stride + (int64_t)hk * a.k_dim + lane * PER;
+    const T* Q = static_cast<const T*>(a.q) + row * a.q_stride + (int64_t)hk * a.k_dim + lane * PER;
+    const bool whole = a.k_dim == DK && PER * sizeof(T) >= 4 && a.k_stride % PER == 0 && a.q_stride % PER == 0 &&
+                       ((uintptr_t)a.k | (uintptr_t)a.q) % (PER * sizeof(T)) == 0;
+    float x[16][PER];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int i = warp * 8 + (r & 7);
+        const T* p = r < 8 ? K + i * a.k_stride : Q + i * a.q_stride;
+        if (i < n && whole) {
+            const Pack<T, PER> in = *reinterpret_cast<const Pack<T, PER>*>(p);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[r][e] = to_f32(in.v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[r][e] = i < n && lane * PER + e < a.k_dim ? to_f32(p[e]) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int i = warp * 8 + (r & 7);
+        float m = 0.0f, ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) m = fmaxf(m, fabsf(x[r][e])), ss = fmaf(x[r][e], x[r][e], ss);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        }
+        float up, down;
+        power_for(m, up, down);
+        __half hi[PER], lo[PER];
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            hi[e] = __float2half_rn(x[r][e] * up);
+            lo[e] = __float2half_rn(x[r][e] * up - __half2float(hi[e]));
+        }
+        uint8_t* at = smem + (r < 8 ? 0 : LIMBS * I::kLimb) + i * I::kPitch + lane * PER * 2;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            reinterpret_cast<__half*>(at)[e] = hi[e];
+            if (LIMBS == 2) reinterpret_cast<__half*>(at + I::kLimb)[e] = lo[e];
+        }
+        if (lane == 0) {
+            if (a.norm) down *= 1.0f / sqrtf(ss + a.eps);
+            (r < 8 ? fk : fq)[i] = i < n ? (r < 8 ? down : down * a.scale) : 0.0f;
+        }
+    }
+    __syncthreads();
+    {  // the image, as the scan will stage it
+        uint4* out = reinterpret_cast<uint4*>(images + (int64_t)blockIdx.x * I::kBytes);
+        for (int i = threadIdx.x; i < I::kBytes / 16; i += kThreads) out[i] = reinterpret_cast<const uint4*>(smem)[i];
+    }
+    {  // warps 0, 1: K K^T; 2, 3: Q K^T; 16 rows each, up to the diagonal
+        const int m0 = (warp & 1) * 16;
+        const uint32_t left = shared_addr(smem) + (warp < 2 ? 0 : LIMBS * I::kLimb) + (m0 + (lane & 15)) * I::kPitch +
+                              (lane >> 4) * 16;
+        const uint32_t right = shared_addr(smem) + ((lane & 7) + ((lane >> 4) << 3)) * I::kPitch + ((lane >> 3) & 1) * 16;
+        float c[4][4] = {}, s[4][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < DK / 16; ++ks) {
+            uint32_t ah[4], al[4];
+            ldmatrix(ah, left + ks * 32);
+            if (LIMBS == 2) ldmatrix(al, left + I::kLimb + ks * 32);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                if (p * 16 > m0) break;
+                uint32_t bh[4], bl[4];
+                ldmatrix(bh, right + p * 16 * I::kPitch + ks * 32);
+                mma(c[2 * p], ah, bh[0], bh[1]);
+                mma(c[2 * p + 1], ah, bh[2], bh[3]);
+                if (LIMBS == 2) {
+                    ldmatrix(bl, right + I::kLimb + p * 16 * I::kPitch + ks * 32);
+                    mma(s[2 * p], ah, bl[0], bl[1]);
+                    mma(s[2 * p + 1], ah, bl[2], bl[3]);
+                    mma(s[2 * p], al, bh[0], bh[1]);
+                    mma(s[2 * p + 1], al, bh[2], bh[3]);
+                }
+            }
+        }
+        float(*out)[kChunk + 1] = warp < 2 ? kk : qk;
+        const float* f = warp < 2 ? fk : fq;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = m0 + (lane >> 2) + (r >> 1) * 8, j = t * 8 + (lane & 3) * 2 + (r & 1);
+                out[i][j] = (c[t][r] + s[t][r]) * f[i] * fk[j];
+            }
+    }
+    __syncthreads();
+    const int per = a.v_heads / a.k_heads;
+    for (int m = warp; m < per; m += kThreads / 32) {
+        const int h = a.tiled ? hk + m * a.k_heads : hk * per + m;
+        float g = 0.0f, beta = 0.0f;
+        if (lane < n) {
+            g = a.gate[(row + lane) * a.gate_stride + h];
+            beta = a.beta[(row + lane) * a.beta_stride + h];
+            gates(a, h, g, beta);
+            // e^-10000 is zero; a sum of these stays a number, so that differences do
+            if (g < -1e4f) g = -1e4f;
+        }
+        double G = (double)g;  // differences of the sums must keep f32's precision
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double up = __shfl_up_sync(0xFFFFFFFFu, G, o);
+            if (lane >= o) G += up;
+        }
+        const double end = __shfl_sync(0xFFFFFFFFu, G, 31);
+        uint8_t* image = images_t + ((int64_t)tile * a.v_heads + h) * kImageT;
+        float scale_t = 0.0f, scale_p = 0.0f;
+        __syncwarp();
+        for (int i = 0; i < kChunk; ++i) {
+            const double Gi = __shfl_sync(0xFFFFFFFFu, G, i);
+            const float bi = __shfl_sync(0xFFFFFFFFu, beta, i);
+            const float e = lane <= i ? expf((float)(Gi - G)) : 0.0f;
+            A[i][lane] = lane < i ? bi * e * kk[i][lane] : 0.0f;
+            const float p = lane <= i ? e * qk[i][lane] : 0.0f;
+            float mx = fabsf(p), up, down;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+            power_for(mx, up, down);
+            const __half hi = __float2half_rn(p * up), lo = __float2half_rn(p * up - __half2float(hi));
+            __half* at = reinterpret_cast<__half*>(image + 2 * kLimbT + i * kPitchT) + lane;
+            at[0] = hi;
+            at[kLimbT / 2] = lo;
+            if (lane == i) scale_p = down;
+        }
+        __syncwarp();
+        // T = (I + A)^-1, a column a lane, row by row
+        float t[kChunk];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            float acc = lane == i ? 1.0f : 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) acc = fmaf(-A[i][j], t[j], acc);
+            t[i] = acc;
+        }
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            float mx = fabsf(t[i]), up, down;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+            power_for(mx, up, down);
+            const __half hi = __float2half_rn(t[i] * up), lo = __float2half_rn(t[i] * up - __half2float(hi));
+            __half* at = reinterpret_cast<__half*>(image + i * kPitchT) + lane;
+            at[0] = hi;
+            at[kLimbT / 2] = lo;
+            if (lane == i) scale_t = down;
+        }
+        float* out = reinterpret_cast<float*>(image + kGates) + lane;
+        const float before = expf((float)G), after = expf((float)(end - G));
+        out[kBeta * kChunk] = beta;
+        out[kXk * kChunk] = beta * before * fk[lane];
+        out[kOq * kChunk] = before * fq[lane];
+        out[kDown * kChunk] = after * fk[lane];
+        out[kScaleT * kChunk] = scale_t;
+        out[kScaleP * kChunk] = scale_p;
+        out[kTotal * kChunk] = expf((float)end);
+    }
+}
+
+// ------------------------------------------------------------------- scan
+
+constexpr int kExchange = 24;  // floats a lane hands to the warp with the other half: 16 of S^T K^T, 8 of S^T Q^T
+
+template <int DK, int LIMBS>
+constexpr int scan_smem() {
+    return 2 * (Image<DK, LIMBS>::kBytes + kImageT) + 4 * kExchange * 32 * 4;
+}
+
+// The largest magnitude of a row of the warp's tile: rows lie across 4 lanes.
+__device__ __forceinline__ float row_max(float m) {
+    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    return fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+}
+
+// Tiles x (16 rows by 8 N columns) as limbs of a left operand, scaled by row;
+// down: what undoes the scale, for the two rows of a lane.
+template <int N>
+__device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N / 2][4], uint32_t (&lo)[N / 2][4],
+                                      float (&down)[2]) {
+    float m0 = 0.0f, m1 = 0.0f, up0, up1;
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+        m0 = fmaxf(m0, fmaxf(fabsf(x[t][0]), fabsf(x[t][1])));
+        m1 = fmaxf(m1, fmaxf(fabsf(x[t][2]), fabsf(x[t][3])));
+    }
+    power_for(row_max(m0), up0, down[0]);
+    power_for(row_max(m1), up1, down[1]);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+        split(x[2 * k][0] * up0, x[2 * k][1] * up0, hi[k][0], lo[k][0]);
+        split(x[2 * k][2] * up1, x[2 * k][3] * up1, hi[k][1], lo[k][1]);
+        split(x[2 * k + 1][0] * up0, x[2 * k + 1][1] * up0, hi[k][2], lo[k][2]);
+        split(x[2 * k + 1][2] * up1, x[2 * k + 1][3] * up1, hi[k][3], lo[k][3]);
+    }
+}
+
+template <typename T, int DK, int LIMBS>
+__global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab,
+                                                                 const uint8_t* __restrict__ images,
+                                                                 const uint8_t* __restrict__ images_t) {
+    using I = Image<DK, LIMBS>;
+    constexpr int HALF = DK / 2, NT = HALF / 8, KS = HALF / 16;
+    constexpr int kStage = I::kBytes + kImageT;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* ex = reinterpret_cast<float*>(smem + 2 * kStage);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1;
+    int b = blockIdx.x;
+    const int cb = b % a.col_blocks;
+    b /= a.col_blocks;
+    const int h = b % a.v_heads;
+    const Seq seq = sequence_at(tab, b / a.v_heads);
+    const int hk = key_head(a, h);
+    const int chunks = (seq.len + kChunk - 1) / kChunk;
+    const int j0 = cb * kCols + (warp >> 1) * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
+    const bool in0 = j0 < a.v_dim, in1 = j1 < a.v_dim;
+    const int tc = (lane & 3) * 2;
+    const int d0 = half * HALF + tc;  // its first row of S
+
+    auto stage = [&](int c) {
+        const int64_t tile = seq.tile0 + c;
+        const uint8_t* src = images + (tile * a.k_heads + hk) * I::kBytes;
+        const uint8_t* src_t = images_t + (tile * a.v_heads + h) * kImageT;
+        const uint32_t dst = shared_addr(smem + (c & 1) * kStage);
+        for (int i = threadIdx.x; i < I::kBytes / 16; i += kThreads) copy16(dst + i * 16, src + i * 16);
+        for (int i = threadIdx.x; i < kImageT / 16; i += kThreads)
+            copy16(dst + I::kBytes + i * 16, src_t + i * 16);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+    stage(0);
+
+    float* S = a.state + ((int64_t)seq.slot * a.v_heads + h) * a.k_dim * a.v_dim;
+    float s[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int d = d0 + t * 8 + (r & 1), j = r < 2 ? j0 : j1;
+            s[t][r] = d < a.k_dim && j < a.v_dim ? S[(int64_t)d * a.v_dim + j] : 0.0f;
+        }
+    const T* V = static_cast<const T*>(a.v) + (int64_t)seq.row * a.v_stride + (int64_t)h * a.v_dim;
+    T* O = static_cast<T*>(a.o) + (int64_t)seq.row * a.o_stride + (int64_t)h * a.v_dim;
+    float v[4][4];
+    auto fetch = [&](int c) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = c * kChunk + t * 8 + tc + (r & 1);
+                const bool in = i < seq.len && (r < 2 ? in0 : in1);
+                v[t][r] = in ? to_f32(V[(int64_t)i * a.v_stride + (r < 2 ? j0 : j1)]) : 0.0f;
+            }
+    };
+    fetch(0);
+
+    const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
+    for (int c = 0; c < chunks; ++c) {
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        __syncthreads();  // the chunk is staged, and every warp is done with the one before
+        if (c + 1 < chunks) stage(c + 1);
+        const uint32_t base = shared_addr(smem + (c & 1) * kStage);
+        const float* gate = reinterpret_cast<const float*>(smem + (c & 1) * kStage + I::kBytes + kGates);
+
+        // this half's part of S^T K^T and S^T Q^T
+        float y[4][4] = {}, o[4][4] = {};
+        {
+            float y2[4][4] = {}, o2[4][4] = {};
+            uint32_t hi[KS][4], lo[KS][4];
+            float down[2];
+            limbs<NT>(s, hi, lo, down);
+            const uint32_t at = base + lane_b * I::kPitch + half * HALF * 2 + ((lane >> 3) & 1) * 16;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    uint32_t bk[4], bq[4];
+                    const uint32_t k_at = at + p * 16 * I::kPitch + ks * 32, q_at = k_at + LIMBS * I::kLimb;
+                    ldmatrix(bk, k_at);
+                    ldmatrix(bq, q_at);
+                    mma(y[2 * p], hi[ks], bk[0], bk[1]);
+                    mma(y[2 * p + 1], hi[ks], bk[2], bk[3]);
+                    mma(o[2 * p], hi[ks], bq[0], bq[1]);
+                    mma(o[2 * p + 1], hi[ks], bq[2], bq[3]);
+                    mma(y2[2 * p], lo[ks], bk[0], bk[1]);
+                    mma(y2[2 * p + 1], lo[ks], bk[2], bk[3]);
+                    mma(o2[2 * p], lo[ks], bq[0], bq[1]);
+                    mma(o2[2 * p + 1], lo[ks], bq[2], bq[3]);
+                    if (LIMBS == 2) {
+                        ldmatrix(bk, k_at + I::kLimb);
+                        ldmatrix(bq, q_at + I::kLimb);
+                        mma(y2[2 * p], hi[ks], bk[0], bk[1]);
+                        mma(y2[2 * p + 1], hi[ks], bk[2], bk[3]);
+                        mma(o2[2 * p], hi[ks], bq[0], bq[1]);
+                        mma(o2[2 * p + 1], hi[ks], bq[2], bq[3]);
+                    }
+                }
+            float* mine = ex + warp * kExchange * 32 + lane;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    y[t][r] = (y[t][r] + y2[t][r]) * down[r >> 1];
+                    o[t][r] = (o[t][r] + o2[t][r]) * down[r >> 1];
+                    mine[(t * 4 + r) * 32] = y[t][r];
+                    // the other warp's tokens
+                    if ((t >> 1) != half) mine[(16 + (t & 1) * 4 + r) * 32] = o[t][r];
+                }
+        }
+        __syncthreads();
+        const float* other = ex + (warp ^ 1) * kExchange * 32 + lane;
+        float x[4][4], out[2][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = t * 8 + tc + (r & 1);
+                const float yy = y[t][r] + other[(t * 4 + r) * 32];
+                x[t][r] = gate[kBeta * kChunk + i] * v[t][r] - gate[kXk * kChunk + i] * yy;
+            }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                out[t][r] = (half ? o[2 + t][r] : o[t][r]) + other[(16 + t * 4 + r) * 32];
+        if (c + 1 < chunks) fetch(c + 1);
+
+        const uint32_t t_at = base + I::kBytes + lane_b * kPitchT + ((lane >> 3) & 1) * 16;
+        // U^T = X^T T^T: token i takes tokens j <= i, so the second half of j only reaches the second half of i
+        float u[4][4];
+        {
+            uint32_t hi[2][4], lo[2][4];
+            float down[2], c1[4][4] = {}, c2[4][4] = {};
+            limbs<4>(x, hi, lo, down);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int p = ks; p < 2; ++p) {
+                    uint32_t bh[4], bl[4];
+                    ldmatrix(bh, t_at + p * 16 * kPitchT + ks * 32);
+                    ldmatrix(bl, t_at + kLimbT + p * 16 * kPitchT + ks * 32);
+                    mma(c1[2 * p], hi[ks], bh[0], bh[1]);
+                    mma(c1[2 * p + 1], hi[ks], bh[2], bh[3]);
+                    mma(c2[2 * p], lo[ks], bh[0], bh[1]);
+                    mma(c2[2 * p + 1], lo[ks], bh[2], bh[3]);
+                    mma(c2[2 * p], hi[ks], bl[0], bl[1]);
+                    mma(c2[2 * p + 1], hi[ks], bl[2], bl[3]);
+                }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    u[t][r] = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleT * kChunk + t * 8 + tc + (r & 1)]);
+        }
+        // this warp's half of the outputs
+        {
+            uint32_t hi[2][4], lo[2][4];
+            float down[2], c1[2][4] = {}, c2[2][4] = {};
+            limbs<4>(u, hi, lo, down);
+            const uint32_t p_at = t_at + 2 * kLimbT + half * 16 * kPitchT;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks > half) break;
+                uint32_t bh[4], bl[4];
+                ldmatrix(bh, p_at + ks * 32);
+                ldmatrix(bl, p_at + kLimbT + ks * 32);
+                mma(c1[0], hi[ks], bh[0], bh[1]);
+                mma(c1[1], hi[ks], bh[2], bh[3]);
+                mma(c2[0], lo[ks], bh[0], bh[1]);
+                mma(c2[1], lo[ks], bh[2], bh[3]);
+                mma(c2[0], hi[ks], bl[0], bl[1]);
+                mma(c2[1], hi[ks], bl[2], bl[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int k = half * 16 + t * 8 + tc + (r & 1), i = c * kChunk + k;
+                    const float y1 = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleP * kChunk + k]);
+                    const float res = fmaf(gate[kOq * kChunk + k], out[t][r], y1);
+                    if (i < seq.len && (r < 2 ? in0 : in1))
+                        from_f32(O[(int64_t)i * a.o_stride + (r < 2 ? j0 : j1)], res);
+                }
+        }
+        // S <- e^{G_C} S + (rows of U scaled to the chunk's end) K
+        {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[t][r] *= gate[kDown * kChunk + t * 8 + tc + (r & 1)];
+            uint32_t hi[2][4], lo[2][4];
+            float down[2];
+            limbs<4>(u, hi, lo, down);
+            const float total = gate[kTotal * kChunk];
+            const uint32_t at = base + (lane & 15) * I::kPitch + half * HALF * 2 + (lane >> 4) * 16;
+#pragma unroll
+            for (int p = 0; p < NT / 2; ++p) {
+                float c1[2][4] = {}, c2[2][4] = {};
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    uint32_t bh[4], bl[4];
+                    ldmatrix_trans(bh, at + ks * 16 * I::kPitch + p * 32);
+                    mma(c1[0], hi[ks], bh[0], bh[1]);
+                    mma(c1[1], hi[ks], bh[2], bh[3]);
+                    mma(c2[0], lo[ks], bh[0], bh[1]);
+                    mma(c2[1], lo[ks], bh[2], bh[3]);
+                    if (LIMBS == 2) {
+                        ldmatrix_trans(bl, at + I::kLimb + ks * 16 * I::kPitch + p * 32);
+                        mma(c2[0], hi[ks], bl[0], bl[1]);
+                        mma(c2[1], hi[ks], bl[2], bl[3]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], (c1[t][r] + c2[t][r]) * down[r >> 1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int d = d0 + t * 8 + (r & 1), j = r < 2 ? j0 : j1;
+            if (d < a.k_dim && j < a.v_dim) S[(int64_t)d * a.v_dim + j] = s[t][r];
+        }
+}
+
+// ------------------------------------------------------------------- host
+
+int padded_dim(int64_t k_dim) { return k_dim <= 32 ? 32 : k_dim <= 64 ? 64 : k_dim <= 96 ? 96 : 128; }
+
+// Bytes of the images of one chunk over all heads.
+struct ChunkBytes {
+    uint64_t keys, rest;
+    uint64_t all() const { return keys + rest; }
+};
+ChunkBytes chunk_bytes(const strata_gated_delta& d) {
+    const uint64_t limbs = d.dtype == STRATA_QUANT_BF16 ? 1 : 2;
+    return ChunkBytes{2 * limbs * kChunk * (uint64_t)(padded_dim(d.k_dim) * 2 + 16) * (uint64_t)d.n_k_head,
+                      (uint64_t)kImageT * (uint64_t)d.n_v_head};
+}
+
+// The launches of a call: groups of sequences, each read in pieces of as many
+// chunks as the workspace bound allows (one per sequence at least). Calls
+// launch(table, tiles) in order.
+template <typename F>
+int plan_chunks(const strata_gated_delta& d, F launch) {
+    const uint64_t fit = kMaxWork / chunk_bytes(d).all();
+    const int64_t cap = fit < 1 ? 1 : (int64_t)fit;
+    auto per_sequence = [&](int64_t n) { return cap / n > 1 ? cap / n : int64_t(1); };
+    if (!d.seq_offsets) {
+        const int64_t group = d.n_seq < cap ? d.n_seq : cap;
+        for (int64_t i = 0; i < d.n_seq; i += group) {
+            const int64_t n = d.n_seq - i < group ? d.n_seq - i : group, step = per_sequence(n) * kChunk;
+            for (int64_t t = 0; t < d.seq_len; t += step) {
+                const int64_t len = d.seq_len - t < step ? d.seq_len - t : step;
+                const SeqTable tab = uniform_table(n, i * d.seq_len + t, d.seq_len, i, len, kChunk);
+                const int rc = launch(tab, n * tab.tiles_all);
+                if (rc) return rc;
+            }
+        }
+        return STRATA_OK;
+    }
+    const int64_t group = cap < kSeqGroup ? cap : kSeqGroup;
+    const int64_t* off = d.seq_offsets;
+    for (int64_t i = 0; i < d.n_seq;) {
+        int64_t end = i, live = 0;  // sequences [i, end), `live` of them with tokens
+        while (end < d.n_seq && live < group) live += off[end + 1] > off[end], ++end;
+        for (int64_t t = 0; live > 0;) {
+            const int64_t step = per_sequence(live) * kChunk;
+            SeqTable tab = ragged_table();
+            int64_t left = 0;
+            for (int64_t k = i; k < end; ++k) {
+                const int64_t len = off[k + 1] - off[k] - t;
+                if (len <= 0) continue;
+                add_sequence(tab, k, off[k] + t, len < step ? len : step, kChunk);
+                left += len > step;
+            }
+            const int rc = launch(tab, (int64_t)tab.tile[tab.n]);
+            if (rc) return rc;
+            t += step;
+            live = left;
+        }
+        i = end;
+    }
+    return STRATA_OK;
+}
+
+template <typename T, int DK, int LIMBS>
+int enqueue(strata_ctx* ctx, const strata_gated_delta& d, DeltaArgs a, uint8_t* work, cudaStream_t s) {
+    auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
+    auto scan = delta_scan_kernel<T, DK, LIMBS>;
+    constexpr int sp = prepare_smem<DK, LIMBS>(), ss = scan_smem<DK, LIMBS>();
+    cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, sp);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ss);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
+    a.col_blocks = (a.v_dim + kCols - 1) / kCols;
+    const uint64_t keys = chunk_bytes(d).keys;
+    return plan_chunks(d, [&](const SeqTable& t, int64_t tiles) {
+        const int64_t gp = tiles * a.k_heads, gs = (int64_t)t.n * a.v_heads * a.col_blocks;
+        if (gp > kMaxTokens || gs > kMaxTokens)
+            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.v_heads);
+        uint8_t* images_t = work + keys * (uint64_t)tiles;
+        prepare<<<(unsigned)gp, kThreads, sp, s>>>(a, t, work, images_t);
+        scan<<<(unsigned)gs, kThreads, ss, s>>>(a, t, work, images_t);
+        return check_launch(ctx, "gated_delta chunk kernels");
+    });
+}
+
+template <typename T, int LIMBS>
+int enqueue_dim(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
+    switch (padded_dim(d.k_dim)) {
+        case 32: return enqueue<T, 32, LIMBS>(ctx, d, a, work, s);
+        case 64: return enqueue<T, 64, LIMBS>(ctx, d, a, work, s);
+        case 96: return enqueue<T, 96, LIMBS>(ctx, d, a, work, s);
+        default: return enqueue<T, 128, LIMBS>(ctx, d, a, work, s);
+    }
+}
+
+}  // namespace
+
+uint64_t delta_chunk_work(const strata_gated_delta& d) {
+    int64_t most = 0;
+    plan_chunks(d, [&](const SeqTable&, int64_t tiles) {
+        if (tiles > most) most = tiles;
+        return (int)STRATA_OK;
+    });
+    return (uint64_t)most * chunk_bytes(d).all();
+}
+
+int delta_chunk_enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, void* work, cudaStream_t s) {
+    uint8_t* w = static_cast<uint8_t*>(work);
+    if (d.dtype == STRATA_QUANT_BF16) return enqueue_dim<__nv_bfloat16, 1>(ctx, d, a, w, s);
+    return enqueue_dim<float, 2>(ctx, d, a, w, s);
+}
+
+}  // namespace strata

@@ -25,68 +25,85 @@ struct DeviceGuard {
 };
 
 // The sequences of one launch, by value in the kernel's parameters: no copy
-// to wait for, nothing to allocate, and a captured graph holds its own. Calls
-// with more ragged sequences than kSeqGroup launch once per group.
-constexpr int kSeqGroup = 256;
+// to wait for, nothing to allocate, and a captured graph holds its own. Empty
+// sequences are left out; calls with more ragged sequences than kSeqGroup
+// launch once per group.
+constexpr int kSeqGroup = 224;  // with its four numbers a sequence, the table stays within 4 KB
 struct SeqTable {
-    int n;                     // sequences in this launch
-    int uniform;               // 1: sequence i holds rows [first + i * len, first + (i + 1) * len)
-    int first, len, tiles;     // uniform: rows and tiles of each sequence
-    int row[kSeqGroup + 1];    // ragged: first row of each sequence, and the row behind the last
-    int tile[kSeqGroup + 1];   // ragged: tiles before each sequence
+    int n;                   // sequences in this launch
+    int uniform;             // 1: sequence i is state `slot0 + i`, rows from first + i * pitch, all len long
+    int first, pitch, slot0, len_all, tiles_all;
+    int row[kSeqGroup];      // ragged: first row,
+    int len[kSeqGroup];      // rows,
+    int slot[kSeqGroup];     // number in the call (its state's),
+    int tile[kSeqGroup + 1]; // and tiles before each sequence
 };
 
-// Tile `b` of the launch: its sequence, that sequence's first row and number
-// of rows, and the tile's number in it.
-__device__ __forceinline__ void find_tile(const SeqTable& t, int b, int& seq, int& row, int& len, int& tile) {
-    if (t.uniform) {
-        seq = b / t.tiles;
-        tile = b - seq * t.tiles;
-        row = t.first + seq * t.len;
-        len = t.len;
-        return;
-    }
+// A sequence of a launch as a kernel sees it.
+struct Seq {
+    int slot, row, len;
+    int tile0;  // tiles of the sequences before it
+};
+
+__device__ __forceinline__ Seq sequence_at(const SeqTable& t, int i) {
+    if (t.uniform) return Seq{t.slot0 + i, t.first + i * t.pitch, t.len_all, i * t.tiles_all};
+    return Seq{t.slot[i], t.row[i], t.len[i], t.tile[i]};
+}
+
+// The sequence that tile `b` of the launch belongs to.
+__device__ __forceinline__ Seq sequence_of_tile(const SeqTable& t, int b) {
+    if (t.uniform) return sequence_at(t, b / t.tiles_all);
     int lo = 0, hi = t.n;  // tile[lo] <= b < tile[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (t.tile[mid] <= b) lo = mid;
         else hi = mid;
     }
-    seq = lo;
-    row = t.row[lo];
-    len = t.row[lo + 1] - row;
-    tile = b - t.tile[lo];
+    return sequence_at(t, lo);
 }
 
-// Calls launch(table, tiles, first sequence) for each group of sequences that has tiles of `rows` rows.
+inline SeqTable uniform_table(int64_t n, int64_t first, int64_t pitch, int64_t slot0, int64_t len, int64_t rows) {
+    SeqTable t;
+    t.n = (int)n;
+    t.uniform = 1;
+    t.first = (int)first;
+    t.pitch = (int)pitch;
+    t.slot0 = (int)slot0;
+    t.len_all = (int)len;
+    t.tiles_all = (int)((len + rows - 1) / rows);
+    return t;
+}
+inline SeqTable ragged_table() {
+    SeqTable t;
+    t.n = t.uniform = 0;
+    t.first = t.pitch = t.slot0 = t.len_all = t.tiles_all = 0;
+    t.tile[0] = 0;
+    return t;
+}
+inline void add_sequence(SeqTable& t, int64_t slot, int64_t row, int64_t len, int64_t rows) {
+    t.slot[t.n] = (int)slot;
+    t.row[t.n] = (int)row;
+    t.len[t.n] = (int)len;
+    t.tile[t.n + 1] = t.tile[t.n] + (int)((len + rows - 1) / rows);
+    ++t.n;
+}
+
+// Calls launch(table, tiles) for each group of sequences, cut into tiles of `rows` rows.
 template <typename F>
 int for_sequence_groups(int64_t n_seq, int64_t seq_len, const int64_t* off, int64_t rows, F launch) {
     if (!off) {
         if (seq_len == 0) return STRATA_OK;
-        SeqTable t;
-        t.n = (int)n_seq;
-        t.uniform = 1;
-        t.first = 0;
-        t.len = (int)seq_len;
-        t.tiles = (int)((seq_len + rows - 1) / rows);
-        return launch(t, n_seq * t.tiles, int64_t(0));
+        const SeqTable t = uniform_table(n_seq, 0, seq_len, 0, seq_len, rows);
+        return launch(t, n_seq * t.tiles_all);
     }
-    for (int64_t s0 = 0; s0 < n_seq; s0 += kSeqGroup) {
-        SeqTable t;
-        t.n = (int)(n_seq - s0 < kSeqGroup ? n_seq - s0 : kSeqGroup);
-        t.uniform = 0;
-        t.first = t.len = t.tiles = 0;
-        int64_t tiles = 0;
-        for (int i = 0; i < t.n; ++i) {
-            t.row[i] = (int)off[s0 + i];
-            t.tile[i] = (int)tiles;
-            tiles += (off[s0 + i + 1] - off[s0 + i] + rows - 1) / rows;
+    SeqTable t = ragged_table();
+    for (int64_t i = 0; i < n_seq; ++i) {
+        if (off[i + 1] > off[i]) add_sequence(t, i, off[i], off[i + 1] - off[i], rows);
+        if (t.n == kSeqGroup || (i + 1 == n_seq && t.n)) {
+            const int rc = launch(t, (int64_t)t.tile[t.n]);
+            if (rc) return rc;
+            t = ragged_table();
         }
-        t.row[t.n] = (int)off[s0 + t.n];
-        t.tile[t.n] = (int)tiles;
-        if (!tiles) continue;
-        const int rc = launch(t, tiles, s0);
-        if (rc) return rc;
     }
     return STRATA_OK;
 }
@@ -96,10 +113,10 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162flo
 __device__ __forceinline__ void from_f32(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f32(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
 
-// VEC elements as they lie in memory: 16-byte accesses where VEC * sizeof(T)
-// is 16, plain ones otherwise.
+// VEC elements as they lie in memory: one access where VEC is a power of two
+// (16 bytes at most), plain ones otherwise.
 template <typename T, int VEC>
-struct alignas(VEC * sizeof(T) >= 16 ? 16 : VEC * sizeof(T)) Pack {
+struct alignas(VEC & (VEC - 1) ? sizeof(T) : VEC * sizeof(T) >= 16 ? 16 : VEC * sizeof(T)) Pack {
     T v[VEC];
 };
 

@@ -29,7 +29,7 @@ struct ConvArgs {
     const void* x;
     const float* w;
     const float* bias;
-    float* state;  // of the launch's first sequence
+    float* state;
     void* y;
     int64_t x_stride, y_stride;
     int channels, blocks;  // blocks of channels
@@ -49,9 +49,8 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvArgs a, const 
     const int block = blockIdx.x / a.blocks;
     const int c = ((blockIdx.x - block * a.blocks) * kThreads + threadIdx.x) * VEC;
     if (c >= a.channels) return;
-    int seq, row, len, tile;
-    find_tile(tab, block, seq, row, len, tile);
-    const int t0 = tile * kTile;
+    const Seq seq = sequence_of_tile(tab, block);
+    const int row = seq.row, len = seq.len, t0 = (block - seq.tile0) * kTile;
     const int n = len - t0 < kTile ? len - t0 : kTile;
     const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.x_stride + c;
     T* y = static_cast<T*>(a.y) + (int64_t)(row + t0) * a.y_stride + c;
@@ -66,7 +65,7 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvArgs a, const 
         bias[v] = a.bias ? a.bias[c + v] : 0.0f;
     }
     if (K > 1) {
-        float* st = a.state + (int64_t)seq * (K - 1) * a.channels + c;
+        float* st = a.state + (int64_t)seq.slot * (K - 1) * a.channels + c;
         if (t0 == 0) {
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
@@ -165,22 +164,19 @@ extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_co
     if (longest == 0) return STRATA_OK;
     const bool bf16 = d.dtype == STRATA_QUANT_BF16, vec = packs(d, x_dev, y_dev);
     const int64_t per = (int64_t)kThreads * (vec ? (bf16 ? 8 : 4) : 1);
-    ConvArgs a{x_dev, w_dev, bias_dev, state_dev, y_dev, d.x_stride, d.y_stride, (int)d.channels,
+    const ConvArgs a{x_dev, w_dev, bias_dev, state_dev, y_dev, d.x_stride, d.y_stride, (int)d.channels,
                (int)((d.channels + per - 1) / per), d.silu};
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kTile, [&](const SeqTable& t, int64_t tiles,
-                                                                            int64_t first) {
+    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kTile, [&](const SeqTable& t, int64_t tiles) {
         if (tiles * a.blocks > kMaxTokens)
             return fail(ctx, STRATA_ERR_INVALID, "short_conv: %lld tiles of %d channel blocks", (long long)tiles,
                         a.blocks);
-        ConvArgs b = a;
-        if (state_dev) b.state = state_dev + first * (d.taps - 1) * d.channels;
         const unsigned grid = (unsigned)(tiles * a.blocks);
-        if (bf16 && vec) launch_conv<__nv_bfloat16, 8>((int)d.taps, b, t, grid, s);
-        else if (bf16) launch_conv<__nv_bfloat16, 1>((int)d.taps, b, t, grid, s);
-        else if (vec) launch_conv<float, 4>((int)d.taps, b, t, grid, s);
-        else launch_conv<float, 1>((int)d.taps, b, t, grid, s);
+        if (bf16 && vec) launch_conv<__nv_bfloat16, 8>((int)d.taps, a, t, grid, s);
+        else if (bf16) launch_conv<__nv_bfloat16, 1>((int)d.taps, a, t, grid, s);
+        else if (vec) launch_conv<float, 4>((int)d.taps, a, t, grid, s);
+        else launch_conv<float, 1>((int)d.taps, a, t, grid, s);
         return check_launch(ctx, "short_conv kernel");
     });
 }
