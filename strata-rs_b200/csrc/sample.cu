@@ -33,13 +33,16 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = kThreads;       // a bin a thread
+constexpr int kBins = kThreads;       // of the wide search: a bin a thread
 constexpr int kBinBits = 9;
 static_assert(kBins == 1 << kBinBits, "a key range is cut into kBins");
-constexpr float kBinsPerNat = 16.0f;  // value histograms: 32 nats, the last bin takes the rest
+constexpr float kBinsPerNat = 16.0f;  // its value histogram: 32 nats, the last bin takes the rest
+constexpr int kFine = 2048;           // of the first pass: kPer bins a thread,
+constexpr int kPer = kFine / kThreads;
+constexpr float kFinePerNat = 128.0f; // 16 nats from 4 above the sample's maximum
 constexpr int kMaxCluster = 8;
 constexpr int kList = 4096;           // tokens a list holds
-constexpr int kExpTable = 128;
+constexpr int kExpTable = 64;
 
 struct SampleArgs {
     const float* logits;
@@ -82,9 +85,9 @@ struct Part {
 
 // A block's part of what the first pass finds.
 struct First {
-    double sum;       // of every token's weight, where the row needs it
-    float best;       // largest logit and its first index
-    int index, alive; // tokens that can be taken
+    double sum;  // of every token's weight, where the row needs it
+    float best;  // largest logit and, where the row takes it, its first index
+    int index;
 };
 
 struct Shared {
@@ -96,7 +99,10 @@ struct Shared {
     uint8_t chain[kWarps][kList / 32];  // the pool's groups of 32 that hold them, in order
     int pool_used;
     int offset[kMaxCluster * kWarps + 1];  // of each warp's tokens in the list of the whole row
-    double exp2_table[kExpTable];
+    double exp2_table[kExpTable][32];  // a copy a lane: no two lanes meet in a bank
+    float dense[kWarps][32 + 128];     // values waiting for their exponentials, 32 at a time
+    alignas(16) uint32_t fine[kFine];              // exchanged: the first pass's histogram
+    double segment[kMaxCluster * kWarps];
     int won, id;                   // the draw: its segment (-1: id is the token)
     double won_before, total, weight;
     Part part[2];                  // exchanged, alternating
@@ -113,15 +119,13 @@ struct Shared {
 struct Row {
     const SampleArgs& a;
     Shared& sh;
-    const float* x;    // this block's slice, in shared or global memory; or a list
-    const int* index;  // a list's indices (nullptr: x is a slice)
-    int base, n;       // its first index and its number of elements
+    const float* x;  // this block's slice, in shared or global memory
+    int base, n;     // its first index and its number of elements
     int seg;         // elements of a warp (contiguous)
     int rank, ranks;
     int turn, hturn;
     cg::cluster_group cluster;
 
-    __device__ __forceinline__ int at(int i) const { return index ? index[i] : base + i; }
     __device__ __forceinline__ void sync() {
         if (ranks == 1) __syncthreads();
         else cluster.sync();
@@ -136,7 +140,7 @@ struct Row {
     __device__ __forceinline__ void each(F f) {
         const int lo = (threadIdx.x >> 5) * seg, hi = min(lo + seg, n);
 #pragma unroll 4
-        for (int i = lo + (threadIdx.x & 31); i < hi; i += 32) f(x[i], at(i));
+        for (int i = lo + (threadIdx.x & 31); i < hi; i += 32) f(x[i], base + i);
     }
 
     // Sums (a, b, n) and bounds (lo, hi) over the cluster, the same in every thread.
@@ -262,7 +266,7 @@ struct Row {
                 const bool hit = i + lane < hi && key_of(x[i + lane]) == key;
                 const unsigned m = __ballot_sync(0xFFFFFFFFu, hit);
                 if (seen + __popc(m) >= want) {
-                    if (hit && seen + __popc(m & ((1u << lane) - 1u)) + 1 == want) found = (uint32_t)at(i + lane);
+                    if (hit && seen + __popc(m & ((1u << lane) - 1u)) + 1 == want) found = (uint32_t)(base + i + lane);
                     break;
                 }
                 seen += __popc(m);
@@ -324,10 +328,7 @@ __device__ Cut cut_top_k(Row& r, float top, uint32_t k) {
     }
 }
 
-// `above`: the mass of kept tokens larger than all of the view's. total: the
-// kept tokens' mass (0: those of the view). `fits` (optional) reports whether
-// the border lies in the view; it does not where the view ends above it.
-__device__ Cut cut_top_p(Row& r, float top, double p, Cut cut, double above, double total, bool* fits) {
+__device__ Cut cut_top_p(Row& r, float top, double p, Cut cut) {
     // the kept tokens' mass, and their histogram
     Part z{0.0, 0.0, 0u, 0u, 0};
     const uint32_t count = r.histogram([&](uint32_t* h) {
@@ -339,12 +340,7 @@ __device__ Cut cut_top_p(Row& r, float top, double p, Cut cut, double above, dou
             }
         });
     });
-    const double mass = r.reduce(z).a;
-    const double target = p * (total > 0.0 ? total : above + mass) - above;
-    if (fits) {
-        *fits = target > 0.0 && target <= mass;
-        if (!*fits) return cut;
-    }
+    const double target = p * r.reduce(z).a;
     const double guess = (double)count * exp(-((double)threadIdx.x + 0.5) / (double)kBinsPerNat);
     double before;
     int bin = r.border<double>(count, guess, target, before), way = 0;
@@ -424,31 +420,43 @@ __device__ Cut cut_top_p(Row& r, float top, double p, Cut cut, double above, dou
     }
 }
 
-// exp(x) by the table method (Tang, 1989): x = (128 m + j) ln2 / 128 + r,
-// exp(x) = 2^m 2^(j/128) exp(r), |r| <= ln2 / 256, four terms of the series.
-// Good to a few 1e-15 of the result for |x| < 700 (the cuts compare sums of
-// thousands of tokens); 0 below -700, infinity above 700.
-__device__ __forceinline__ double exp_table(double x, const double* table) {
-    constexpr double kLn2 = 0.69314718055994530942, kMagic = 6755399441055744.0;  // 1.5 * 2^52
-    if (!(x > -700.0)) return 0.0;
-    if (x > 700.0) return INFINITY;
-    const double t = fma(x, kExpTable / kLn2, kMagic);
-    const int n = __double2loint(t);
-    const double r = fma(t - kMagic, -kLn2 / kExpTable, x);
-    const double q = fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0);
-    const double b = table[n & (kExpTable - 1)];
-    const double y = fma(b * r, q, b);
-    return __hiloint2double(__double2hiint(y) + ((n >> 7) << 20), __double2loint(y));
-}
+// exp by the table method (Tang, 1989): v f + c = (64 m + j) ln2 / 64 + r,
+// exp = 2^m 2^(j/64) exp(r), |r| <= ln2 / 128, four terms of exp(r) - 1. Good
+// to 4e-14 of the result while |v f + c| < 700.
+struct Exp {
+    const double (*table)[32];
+    double f, c, tf, tc;  // the argument, and 64 / ln2 times it plus the rounding constant
+    __device__ Exp(const double (*t)[32], double f_, double c_) : table(t), f(f_), c(c_) {
+        constexpr double kLn2 = 0.69314718055994530942, kMagic = 6755399441055744.0;  // 1.5 * 2^52
+        tf = f * (kExpTable / kLn2);
+        tc = c * (kExpTable / kLn2) + kMagic;
+    }
+    __device__ __forceinline__ double operator()(float v) const {
+        constexpr double kLn2 = 0.69314718055994530942, kMagic = 6755399441055744.0;
+        const double x = (double)v;
+        const double t = fma(x, tf, tc);
+        const int n = __double2loint(t);
+        const double r = fma(t - kMagic, -kLn2 / kExpTable, fma(x, f, c));
+        const double b = table[n & (kExpTable - 1)][threadIdx.x & 31];
+        const double q = fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0);
+        const double y = fma(b * r, q, b);
+        return __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));
+    }
+};
 
-// The value histogram of the first pass: `high` falls into bin 0.
-__device__ __forceinline__ int value_bin(float v, float high) {
-    return (int)fminf(fmaxf((high - v) * kBinsPerNat, 0.0f), (float)(kBins - 1));
-}
+// The value histogram of the first pass. One fused operation and two bounds,
+// all monotone: a larger value is never in a later bin.
+struct Fine {
+    float high;  // (what falls into bin 0) * kFinePerNat + 2^23: the sum's last bits are the bin
+    __device__ __forceinline__ int operator()(float v) const {
+        const float b = fminf(fmaxf(fmaf(v, -kFinePerNat, high), 8388608.0f), 8388608.0f + (kFine - 1));
+        return (int)(__float_as_uint(b) & (kFine - 1));
+    }
+};
 
-constexpr int kListBytes = kList * 16;          // the pool of this block's tokens, and the row's list
-constexpr int64_t kMaxSlice = 128 * 1024;       // bytes of a slice that is kept in shared memory,
-constexpr int64_t kPairSlice = 38 * 1024;       // and that leave room for two blocks a multiprocessor
+constexpr int kListBytes = kList * 16;     // the pool of this block's tokens, and the row's list
+constexpr int64_t kMaxSlice = 116 * 1024;  // bytes of a slice that is kept in shared memory,
+constexpr int64_t kPairSlice = 5 * 1024;    // and that leave room for two blocks a multiprocessor
 
 // Four elements of a lane: neighbours where the row is 16-byte packs, 32 apart otherwise.
 template <bool PACKS>
@@ -460,12 +468,9 @@ template <bool PACKS>
 __device__ __forceinline__ void load4(const float* x, int i, int hi, float (&v)[4]) {
     if (PACKS) {
         const int at = element<true>(i, 0);
-        if (at < hi) {
-            const float4 p = *reinterpret_cast<const float4*>(x + at);
-            v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w;
-        } else {
-            v[0] = v[1] = v[2] = v[3] = -INFINITY;
-        }
+        float4 p = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (at < hi) p = *reinterpret_cast<const float4*>(x + at);
+        v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -475,62 +480,107 @@ __device__ __forceinline__ void load4(const float* x, int i, int hi, float (&v)[
     }
 }
 
-// The first element, in index order, of [lo, hi) of the block's slice whose
-// running sum of weights exceeds `target` (the last one with a weight if none
-// does): the block's warps take a part each, the warp that holds it walks its part.
-template <typename W>
-__device__ int locate(Row& r, int lo, int hi, double target, double* weight_out, W weight) {
+// Inclusive sum over the block's threads, and the total.
+__device__ __forceinline__ double block_scan(Shared& sh, double v, double& total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int part = ((hi - lo + kThreads - 1) / kThreads) * 32;
-    const int from = min(lo + warp * part, hi), to = min(from + part, hi);
-    double w = 0.0;
-    for (int i = from + lane; i < to; i += 32) w += weight(r.x[i], r.base + i);
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
-    __syncthreads();
-    if (lane == 0) r.sh.wsum[0][warp] = w;
-    if (threadIdx.x == 0) r.sh.found = -1, r.sh.pick_bin = INT_MAX;
-    __syncthreads();
-    double run = 0.0;
-    bool mine = w > 0.0;  // the first warp whose sum goes past the target, else the last with a weight
-    for (int k = 0; k < kWarps; ++k) {
-        if (k < warp) run += r.sh.wsum[0][k];
-        else if (k > warp && run + w <= target && r.sh.wsum[0][k] > 0.0) mine = false;
-    }
-    if (run > target) mine = false;
-    if (mine) {
-        int found = INT_MAX, last = -1;
-        for (int i = from; i < to; i += 32) {
-            const double wi = i + lane < to ? weight(r.x[i + lane], r.base + i + lane) : 0.0;
-            double incl = wi;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            if (wi > 0.0) {
-                last = i + lane;
-                if (run + incl > target) found = i + lane;
-            }
-            run += __shfl_sync(0xFFFFFFFFu, incl, 31);
-            if (__any_sync(0xFFFFFFFFu, found != INT_MAX)) break;
-        }
-        if (found != INT_MAX) atomicMin(&r.sh.pick_bin, found);
-        if (last >= 0) atomicMax(&r.sh.found, last);
+    for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += up;
     }
     __syncthreads();
-    const int at = r.sh.pick_bin != INT_MAX ? r.sh.pick_bin : r.sh.found;
-    *weight_out = at >= 0 ? weight(r.x[at], r.base + at) : 0.0;
-    return at >= 0 ? r.base + at : -1;
+    if (lane == 31) sh.wsum[0][warp] = v;
+    __syncthreads();
+    double before = 0.0;
+    total = 0.0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before = total;
+        total += sh.wsum[0][w];
+    }
+    return before + v;
+}
+
+// Among the block's weights w[e] (element threadIdx.x * PER + e), the first
+// whose running sum exceeds `target` of the total `u` asks for; the last one
+// with a weight where none does (u >= 1, or a border's rounding). -1: none.
+template <int PER>
+__device__ int pick(Shared& sh, const double (&w)[PER], double u, double offset, double& total, double& weight) {
+    double own = 0.0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) own += w[e];
+    double run = block_scan(sh, own, total) - own;
+    const double target = u >= 0.0 ? u * total : offset;
+    if (threadIdx.x == 0) sh.pick_bin = INT_MAX, sh.found = -1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        run += w[e];
+        if (w[e] > 0.0) {
+            atomicMax(&sh.found, (int)threadIdx.x * PER + e);
+            if (run > target) atomicMin(&sh.pick_bin, (int)threadIdx.x * PER + e);
+        }
+    }
+    __syncthreads();
+    const int at = sh.pick_bin != INT_MAX ? sh.pick_bin : sh.found;
+    if (at >= 0 && at / PER == (int)threadIdx.x) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (at % PER == e) sh.weight = w[e], sh.won_before = run;
+    }
+    __syncthreads();
+    weight = sh.weight;
+    return at;
+}
+
+// The bins of the first pass, kPer a thread: the first whose running sum
+// reaches `target`, the last one with a count if none does.
+template <typename W>
+__device__ int fine_border(Shared& sh, const uint32_t (&count)[kPer], const W (&weight)[kPer], W target) {
+    double own = 0.0, total;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) own += (double)weight[e];
+    double run = block_scan(sh, own, total) - own;
+    if (threadIdx.x == 0) sh.pick_bin = INT_MAX, sh.found = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        run += (double)weight[e];
+        if (count[e]) {
+            atomicMax(&sh.found, (int)threadIdx.x * kPer + e);
+            if (run >= (double)target) atomicMin(&sh.pick_bin, (int)threadIdx.x * kPer + e);
+        }
+    }
+    __syncthreads();
+    const int bin = sh.pick_bin != INT_MAX ? sh.pick_bin : sh.found;
+    __syncthreads();
+    return bin;
+}
+
+// Sorts x[0, n), n a power of two from 64, rising. Strides up to 32 stay within
+// the 64 values of a warp.
+__device__ void sort_list(unsigned long long* x, int n) {
+    for (int size = 2; size <= n; size <<= 1) {
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            for (int t = threadIdx.x; t < n / 2; t += kThreads) {
+                const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+                const unsigned long long a = x[i], b = x[j];
+                if ((a > b) == ((i & size) == 0)) x[i] = b, x[j] = a;
+            }
+            if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads();
+            else __syncwarp();
+        }
+    }
+    __syncthreads();
 }
 
 // The search over whole slices: for rows whose cut no list holds.
-__device__ void sample_wide(Row& r, const float* logits, float top, int top_index, int alive, float t, int k, float p,
-                            float mp, double u_in, int& id, float& logp) {
+__device__ void sample_wide(Row& r, const float* logits, float top, uint32_t k, float p, float mp, float t, double u,
+                            int& id, float& logp) {
     Shared& sh = r.sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Cut cut{1u, INT_MAX};  // no element has key 1: everything but the excluded
-    if (k > 0 && k < alive) cut = cut_top_k(r, top, (uint32_t)k);
-    if (p < 1.0f) cut = cut_top_p(r, top, (double)p, cut, 0.0, 0.0, nullptr);
+    if (k > 0) cut = cut_top_k(r, top, k);
+    if (p < 1.0f) cut = cut_top_p(r, top, (double)p, cut);
     const bool by_min = mp > 0.0f;
     const double least = (double)mp, log_least = by_min ? log(least) : 0.0;
     const double inv_t = 1.0 / (double)t;
@@ -561,7 +611,7 @@ __device__ void sample_wide(Row& r, const float* logits, float top, int top_inde
         all += r.of(&sh.part[r.turn], i)->a;
     }
     r.turn ^= 1;
-    const double target = u_in * all;
+    const double target = u * all;
     // The first element whose running sum exceeds the target. The sums of
     // blocks, warps and elements are each taken in index order; where their
     // roundings disagree at a border (or u >= 1) the last element with a
@@ -572,11 +622,11 @@ __device__ void sample_wide(Row& r, const float* logits, float top, int top_inde
         const int lo = warp * r.seg, hi = min(lo + r.seg, r.n);
         const bool here = from + w > target;  // uniform in the warp
         // surely before the border, or surely behind it (an earlier warp finds it)
-        const bool skip = (!here && u_in < 1.0 && from + w < target * (1.0 - 1e-9)) || from > target * (1.0 + 1e-9);
+        const bool skip = (!here && u < 1.0 && from + w < target * (1.0 - 1e-9)) || from > target * (1.0 + 1e-9);
         double run = from;
         if (!skip)
             for (int i = lo; i < hi; i += 32) {
-                const double wi = i + lane < hi ? weight(r.x[i + lane], r.at(i + lane)) : 0.0;
+                const double wi = i + lane < hi ? weight(r.x[i + lane], r.base + i + lane) : 0.0;
                 double incl = wi;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -584,8 +634,8 @@ __device__ void sample_wide(Row& r, const float* logits, float top, int top_inde
                     if (lane >= o) incl += up;
                 }
                 if (wi > 0.0) {
-                    last = max(last, (uint32_t)r.at(i + lane) + 1u);
-                    if (run + incl > target) found = min(found, (uint32_t)r.at(i + lane));
+                    last = max(last, (uint32_t)(r.base + i + lane) + 1u);
+                    if (run + incl > target) found = min(found, (uint32_t)(r.base + i + lane));
                 }
                 run += __shfl_sync(0xFFFFFFFFu, incl, 31);
                 if (__any_sync(0xFFFFFFFFu, found != 0xFFFFFFFFu)) break;
@@ -597,10 +647,107 @@ __device__ void sample_wide(Row& r, const float* logits, float top, int top_inde
     logp = (float)((d == 0.0 ? 0.0 : d * inv_t) - log(all));
 }
 
+// The first element, in index order, of [lo, hi) of the block's slice whose
+// running sum of weights exceeds `target`: the warps sum a part each, then the
+// block looks at the one part that holds it.
+template <typename W>
+__device__ int locate(Row& r, int lo, int hi, double target, double& weight_out, W weight) {
+    Shared& sh = r.sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    while (hi - lo > 2 * kThreads) {
+        const int part = ((hi - lo + kThreads - 1) / kThreads) * 32;
+        const int from = min(lo + warp * part, hi), to = min(from + part, hi);
+        double w = 0.0;
+        for (int i = from + lane; i < to; i += 32) w += weight(r.x[i], r.base + i);
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+        __syncthreads();
+        if (lane == 0) sh.wsum[1][warp] = w;
+        __syncthreads();
+        double run = 0.0, before = 0.0;
+        int at = -1;  // the first part past the target, else the last with a weight
+        for (int k = 0; k < kWarps; ++k) {
+            const double wk = sh.wsum[1][k];
+            if (wk > 0.0) at = k, before = run;
+            run += wk;
+            if (wk > 0.0 && run > target) break;
+        }
+        __syncthreads();
+        if (at < 0) return -1;
+        const int end = hi;
+        lo = min(lo + at * part, end), hi = min(lo + part, end);
+        target -= before;
+    }
+    double w[2], total;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = lo + (int)threadIdx.x * 2 + e;
+        w[e] = i < hi ? weight(r.x[i], r.base + i) : 0.0;
+    }
+    const int at = pick<2>(sh, w, -1.0, target, total, weight_out);
+    return at < 0 ? -1 : r.base + lo + at;
+}
+
+// The list's order and cut. On entry list / list_index hold `listed` tokens in
+// index order; on return out[i] is token i's weight in the draw (0 where it is
+// not kept). above: mass of larger tokens outside the list, all: mass that p
+// refers to (0: the first k of the list), both relative to `ref` as `mass`
+// gives it. False where the border of p lies outside a list that has tokens above it.
+template <typename M, typename D>
+__device__ bool settle_list(Shared& sh, const float* list, unsigned long long* order, double* out, int listed, int k,
+                            float p, double above, double all, bool sure, M mass, D draw) {
+    int n = 64;
+    while (n < listed) n <<= 1;
+    for (int i = threadIdx.x; i < n; i += kThreads)
+        order[i] = i < listed ? (unsigned long long)~key_of(list[i]) << 32 | (unsigned)i : ~0ull;
+    __syncthreads();
+    sort_list(order, n);
+    constexpr int PER = kList / kThreads;
+    const int per = n > kThreads ? n / kThreads : 1;
+    unsigned long long mine[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int r = threadIdx.x * per + e;
+        mine[e] = e < per && r < n ? order[r] : ~0ull;
+    }
+    int kept = k > 0 && k < listed ? k : listed;
+    bool holds = true;
+    if (p < 1.0f) {
+        double m[PER], own = 0.0, total;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int r = threadIdx.x * per + e;
+            m[e] = e < per && r < kept ? mass(logit_of(~(uint32_t)(mine[e] >> 32))) : 0.0;
+            own += m[e];
+        }
+        double run = above + (block_scan(sh, own, total) - own);
+        const double target = (double)p * (all > 0.0 ? all : total);
+        if (sure) holds = target > above && target <= above + total;
+        if (threadIdx.x == 0) sh.found = 1;  // the first token always stays
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int r = threadIdx.x * per + e;
+            if (e < per && r < kept && run < target) atomicMax(&sh.found, r + 1);
+            run += m[e];
+        }
+        __syncthreads();
+        kept = sh.found;
+    }
+    __syncthreads();  // every thread holds its part of the order; its place takes the weights
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int r = threadIdx.x * per + e;
+        if (e < per && r < n && mine[e] != ~0ull)
+            out[(uint32_t)mine[e]] = r < kept ? draw(logit_of(~(uint32_t)(mine[e] >> 32))) : 0.0;
+    }
+    __syncthreads();
+    return holds;
+}
+
 template <bool PACKS>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t dynamic[];
-    float* pool = reinterpret_cast<float*>(dynamic);             // values, then indices
+    float* pool = reinterpret_cast<float*>(dynamic);  // this block's tokens for the list: values, then indices
     int* pool_index = reinterpret_cast<int*>(pool + kList);
     float* list = pool + 2 * kList;
     int* list_index = reinterpret_cast<int*>(pool + 3 * kList);
@@ -612,65 +759,104 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const float* logits = a.logits + row * a.stride;
     const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
     const int seg = ((n + kWarps * 128 - 1) / (kWarps * 128)) * 128;
-    Row r{a, sh, a.resident ? held : logits + base, nullptr, base, n, seg, rank, ranks, 0, 0, cluster};
+    Row r{a, sh, a.resident ? held : logits + base, base, n, seg, rank, ranks, 0, 0, cluster};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int lo = warp * seg, hi = min(lo + seg, n);
+    const int lo = min(warp * seg, n), hi = min(lo + seg, n);
 
     const float t = a.temperature ? a.temperature[row] : 1.0f;
     int k = a.top_k ? a.top_k[row] : 0;
-    if (k >= a.vocab) k = 0;
+    if (k < 0 || k >= a.vocab) k = 0;
     float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f;
     if (!(p < 1.0f)) p = 1.0f;
     if (!(mp > 0.0f)) mp = 0.0f;
     double u = a.uniform[row];
     u = u > 0.0 ? u : 0.0;
+    // rows that take the largest logit; at a positive temperature it has all the weight
     const bool greedy = !(t > 0.0f) || p <= 0.0f || mp > 1.0f || k == 1;
     const double inv_t = 1.0 / (double)t;
-    const bool sums_all = !greedy && k <= 0 && (p < 1.0f || mp == 0.0f);  // the first pass sums every weight
+    const bool sums_all = !greedy && k == 0 && (p < 1.0f || mp == 0.0f);  // the first pass sums every weight,
     const bool draws_all = sums_all && p >= 1.0f;                         // at the draw's temperature
 
     // Where the histogram lies and what the sums refer to: the largest of a
     // sample of the row, the same for all its blocks.
-    for (int i = threadIdx.x; i < kExpTable; i += kThreads) sh.exp2_table[i] = exp2((double)i / kExpTable);
+    for (int i = threadIdx.x; i < kExpTable * 32; i += kThreads) {
+        if (lane == 0) sh.exp2_table[i / 32][0] = exp2((double)(i / 32) / kExpTable);
+        __syncwarp();
+        if (lane != 0) sh.exp2_table[i / 32][lane] = sh.exp2_table[i / 32][0];
+    }
     if (threadIdx.x == 0) sh.pool_used = 0;
-    sh.hist[0][threadIdx.x] = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sh.fine[threadIdx.x * kPer + e] = 0;
     float center = logits[(int64_t)threadIdx.x * a.vocab / kThreads];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) center = fmaxf(center, __shfl_xor_sync(0xFFFFFFFFu, center, o));
     if (lane == 0) sh.wlo[warp] = __float_as_uint(center);
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) center = fmaxf(center, __uint_as_float(sh.wlo[w]));
-    if (!(fabsf(center) < 1e30f)) center = 0.0f;  // a masked or infinite sample
-    const float high = center + 8.0f;
+    if (!(fabsf(center) < 1e4f)) center = 0.0f;  // a masked sample, or values too large for the bins
+    const Fine bin_of{(center + 4.0f) * kFinePerNat + 8388608.0f};
     const double ref = (double)center;
+    const Exp mass(sh.exp2_table, 1.0, -ref);                  // relative to the sample's maximum
+    const Exp draw(sh.exp2_table, inv_t, -ref * inv_t);
+    // what lies so far below it that its exponential is zero at either temperature
+    auto lowest = [](double x) { return x > -3e38 ? (float)x : -INFINITY; };
+    const float mass_floor = (float)(ref - 600.0), draw_floor = lowest(ref - 600.0 * (double)t);
 
     // first pass
     {
         double sum = 0.0;
         float best = -INFINITY;
-        int index = INT_MAX, alive = 0;
-        const double f = draws_all ? inv_t : 1.0;
-        for (int i = lo; i < hi; i += 128) {
-            float v[4];
-            load4<PACKS>(logits + base, i, hi, v);
-            if (a.resident) {
-                if (PACKS) {
-                    if (element<true>(i, 0) < hi)
-                        *reinterpret_cast<float4*>(held + element<true>(i, 0)) = make_float4(v[0], v[1], v[2], v[3]);
-                } else {
+        int index = INT_MAX;
+        constexpr int STEPS = PACKS ? 4 : 2;  // loads in flight
+        const float floor_of = draws_all ? draw_floor : mass_floor;
+        const Exp f(sh.exp2_table, draws_all ? inv_t : 1.0, draws_all ? -ref * inv_t : -ref);
+        for (int i = lo; i < hi; i += 128 * STEPS) {
+            float v[STEPS][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (element<false>(i, e) < hi) held[element<false>(i, e)] = v[e];
+            for (int q = 0; q < STEPS; ++q) load4<PACKS>(logits + base, i + 128 * q, hi, v[q]);
+            if (a.resident) {
+#pragma unroll
+                for (int q = 0; q < STEPS; ++q) {
+                    if (PACKS) {
+                        const int at = element<true>(i + 128 * q, 0);
+                        if (at < hi)
+                            *reinterpret_cast<float4*>(held + at) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int at = element<false>(i + 128 * q, e);
+                            if (at < hi) held[at] = v[q][e];
+                        }
+                    }
                 }
             }
+            if (greedy) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!(v[e] > -INFINITY)) continue;
-                ++alive;
-                if (v[e] > best) best = v[e], index = base + element<PACKS>(i, e);
-                if (greedy) continue;
-                if (!draws_all) atomicAdd(&sh.hist[0][value_bin(v[e], high)], 1u);
-                if (sums_all) sum += exp_table(((double)v[e] - ref) * f, sh.exp2_table);
+                for (int q = 0; q < STEPS; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (v[q][e] > best) best = v[q][e], index = base + element<PACKS>(i + 128 * q, e);
+                continue;
+            }
+#pragma unroll
+            for (int q = 0; q < STEPS; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best = fmaxf(best, v[q][e]);  // a NaN is passed over
+            if (!draws_all) {
+#pragma unroll
+                for (int q = 0; q < STEPS; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (v[q][e] > -INFINITY) atomicAdd(&sh.fine[bin_of(v[q][e])], 1u);
+            }
+            if (sums_all) {
+#pragma unroll
+                for (int q = 0; q < STEPS; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const double w = f(v[q][e]);
+                        if (v[q][e] > floor_of) sum += w;
+                    }
             }
         }
 #pragma unroll
@@ -679,109 +865,146 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             const int i2 = __shfl_xor_sync(0xFFFFFFFFu, index, o);
             if (b2 > best || (b2 == best && i2 < index)) best = b2, index = i2;
             sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            alive += __shfl_xor_sync(0xFFFFFFFFu, alive, o);
         }
         if (lane == 0) {
-            sh.wsum[0][warp] = sum, sh.wn[warp] = alive;
+            sh.wsum[0][warp] = sum;
             sh.wlo[warp] = __float_as_uint(best), sh.whi[warp] = (uint32_t)index;
             sh.seg[warp] = draws_all ? sum : 0.0;
         }
         __syncthreads();
         if (threadIdx.x == 0) {
-            First m{0.0, -INFINITY, INT_MAX, 0};
+            First m{0.0, -INFINITY, INT_MAX};
             for (int w = 0; w < kWarps; ++w) {
                 const float b2 = __uint_as_float(sh.wlo[w]);
                 const int i2 = (int)sh.whi[w];
                 if (b2 > m.best || (b2 == m.best && i2 < m.index)) m.best = b2, m.index = i2;
-                m.sum += sh.wsum[0][w], m.alive += sh.wn[w];
+                m.sum += sh.wsum[0][w];
             }
             sh.first = m;
         }
     }
     r.sync();
-    First m{0.0, -INFINITY, INT_MAX, 0};
-    uint32_t count = 0;
+    First m{0.0, -INFINITY, INT_MAX};
     for (int i = 0; i < ranks; ++i) {
         const First q = *r.of(&sh.first, i);
         if (q.best > m.best) m.best = q.best, m.index = q.index;  // ranks hold rising indices
-        m.sum += q.sum, m.alive += q.alive;
-        count += r.of(sh.hist[0], i)[threadIdx.x];
+        m.sum += q.sum;
     }
-    r.hturn = 1;
     const float top = m.best;
-
-    int id = -1;
-    float logp = -INFINITY;
-    bool done = true, wide = false;
-    if (m.alive > 0 && greedy) {
-        id = m.index;
-        // the one kept token; at a positive temperature it has all the weight
-        logp = 0.0f;
-    } else if (m.alive > 0) {
-        done = false;
+    if (!(top > -INFINITY) || greedy) {
+        if (rank == 0 && threadIdx.x == 0) {
+            a.ids[row] = top > -INFINITY ? m.index : -1;
+            if (a.logprobs) a.logprobs[row] = top > -INFINITY ? 0.0f : -INFINITY;
+        }
+        if (ranks > 1) cluster.sync();  // no block leaves while another may read its shared memory
+        return;
     }
 
     // Which bins the list takes ([first, last]); bins before it are kept for sure.
     int first = 0, last = -1;
-    bool sure = false, by_k = false;
-    if (!done) {
-        by_k = k > 0 && k < m.alive;
-        // a range that the sample misjudged, or infinite logits
-        if (sums_all && !(m.sum > 1e-250 && m.sum < 1e250 && top < 1e30f)) wide = true;
-        if (wide || draws_all) {
-        } else if (k > 0 || mp > 0.0f) {
+    const bool sure = sums_all && p < 1.0f && mp == 0.0f;
+    // a range that the sample misjudged, or infinite logits
+    bool wide = sums_all && !(m.sum > 1e-250 && m.sum < 1e250 && top < center + 500.0f * fminf(t, 1.0f));
+    if (!draws_all && !wide) {
+        uint32_t count[kPer] = {};
+        for (int i = 0; i < ranks; ++i) {
+            const uint4 c = *reinterpret_cast<const uint4*>(r.of(sh.fine, i) + threadIdx.x * kPer);
+            count[0] += c.x, count[1] += c.y, count[2] += c.z, count[3] += c.w;
+        }
+        if (!sure) {
             // top-p behind top-k needs the mass of all k; otherwise nothing below min-p's bin matters
-            const int by_min = mp > 0.0f && !(k > 0 && p < 1.0f)
-                                   ? value_bin(__double2float_rd((double)top + log((double)mp) - 1e-4), high)
-                                   : kBins - 1;
-            last = by_min;
-            if (by_k) {
-                uint32_t before;
-                last = r.border<uint32_t>(count, count, (uint32_t)k, before);
-                if (last > by_min) last = by_min, by_k = false;  // what min-p keeps is less than k
+            last = mp > 0.0f && !(k > 0 && p < 1.0f)
+                       ? bin_of(__double2float_rd((double)top + log((double)mp) - 1e-4))
+                       : kFine - 1;
+            if (k > 0) {
+                const int by_k = fine_border<uint32_t>(sh, count, count, (uint32_t)k);
+                if (by_k > last) k = 0;  // what min-p keeps is less than k
+                else last = by_k;
             }
         } else {
-            // the bins around the estimated border, far enough that the estimate's error cannot matter
-            const double guess = (double)count * exp(-((double)threadIdx.x + 0.5) / (double)kBinsPerNat);
-            double before, mass = guess;
+            // The bins around the border. A bin's tokens are estimated at its
+            // middle, each off by 1/256 of its mass at most and by independent
+            // amounts: six spreads of their sum (a spread of 1/443 each), and
+            // 1e-4 for bins on a slope. The first bin takes what the sum has
+            // beyond the others. Where that is not enough, the list does not
+            // hold the border and the wide search settles the row.
+            double guess[kPer], own = 0.0, squares = 0.0, others, spread;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xFFFFFFFFu, mass, o);
-            __syncthreads();
-            if (lane == 0) sh.wsum[1][warp] = mass;
-            __syncthreads();
-            mass = 0.0;
-            for (int w = 0; w < kWarps; ++w) mass += sh.wsum[1][w];
-            first = r.border<double>(count, guess, (double)p * mass * (1.0 - 1e-3), before);
-            last = r.border<double>(count, guess, (double)p * mass * (1.0 + 1e-3), before);
-            sure = true;
+            for (int e = 0; e < kPer; ++e) {
+                const int b = threadIdx.x * kPer + e;
+                const double one = exp(((double)bin_of.high - 8388608.0 - (double)b) / kFinePerNat - ref);
+                guess[e] = b ? (double)count[e] * one : 0.0;
+                own += guess[e], squares += guess[e] * one;
+            }
+            block_scan(sh, own, others);
+            block_scan(sh, squares, spread);
+            if (threadIdx.x == 0) guess[0] = fmax(m.sum - others, 0.0);
+            const double border = (double)p * m.sum;
+            const double off = fmin(m.sum / 250.0, 6.0 / 443.0 * sqrt(spread) + 1e-4 * m.sum);
+            first = fine_border<double>(sh, count, guess, border - off);
+            last = fine_border<double>(sh, count, guess, border + off);
         }
     }
-    auto sure_weight = [&](float v) { return exp_table(((double)v - ref) * inv_t, sh.exp2_table); };
 
     // second pass: the list's tokens, and the sums of what lies above them
-    if (!done && !wide && !draws_all) {
-        double above = 0.0, weights = 0.0;
-        int mine = 0;
+    int listed = 0;
+    double above = 0.0;
+    if (!draws_all && !wide) {
+        double sum = 0.0, weights = 0.0;
+        int mine = 0, waiting = 0;
+        float* dense = sh.dense[warp];
+        auto flush = [&](int c) {  // the first c of the waiting values
+            if (lane < c) {
+                const float v = dense[lane];
+                if (v > mass_floor) sum += mass(v);
+                if (v > draw_floor) weights += draw(v);
+            }
+        };
+#pragma unroll 2
         for (int i = lo; i < hi; i += 128) {
             float v[4];
             load4<PACKS>(r.x, i, hi, v);
-            int take = 0, bits = 0;
+            int take = 0, over = 0;  // bits: tokens of the list, tokens above it
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (!(v[e] > -INFINITY)) continue;
-                const int b = value_bin(v[e], high);
-                if (b > last) continue;
-                if (b >= first) {
-                    bits |= 1 << e, ++take;
-                } else {
-                    above += exp_table((double)v[e] - ref, sh.exp2_table);
-                    weights += sure_weight(v[e]);
+                const int b = bin_of(v[e]);
+                const bool in = v[e] > -INFINITY && b <= last;
+                take |= (in && b >= first) << e;
+                over |= (in && b < first) << e;
+            }
+            if (sure && __any_sync(0xFFFFFFFFu, over)) {
+                int incl = __popc(over);
+                const int c = incl;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                    if (lane >= o) incl += up;
+                }
+                int at = waiting + incl - c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (over >> e & 1) dense[at++] = v[e];
+                waiting += __shfl_sync(0xFFFFFFFFu, incl, 31);
+                __syncwarp();
+                if (waiting >= 32) {
+                    int from = 0;
+                    for (; from + 32 <= waiting; from += 32) {
+                        const float w = dense[from + lane];
+                        if (w > mass_floor) sum += mass(w);
+                        if (w > draw_floor) weights += draw(w);
+                    }
+                    waiting -= from;
+                    const float rest = lane < waiting ? dense[from + lane] : 0.0f;
+                    __syncwarp();
+                    if (lane < waiting) dense[lane] = rest;
+                    __syncwarp();
                 }
             }
             if (!__any_sync(0xFFFFFFFFu, take)) continue;
             int pos[4], all = 0;  // places of this step's tokens, in index order
             if (PACKS) {
-                int incl = take;
+                const int c = __popc(take);
+                int incl = c;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
@@ -789,11 +1012,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 }
                 all = __shfl_sync(0xFFFFFFFFu, incl, 31);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pos[e] = incl - take + __popc(bits & ((1 << e) - 1));
+                for (int e = 0; e < 4; ++e) pos[e] = incl - c + __popc(take & ((1 << e) - 1));
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const unsigned votes = __ballot_sync(0xFFFFFFFFu, bits >> e & 1);
+                    const unsigned votes = __ballot_sync(0xFFFFFFFFu, take >> e & 1);
                     pos[e] = all + __popc(votes & ((1u << lane) - 1u));
                     all += __popc(votes);
                 }
@@ -807,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int slot = mine + pos[e];
-                if ((bits >> e & 1) && slot < kList) {
+                if ((take >> e & 1) && slot < kList) {
                     const int to = sh.chain[warp][slot / 32] * 32 + slot % 32;
                     pool[to] = v[e];
                     pool_index[to] = base + element<PACKS>(i, e);
@@ -815,216 +1038,163 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             }
             mine += all;
         }
+        flush(waiting);
+#pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
+            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             weights += __shfl_xor_sync(0xFFFFFFFFu, weights, o);
         }
-        if (lane == 0) sh.listed[warp] = mine, sh.seg[warp] = weights, sh.wsum[0][warp] = above;
+        if (lane == 0) sh.listed[warp] = mine, sh.seg[warp] = weights, sh.wsum[1][warp] = sum;
         __syncthreads();
         if (threadIdx.x == 0) {
             double s = 0.0;
             int c = sh.pool_used > kList / 32 ? kList + 1 : 0;  // more than the pool holds
-            for (int w = 0; w < kWarps; ++w) s += sh.wsum[0][w], c += sh.listed[w];
+            for (int w = 0; w < kWarps; ++w) s += sh.wsum[1][w], c += sh.listed[w];
             sh.above = s, sh.block_listed = c;
         }
         r.sync();
-    }
-    // every block: does the list hold?
-    int listed = 0;
-    double above = 0.0;
-    if (!done && !wide && !draws_all) {
         for (int i = 0; i < ranks; ++i) {
             listed += *r.of(&sh.block_listed, i);
             above += *r.of(&sh.above, i);
         }
-        if (listed > kList) wide = true;
+        if (listed > kList) wide = true;  // every block sees the same sum
     }
 
-    // the first block settles the cut and finds the draw's segment
-    Cut cut{1u, INT_MAX};
-    if (!done && !wide && rank == 0) {
-        const int segs = ranks * kWarps;
-        if (threadIdx.x == 0) sh.won = -1, sh.id = -1;
-        bool fits = true;
-        if (!draws_all) {
-            if (warp == 0) {  // where each warp's tokens start in the list
-                int before = 0;
-                for (int g = 0; g < segs; g += 32) {
-                    int c = g + lane < segs ? r.of(sh.listed, (g + lane) / kWarps)[(g + lane) % kWarps] : 0, own_c = c;
+    // The first block settles the cut; the draw is one of the list's tokens,
+    // or lies in one warp's segment of the row.
+    if (!wide) {
+        double* weight_of = reinterpret_cast<double*>(pool);  // of the list's tokens: the pool has been read by then
+        if (rank == 0) {
+            const int segs = ranks * kWarps;
+            bool holds = true;
+            if (threadIdx.x == 0) sh.won = -1;
+            if (!draws_all) {
+                if (warp == 0) {  // where each warp's tokens start in the list
+                    int before = 0;
+                    for (int g = 0; g < segs; g += 32) {
+                        const int c = g + lane < segs ? r.of(sh.listed, (g + lane) / kWarps)[(g + lane) % kWarps] : 0;
+                        int incl = c;
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int up = __shfl_up_sync(0xFFFFFFFFu, c, o);
-                        if (lane >= o) c += up;
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                            if (lane >= o) incl += up;
+                        }
+                        if (g + lane < segs) sh.offset[g + lane] = before + incl - c;
+                        before += __shfl_sync(0xFFFFFFFFu, incl, 31);
                     }
-                    if (g + lane < segs) sh.offset[g + lane] = before + c - own_c;
-                    before += __shfl_sync(0xFFFFFFFFu, c, 31);
+                    if (lane == 0) sh.offset[segs] = before;
                 }
-                if (lane == 0) sh.offset[segs] = before;
-            }
-            __syncthreads();
-            for (int g = warp; g < segs; g += kWarps) {
-                const int q = g / kWarps, from = sh.offset[g], c = sh.offset[g + 1] - from;
-                const uint8_t* chain = r.of(&sh.chain[0][0], q) + (g % kWarps) * (kList / 32);
-                const float* pv = r.of(pool, q);
-                const int* pi = r.of(pool_index, q);
-                for (int i = lane; i < c; i += 32) {
-                    const int at = chain[i / 32] * 32 + i % 32;
-                    list[from + i] = pv[at];
-                    list_index[from + i] = pi[at];
+                __syncthreads();
+                for (int g = warp; g < segs; g += kWarps) {
+                    const int q = g / kWarps, from = sh.offset[g], c = sh.offset[g + 1] - from;
+                    const uint8_t* chain = r.of(&sh.chain[0][0], q) + (g % kWarps) * (kList / 32);
+                    const float* pv = r.of(pool, q);
+                    const int* pi = r.of(pool_index, q);
+                    for (int i = lane; i < c; i += 32) {
+                        const int at = chain[i / 32] * 32 + i % 32;
+                        list[from + i] = pv[at];
+                        list_index[from + i] = pi[at];
+                    }
                 }
-            }
-            __syncthreads();
-            Row l{a, sh, list, list_index, 0, listed, ((listed + kThreads - 1) / kThreads) * 32, 0, 1, r.turn, r.hturn, cluster};
-            if (by_k) cut = cut_top_k(l, top, (uint32_t)k);
-            if (p < 1.0f) {
-                if (sure) {
-                    const double scale = exp(ref - (double)top);
-                    cut = cut_top_p(l, top, (double)p, cut, above * scale, m.sum * scale, &fits);
-                } else if (k > 0) {
-                    cut = cut_top_p(l, top, (double)p, cut, 0.0, 0.0, nullptr);
-                } else {
-                    // the list ends at min-p's bin: top-p's border may lie behind it, and then cuts nothing here
-                    bool inside;
-                    cut = cut_top_p(l, top, (double)p, cut, 0.0, m.sum * exp(ref - (double)top), &inside);
-                }
-            }
-            r.turn = l.turn, r.hturn = l.hturn;
-        }
-        if (!fits) {
-            if (threadIdx.x == 0) sh.won = -2;
-        } else if (!sure && !draws_all) {
-            // the draw is among the list's tokens
-            const bool by_min = mp > 0.0f;
-            const double least = (double)mp, log_least = by_min ? log(least) : 0.0;
-            constexpr int PER = kList / kThreads;
-            double w[PER], own = 0.0;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                const int i = threadIdx.x * PER + e;
-                w[e] = 0.0;
-                if (i < listed) {
-                    const float v = list[i];
+                __syncthreads();
+                const double least = (double)mp, log_least = mp > 0.0f ? log(least) : 0.0;
+                auto kept_weight = [&](float v) -> double {
                     const double d = below(v, top);
-                    const bool small = by_min && (d < log_least - 1e-9 || (d < log_least + 1e-9 && exp(d) < least));
-                    if (cut.keeps(key_of(v), list_index[i]) && !small)
-                        w[e] = d == 0.0 ? 1.0 : d < -1e300 ? 0.0 : exp(d * inv_t);
-                }
-                own += w[e];
+                    // min-p's comparison of exponentials, decided by the logs unless they are close
+                    if (mp > 0.0f && (d < log_least - 1e-9 || (d < log_least + 1e-9 && exp(d) < least))) return 0.0;
+                    if (sure) return v > draw_floor ? draw(v) : 0.0;
+                    return d == 0.0 ? 1.0 : d < -1e300 ? 0.0 : exp(d * inv_t);
+                };
+                auto list_mass = [&](float v) -> double {
+                    if (sums_all) return v > mass_floor ? mass(v) : 0.0;
+                    return exp(below(v, top));
+                };
+                holds = settle_list(sh, list, reinterpret_cast<unsigned long long*>(pool), weight_of, listed, k, p,
+                                    above, sums_all ? m.sum : 0.0, sure, list_mass, kept_weight);
             }
-            double incl = own;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            __syncthreads();
-            if (lane == 31) sh.wsum[0][warp] = incl;
-            if (threadIdx.x == 0) sh.pick_bin = INT_MAX, sh.found = -1;
-            __syncthreads();
-            double before = 0.0, total = 0.0;
-            for (int i = 0; i < kWarps; ++i) {
-                if (i < warp) before += sh.wsum[0][i];
-                total += sh.wsum[0][i];
-            }
-            const double target = u * total;
-            double run = before + (incl - own);
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                run += w[e];
-                if (w[e] > 0.0) {
-                    atomicMax(&sh.found, threadIdx.x * PER + e);
-                    if (run > target) atomicMin(&sh.pick_bin, threadIdx.x * PER + e);
-                }
-            }
-            __syncthreads();
-            const int at = sh.pick_bin != INT_MAX ? sh.pick_bin : sh.found;
-            if (at / PER == (int)threadIdx.x) {
-                double mine = 0.0;
-#pragma unroll
-                for (int e = 0; e < PER; ++e)
-                    if (at % PER == e) mine = w[e];
-                sh.id = list_index[at], sh.weight = mine, sh.total = total;
-            }
-        } else {
-            // the segment that holds the draw: each one's sure weights and its kept tokens of the list
-            double w = 0.0;
-            const int g = threadIdx.x;
-            if (g < segs) {
-                w = r.of(sh.seg, g / kWarps)[g % kWarps];
-                if (!draws_all)
-                    for (int i = sh.offset[g]; i < sh.offset[g + 1]; ++i)
-                        if (cut.keeps(key_of(list[i]), list_index[i])) w += sure_weight(list[i]);
-            }
-            double incl = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            __syncthreads();
-            if (lane == 31) sh.wsum[0][warp] = incl;
-            if (threadIdx.x == 0) sh.pick_bin = INT_MAX, sh.found = -1;
-            __syncthreads();
-            double before = 0.0, total = 0.0;
-            for (int i = 0; i < kWarps; ++i) {
-                if (i < warp) before += sh.wsum[0][i];
-                total += sh.wsum[0][i];
-            }
-            const double target = u * total;
-            if (w > 0.0) {
-                atomicMax(&sh.found, g);
-                if (before + incl > target) atomicMin(&sh.pick_bin, g);
-            }
-            __syncthreads();
-            const int won = sh.pick_bin != INT_MAX ? sh.pick_bin : sh.found;
-            if (!(total > 1e-250 && total < 1e250)) {  // a temperature that takes the weights out of range
+            if (!holds) {
                 if (threadIdx.x == 0) sh.won = -2;
-            } else if (won == g) {
-                sh.won = won, sh.won_before = target - (before + (incl - w)), sh.total = total;
-                sh.part[0].lo = cut.key, sh.part[0].n = cut.index;
+            } else if (!sure && !draws_all) {
+                constexpr int PER = kList / kThreads;
+                const int per = (listed + kThreads - 1) / kThreads;
+                double w[PER], total, weight;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const int i = threadIdx.x * per + e;
+                    w[e] = e < per && i < listed ? weight_of[i] : 0.0;
+                }
+                // pick counts PER elements a thread; only the first `per` have a weight
+                const int at = pick<PER>(sh, w, u, 0.0, total, weight);
+                if (threadIdx.x == 0)
+                    sh.id = list_index[(at / PER) * per + at % PER], sh.weight = weight, sh.total = total;
+            } else {
+                // each segment's sure weights and its kept tokens of the list
+                double* sums = sh.segment;
+                for (int g = warp; g < segs; g += kWarps) {
+                    double w = 0.0;
+                    if (!draws_all)
+                        for (int i = sh.offset[g] + lane; i < sh.offset[g + 1]; i += 32) w += weight_of[i];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+                    if (lane == 0) sums[g] = w + r.of(sh.seg, g / kWarps)[g % kWarps];
+                }
+                __syncthreads();
+                double w[1] = {(int)threadIdx.x < segs ? sums[threadIdx.x] : 0.0}, total, weight;
+                const int won = pick<1>(sh, w, u, 0.0, total, weight);
+                if (threadIdx.x == 0) {
+                    // a temperature that takes the weights out of range
+                    sh.won = total > 1e-250 && total < 1e250 ? won : -2;
+                    sh.won_before = u * total - (sh.won_before - weight);  // the target within the segment
+                    sh.total = total;
+                }
             }
         }
-    }
-    if (!done && !wide) {
         r.sync();
         const int won = *r.of(&sh.won, 0);
         const double total = *r.of(&sh.total, 0);
-        if (won == -2) {
-            wide = true;
-        } else if (won < 0) {
-            id = *r.of(&sh.id, 0);
-            logp = (float)log(*r.of(&sh.weight, 0) / total);
-        } else {
-            const Part* q = r.of(&sh.part[0], 0);
-            const Cut c{q->lo, q->n};
+        if (won >= 0 && won / kWarps == rank) {
+            const int from = min((won % kWarps) * seg, n), to = min(from + seg, n);
             const double target = *r.of(&sh.won_before, 0);
-            if (won / kWarps == rank) {
-                const int from = (won % kWarps) * seg, to = min(from + seg, n);
-                double w;
-                const int got = locate(r, from, to, target, &w, [&](float v, int i) -> double {
-                    if (!(v > -INFINITY)) return 0.0;
-                    if (!draws_all) {
-                        const int b = value_bin(v, high);
-                        if (b > last || (b >= first && !c.keeps(key_of(v), i))) return 0.0;
-                    }
-                    return sure_weight(v);
-                });
-                if (threadIdx.x == 0) {
-                    a.ids[row] = got;
-                    if (a.logprobs) a.logprobs[row] = (float)log(w / total);
+            const double* all_weights = r.of(weight_of, 0);
+            const int* all_index = r.of(list_index, 0);
+            const int* offsets = r.of(sh.offset, 0);
+            const int l0 = draws_all ? 0 : offsets[won], l1 = draws_all ? 0 : offsets[won + 1];
+            double w;
+            const int got = locate(r, from, to, target, w, [&](float v, int i) -> double {
+                if (!(v > draw_floor)) return 0.0;
+                if (draws_all) return draw(v);
+                const int b = bin_of(v);
+                if (b > last) return 0.0;
+                if (b < first) return draw(v);
+                int lo_i = l0, hi_i = l1;  // a token of the list: its weight there
+                while (hi_i - lo_i > 1) {
+                    const int mid = (lo_i + hi_i) >> 1;
+                    if (all_index[mid] <= i) lo_i = mid;
+                    else hi_i = mid;
                 }
+                return all_weights[lo_i];
+            });
+            if (threadIdx.x == 0) {
+                a.ids[row] = got;
+                if (a.logprobs) a.logprobs[row] = (float)log(w / total);
             }
         }
-        if (won >= 0) {
-            if (ranks > 1) cluster.sync();  // no block leaves while another may read its shared memory
-            return;
+        if (won == -1 && rank == 0 && threadIdx.x == 0) {
+            a.ids[row] = sh.id;
+            if (a.logprobs) a.logprobs[row] = (float)log(sh.weight / sh.total);
         }
-        r.sync();  // the first block's words have been read
+        if (ranks > 1) cluster.sync();  // the first block's words have been read
+        if (won != -2) return;
     }
-    if (wide) {
-        r.turn = 0, r.hturn = 1;  // the same in every block
-        sample_wide(r, logits, top, m.index, m.alive, t, k, p, mp, u, id, logp);
+    int id;
+    float logp;
+    r.turn = 0, r.hturn = 0;  // the same in every block
+    if (k > 0) {  // against the tokens that can be taken
+        Part alive{0.0, 0.0, 0u, 0u, 0};
+        r.each([&](float v, int) { alive.n += v > -INFINITY; });
+        if (k >= r.reduce(alive).n) k = 0;
     }
+    sample_wide(r, logits, top, (uint32_t)k, p, mp, t, u, id, logp);
     if (rank == 0 && threadIdx.x == 0) {
         a.ids[row] = id;
         if (a.logprobs) a.logprobs[row] = logp;
