@@ -39,10 +39,11 @@ static_assert(kBins == 1 << kBinBits, "a key range is cut into kBins");
 constexpr float kBinsPerNat = 16.0f;  // its value histogram: 32 nats, the last bin takes the rest
 constexpr int kFine = 2048;           // of the first pass: kPer bins a thread,
 constexpr int kPer = kFine / kThreads;
-constexpr float kFinePerNat = 128.0f; // 16 nats from 4 above the sample's maximum
+constexpr float kFinePerNat = 64.0f;  // 32 nats
 constexpr int kMaxCluster = 8;
 constexpr int kList = 4096;           // tokens a list holds
 constexpr int kExpTable = 64;
+constexpr int kSub = 4;               // parts of a warp's segment whose weights are summed apart
 
 struct SampleArgs {
     const float* logits;
@@ -93,20 +94,20 @@ struct First {
 struct Shared {
     First first;                   // exchanged
     double above;                  // exchanged: mass above the list
-    double seg[kWarps];            // exchanged: weights of each warp's tokens above the list
-    int listed[kWarps];            // exchanged: tokens each warp put into the list
+    double seg[kWarps * kSub];     // exchanged: weights of the tokens above the list, by part of the slice
+    int listed[kWarps];            // exchanged: tokens each warp put into the list,
+    int listed_part[kWarps * kSub];  // and how many of them by the end of each part
     int block_listed;              // exchanged: their sum
     uint8_t chain[kWarps][kList / 32];  // the pool's groups of 32 that hold them, in order
     int pool_used;
     int offset[kMaxCluster * kWarps + 1];  // of each warp's tokens in the list of the whole row
+    int part_end[kMaxCluster * kWarps * kSub];  // and the list's length by the end of each part
     double exp2_table[kExpTable][32];  // a copy a lane: no two lanes meet in a bank
-    float dense[kWarps][32 + 128];     // values waiting for their exponentials, 32 at a time
-    alignas(16) uint32_t fine[kFine];              // exchanged: the first pass's histogram
-    double segment[kMaxCluster * kWarps];
+    alignas(16) uint32_t fine[kFine + 32];              // exchanged: the first pass's histogram
+    double segment[kMaxCluster * kWarps * kSub];
     int won, id;                   // the draw: its segment (-1: id is the token)
     double won_before, total, weight;
     Part part[2];                  // exchanged, alternating
-    uint32_t hist[2][kBins];       // exchanged, alternating
     double wsum[2][kWarps];
     uint32_t wlo[kWarps], whi[kWarps];
     int wn[kWarps];
@@ -187,7 +188,7 @@ struct Row {
     // The cluster's count of this thread's bin. `fill` adds to the block's histogram.
     template <typename F>
     __device__ uint32_t histogram(F fill) {
-        uint32_t* h = sh.hist[hturn];
+        uint32_t* h = sh.fine + hturn * kBins;  // the first pass is done with its own
         h[threadIdx.x] = 0;
         __syncthreads();
         fill(h);
@@ -444,19 +445,27 @@ struct Exp {
     }
 };
 
-// The value histogram of the first pass. One fused operation and two bounds,
-// all monotone: a larger value is never in a later bin.
+// The value histogram of the first pass: bin round(high - v * kFinePerNat), by
+// one fused operation whose last bits are the bin, and bounds, all monotone: a
+// larger value is never in a later bin. What lies below the last bin has none.
 struct Fine {
-    float high;  // (what falls into bin 0) * kFinePerNat + 2^23: the sum's last bits are the bin
-    __device__ __forceinline__ int operator()(float v) const {
-        const float b = fminf(fmaxf(fmaf(v, -kFinePerNat, high), 8388608.0f), 8388608.0f + (kFine - 1));
-        return (int)(__float_as_uint(b) & (kFine - 1));
+    float high;  // what falls into bin 0, times kFinePerNat, plus 2^23
+    __device__ __forceinline__ unsigned raw(float v) const {
+        return __float_as_uint(fmaxf(fmaf(v, -kFinePerNat, high), 8388608.0f)) - 0x4B000000u;
+    }
+    __device__ __forceinline__ int operator()(float v) const { return (int)min(raw(v), (unsigned)kFine); }
+    // The smallest value that falls into bin `b` or an earlier one.
+    __device__ float start(int b) const {
+        float v = (high - 8388608.0f - (float)b - 0.5f) / kFinePerNat;
+        for (int i = 0; i < 64 && (*this)(v) > b; ++i) v = nextafterf(v, INFINITY);
+        for (int i = 0; i < 64 && (*this)(nextafterf(v, -INFINITY)) <= b; ++i) v = nextafterf(v, -INFINITY);
+        return v;
     }
 };
 
 constexpr int kListBytes = kList * 16;     // the pool of this block's tokens, and the row's list
-constexpr int64_t kMaxSlice = 116 * 1024;  // bytes of a slice that is kept in shared memory,
-constexpr int64_t kPairSlice = 5 * 1024;    // and that leave room for two blocks a multiprocessor
+constexpr int64_t kMaxSlice = 124 * 1024;  // bytes of a slice that is kept in shared memory,
+constexpr int64_t kPairSlice = 13 * 1024;  // and that leave room for two blocks a multiprocessor
 
 // Four elements of a lane: neighbours where the row is 16-byte packs, 32 apart otherwise.
 template <bool PACKS>
@@ -533,25 +542,22 @@ __device__ int pick(Shared& sh, const double (&w)[PER], double u, double offset,
 }
 
 // The bins of the first pass, kPer a thread: the first whose running sum
-// reaches `target`, the last one with a count if none does.
+// reaches `target`; kFine, for what has no bin, if none does.
 template <typename W>
-__device__ int fine_border(Shared& sh, const uint32_t (&count)[kPer], const W (&weight)[kPer], W target) {
+__device__ int fine_border(Shared& sh, const W (&weight)[kPer], W target) {
     double own = 0.0, total;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) own += (double)weight[e];
     double run = block_scan(sh, own, total) - own;
-    if (threadIdx.x == 0) sh.pick_bin = INT_MAX, sh.found = 0;
+    if (threadIdx.x == 0) sh.pick_bin = kFine;
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         run += (double)weight[e];
-        if (count[e]) {
-            atomicMax(&sh.found, (int)threadIdx.x * kPer + e);
-            if (run >= (double)target) atomicMin(&sh.pick_bin, (int)threadIdx.x * kPer + e);
-        }
+        if (weight[e] > 0 && run >= (double)target) atomicMin(&sh.pick_bin, (int)threadIdx.x * kPer + e);
     }
     __syncthreads();
-    const int bin = sh.pick_bin != INT_MAX ? sh.pick_bin : sh.found;
+    const int bin = sh.pick_bin;
     __syncthreads();
     return bin;
 }
@@ -687,12 +693,13 @@ __device__ int locate(Row& r, int lo, int hi, double target, double& weight_out,
     return at < 0 ? -1 : r.base + lo + at;
 }
 
-// The list's order and cut. On entry list / list_index hold `listed` tokens in
-// index order; on return out[i] is token i's weight in the draw (0 where it is
-// not kept). above: mass of larger tokens outside the list, all: mass that p
-// refers to (0: the first k of the list), both relative to `ref` as `mass`
-// gives it. False where the border of p lies outside a list that has tokens above it.
-template <typename M, typename D>
+// The list's order and cut. On entry list holds `listed` tokens in index order;
+// on return out[i] is token i's weight in the draw (0 where it is not kept).
+// above: mass of larger tokens outside the list; all: mass that p refers to
+// (0: that of the first k). False where the border of p lies outside a list
+// that has tokens above it. A thread holds PER neighbours of the order (one
+// for the usual short list, to keep the code that a row runs through short).
+template <int PER, typename M, typename D>
 __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* order, double* out, int listed, int k,
                             float p, double above, double all, bool sure, M mass, D draw) {
     int n = 64;
@@ -701,13 +708,11 @@ __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* o
         order[i] = i < listed ? (unsigned long long)~key_of(list[i]) << 32 | (unsigned)i : ~0ull;
     __syncthreads();
     sort_list(order, n);
-    constexpr int PER = kList / kThreads;
-    const int per = n > kThreads ? n / kThreads : 1;
     unsigned long long mine[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int r = threadIdx.x * per + e;
-        mine[e] = e < per && r < n ? order[r] : ~0ull;
+        const int r = threadIdx.x * PER + e;
+        mine[e] = r < listed ? order[r] : ~0ull;
     }
     int kept = k > 0 && k < listed ? k : listed;
     bool holds = true;
@@ -715,8 +720,7 @@ __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* o
         double m[PER], own = 0.0, total;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const int r = threadIdx.x * per + e;
-            m[e] = e < per && r < kept ? mass(logit_of(~(uint32_t)(mine[e] >> 32))) : 0.0;
+            m[e] = (int)threadIdx.x * PER + e < kept ? mass(logit_of(~(uint32_t)(mine[e] >> 32))) : 0.0;
             own += m[e];
         }
         double run = above + (block_scan(sh, own, total) - own);
@@ -726,8 +730,8 @@ __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* o
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const int r = threadIdx.x * per + e;
-            if (e < per && r < kept && run < target) atomicMax(&sh.found, r + 1);
+            const int r = threadIdx.x * PER + e;
+            if (r < kept && run < target) atomicMax(&sh.found, r + 1);
             run += m[e];
         }
         __syncthreads();
@@ -736,9 +740,8 @@ __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* o
     __syncthreads();  // every thread holds its part of the order; its place takes the weights
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int r = threadIdx.x * per + e;
-        if (e < per && r < n && mine[e] != ~0ull)
-            out[(uint32_t)mine[e]] = r < kept ? draw(logit_of(~(uint32_t)(mine[e] >> 32))) : 0.0;
+        const int r = threadIdx.x * PER + e;
+        if (r < listed) out[(uint32_t)mine[e]] = r < kept ? draw(logit_of(~(uint32_t)(mine[e] >> 32))) : 0.0;
     }
     __syncthreads();
     return holds;
@@ -758,10 +761,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const int64_t row = blockIdx.x / ranks;
     const float* logits = a.logits + row * a.stride;
     const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
-    const int seg = ((n + kWarps * 128 - 1) / (kWarps * 128)) * 128;
+    const int seg = ((n + kWarps * 256 - 1) / (kWarps * 256)) * 256;
     Row r{a, sh, a.resident ? held : logits + base, base, n, seg, rank, ranks, 0, 0, cluster};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int lo = min(warp * seg, n), hi = min(lo + seg, n);
+    const int part = ((seg / 256 + kSub - 1) / kSub) * 256;  // elements of a part of the segment
 
     const float t = a.temperature ? a.temperature[row] : 1.0f;
     int k = a.top_k ? a.top_k[row] : 0;
@@ -779,22 +783,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
     // Where the histogram lies and what the sums refer to: the largest of a
     // sample of the row, the same for all its blocks.
-    for (int i = threadIdx.x; i < kExpTable * 32; i += kThreads) {
-        if (lane == 0) sh.exp2_table[i / 32][0] = exp2((double)(i / 32) / kExpTable);
-        __syncwarp();
-        if (lane != 0) sh.exp2_table[i / 32][lane] = sh.exp2_table[i / 32][0];
-    }
+    const bool exps = !greedy && (sums_all || p < 1.0f);
+    if (exps && threadIdx.x < kExpTable) sh.segment[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
     if (threadIdx.x == 0) sh.pool_used = 0;
+    if (threadIdx.x < kWarps * kSub) sh.seg[threadIdx.x] = 0.0, sh.listed_part[threadIdx.x] = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sh.fine[threadIdx.x * kPer + e] = 0;
-    float center = logits[(int64_t)threadIdx.x * a.vocab / kThreads];
+    float center = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // 32 neighbours from each of 32 places
+        const int64_t at = (int64_t)(warp * 2 + e) * a.vocab / (2 * kWarps) + lane;
+        if (at < a.vocab) center = fmaxf(center, logits[at]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) center = fmaxf(center, __shfl_xor_sync(0xFFFFFFFFu, center, o));
     if (lane == 0) sh.wlo[warp] = __float_as_uint(center);
     __syncthreads();
-    for (int w = 0; w < kWarps; ++w) center = fmaxf(center, __uint_as_float(sh.wlo[w]));
-    if (!(fabsf(center) < 1e4f)) center = 0.0f;  // a masked sample, or values too large for the bins
-    const Fine bin_of{(center + 4.0f) * kFinePerNat + 8388608.0f};
+    if (exps) {
+#pragma unroll
+        for (int i = 0; i < kExpTable / kWarps; ++i)
+            sh.exp2_table[i * kWarps + warp][lane] = sh.segment[i * kWarps + warp];
+    }
+    center = __uint_as_float(sh.wlo[lane % kWarps]);
+    // the fourth largest of the warps' maxima: six in a thousand tokens or so are above it
+    int larger = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const float other = __shfl_sync(0xFFFFFFFFu, center, w);
+        larger += other > center || (other == center && w < lane % kWarps);
+    }
+    float upper = __shfl_sync(0xFFFFFFFFu, center, __ffs(__ballot_sync(0xFFFFFFFFu, larger == 3)) - 1);
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) center = fmaxf(center, __shfl_xor_sync(0xFFFFFFFFu, center, o));
+    __syncthreads();
+    // a masked sample, or values too large for the bins
+    if (!(fabsf(center) < 1e4f)) center = upper = 0.0f;
+    if (!(fabsf(upper) < 1e4f)) upper = center;
+    // Top-p's border is mostly below the few largest tokens: they share the
+    // first bin, whose mass follows from the sum and needs no estimate.
+    const bool sure = sums_all && p < 1.0f && mp == 0.0f;  // tokens above the border's bins are not listed
+    const Fine bin_of{(sure ? upper : center + 8.0f) * kFinePerNat + 8388608.0f};
     const double ref = (double)center;
     const Exp mass(sh.exp2_table, 1.0, -ref);                  // relative to the sample's maximum
     const Exp draw(sh.exp2_table, inv_t, -ref * inv_t);
@@ -807,29 +835,42 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         double sum = 0.0;
         float best = -INFINITY;
         int index = INT_MAX;
-        constexpr int STEPS = PACKS ? 4 : 2;  // loads in flight
+        constexpr int STEPS = 2;  // loads in flight, eight elements a lane
         const float floor_of = draws_all ? draw_floor : mass_floor;
         const Exp f(sh.exp2_table, draws_all ? inv_t : 1.0, draws_all ? -ref * inv_t : -ref);
-        for (int i = lo; i < hi; i += 128 * STEPS) {
-            float v[STEPS][4];
+        int next = part;  // where the part ends
+        double before = 0.0;
+        // The slice comes in by asynchronous copies, kAhead steps ahead, each
+        // lane's elements by itself: into place where the slice is kept, else
+        // into a ring of the warp's own.
+        constexpr int kAhead = 3, kStep = 128 * STEPS;
+        float* ring = pool + warp * (4 * kStep);
+        auto place = [&](int i, int step) { return a.resident ? held + i : ring + (step & 3) * kStep; };
+        auto copy = [&](int i, int step) {
+            if (i < hi) {
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(place(i, step));
 #pragma unroll
-            for (int q = 0; q < STEPS; ++q) load4<PACKS>(logits + base, i + 128 * q, hi, v[q]);
-            if (a.resident) {
+                for (int q = 0; q < STEPS; ++q)
 #pragma unroll
-                for (int q = 0; q < STEPS; ++q) {
-                    if (PACKS) {
-                        const int at = element<true>(i + 128 * q, 0);
-                        if (at < hi)
-                            *reinterpret_cast<float4*>(held + at) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int at = element<false>(i + 128 * q, e);
-                            if (at < hi) held[at] = v[q][e];
-                        }
+                    for (int e = 0; e < (PACKS ? 1 : 4); ++e) {
+                        const int at = element<PACKS>(128 * q, e);
+                        if (i + at < hi)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst + at * 4),
+                                         "l"(logits + base + i + at), "n"(PACKS ? 16 : 4)
+                                         : "memory");
                     }
-                }
             }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        };
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) copy(lo + d * kStep, d);
+        float v[STEPS][4];
+        for (int i = lo, step = 0; i < hi; i += kStep, ++step) {
+            copy(i + kAhead * kStep, step + kAhead);
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kAhead) : "memory");
+            const float* in = place(i, step);
+#pragma unroll
+            for (int q = 0; q < STEPS; ++q) load4<PACKS>(in, 128 * q, hi - i, v[q]);
             if (greedy) {
 #pragma unroll
                 for (int q = 0; q < STEPS; ++q)
@@ -841,22 +882,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 #pragma unroll
             for (int q = 0; q < STEPS; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) best = fmaxf(best, v[q][e]);  // a NaN is passed over
+                for (int e = 0; e < 4; ++e) {
+                    best = fmaxf(best, v[q][e]);              // a NaN is passed over,
+                    v[q][e] = fmaxf(v[q][e], floor_of);       // and counts, as -inf does, as nothing
+                }
             if (!draws_all) {
 #pragma unroll
                 for (int q = 0; q < STEPS; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (v[q][e] > -INFINITY) atomicAdd(&sh.fine[bin_of(v[q][e])], 1u);
+                    for (int e = 0; e < 4; ++e)  // what has no bin goes to a word of the lane's own
+                        atomicAdd(&sh.fine[min(bin_of.raw(v[q][e]), (unsigned)(kFine + lane))], 1u);
             }
             if (sums_all) {
 #pragma unroll
                 for (int q = 0; q < STEPS; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const double w = f(v[q][e]);
-                        if (v[q][e] > floor_of) sum += w;
-                    }
+                    for (int e = 0; e < 4; ++e) sum += f(v[q][e]);
+                if (draws_all && (i + 128 * STEPS - lo >= next || i + 128 * STEPS >= hi)) {
+                    double w = sum - before;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+                    if (lane == 0) sh.seg[warp * kSub + next / part - 1] = w;
+                    before = sum, next += part;
+                }
             }
         }
 #pragma unroll
@@ -869,7 +917,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         if (lane == 0) {
             sh.wsum[0][warp] = sum;
             sh.wlo[warp] = __float_as_uint(best), sh.whi[warp] = (uint32_t)index;
-            sh.seg[warp] = draws_all ? sum : 0.0;
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -885,11 +932,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
     r.sync();
     First m{0.0, -INFINITY, INT_MAX};
-    for (int i = 0; i < ranks; ++i) {
-        const First q = *r.of(&sh.first, i);
-        if (q.best > m.best) m.best = q.best, m.index = q.index;  // ranks hold rising indices
-        m.sum += q.sum;
+    if (lane < ranks) m = *r.of(&sh.first, lane);
+#pragma unroll
+    for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+        const float b2 = __shfl_xor_sync(0xFFFFFFFFu, m.best, o);
+        const int i2 = __shfl_xor_sync(0xFFFFFFFFu, m.index, o);
+        if (b2 > m.best || (b2 == m.best && i2 < m.index)) m.best = b2, m.index = i2;
+        m.sum += __shfl_xor_sync(0xFFFFFFFFu, m.sum, o);
     }
+    m.best = __shfl_sync(0xFFFFFFFFu, m.best, 0), m.index = __shfl_sync(0xFFFFFFFFu, m.index, 0);
+    m.sum = __shfl_sync(0xFFFFFFFFu, m.sum, 0);
     const float top = m.best;
     if (!(top > -INFINITY) || greedy) {
         if (rank == 0 && threadIdx.x == 0) {
@@ -902,12 +954,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
     // Which bins the list takes ([first, last]); bins before it are kept for sure.
     int first = 0, last = -1;
-    const bool sure = sums_all && p < 1.0f && mp == 0.0f;
     // a range that the sample misjudged, or infinite logits
     bool wide = sums_all && !(m.sum > 1e-250 && m.sum < 1e250 && top < center + 500.0f * fminf(t, 1.0f));
     if (!draws_all && !wide) {
         uint32_t count[kPer] = {};
-        for (int i = 0; i < ranks; ++i) {
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i) {
+            if (i >= ranks) break;
             const uint4 c = *reinterpret_cast<const uint4*>(r.of(sh.fine, i) + threadIdx.x * kPer);
             count[0] += c.x, count[1] += c.y, count[2] += c.z, count[3] += c.w;
         }
@@ -915,34 +968,36 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             // top-p behind top-k needs the mass of all k; otherwise nothing below min-p's bin matters
             last = mp > 0.0f && !(k > 0 && p < 1.0f)
                        ? bin_of(__double2float_rd((double)top + log((double)mp) - 1e-4))
-                       : kFine - 1;
+                       : kFine;
             if (k > 0) {
-                const int by_k = fine_border<uint32_t>(sh, count, count, (uint32_t)k);
+                const int by_k = fine_border<uint32_t>(sh, count, (uint32_t)k);
                 if (by_k > last) k = 0;  // what min-p keeps is less than k
                 else last = by_k;
             }
         } else {
             // The bins around the border. A bin's tokens are estimated at its
-            // middle, each off by 1/256 of its mass at most and by independent
-            // amounts: six spreads of their sum (a spread of 1/443 each), and
-            // 1e-4 for bins on a slope. The first bin takes what the sum has
-            // beyond the others. Where that is not enough, the list does not
-            // hold the border and the wide search settles the row.
+            // middle, each off by 1/128 of its mass at most and by independent
+            // amounts: six spreads of their sum (a spread of 1/222 each), and
+            // 1e-4 for bins on a slope. What has no bin is below e^-24 a token.
+            // The first bin takes what the sum has beyond the others. Where
+            // that is not enough, the list does not hold the border and the
+            // wide search settles the row.
             double guess[kPer], own = 0.0, squares = 0.0, others, spread;
+            double one = exp(((double)bin_of.high - 8388608.0 - (double)(threadIdx.x * kPer)) / kFinePerNat - ref);
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
-                const int b = threadIdx.x * kPer + e;
-                const double one = exp(((double)bin_of.high - 8388608.0 - (double)b) / kFinePerNat - ref);
-                guess[e] = b ? (double)count[e] * one : 0.0;
+                guess[e] = threadIdx.x * kPer + e ? (double)count[e] * one : 0.0;
                 own += guess[e], squares += guess[e] * one;
+                one *= 0.98449643700540845;  // exp(-1 / kFinePerNat)
             }
             block_scan(sh, own, others);
             block_scan(sh, squares, spread);
             if (threadIdx.x == 0) guess[0] = fmax(m.sum - others, 0.0);
             const double border = (double)p * m.sum;
-            const double off = fmin(m.sum / 250.0, 6.0 / 443.0 * sqrt(spread) + 1e-4 * m.sum);
-            first = fine_border<double>(sh, count, guess, border - off);
-            last = fine_border<double>(sh, count, guess, border + off);
+            const double none = 3.8e-11 * (double)a.vocab;
+            const double off = fmin(m.sum / 125.0, 6.0 / 222.0 * sqrt(spread) + 1e-4 * m.sum) + none;
+            first = fine_border<double>(sh, guess, border - off);
+            last = fine_border<double>(sh, guess, border + off);
         }
     }
 
@@ -950,113 +1005,134 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     int listed = 0;
     double above = 0.0;
     if (!draws_all && !wide) {
+        // the bins' borders as values: the list takes v >= from, those above it v >= over
+        const float from = last == kFine ? -INFINITY : bin_of.start(last);
+        const float over = first == 0 ? INFINITY : bin_of.start(first - 1);
         double sum = 0.0, weights = 0.0;
-        int mine = 0, waiting = 0;
-        float* dense = sh.dense[warp];
-        auto flush = [&](int c) {  // the first c of the waiting values
-            if (lane < c) {
-                const float v = dense[lane];
-                if (v > mass_floor) sum += mass(v);
-                if (v > draw_floor) weights += draw(v);
-            }
+        int mine = 0, waiting = 0, next = part;
+        // Values above the list wait in a column of the lane's own (the list's
+        // place, not needed yet), so that their exponentials are computed with
+        // most of the warp's lanes at work.
+        constexpr int kStep = 256, kDeep = 16;
+        float* queue = list + warp * (kDeep * 32) + lane;
+        auto drain = [&] {
+            for (int d = 0; __any_sync(0xFFFFFFFFu, d < waiting); ++d)
+                if (d < waiting) {
+                    const float w = queue[d * 32];
+                    const double e = mass(w);
+                    sum += e;
+                    weights += t == 1.0f ? e : draw(fmaxf(w, draw_floor));
+                }
+            waiting = 0;
         };
-#pragma unroll 2
-        for (int i = lo; i < hi; i += 128) {
-            float v[4];
-            load4<PACKS>(r.x, i, hi, v);
-            int take = 0, over = 0;  // bits: tokens of the list, tokens above it
+        float v[2][4], ahead[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int b = bin_of(v[e]);
-                const bool in = v[e] > -INFINITY && b <= last;
-                take |= (in && b >= first) << e;
-                over |= (in && b < first) << e;
+        for (int q = 0; q < 2; ++q) load4<PACKS>(r.x, lo + 128 * q, hi, ahead[q]);
+        for (int i = lo; i < hi; i += kStep) {
+            bool take = false;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[q][e] = ahead[q][e];
+                load4<PACKS>(r.x, i + kStep + 128 * q, hi, ahead[q]);
             }
-            if (sure && __any_sync(0xFFFFFFFFu, over)) {
-                int incl = __popc(over);
-                const int c = incl;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                    if (lane >= o) incl += up;
-                }
-                int at = waiting + incl - c;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (over >> e & 1) dense[at++] = v[e];
-                waiting += __shfl_sync(0xFFFFFFFFu, incl, 31);
-                __syncwarp();
-                if (waiting >= 32) {
-                    int from = 0;
-                    for (; from + 32 <= waiting; from += 32) {
-                        const float w = dense[from + lane];
-                        if (w > mass_floor) sum += mass(w);
-                        if (w > draw_floor) weights += draw(w);
-                    }
-                    waiting -= from;
-                    const float rest = lane < waiting ? dense[from + lane] : 0.0f;
-                    __syncwarp();
-                    if (lane < waiting) dense[lane] = rest;
-                    __syncwarp();
-                }
-            }
-            if (!__any_sync(0xFFFFFFFFu, take)) continue;
-            int pos[4], all = 0;  // places of this step's tokens, in index order
-            if (PACKS) {
-                const int c = __popc(take);
-                int incl = c;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                    if (lane >= o) incl += up;
-                }
-                all = __shfl_sync(0xFFFFFFFFu, incl, 31);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pos[e] = incl - c + __popc(take & ((1 << e) - 1));
-            } else {
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const unsigned votes = __ballot_sync(0xFFFFFFFFu, take >> e & 1);
-                    pos[e] = all + __popc(votes & ((1u << lane) - 1u));
-                    all += __popc(votes);
+                    const bool in = v[q][e] >= over;  // over is infinite where nothing is sure
+                    if (sure) queue[waiting * 32] = v[q][e];  // the next one overwrites what does not count
+                    waiting += in && sure;
+                    take |= v[q][e] >= from && v[q][e] > -INFINITY && !(in && sure);
+                }
+            if (sure && __any_sync(0xFFFFFFFFu, waiting > kDeep - 8)) drain();
+            if (__any_sync(0xFFFFFFFFu, take)) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    int bits = 0, pos[4], all = 0;  // places of these tokens, in index order
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        bits |= (v[q][e] >= from && v[q][e] > -INFINITY && !(sure && v[q][e] >= over)) << e;
+                    const unsigned some = __ballot_sync(0xFFFFFFFFu, bits);
+                    if (!some) continue;
+                    if (PACKS) {
+                        const int c = __popc(bits);
+                        int before = __popc(some & ((1u << lane) - 1u));
+                        all = __popc(some);
+                        if (__any_sync(0xFFFFFFFFu, c > 1)) {
+                            int incl = c;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                                if (lane >= o) incl += up;
+                            }
+                            all = __shfl_sync(0xFFFFFFFFu, incl, 31);
+                            before = incl - c;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) pos[e] = before + __popc(bits & ((1 << e) - 1));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned votes = __ballot_sync(0xFFFFFFFFu, bits >> e & 1);
+                            pos[e] = all + __popc(votes & ((1u << lane) - 1u));
+                            all += __popc(votes);
+                        }
+                    }
+                    if ((mine + 31) / 32 < (mine + all + 31) / 32) {
+                        if (lane == 0)  // groups of 32 from the pool, up to the last of them
+                            for (int g = (mine + 31) / 32; g < (mine + all + 31) / 32; ++g) {
+                                const int got = atomicAdd(&sh.pool_used, 1);
+                                if (g < kList / 32) sh.chain[warp][g] = (uint8_t)min(got, kList / 32 - 1);
+                            }
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int slot = mine + pos[e];
+                        if ((bits >> e & 1) && slot < kList) {
+                            const int to = sh.chain[warp][slot / 32] * 32 + slot % 32;
+                            pool[to] = v[q][e];
+                            pool_index[to] = base + element<PACKS>(i + 128 * q, e);
+                        }
+                    }
+                    mine += all;
                 }
             }
-            if (lane == 0)  // groups of 32 from the pool, up to the last of them
-                for (int g = (mine + 31) / 32; g < (mine + all + 31) / 32; ++g) {
-                    const int got = atomicAdd(&sh.pool_used, 1);
-                    if (g < kList / 32) sh.chain[warp][g] = (uint8_t)min(got, kList / 32 - 1);
-                }
-            __syncwarp();
+            if (sure && (i + kStep - lo >= next || i + kStep >= hi)) {  // a part ends
+                drain();
+                double w = weights;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int slot = mine + pos[e];
-                if ((take >> e & 1) && slot < kList) {
-                    const int to = sh.chain[warp][slot / 32] * 32 + slot % 32;
-                    pool[to] = v[e];
-                    pool_index[to] = base + element<PACKS>(i, e);
-                }
+                for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+                if (lane == 0) sh.seg[warp * kSub + next / part - 1] = w, sh.listed_part[warp * kSub + next / part - 1] = mine;
+                weights = 0.0, next += part;
             }
-            mine += all;
         }
-        flush(waiting);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            weights += __shfl_xor_sync(0xFFFFFFFFu, weights, o);
-        }
-        if (lane == 0) sh.listed[warp] = mine, sh.seg[warp] = weights, sh.wsum[1][warp] = sum;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (lane == 0) sh.listed[warp] = mine, sh.wsum[1][warp] = sum;
+        if (lane == 0)
+            for (int e = next / part - 1; e < kSub; ++e) sh.listed_part[warp * kSub + e] = mine;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            double s = 0.0;
-            int c = sh.pool_used > kList / 32 ? kList + 1 : 0;  // more than the pool holds
-            for (int w = 0; w < kWarps; ++w) s += sh.wsum[1][w], c += sh.listed[w];
-            sh.above = s, sh.block_listed = c;
+        if (warp == 0) {
+            double s = sh.wsum[1][lane % kWarps];
+            int c = sh.listed[lane % kWarps];
+#pragma unroll
+            for (int o = kWarps / 2; o > 0; o >>= 1) {
+                s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+                c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+            }
+            // more than the pool holds
+            if (lane == 0) sh.above = s, sh.block_listed = sh.pool_used > kList / 32 ? kList + 1 : c;
         }
         r.sync();
-        for (int i = 0; i < ranks; ++i) {
-            listed += *r.of(&sh.block_listed, i);
-            above += *r.of(&sh.above, i);
+        if (lane < ranks) listed = *r.of(&sh.block_listed, lane), above = *r.of(&sh.above, lane);
+#pragma unroll
+        for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+            listed += __shfl_xor_sync(0xFFFFFFFFu, listed, o);
+            above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
         }
+        listed = __shfl_sync(0xFFFFFFFFu, listed, 0), above = __shfl_sync(0xFFFFFFFFu, above, 0);
         if (listed > kList) wide = true;  // every block sees the same sum
     }
 
@@ -1085,17 +1161,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                     if (lane == 0) sh.offset[segs] = before;
                 }
                 __syncthreads();
-                for (int g = warp; g < segs; g += kWarps) {
-                    const int q = g / kWarps, from = sh.offset[g], c = sh.offset[g + 1] - from;
-                    const uint8_t* chain = r.of(&sh.chain[0][0], q) + (g % kWarps) * (kList / 32);
-                    const float* pv = r.of(pool, q);
-                    const int* pi = r.of(pool_index, q);
-                    for (int i = lane; i < c; i += 32) {
-                        const int at = chain[i / 32] * 32 + i % 32;
-                        list[from + i] = pv[at];
-                        list_index[from + i] = pi[at];
+                for (int i = threadIdx.x; i < listed; i += kThreads) {
+                    int g = 0, end = segs;  // the warp that put it there: offset[g] <= i < offset[g + 1]
+                    while (end - g > 1) {
+                        const int mid = (g + end) >> 1;
+                        if (sh.offset[mid] <= i) g = mid;
+                        else end = mid;
                     }
+                    const int q = g / kWarps, at = i - sh.offset[g];
+                    const int from = r.of(&sh.chain[0][0], q)[(g % kWarps) * (kList / 32) + at / 32] * 32 + at % 32;
+                    list[i] = r.of(pool, q)[from];
+                    list_index[i] = r.of(pool_index, q)[from];
                 }
+                if (sure)
+                    for (int g = threadIdx.x; g < segs * kSub; g += kThreads)
+                        sh.part_end[g] = sh.offset[g / kSub] + r.of(sh.listed_part, g / (kWarps * kSub))[g % (kWarps * kSub)];
                 __syncthreads();
                 const double least = (double)mp, log_least = mp > 0.0f ? log(least) : 0.0;
                 auto kept_weight = [&](float v) -> double {
@@ -1109,38 +1189,56 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                     if (sums_all) return v > mass_floor ? mass(v) : 0.0;
                     return exp(below(v, top));
                 };
-                holds = settle_list(sh, list, reinterpret_cast<unsigned long long*>(pool), weight_of, listed, k, p,
-                                    above, sums_all ? m.sum : 0.0, sure, list_mass, kept_weight);
+                unsigned long long* order = reinterpret_cast<unsigned long long*>(pool);
+                const double all = sums_all ? m.sum : 0.0;
+                if (listed <= kThreads)
+                    holds = settle_list<1>(sh, list, order, weight_of, listed, k, p, above, all, sure, list_mass, kept_weight);
+                else
+                    holds = settle_list<kList / kThreads>(sh, list, order, weight_of, listed, k, p, above, all, sure,
+                                                          list_mass, kept_weight);
             }
             if (!holds) {
                 if (threadIdx.x == 0) sh.won = -2;
             } else if (!sure && !draws_all) {
                 constexpr int PER = kList / kThreads;
-                const int per = (listed + kThreads - 1) / kThreads;
+                double total, weight;
+                int at;
+                if (listed <= kThreads) {
+                    const double w[1] = {(int)threadIdx.x < listed ? weight_of[threadIdx.x] : 0.0};
+                    at = pick<1>(sh, w, u, 0.0, total, weight);
+                } else {
+                    double w[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) {
+                        const int i = threadIdx.x * PER + e;
+                        w[e] = i < listed ? weight_of[i] : 0.0;
+                    }
+                    at = pick<PER>(sh, w, u, 0.0, total, weight);
+                }
+                if (threadIdx.x == 0) sh.id = list_index[at], sh.weight = weight, sh.total = total;
+            } else {
+                // each part's weights: what lies above the list, and its kept tokens of the list
+                constexpr int PER = kMaxCluster * kWarps * kSub / kThreads;
+                const int parts = segs * kSub;
+                if (!draws_all) {
+                    for (int g = warp; g < parts; g += kWarps) {
+                        double w = 0.0;
+                        for (int i = (g ? sh.part_end[g - 1] : 0) + lane; i < sh.part_end[g]; i += 32) w += weight_of[i];
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+                        if (lane == 0) sh.segment[g] = w;
+                    }
+                    __syncthreads();
+                }
                 double w[PER], total, weight;
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const int i = threadIdx.x * per + e;
-                    w[e] = e < per && i < listed ? weight_of[i] : 0.0;
+                    const int g = threadIdx.x * PER + e;
+                    w[e] = 0.0;
+                    if (g < parts)
+                        w[e] = (draws_all ? 0.0 : sh.segment[g]) + r.of(sh.seg, g / (kWarps * kSub))[g % (kWarps * kSub)];
                 }
-                // pick counts PER elements a thread; only the first `per` have a weight
-                const int at = pick<PER>(sh, w, u, 0.0, total, weight);
-                if (threadIdx.x == 0)
-                    sh.id = list_index[(at / PER) * per + at % PER], sh.weight = weight, sh.total = total;
-            } else {
-                // each segment's sure weights and its kept tokens of the list
-                double* sums = sh.segment;
-                for (int g = warp; g < segs; g += kWarps) {
-                    double w = 0.0;
-                    if (!draws_all)
-                        for (int i = sh.offset[g] + lane; i < sh.offset[g + 1]; i += 32) w += weight_of[i];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
-                    if (lane == 0) sums[g] = w + r.of(sh.seg, g / kWarps)[g % kWarps];
-                }
-                __syncthreads();
-                double w[1] = {(int)threadIdx.x < segs ? sums[threadIdx.x] : 0.0}, total, weight;
-                const int won = pick<1>(sh, w, u, 0.0, total, weight);
+                const int won = pick<PER>(sh, w, u, 0.0, total, weight);
                 if (threadIdx.x == 0) {
                     // a temperature that takes the weights out of range
                     sh.won = total > 1e-250 && total < 1e250 ? won : -2;
@@ -1152,13 +1250,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         r.sync();
         const int won = *r.of(&sh.won, 0);
         const double total = *r.of(&sh.total, 0);
-        if (won >= 0 && won / kWarps == rank) {
-            const int from = min((won % kWarps) * seg, n), to = min(from + seg, n);
+        if (won >= 0 && won / (kWarps * kSub) == rank) {
+            const int at = won % (kWarps * kSub), end = min((at / kSub + 1) * seg, n);
+            const int from = min((at / kSub) * seg + (at % kSub) * part, end), to = min(from + part, end);
             const double target = *r.of(&sh.won_before, 0);
             const double* all_weights = r.of(weight_of, 0);
             const int* all_index = r.of(list_index, 0);
-            const int* offsets = r.of(sh.offset, 0);
-            const int l0 = draws_all ? 0 : offsets[won], l1 = draws_all ? 0 : offsets[won + 1];
+            const int* ends = r.of(sh.part_end, 0);
+            const int l0 = draws_all || won == 0 ? 0 : ends[won - 1], l1 = draws_all ? 0 : ends[won];
             double w;
             const int got = locate(r, from, to, target, w, [&](float v, int i) -> double {
                 if (!(v > draw_floor)) return 0.0;
