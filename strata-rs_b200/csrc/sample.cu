@@ -24,6 +24,8 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "sequence.cuh"
 
 namespace cg = cooperative_groups;
@@ -218,10 +220,9 @@ struct Row {
         W base_sum = 0;
         for (int w = 0; w < warp; ++w) base_sum += tot[w];
         incl += base_sum;
-        if (count) {
-            atomicMax(&sh.found, (int)threadIdx.x);
-            if (incl >= target) atomicMin(&sh.pick_bin, (int)threadIdx.x);
-        }
+        const int past = __reduce_min_sync(0xFFFFFFFFu, count && incl >= target ? (int)threadIdx.x : kBins);
+        const int last = __reduce_max_sync(0xFFFFFFFFu, count ? (int)threadIdx.x : -1);
+        if (lane == 0) atomicMin(&sh.pick_bin, past), atomicMax(&sh.found, last);
         __syncthreads();
         const int bin = sh.pick_bin < kBins ? sh.pick_bin : sh.found;
         if ((int)threadIdx.x == bin) sh.pick_mass = (double)(incl - weight);
@@ -500,13 +501,15 @@ __device__ __forceinline__ double block_scan(Shared& sh, double v, double& total
     __syncthreads();
     if (lane == 31) sh.wsum[0][warp] = v;
     __syncthreads();
-    double before = 0.0;
-    total = 0.0;
-    for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) before = total;
-        total += sh.wsum[0][w];
+    double w = sh.wsum[0][lane % kWarps];
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+        const double up = __shfl_up_sync(0xFFFFFFFFu, w, o, kWarps);
+        if (lane % kWarps >= o) w += up;
     }
-    return before + v;
+    total = __shfl_sync(0xFFFFFFFFu, w, kWarps - 1);
+    const double before = __shfl_sync(0xFFFFFFFFu, w, warp > 0 ? warp - 1 : 0);
+    return (warp > 0 ? before : 0.0) + v;
 }
 
 // Among the block's weights w[e] (element threadIdx.x * PER + e), the first
@@ -521,20 +524,30 @@ __device__ int pick(Shared& sh, const double (&w)[PER], double u, double offset,
     const double target = u >= 0.0 ? u * total : offset;
     if (threadIdx.x == 0) sh.pick_bin = INT_MAX, sh.found = -1;
     __syncthreads();
+    int past = INT_MAX, last = -1;  // the first past the target, the last with a weight
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         run += w[e];
         if (w[e] > 0.0) {
-            atomicMax(&sh.found, (int)threadIdx.x * PER + e);
-            if (run > target) atomicMin(&sh.pick_bin, (int)threadIdx.x * PER + e);
+            last = (int)threadIdx.x * PER + e;
+            if (run > target && past == INT_MAX) past = last;
         }
+    }
+    past = __reduce_min_sync(0xFFFFFFFFu, past), last = __reduce_max_sync(0xFFFFFFFFu, last);
+    if ((threadIdx.x & 31) == 0) {
+        if (past != INT_MAX) atomicMin(&sh.pick_bin, past);
+        if (last >= 0) atomicMax(&sh.found, last);
     }
     __syncthreads();
     const int at = sh.pick_bin != INT_MAX ? sh.pick_bin : sh.found;
     if (at >= 0 && at / PER == (int)threadIdx.x) {
+        double upto = run - own;  // the sum up to the element itself
 #pragma unroll
         for (int e = 0; e < PER; ++e)
-            if (at % PER == e) sh.weight = w[e], sh.won_before = run;
+            if (e <= at % PER) upto += w[e];
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (at % PER == e) sh.weight = w[e], sh.won_before = upto;
     }
     __syncthreads();
     weight = sh.weight;
@@ -551,32 +564,65 @@ __device__ int fine_border(Shared& sh, const W (&weight)[kPer], W target) {
     double run = block_scan(sh, own, total) - own;
     if (threadIdx.x == 0) sh.pick_bin = kFine;
     __syncthreads();
+    int reached = kFine;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         run += (double)weight[e];
-        if (weight[e] > 0 && run >= (double)target) atomicMin(&sh.pick_bin, (int)threadIdx.x * kPer + e);
+        if (weight[e] > 0 && run >= (double)target) reached = min(reached, (int)threadIdx.x * kPer + e);
     }
+    reached = __reduce_min_sync(0xFFFFFFFFu, reached);
+    if ((threadIdx.x & 31) == 0) atomicMin(&sh.pick_bin, reached);
     __syncthreads();
     const int bin = sh.pick_bin;
     __syncthreads();
     return bin;
 }
 
-// Sorts x[0, n), n a power of two from 64, rising. Strides up to 32 stay within
-// the 64 values of a warp.
-__device__ void sort_list(unsigned long long* x, int n) {
-    for (int size = 2; size <= n; size <<= 1) {
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            for (int t = threadIdx.x; t < n / 2; t += kThreads) {
-                const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-                const unsigned long long a = x[i], b = x[j];
-                if ((a > b) == ((i & size) == 0)) x[i] = b, x[j] = a;
+// Sorts the block's kThreads * PER values x[e] (place threadIdx.x * PER + e),
+// rising: a bitonic network whose short strides stay within a thread or a
+// warp's registers; `buffer` holds kThreads * PER values.
+template <int PER>
+__device__ void sort_block(unsigned long long (&x)[PER], unsigned long long* buffer) {
+    constexpr int N = kThreads * PER;
+    const int first = threadIdx.x * PER;
+#pragma unroll 1
+    for (int size = 2; size <= N; size <<= 1) {
+        int stride = size >> 1;
+#pragma unroll 1
+        for (; stride >= 32 * PER; stride >>= 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < PER; ++e) buffer[e * kThreads + threadIdx.x] = x[e];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const unsigned long long y = buffer[e * kThreads + (threadIdx.x ^ (stride / PER))];
+                const bool low = (((first + e) & stride) == 0) == (((first + e) & size) == 0);
+                x[e] = low ? min(x[e], y) : max(x[e], y);
             }
-            if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads();
-            else __syncwarp();
+        }
+#pragma unroll 1
+        for (; stride >= PER; stride >>= 1) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const unsigned long long y = __shfl_xor_sync(0xFFFFFFFFu, x[e], stride / PER);
+                const bool low = (((first + e) & stride) == 0) == (((first + e) & size) == 0);
+                x[e] = low ? min(x[e], y) : max(x[e], y);
+            }
+        }
+#pragma unroll
+        for (int s = PER / 2; s > 0; s >>= 1) {
+            if (s >= size) continue;
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                if (!(e & s)) {
+                    const unsigned long long a = x[e], b = x[e | s];
+                    const bool rising = ((first + e) & size) == 0;
+                    x[e] = rising ? min(a, b) : max(a, b);
+                    x[e | s] = rising ? max(a, b) : min(a, b);
+                }
         }
     }
-    __syncthreads();
 }
 
 // The search over whole slices: for rows whose cut no list holds.
@@ -697,23 +743,17 @@ __device__ int locate(Row& r, int lo, int hi, double target, double& weight_out,
 // on return out[i] is token i's weight in the draw (0 where it is not kept).
 // above: mass of larger tokens outside the list; all: mass that p refers to
 // (0: that of the first k). False where the border of p lies outside a list
-// that has tokens above it. A thread holds PER neighbours of the order (one
-// for the usual short list, to keep the code that a row runs through short).
+// that has tokens above it. A thread holds PER neighbours of the order.
 template <int PER, typename M, typename D>
 __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* order, double* out, int listed, int k,
                             float p, double above, double all, bool sure, M mass, D draw) {
-    int n = 64;
-    while (n < listed) n <<= 1;
-    for (int i = threadIdx.x; i < n; i += kThreads)
-        order[i] = i < listed ? (unsigned long long)~key_of(list[i]) << 32 | (unsigned)i : ~0ull;
-    __syncthreads();
-    sort_list(order, n);
     unsigned long long mine[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int r = threadIdx.x * PER + e;
-        mine[e] = r < listed ? order[r] : ~0ull;
+        const int i = e * kThreads + threadIdx.x;
+        mine[e] = i < listed ? (unsigned long long)~key_of(list[i]) << 32 | (unsigned)i : ~0ull;
     }
+    sort_block<PER>(mine, order);
     int kept = k > 0 && k < listed ? k : listed;
     bool holds = true;
     if (p < 1.0f) {
@@ -728,12 +768,15 @@ __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* o
         if (sure) holds = target > above && target <= above + total;
         if (threadIdx.x == 0) sh.found = 1;  // the first token always stays
         __syncthreads();
+        int last = 0;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int r = threadIdx.x * PER + e;
-            if (r < kept && run < target) atomicMax(&sh.found, r + 1);
+            if (r < kept && run < target) last = r + 1;
             run += m[e];
         }
+        last = __reduce_max_sync(0xFFFFFFFFu, last);
+        if ((threadIdx.x & 31) == 0) atomicMax(&sh.found, last);
         __syncthreads();
         kept = sh.found;
     }
@@ -1191,11 +1234,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 };
                 unsigned long long* order = reinterpret_cast<unsigned long long*>(pool);
                 const double all = sums_all ? m.sum : 0.0;
-                if (listed <= kThreads)
-                    holds = settle_list<1>(sh, list, order, weight_of, listed, k, p, above, all, sure, list_mass, kept_weight);
-                else
-                    holds = settle_list<kList / kThreads>(sh, list, order, weight_of, listed, k, p, above, all, sure,
-                                                          list_mass, kept_weight);
+                auto settle = [&](auto per) {
+                    return settle_list<decltype(per)::value>(sh, list, order, weight_of, listed, k, p, above, all, sure,
+                                                             list_mass, kept_weight);
+                };
+                holds = listed <= kThreads       ? settle(std::integral_constant<int, 1>())
+                        : listed <= 2 * kThreads ? settle(std::integral_constant<int, 2>())
+                                                 : settle(std::integral_constant<int, kList / kThreads>());
             }
             if (!holds) {
                 if (threadIdx.x == 0) sh.won = -2;
@@ -1220,23 +1265,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 // each part's weights: what lies above the list, and its kept tokens of the list
                 constexpr int PER = kMaxCluster * kWarps * kSub / kThreads;
                 const int parts = segs * kSub;
-                if (!draws_all) {
-                    for (int g = warp; g < parts; g += kWarps) {
-                        double w = 0.0;
-                        for (int i = (g ? sh.part_end[g - 1] : 0) + lane; i < sh.part_end[g]; i += 32) w += weight_of[i];
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
-                        if (lane == 0) sh.segment[g] = w;
-                    }
-                    __syncthreads();
-                }
                 double w[PER], total, weight;
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
                     const int g = threadIdx.x * PER + e;
                     w[e] = 0.0;
-                    if (g < parts)
-                        w[e] = (draws_all ? 0.0 : sh.segment[g]) + r.of(sh.seg, g / (kWarps * kSub))[g % (kWarps * kSub)];
+                    if (g < parts) {
+                        w[e] = r.of(sh.seg, g / (kWarps * kSub))[g % (kWarps * kSub)];
+                        if (!draws_all)
+                            for (int i = g ? sh.part_end[g - 1] : 0; i < sh.part_end[g]; ++i) w[e] += weight_of[i];
+                    }
                 }
                 const int won = pick<PER>(sh, w, u, 0.0, total, weight);
                 if (threadIdx.x == 0) {
