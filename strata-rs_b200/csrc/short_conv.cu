@@ -6,10 +6,11 @@
 //
 // Bound by memory: each x is read and each y written once, 2 K flops between
 // them. A thread owns VEC neighbouring channels (one 16-byte access) and walks
-// a tile of kTile tokens with the last K - 1 inputs in registers, so a tile
-// re-reads only its K - 1 rows of halo (from L2). The rows of a tile are
-// loaded kAhead at a time, so that many independent 16-byte loads are in
-// flight per thread.
+// a tile of tokens with the last K - 1 inputs in registers, so a tile re-reads
+// only its K - 1 rows of halo (from L2). Rows are loaded kAhead at a time, one
+// batch ahead of the one that is computed, so that independent 16-byte loads
+// are always in flight. Tiles are as long as a full GPU allows (their weights
+// and halo are then a small part), one token where sequences have one.
 //
 // The state of a sequence is read and replaced by the same thread (the one
 // that has its first tile; the new state is the sequence's last K - 1 inputs,
@@ -21,8 +22,7 @@
 namespace strata {
 namespace {
 
-constexpr int kTile = 16;
-constexpr int kAhead = 8;
+constexpr int kMinTile = 8, kMaxTile = 64;  // tokens of a tile; at least the longest halo
 constexpr int kThreads = 128;
 
 struct ConvArgs {
@@ -33,7 +33,9 @@ struct ConvArgs {
     void* y;
     int64_t x_stride, y_stride;
     int channels, blocks;  // blocks of channels
+    int tile;
     int silu;
+    int wide_w;            // w can be read in 16-byte packs
 };
 
 // z / (1 + exp(-z)). For bf16 outputs the approximate exponential is far below
@@ -44,82 +46,99 @@ __device__ __forceinline__ float silu(float z) {
     return __fdividef(z, 1.0f + (sizeof(T) == 2 ? __expf(-z) : expf(-z)));
 }
 
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&d)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) d[v] = to_f32(p.v[v]);
+}
+
 template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(kThreads) conv_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
+__global__ void __launch_bounds__(kThreads, K <= 4 ? 4 : 1)
+    conv_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
+    constexpr int kAhead = VEC == 1 ? 8 : 4;
     const int block = blockIdx.x / a.blocks;
     const int c = ((blockIdx.x - block * a.blocks) * kThreads + threadIdx.x) * VEC;
     if (c >= a.channels) return;
     const Seq seq = sequence_of_tile(tab, block);
-    const int row = seq.row, len = seq.len, t0 = (block - seq.tile0) * kTile;
-    const int n = len - t0 < kTile ? len - t0 : kTile;
+    const int row = seq.row, len = seq.len, t0 = (block - seq.tile0) * a.tile;
+    const int n = len - t0 < a.tile ? len - t0 : a.tile;
     const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.x_stride + c;
     T* y = static_cast<T*>(a.y) + (int64_t)(row + t0) * a.y_stride + c;
     using P = Pack<T, VEC>;
+    using F = Pack<float, VEC>;
 
+    auto load = [&](P(&in)[kAhead], int t) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (t + u < n) in[u] = *reinterpret_cast<const P*>(x + (int64_t)(t0 + t + u) * a.x_stride);
+    };
+    P now[kAhead], next[kAhead];
+    load(now, 0);
     float w[K][VEC], past[K][VEC];  // past[0 .. K-2]: the inputs before the tile (one spare row keeps K = 1 legal)
-    float bias[VEC];
+    if (K == 4 && a.wide_w) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
+        for (int v = 0; v < VEC; ++v) {
+            const float4 q = *reinterpret_cast<const float4*>(a.w + (int64_t)(c + v) * 4);
+            w[0][v] = q.x, w[K > 1 ? 1 : 0][v] = q.y, w[K > 2 ? 2 : 0][v] = q.z, w[K > 3 ? 3 : 0][v] = q.w;
+        }
+    } else {
 #pragma unroll
-        for (int j = 0; j < K; ++j) w[j][v] = a.w[(int64_t)(c + v) * K + j];
-        bias[v] = a.bias ? a.bias[c + v] : 0.0f;
+        for (int v = 0; v < VEC; ++v)
+#pragma unroll
+            for (int j = 0; j < K; ++j) w[j][v] = a.w[(int64_t)(c + v) * K + j];
     }
+    float bias[VEC] = {};
+    if (a.bias) unpack<float, VEC>(*reinterpret_cast<const F*>(a.bias + c), bias);
     if (K > 1) {
         float* st = a.state + (int64_t)seq.slot * (K - 1) * a.channels + c;
         if (t0 == 0) {
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) past[j][v] = st[(int64_t)j * a.channels + v];
+                unpack<float, VEC>(*reinterpret_cast<const F*>(st + (int64_t)j * a.channels), past[j]);
             // the new state: input len - (K - 1) + j, or where that is before the call, old row len + j
 #pragma unroll
             for (int j = 0; j < K - 1; ++j) {
                 const int p = len - (K - 1) + j;
+                F out;
                 if (p >= 0) {
-                    const P in = *reinterpret_cast<const P*>(x + (int64_t)p * a.x_stride);
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) st[(int64_t)j * a.channels + v] = to_f32(in.v[v]);
+                    unpack<T, VEC>(*reinterpret_cast<const P*>(x + (int64_t)p * a.x_stride), out.v);
                 } else {
 #pragma unroll
                     for (int m = j + 1; m < K - 1; ++m)
                         if (m == j + len)
 #pragma unroll
-                            for (int v = 0; v < VEC; ++v) st[(int64_t)j * a.channels + v] = past[m][v];
+                            for (int v = 0; v < VEC; ++v) out.v[v] = past[m][v];
                 }
+                *reinterpret_cast<F*>(st + (int64_t)j * a.channels) = out;
             }
-        } else {  // t0 >= kTile > K - 1: the halo lies inside the sequence
+        } else {  // t0 >= kMinTile > K - 1: the halo lies inside the sequence
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) {
-                const P in = *reinterpret_cast<const P*>(x + (int64_t)(t0 - (K - 1) + j) * a.x_stride);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) past[j][v] = to_f32(in.v[v]);
-            }
+            for (int j = 0; j < K - 1; ++j)
+                unpack<T, VEC>(*reinterpret_cast<const P*>(x + (int64_t)(t0 - (K - 1) + j) * a.x_stride), past[j]);
         }
     }
-    x += (int64_t)t0 * a.x_stride;
     for (int t = 0; t < n; t += kAhead) {
-        P in[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (t + u < n) in[u] = *reinterpret_cast<const P*>(x + (int64_t)(t + u) * a.x_stride);
+        load(next, t + kAhead);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (t + u >= n) break;
             P out;
+            float in[VEC];
+            unpack<T, VEC>(now[u], in);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float now = to_f32(in[u].v[v]);
                 float z = bias[v];
 #pragma unroll
                 for (int j = 0; j < K - 1; ++j) z = fmaf(w[j][v], past[j][v], z);
-                z = fmaf(w[K - 1][v], now, z);
+                z = fmaf(w[K - 1][v], in[v], z);
 #pragma unroll
                 for (int j = 0; j + 1 < K - 1; ++j) past[j][v] = past[j + 1][v];
-                if (K > 1) past[K >= 2 ? K - 2 : 0][v] = now;
+                if (K > 1) past[K >= 2 ? K - 2 : 0][v] = in[v];
                 from_f32(out.v[v], a.silu ? silu<T>(z) : z);
             }
-            *reinterpret_cast<P*>(y + (int64_t)(t + u) * a.y_stride) = out;
+            if (t + u < n) *reinterpret_cast<P*>(y + (int64_t)(t + u) * a.y_stride) = out;
         }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) now[u] = next[u];
     }
 }
 
@@ -138,10 +157,10 @@ void launch_conv(int taps, const ConvArgs& a, const SeqTable& t, unsigned grid, 
 }
 
 // The 16-byte form needs whole packs in every row and 16-byte rows.
-bool packs(const strata_short_conv& d, const void* x, const void* y) {
+bool packs(const strata_short_conv& d, const void* x, const void* y, const float* bias, const float* state) {
     const int64_t vec = 16 / dtype_bytes(d.dtype);
-    return d.channels % vec == 0 && d.x_stride % vec == 0 && d.y_stride % vec == 0 && (uintptr_t)x % 16 == 0 &&
-           (uintptr_t)y % 16 == 0;
+    return d.channels % vec == 0 && d.x_stride % vec == 0 && d.y_stride % vec == 0 &&
+           ((uintptr_t)x | (uintptr_t)y | (uintptr_t)bias | (uintptr_t)state) % 16 == 0;
 }
 
 }  // namespace
@@ -162,13 +181,17 @@ extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_co
     if (!rc) rc = check_short_conv_buffers(why, d, tokens, x_dev, w_dev, bias_dev, state_dev, y_dev);
     if (rc) return fail(ctx, rc, "short_conv: %s", why.text);
     if (longest == 0) return STRATA_OK;
-    const bool bf16 = d.dtype == STRATA_QUANT_BF16, vec = packs(d, x_dev, y_dev);
+    const bool bf16 = d.dtype == STRATA_QUANT_BF16, vec = packs(d, x_dev, y_dev, bias_dev, state_dev);
     const int64_t per = (int64_t)kThreads * (vec ? (bf16 ? 8 : 4) : 1);
-    const ConvArgs a{x_dev, w_dev, bias_dev, state_dev, y_dev, d.x_stride, d.y_stride, (int)d.channels,
-               (int)((d.channels + per - 1) / per), d.silu};
+    const int64_t blocks = (d.channels + per - 1) / per;
+    // the longest tile that still gives every multiprocessor twelve blocks
+    const int64_t fit = tokens * blocks / (12 * (int64_t)ctx->sm_count) & ~int64_t(7);
+    const int64_t tile = fit < kMinTile ? kMinTile : fit > kMaxTile ? kMaxTile : fit;
+    const ConvArgs a{x_dev, w_dev, bias_dev, state_dev, y_dev, d.x_stride, d.y_stride, (int)d.channels, (int)blocks,
+                     (int)tile, d.silu, (uintptr_t)w_dev % 16 == 0};
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kTile, [&](const SeqTable& t, int64_t tiles) {
+    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, tile, [&](const SeqTable& t, int64_t tiles) {
         if (tiles * a.blocks > kMaxTokens)
             return fail(ctx, STRATA_ERR_INVALID, "short_conv: %lld tiles of %d channel blocks", (long long)tiles,
                         a.blocks);
