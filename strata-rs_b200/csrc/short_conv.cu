@@ -7,10 +7,13 @@
 // Bound by memory: each x is read and each y written once, 2 K flops between
 // them. A thread owns VEC neighbouring channels (one 16-byte access) and walks
 // a tile of tokens with the last K - 1 inputs in registers, so a tile re-reads
-// only its K - 1 rows of halo (from L2). Rows are loaded kAhead at a time, one
-// batch ahead of the one that is computed, so that independent 16-byte loads
-// are always in flight. Tiles are as long as a full GPU allows (their weights
-// and halo are then a small part), one token where sequences have one.
+// only its K - 1 rows of halo (from L2). Rows come kAhead at a time: 16-byte
+// packs by asynchronous copies into shared memory, three batches ahead and
+// without holding registers (each lane copies and reads its own packs, so
+// nothing has to be waited for but its own copies); odd shapes element-wise
+// into registers, one batch ahead. Tiles are as long as a full GPU allows
+// (their weights and halo are then a small part), one token where sequences
+// have one.
 //
 // The state of a sequence is read and replaced by the same thread (the one
 // that has its first tile; the new state is the sequence's last K - 1 inputs,
@@ -24,6 +27,7 @@ namespace {
 
 constexpr int kMinTile = 8, kMaxTile = 64;  // tokens of a tile; at least the longest halo
 constexpr int kThreads = 128;
+constexpr int kRingBatches = 4;
 
 struct ConvArgs {
     const void* x;
@@ -38,12 +42,20 @@ struct ConvArgs {
     int wide_w;            // w can be read in 16-byte packs
 };
 
-// z / (1 + exp(-z)). For bf16 outputs the approximate exponential is far below
-// the rounding; f32 outputs take the accurate one. The quick division is good
-// to 2 ulp, and gives 0 where exp(-z) > 2^126 (the true value is below 1e-36).
+// z / (1 + exp(-z)). For bf16 outputs the approximate exponential (its
+// argument rounds, 2^-24 |z| of the result) and reciprocal (1 ulp) are far below
+// the rounding; f32 outputs take the accurate exponential. The quick division
+// is good to 2 ulp, and gives 0 where exp(-z) > 2^126 (the true value is below
+// 1e-36).
 template <typename T>
 __device__ __forceinline__ float silu(float z) {
-    return __fdividef(z, 1.0f + (sizeof(T) == 2 ? __expf(-z) : expf(-z)));
+    if (sizeof(T) == 2) {
+        float e, r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+        return z * r;
+    }
+    return __fdividef(z, 1.0f + expf(-z));
 }
 
 template <typename T, int VEC>
@@ -53,7 +65,7 @@ __device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&d)[VEC]) {
 }
 
 template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(kThreads, K <= 4 ? 4 : 1)
+__global__ void __launch_bounds__(kThreads, K <= 4 ? (VEC == 8 ? 5 : 6) : 1)
     conv_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
     constexpr int kAhead = VEC == 1 ? 8 : 4;
     const int block = blockIdx.x / a.blocks;
@@ -67,13 +79,30 @@ __global__ void __launch_bounds__(kThreads, K <= 4 ? 4 : 1)
     using P = Pack<T, VEC>;
     using F = Pack<float, VEC>;
 
+    constexpr bool kRing = VEC > 1;
+    __shared__ P ring[kRing ? kRingBatches * kAhead : 1][kRing ? kThreads : 1];
+    P now[kAhead], next[kAhead];
+    // Brings in the rows from t on: into `in`, or batch t / kAhead of the ring.
     auto load = [&](P(&in)[kAhead], int t) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (t + u < n) in[u] = *reinterpret_cast<const P*>(x + (int64_t)(t0 + t + u) * a.x_stride);
+        for (int u = 0; u < kAhead; ++u) {
+            const T* p = x + (int64_t)(t0 + t + u) * a.x_stride;
+            if (t + u < n) {
+                if (kRing)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(
+                                     &ring[kRing ? (t + u) % (kRingBatches * kAhead) : 0][kRing ? threadIdx.x : 0])),
+                                 "l"(p)
+                                 : "memory");
+                else
+                    in[u] = *reinterpret_cast<const P*>(p);
+            }
+        }
+        if (kRing) asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
-    P now[kAhead], next[kAhead];
     load(now, 0);
+    if (kRing)
+#pragma unroll
+        for (int q = 1; q < kRingBatches - 1; ++q) load(now, q * kAhead);
     float w[K][VEC], past[K][VEC];  // past[0 .. K-2]: the inputs before the tile (one spare row keeps K = 1 legal)
     if (K == 4 && a.wide_w) {
 #pragma unroll
@@ -95,20 +124,14 @@ __global__ void __launch_bounds__(kThreads, K <= 4 ? 4 : 1)
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
                 unpack<float, VEC>(*reinterpret_cast<const F*>(st + (int64_t)j * a.channels), past[j]);
-            // the new state: input len - (K - 1) + j, or where that is before the call, old row len + j
+            // the new state: input len - (K - 1) + j, or where that is before the
+            // call, old row len + j, which lies behind row j and is not yet replaced
 #pragma unroll
             for (int j = 0; j < K - 1; ++j) {
                 const int p = len - (K - 1) + j;
                 F out;
-                if (p >= 0) {
-                    unpack<T, VEC>(*reinterpret_cast<const P*>(x + (int64_t)p * a.x_stride), out.v);
-                } else {
-#pragma unroll
-                    for (int m = j + 1; m < K - 1; ++m)
-                        if (m == j + len)
-#pragma unroll
-                            for (int v = 0; v < VEC; ++v) out.v[v] = past[m][v];
-                }
+                if (p >= 0) unpack<T, VEC>(*reinterpret_cast<const P*>(x + (int64_t)p * a.x_stride), out.v);
+                else out = *reinterpret_cast<const F*>(st + (int64_t)(len + j) * a.channels);
                 *reinterpret_cast<F*>(st + (int64_t)j * a.channels) = out;
             }
         } else {  // t0 >= kMinTile > K - 1: the halo lies inside the sequence
@@ -118,7 +141,13 @@ __global__ void __launch_bounds__(kThreads, K <= 4 ? 4 : 1)
         }
     }
     for (int t = 0; t < n; t += kAhead) {
-        load(next, t + kAhead);
+        load(next, t + (kRing ? kRingBatches - 1 : 1) * kAhead);
+        if (kRing) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kRingBatches - 1) : "memory");
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                now[u] = ring[kRing ? (t + u) % (kRingBatches * kAhead) : 0][kRing ? threadIdx.x : 0];
+        }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             P out;
@@ -137,8 +166,9 @@ __global__ void __launch_bounds__(kThreads, K <= 4 ? 4 : 1)
             }
             if (t + u < n) *reinterpret_cast<P*>(y + (int64_t)(t + u) * a.y_stride) = out;
         }
+        if (!kRing)
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+            for (int u = 0; u < kAhead; ++u) now[u] = next[u];
     }
 }
 
