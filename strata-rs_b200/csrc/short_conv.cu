@@ -58,16 +58,21 @@ __device__ __forceinline__ float silu(float z) {
     return __fdividef(z, 1.0f + expf(-z));
 }
 
+// Blocks a multiprocessor runs side by side (up to four taps), as their registers allow.
+constexpr int resident(int vec, bool few) { return few ? (vec == 8 ? 5 : 8) : vec == 8 ? 4 : vec == 4 ? 6 : 8; }
+
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&d)[VEC]) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) d[v] = to_f32(p.v[v]);
 }
 
-template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(kThreads, K <= 4 ? (VEC == 8 ? 5 : 6) : 1)
+// SHORT: for sequences of a few tokens, where registers spent on reading ahead
+// would only keep blocks from running side by side.
+template <typename T, int K, int VEC, bool SHORT>
+__global__ void __launch_bounds__(kThreads, K <= 4 ? resident(VEC, SHORT) : 1)
     conv_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
-    constexpr int kAhead = VEC == 1 ? 8 : 4;
+    constexpr int kAhead = SHORT ? 1 : VEC == 1 ? 8 : 4;
     const int block = blockIdx.x / a.blocks;
     const int c = ((blockIdx.x - block * a.blocks) * kThreads + threadIdx.x) * VEC;
     if (c >= a.channels) return;
@@ -79,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, K <= 4 ? (VEC == 8 ? 5 : 6) : 1)
     using P = Pack<T, VEC>;
     using F = Pack<float, VEC>;
 
-    constexpr bool kRing = VEC > 1;
+    constexpr bool kRing = VEC > 1 && !SHORT;
     __shared__ P ring[kRing ? kRingBatches * kAhead : 1][kRing ? kThreads : 1];
     P now[kAhead], next[kAhead];
     // Brings in the rows from t on: into `in`, or batch t / kAhead of the ring.
@@ -164,26 +169,32 @@ __global__ void __launch_bounds__(kThreads, K <= 4 ? (VEC == 8 ? 5 : 6) : 1)
                 if (K > 1) past[K >= 2 ? K - 2 : 0][v] = in[v];
                 from_f32(out.v[v], a.silu ? silu<T>(z) : z);
             }
-            if (t + u < n) *reinterpret_cast<P*>(y + (int64_t)(t + u) * a.y_stride) = out;
+            if (t + u < n) *reinterpret_cast<P*>(y + u * a.y_stride) = out;
         }
+        y += kAhead * a.y_stride;
         if (!kRing)
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) now[u] = next[u];
     }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHORT>
 void launch_conv(int taps, const ConvArgs& a, const SeqTable& t, unsigned grid, cudaStream_t s) {
     switch (taps) {
-        case 1: conv_kernel<T, 1, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        case 2: conv_kernel<T, 2, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        case 3: conv_kernel<T, 3, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        case 4: conv_kernel<T, 4, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        case 5: conv_kernel<T, 5, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        case 6: conv_kernel<T, 6, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        case 7: conv_kernel<T, 7, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
-        default: conv_kernel<T, 8, VEC><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 1: conv_kernel<T, 1, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 2: conv_kernel<T, 2, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 3: conv_kernel<T, 3, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 4: conv_kernel<T, 4, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 5: conv_kernel<T, 5, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 6: conv_kernel<T, 6, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        case 7: conv_kernel<T, 7, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
+        default: conv_kernel<T, 8, VEC, SHORT><<<grid, kThreads, 0, s>>>(a, t); break;
     }
+}
+template <typename T, int VEC>
+void launch_conv(bool few, int taps, const ConvArgs& a, const SeqTable& t, unsigned grid, cudaStream_t s) {
+    if (few) launch_conv<T, VEC, true>(taps, a, t, grid, s);
+    else launch_conv<T, VEC, false>(taps, a, t, grid, s);
 }
 
 // The 16-byte form needs whole packs in every row and 16-byte rows.
@@ -214,8 +225,11 @@ extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_co
     const bool bf16 = d.dtype == STRATA_QUANT_BF16, vec = packs(d, x_dev, y_dev, bias_dev, state_dev);
     const int64_t per = (int64_t)kThreads * (vec ? (bf16 ? 8 : 4) : 1);
     const int64_t blocks = (d.channels + per - 1) / per;
-    // the longest tile that still gives every multiprocessor twelve blocks
-    const int64_t fit = tokens * blocks / (12 * (int64_t)ctx->sm_count) & ~int64_t(7);
+    // tiles for two whole rounds of the blocks that run side by side
+    const int64_t at_once = 2 * (int64_t)ctx->sm_count * resident(vec ? (bf16 ? 8 : 4) : 1, false);
+    const int64_t share = at_once / blocks > 0 ? at_once / blocks : 1;
+    const int64_t fit = (tokens + share - 1) / share;
+    const bool few = longest <= 4;
     const int64_t tile = fit < kMinTile ? kMinTile : fit > kMaxTile ? kMaxTile : fit;
     const ConvArgs a{x_dev, w_dev, bias_dev, state_dev, y_dev, d.x_stride, d.y_stride, (int)d.channels, (int)blocks,
                      (int)tile, d.silu, (uintptr_t)w_dev % 16 == 0};
@@ -226,10 +240,10 @@ extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_co
             return fail(ctx, STRATA_ERR_INVALID, "short_conv: %lld tiles of %d channel blocks", (long long)tiles,
                         a.blocks);
         const unsigned grid = (unsigned)(tiles * a.blocks);
-        if (bf16 && vec) launch_conv<__nv_bfloat16, 8>((int)d.taps, a, t, grid, s);
-        else if (bf16) launch_conv<__nv_bfloat16, 1>((int)d.taps, a, t, grid, s);
-        else if (vec) launch_conv<float, 4>((int)d.taps, a, t, grid, s);
-        else launch_conv<float, 1>((int)d.taps, a, t, grid, s);
+        if (bf16 && vec) launch_conv<__nv_bfloat16, 8>(few, (int)d.taps, a, t, grid, s);
+        else if (bf16) launch_conv<__nv_bfloat16, 1>(few, (int)d.taps, a, t, grid, s);
+        else if (vec) launch_conv<float, 4>(few, (int)d.taps, a, t, grid, s);
+        else launch_conv<float, 1>(few, (int)d.taps, a, t, grid, s);
         return check_launch(ctx, "short_conv kernel");
     });
 }
