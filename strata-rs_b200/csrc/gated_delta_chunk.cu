@@ -23,15 +23,15 @@
 // where the addition rounds to nearest.
 //
 // Layout of the scan. The columns of S are independent, and products are
-// written transposed: a warp's tile is 16 columns of S as the 16 rows of an
-// m16n8k16 product, S^T K^T, X^T T^T, U^T P^T, U^T K. An accumulator tile is
+// written transposed: a group of warps has 16 columns of S as the 16 rows of
+// m16n8k16 products, S^T K^T, X^T T^T, U^T P^T, U^T K. An accumulator tile is
 // then, split into limbs, the left operand of the next product without leaving
 // the registers, and the right operands (keys, queries, T, P) are the same for
-// all columns: they are staged in shared memory by asynchronous copies one
-// chunk ahead. Two warps share a tile's 16 columns, each with half of k_dim:
-// they exchange their halves of S^T K^T and S^T Q^T through shared memory, and
-// each computes half of the chunk's outputs. A long sequence is bound by one
-// chunk's chain of products and exchanges, a batch by the tensor cores.
+// all columns: they are staged in shared memory by bulk copies one chunk ahead. The warps of a group have a part of k_dim each (Split): they
+// exchange their parts of S^T K^T and S^T Q^T through shared memory, each
+// computes U for itself, and each a part of the chunk's outputs. One sequence
+// is bound by a chunk's chain of products and exchanges, which the split
+// shortens; a batch by the tensor cores, and its blocks take twice the columns.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -41,8 +41,7 @@ namespace strata {
 namespace {
 
 constexpr int kChunk = 32;
-constexpr int kThreads = 128;
-constexpr int kCols = 32;                      // columns of S a scan block holds
+constexpr int kThreads = 128;                  // of a prepare block
 constexpr int kPitchT = kChunk * 2 + 16;       // bytes of a row of T or P: 16-byte steps that no two of 8 rows share
 constexpr int kLimbT = kChunk * kPitchT;
 constexpr int kGates = 4 * kLimbT;             // T hi, T lo, P hi, P lo, then the gate rows
@@ -77,7 +76,7 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& 
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(  // no state but its registers: free to be scheduled
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -95,19 +94,68 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+
+// Copies `bytes` (a multiple of 16) into shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+// Waits for a phase of `bar`, a second at most: false if it has not completed by then.
+__device__ __forceinline__ bool bulk_wait(uint32_t bar, uint32_t parity) {
+    uint64_t begun = 0;
+    for (long long i = 0; i < kSpinLimit; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 255) == 255) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (begun == 0) begun = now;
+            else if (now - begun > 1000000000ull) break;
+        }
+    }
+    return false;
 }
 
 // ---------------------------------------------------------------- prepare
 
+constexpr int kPitchA = kChunk + 4;  // floats of a row of A: 16-byte steps that no two of 8 rows share
+
+// The image, then the two products and the row factors; the warps' scratch
+// takes the image's place once that has been used.
 template <int DK, int LIMBS>
 constexpr int prepare_smem() {
-    return Image<DK, LIMBS>::kBytes + (2 * kChunk * (kChunk + 1) + 2 * kChunk + 4 * kChunk * (kChunk + 4)) * 4;
+    constexpr int scratch = 4 * kChunk * kPitchA * 4, image = Image<DK, LIMBS>::kBytes;
+    return (image > scratch ? image : scratch) + (2 * kChunk * (kChunk + 1) + 2 * kChunk) * 4;
 }
 
-// One block per chunk and key head: limbs of K and Q, K K^T and Q K^T; then
-// one warp per value head of that key head: T and P.
+// 32 values of a row as two limbs of halves, scaled to the row's largest
+// magnitude; returns what undoes the scale.
+__device__ __forceinline__ float store_row(const float (&v)[kChunk], uint8_t* hi_at, uint8_t* lo_at) {
+    float m = 0.0f, up, down;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) m = fmaxf(m, fabsf(v[j]));
+    power_for(m, up, down);
+#pragma unroll
+    for (int j = 0; j < kChunk; j += 8) {
+        uint4 hi, lo;
+        split(v[j] * up, v[j + 1] * up, hi.x, lo.x);
+        split(v[j + 2] * up, v[j + 3] * up, hi.y, lo.y);
+        split(v[j + 4] * up, v[j + 5] * up, hi.z, lo.z);
+        split(v[j + 6] * up, v[j + 7] * up, hi.w, lo.w);
+        *reinterpret_cast<uint4*>(hi_at + j * 2) = hi;
+        *reinterpret_cast<uint4*>(lo_at + j * 2) = lo;
+    }
+    return down;
+}
+
+// One block per chunk and key head: limbs of K and Q, K K^T and Q K^T; then,
+// for each value head of that key head, one warp for T and one for P.
 template <typename T, int DK, int LIMBS>
 __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab,
                                                                  uint8_t* __restrict__ images,
@@ -115,12 +163,13 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
     using I = Image<DK, LIMBS>;
     constexpr int PER = DK / 32;  // elements of a row a lane holds
     extern __shared__ __align__(16) uint8_t smem[];
-    float(*kk)[kChunk + 1] = reinterpret_cast<float(*)[kChunk + 1]>(smem + I::kBytes);
+    float(*kk)[kChunk + 1] =
+        reinterpret_cast<float(*)[kChunk + 1]>(smem + prepare_smem<DK, LIMBS>() - (2 * kChunk * (kChunk + 1) + 2 * kChunk) * 4);
     float(*qk)[kChunk + 1] = kk + kChunk;
     float* fk = &qk[kChunk][0];  // what a row of limbs is to be multiplied with
     float* fq = fk + kChunk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float(*A)[kChunk + 4] = reinterpret_cast<float(*)[kChunk + 4]>(fq + kChunk) + warp * kChunk;
+    float(*A)[kPitchA] = reinterpret_cast<float(*)[kPitchA]>(smem) + warp * kChunk;
     const int tile = blockIdx.x / a.k_heads, hk = blockIdx.x - tile * a.k_heads;
     const Seq seq = sequence_of_tile(tab, tile);
     const int t0 = (tile - seq.tile0) * kChunk, n = min(kChunk, seq.len - t0);
@@ -218,7 +267,8 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
     }
     __syncthreads();
     const int per = a.v_heads / a.k_heads;
-    for (int m = warp; m < per; m += kThreads / 32) {
+    for (int task = warp; task < 2 * per; task += kThreads / 32) {
+        const int m = task >> 1;
         const int h = a.tiled ? hk + m * a.k_heads : hk * per + m;
         float g = 0.0f, beta = 0.0f;
         if (lane < n) {
@@ -234,67 +284,76 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             const double up = __shfl_up_sync(0xFFFFFFFFu, G, o);
             if (lane >= o) G += up;
         }
-        const double end = __shfl_sync(0xFFFFFFFFu, G, 31);
         uint8_t* image = images_t + ((int64_t)tile * a.v_heads + h) * kImageT;
-        float scale_t = 0.0f, scale_p = 0.0f;
-        __syncwarp();
-        for (int i = 0; i < kChunk; ++i) {
-            const double Gi = __shfl_sync(0xFFFFFFFFu, G, i);
-            const float bi = __shfl_sync(0xFFFFFFFFu, beta, i);
-            const float e = lane <= i ? expf((float)(Gi - G)) : 0.0f;
-            A[i][lane] = lane < i ? bi * e * kk[i][lane] : 0.0f;
-            const float p = lane <= i ? e * qk[i][lane] : 0.0f;
-            float mx = fabsf(p), up, down;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-            power_for(mx, up, down);
-            const __half hi = __float2half_rn(p * up), lo = __float2half_rn(p * up - __half2float(hi));
-            __half* at = reinterpret_cast<__half*>(image + 2 * kLimbT + i * kPitchT) + lane;
-            at[0] = hi;
-            at[kLimbT / 2] = lo;
-            if (lane == i) scale_p = down;
-        }
-        __syncwarp();
-        // T = (I + A)^-1, a column a lane, row by row
-        float t[kChunk];
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            float acc = lane == i ? 1.0f : 0.0f;
-#pragma unroll
-            for (int j = 0; j < i; ++j) acc = fmaf(-A[i][j], t[j], acc);
-            t[i] = acc;
-        }
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            float mx = fabsf(t[i]), up, down;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-            power_for(mx, up, down);
-            const __half hi = __float2half_rn(t[i] * up), lo = __float2half_rn(t[i] * up - __half2float(hi));
-            __half* at = reinterpret_cast<__half*>(image + i * kPitchT) + lane;
-            at[0] = hi;
-            at[kLimbT / 2] = lo;
-            if (lane == i) scale_t = down;
-        }
         float* out = reinterpret_cast<float*>(image + kGates) + lane;
-        const float before = expf((float)G), after = expf((float)(end - G));
-        out[kBeta * kChunk] = beta;
-        out[kXk * kChunk] = beta * before * fk[lane];
-        out[kOq * kChunk] = before * fq[lane];
-        out[kDown * kChunk] = after * fk[lane];
-        out[kScaleT * kChunk] = scale_t;
-        out[kScaleP * kChunk] = scale_p;
-        out[kTotal * kChunk] = expf((float)end);
+        float v[kChunk];  // a row a lane: beta_i e^{G_i - G_j} k_i . k_j, or e^{G_i - G_j} q_i . k_j
+        const float(*products)[kChunk + 1] = task & 1 ? qk : kk;
+        const int diagonal = task & 1 ? lane : lane - 1;  // the row's last column
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            const double Gj = __shfl_sync(0xFFFFFFFFu, G, j);
+            v[j] = j <= diagonal ? expf((float)(G - Gj)) * products[lane][j] : 0.0f;
+        }
+        if (task & 1) {
+            const float down = store_row(v, image + 2 * kLimbT + lane * kPitchT, image + 3 * kLimbT + lane * kPitchT);
+            out[kScaleP * kChunk] = down;
+            const double end = __shfl_sync(0xFFFFFFFFu, G, 31);
+            const float before = expf((float)G), after = expf((float)(end - G));
+            out[kBeta * kChunk] = beta;
+            out[kXk * kChunk] = beta * before * fk[lane];
+            out[kOq * kChunk] = before * fq[lane];
+            out[kDown * kChunk] = after * fk[lane];
+            out[kTotal * kChunk] = expf((float)end);
+            continue;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kChunk; j += 4)
+            *reinterpret_cast<float4*>(&A[lane][j]) =
+                make_float4(-beta * v[j], -beta * v[j + 1], -beta * v[j + 2], -beta * v[j + 3]);
+        __syncwarp();
+        // T = (I + A)^-1, a column a lane, row by row (A holds its negative)
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            float acc[2] = {lane == i ? 1.0f : 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j + 4 <= i; j += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(&A[i][j]);
+                acc[0] = fmaf(w.x, v[j], acc[0]), acc[1] = fmaf(w.y, v[j + 1], acc[1]);
+                acc[0] = fmaf(w.z, v[j + 2], acc[0]), acc[1] = fmaf(w.w, v[j + 3], acc[1]);
+            }
+#pragma unroll
+            for (int j = i & ~3; j < i; ++j) acc[j & 1] = fmaf(A[i][j], v[j], acc[j & 1]);
+            v[i] = acc[0] + acc[1];
+        }
+        // and back to a row a lane
+        __syncwarp();
+        float* flat = &A[0][0];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) flat[i * (kChunk + 1) + lane] = v[i];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) v[j] = flat[lane * (kChunk + 1) + j];
+        out[kScaleT * kChunk] = store_row(v, image + lane * kPitchT, image + kLimbT + lane * kPitchT);
     }
 }
 
 // ------------------------------------------------------------------- scan
 
-constexpr int kExchange = 24;  // floats a lane hands to the warp with the other half: 16 of S^T K^T, 8 of S^T Q^T
+// How a scan block is laid out: GROUPS groups of kWarps warps, 16 columns a
+// group, DK / kWarps rows of S a warp.
+template <int DK, int GROUPS>
+struct Split {
+    static constexpr int kWarps = 2;
+    static constexpr int kThreads = 32 * kWarps * GROUPS, kCols = 16 * GROUPS;
+    static constexpr int kRows = DK / kWarps, kTiles = 4 / kWarps;  // token tiles whose outputs a warp writes
+    static constexpr int kExchange = 32;  // floats a lane hands on: 16 of S^T K^T, 16 of S^T Q^T
+};
 
-template <int DK, int LIMBS>
+template <int DK, int LIMBS, int GROUPS>
 constexpr int scan_smem() {
-    return 2 * (Image<DK, LIMBS>::kBytes + kImageT) + 4 * kExchange * 32 * 4;
+    using L = Split<DK, GROUPS>;
+    return 2 * (Image<DK, LIMBS>::kBytes + kImageT) + L::kThreads * L::kExchange * 4;
 }
 
 // The largest magnitude of a row of the warp's tile: rows lie across 4 lanes.
@@ -325,16 +384,18 @@ __device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N /
     }
 }
 
-template <typename T, int DK, int LIMBS>
-__global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab,
-                                                                 const uint8_t* __restrict__ images,
-                                                                 const uint8_t* __restrict__ images_t) {
+template <typename T, int DK, int LIMBS, int GROUPS>
+__global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
+    delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab, const uint8_t* __restrict__ images,
+                      const uint8_t* __restrict__ images_t, int* err) {
     using I = Image<DK, LIMBS>;
-    constexpr int HALF = DK / 2, NT = HALF / 8, KS = HALF / 16;
+    using L = Split<DK, GROUPS>;
+    constexpr int ROWS = L::kRows, NT = ROWS / 8, KS = ROWS / 16, TILES = L::kTiles;
     constexpr int kStage = I::kBytes + kImageT;
     extern __shared__ __align__(16) uint8_t smem[];
     float* ex = reinterpret_cast<float*>(smem + 2 * kStage);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = warp / L::kWarps, part = warp % L::kWarps;
     int b = blockIdx.x;
     const int cb = b % a.col_blocks;
     b /= a.col_blocks;
@@ -342,22 +403,26 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs
     const Seq seq = sequence_at(tab, b / a.v_heads);
     const int hk = key_head(a, h);
     const int chunks = (seq.len + kChunk - 1) / kChunk;
-    const int j0 = cb * kCols + (warp >> 1) * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
+    const int j0 = cb * L::kCols + group * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
     const bool in0 = j0 < a.v_dim, in1 = j1 < a.v_dim;
     const int tc = (lane & 3) * 2;
-    const int d0 = half * HALF + tc;  // its first row of S
+    const int d0 = part * ROWS + tc;  // its first row of S
 
-    auto stage = [&](int c) {
+    __shared__ __align__(8) uint64_t arrived[2];
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_addr(&arrived[i])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    auto stage = [&](int c) {  // by one thread
         const int64_t tile = seq.tile0 + c;
-        const uint8_t* src = images + (tile * a.k_heads + hk) * I::kBytes;
-        const uint8_t* src_t = images_t + (tile * a.v_heads + h) * kImageT;
-        const uint32_t dst = shared_addr(smem + (c & 1) * kStage);
-        for (int i = threadIdx.x; i < I::kBytes / 16; i += kThreads) copy16(dst + i * 16, src + i * 16);
-        for (int i = threadIdx.x; i < kImageT / 16; i += kThreads)
-            copy16(dst + I::kBytes + i * 16, src_t + i * 16);
-        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        const uint32_t dst = shared_addr(smem + (c & 1) * kStage), bar = shared_addr(&arrived[c & 1]);
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kStage) : "memory");
+        bulk_copy(dst, images + (tile * a.k_heads + hk) * I::kBytes, I::kBytes, bar);
+        bulk_copy(dst + I::kBytes, images_t + (tile * a.v_heads + h) * kImageT, kImageT, bar);
     };
-    stage(0);
+    if (threadIdx.x == 0) stage(0);
 
     float* S = a.state + ((int64_t)seq.slot * a.v_heads + h) * a.k_dim * a.v_dim;
     float s[NT][4];
@@ -385,20 +450,26 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs
 
     const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
     for (int c = 0; c < chunks; ++c) {
-        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-        __syncthreads();  // the chunk is staged, and every warp is done with the one before
-        if (c + 1 < chunks) stage(c + 1);
+        bool there = bulk_wait(shared_addr(&arrived[c & 1]), (c >> 1) & 1);
+        // the chunk is staged, and every warp is done with the one before
+        if (__syncthreads_or(!there)) {
+            // a copy that does not come: wait for it once more, report, leave the state as it was
+            if (!there) bulk_wait(shared_addr(&arrived[c & 1]), (c >> 1) & 1);
+            if (threadIdx.x == 0) atomicExch(err, 1);
+            return;
+        }
+        if (threadIdx.x == 0 && c + 1 < chunks) stage(c + 1);
         const uint32_t base = shared_addr(smem + (c & 1) * kStage);
         const float* gate = reinterpret_cast<const float*>(smem + (c & 1) * kStage + I::kBytes + kGates);
 
-        // this half's part of S^T K^T and S^T Q^T
-        float y[4][4] = {}, o[4][4] = {};
+        // this warp's part of S^T K^T and S^T Q^T
         {
+            float y[4][4] = {}, o[4][4] = {};
             float y2[4][4] = {}, o2[4][4] = {};
             uint32_t hi[KS][4], lo[KS][4];
             float down[2];
             limbs<NT>(s, hi, lo, down);
-            const uint32_t at = base + lane_b * I::kPitch + half * HALF * 2 + ((lane >> 3) & 1) * 16;
+            const uint32_t at = base + lane_b * I::kPitch + part * ROWS * 2 + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -424,34 +495,39 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs
                         mma(o2[2 * p + 1], hi[ks], bq[2], bq[3]);
                     }
                 }
-            float* mine = ex + warp * kExchange * 32 + lane;
+            float* mine = ex + warp * L::kExchange * 32 + lane;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    y[t][r] = (y[t][r] + y2[t][r]) * down[r >> 1];
-                    o[t][r] = (o[t][r] + o2[t][r]) * down[r >> 1];
-                    mine[(t * 4 + r) * 32] = y[t][r];
-                    // the other warp's tokens
-                    if ((t >> 1) != half) mine[(16 + (t & 1) * 4 + r) * 32] = o[t][r];
+                    mine[(t * 4 + r) * 32] = (y[t][r] + y2[t][r]) * down[r >> 1];
+                    mine[(16 + t * 4 + r) * 32] = (o[t][r] + o2[t][r]) * down[r >> 1];
                 }
         }
-        __syncthreads();
-        const float* other = ex + (warp ^ 1) * kExchange * 32 + lane;
-        float x[4][4], out[2][4];
+        // the warps of the group only
+        asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(L::kWarps * 32) : "memory");
+        // all parts in the order of the warps, so that every warp has the same bits
+        const float* parts = ex + group * L::kWarps * L::kExchange * 32 + lane;
+        float x[4][4], out[TILES][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = t * 8 + tc + (r & 1);
-                const float yy = y[t][r] + other[(t * 4 + r) * 32];
+                float yy = parts[(t * 4 + r) * 32];
+#pragma unroll
+                for (int q = 1; q < L::kWarps; ++q) yy += parts[(q * L::kExchange + t * 4 + r) * 32];
                 x[t][r] = gate[kBeta * kChunk + i] * v[t][r] - gate[kXk * kChunk + i] * yy;
             }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int k = 0; k < TILES; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                out[t][r] = (half ? o[2 + t][r] : o[t][r]) + other[(16 + t * 4 + r) * 32];
+            for (int r = 0; r < 4; ++r) {
+                const float* at = parts + (16 + (part * TILES + k) * 4 + r) * 32;
+                out[k][r] = at[0];
+#pragma unroll
+                for (int q = 1; q < L::kWarps; ++q) out[k][r] += at[q * L::kExchange * 32];
+            }
         if (c + 1 < chunks) fetch(c + 1);
 
         const uint32_t t_at = base + I::kBytes + lane_b * kPitchT + ((lane >> 3) & 1) * 16;
@@ -481,47 +557,18 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs
                 for (int r = 0; r < 4; ++r)
                     u[t][r] = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleT * kChunk + t * 8 + tc + (r & 1)]);
         }
-        // this warp's half of the outputs
-        {
-            uint32_t hi[2][4], lo[2][4];
-            float down[2], c1[2][4] = {}, c2[2][4] = {};
-            limbs<4>(u, hi, lo, down);
-            const uint32_t p_at = t_at + 2 * kLimbT + half * 16 * kPitchT;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks > half) break;
-                uint32_t bh[4], bl[4];
-                ldmatrix(bh, p_at + ks * 32);
-                ldmatrix(bl, p_at + kLimbT + ks * 32);
-                mma(c1[0], hi[ks], bh[0], bh[1]);
-                mma(c1[1], hi[ks], bh[2], bh[3]);
-                mma(c2[0], lo[ks], bh[0], bh[1]);
-                mma(c2[1], lo[ks], bh[2], bh[3]);
-                mma(c2[0], hi[ks], bl[0], bl[1]);
-                mma(c2[1], hi[ks], bl[2], bl[3]);
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int k = half * 16 + t * 8 + tc + (r & 1), i = c * kChunk + k;
-                    const float y1 = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleP * kChunk + k]);
-                    const float res = fmaf(gate[kOq * kChunk + k], out[t][r], y1);
-                    if (i < seq.len && (r < 2 ? in0 : in1))
-                        from_f32(O[(int64_t)i * a.o_stride + (r < 2 ? j0 : j1)], res);
-                }
-        }
         // S <- e^{G_C} S + (rows of U scaled to the chunk's end) K
         {
+            float e[4][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) u[t][r] *= gate[kDown * kChunk + t * 8 + tc + (r & 1)];
+                for (int r = 0; r < 4; ++r) e[t][r] = u[t][r] * gate[kDown * kChunk + t * 8 + tc + (r & 1)];
             uint32_t hi[2][4], lo[2][4];
             float down[2];
-            limbs<4>(u, hi, lo, down);
+            limbs<4>(e, hi, lo, down);
             const float total = gate[kTotal * kChunk];
-            const uint32_t at = base + (lane & 15) * I::kPitch + half * HALF * 2 + (lane >> 4) * 16;
+            const uint32_t at = base + (lane & 15) * I::kPitch + part * ROWS * 2 + (lane >> 4) * 16;
 #pragma unroll
             for (int p = 0; p < NT / 2; ++p) {
                 float c1[2][4] = {}, c2[2][4] = {};
@@ -545,6 +592,36 @@ __global__ void __launch_bounds__(kThreads, 2) delta_scan_kernel(const DeltaArgs
                     for (int r = 0; r < 4; ++r)
                         s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], (c1[t][r] + c2[t][r]) * down[r >> 1]);
             }
+        }
+        // the outputs of this warp's tokens (columns of P behind them are zero)
+        {
+            uint32_t hi[2][4], lo[2][4];
+            float down[2];
+            limbs<4>(u, hi, lo, down);
+            const uint32_t p_at = t_at + 2 * kLimbT + part * TILES * 8 * kPitchT;
+            float c1[2][4] = {}, c2[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                uint32_t bh[4], bl[4];  // two tiles of tokens; the second is another warp's where a warp has one
+                ldmatrix(bh, p_at + ks * 32);
+                ldmatrix(bl, p_at + kLimbT + ks * 32);
+#pragma unroll
+                for (int k = 0; k < TILES; ++k) {
+                    mma(c1[k], hi[ks], bh[2 * k], bh[2 * k + 1]);
+                    mma(c2[k], lo[ks], bh[2 * k], bh[2 * k + 1]);
+                    mma(c2[k], hi[ks], bl[2 * k], bl[2 * k + 1]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int k = (part * TILES + t) * 8 + tc + (r & 1), i = c * kChunk + k;
+                    const float y1 = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleP * kChunk + k]);
+                    const float res = fmaf(gate[kOq * kChunk + k], out[t][r], y1);
+                    if (i < seq.len && (r < 2 ? in0 : in1))
+                        from_f32(O[(int64_t)i * a.o_stride + (r < 2 ? j0 : j1)], res);
+                }
         }
     }
 #pragma unroll
@@ -617,24 +694,40 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
     return STRATA_OK;
 }
 
-template <typename T, int DK, int LIMBS>
-int enqueue(strata_ctx* ctx, const strata_gated_delta& d, DeltaArgs a, uint8_t* work, cudaStream_t s) {
-    auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
-    auto scan = delta_scan_kernel<T, DK, LIMBS>;
-    constexpr int sp = prepare_smem<DK, LIMBS>(), ss = scan_smem<DK, LIMBS>();
-    cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, sp);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ss);
+template <typename T, int DK, int LIMBS, int GROUPS>
+int enqueue_scan(strata_ctx* ctx, DeltaArgs a, const SeqTable& t, const uint8_t* images, const uint8_t* images_t,
+                 cudaStream_t s) {
+    using L = Split<DK, GROUPS>;
+    auto scan = delta_scan_kernel<T, DK, LIMBS, GROUPS>;
+    constexpr int smem = scan_smem<DK, LIMBS, GROUPS>();
+    const cudaError_t e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
-    a.col_blocks = (a.v_dim + kCols - 1) / kCols;
+    a.col_blocks = (a.v_dim + L::kCols - 1) / L::kCols;
+    const int64_t grid = (int64_t)t.n * a.v_heads * a.col_blocks;
+    if (grid > kMaxTokens) return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %d sequences of %d heads", t.n, a.v_heads);
+    scan<<<(unsigned)grid, L::kThreads, smem, s>>>(a, t, images, images_t, ctx->err_dev);
+    return check_launch(ctx, "gated_delta scan kernel");
+}
+
+template <typename T, int DK, int LIMBS>
+int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
+    auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
+    constexpr int smem = prepare_smem<DK, LIMBS>();
+    const cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
     const uint64_t keys = chunk_bytes(d).keys;
     return plan_chunks(d, [&](const SeqTable& t, int64_t tiles) {
-        const int64_t gp = tiles * a.k_heads, gs = (int64_t)t.n * a.v_heads * a.col_blocks;
-        if (gp > kMaxTokens || gs > kMaxTokens)
-            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.v_heads);
+        const int64_t grid = tiles * a.k_heads;
+        if (grid > kMaxTokens)
+            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.k_heads);
         uint8_t* images_t = work + keys * (uint64_t)tiles;
-        prepare<<<(unsigned)gp, kThreads, sp, s>>>(a, t, work, images_t);
-        scan<<<(unsigned)gs, kThreads, ss, s>>>(a, t, work, images_t);
-        return check_launch(ctx, "gated_delta chunk kernels");
+        prepare<<<(unsigned)grid, kThreads, smem, s>>>(a, t, work, images_t);
+        int rc = check_launch(ctx, "gated_delta prepare kernel");
+        if (rc) return rc;
+        // narrow blocks while they fit the multiprocessors side by side
+        const int64_t narrow = (int64_t)t.n * a.v_heads * ((a.v_dim + 31) / 32);
+        return narrow <= ctx->sm_count ? enqueue_scan<T, DK, LIMBS, 2>(ctx, a, t, work, images_t, s)
+                                       : enqueue_scan<T, DK, LIMBS, 4>(ctx, a, t, work, images_t, s);
     });
 }
 
