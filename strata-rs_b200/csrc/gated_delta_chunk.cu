@@ -16,9 +16,9 @@
 //
 // Precision. The products run on the tensor cores as f16 limbs: x 2^e = hi + lo
 // with the exponent e taken per row from the row's largest magnitude, so a
-// limb pair carries 22 bits of it, and hi hi + hi lo + lo hi is summed in f32
-// (the two small products in accumulators of their own). That keeps f32-like
-// results at f16 rate; plain tf32 would carry 11 bits. Keys and queries given
+// limb pair carries 22 bits of it, and lo hi + hi lo + hi hi is summed in f32,
+// the two small products first. That keeps f32-like results at f16 rate; plain
+// tf32 would carry 11 bits. Keys and queries given
 // as bf16 are exact in one limb. The scan adds to S outside the tensor core,
 // where the addition rounds to nearest.
 //
@@ -27,11 +27,11 @@
 // m16n8k16 products, S^T K^T, X^T T^T, U^T P^T, U^T K. An accumulator tile is
 // then, split into limbs, the left operand of the next product without leaving
 // the registers, and the right operands (keys, queries, T, P) are the same for
-// all columns: they are staged in shared memory by bulk copies one chunk ahead. The warps of a group have a part of k_dim each (Split): they
-// exchange their parts of S^T K^T and S^T Q^T through shared memory, each
-// computes U for itself, and each a part of the chunk's outputs. One sequence
-// is bound by a chunk's chain of products and exchanges, which the split
-// shortens; a batch by the tensor cores, and its blocks take twice the columns.
+// all columns: they are staged in shared memory by bulk copies one chunk ahead.
+// Two warps of a group hold S, half of k_dim each, and follow the chain from
+// chunk to chunk; they exchange their halves of S^T K^T through shared memory.
+// The other two take S's limbs and U from shared memory and compute half of the
+// chunk's outputs each, off the chain and on the other half of the tensor time.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -340,20 +340,32 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
 
 // ------------------------------------------------------------------- scan
 
-// How a scan block is laid out: GROUPS groups of kWarps warps, 16 columns a
-// group, DK / kWarps rows of S a warp.
-template <int DK, int GROUPS>
-struct Split {
-    static constexpr int kWarps = 2;
-    static constexpr int kThreads = 32 * kWarps * GROUPS, kCols = 16 * GROUPS;
-    static constexpr int kRows = DK / kWarps, kTiles = 4 / kWarps;  // token tiles whose outputs a warp writes
-    static constexpr int kExchange = 32;  // floats a lane hands on: 16 of S^T K^T, 16 of S^T Q^T
+// A scan block: kGroups groups of 16 columns of S, each with two warps for S
+// and two for the outputs.
+constexpr int kGroups = 2, kScanThreads = kGroups * 4 * 32, kCols = kGroups * 16;
+constexpr int kStages = 3;  // the chunk being read, the next, and the one whose outputs are still to come
+
+// What a group's warps hand on: halves of S^T K^T, S's limbs and their row
+// factors, U.
+template <int DK>
+struct Handoff {
+    float4 y[2][4][32];
+    uint4 hi[DK / 16][32], lo[DK / 16][32];
+    float2 down[2][32];
+    float4 u[4][32];
 };
 
-template <int DK, int LIMBS, int GROUPS>
+template <int DK, int LIMBS>
 constexpr int scan_smem() {
-    using L = Split<DK, GROUPS>;
-    return 2 * (Image<DK, LIMBS>::kBytes + kImageT) + L::kThreads * L::kExchange * 4;
+    return kStages * (Image<DK, LIMBS>::kBytes + kImageT) + 2 * kGroups * (int)sizeof(Handoff<DK>);
+}
+
+// Named barriers of a group: `threads` of them arrive in all.
+__device__ __forceinline__ void group_sync(int id, int threads) {
+    asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void group_arrive(int id, int threads) {
+    asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
 }
 
 // The largest magnitude of a row of the warp's tile: rows lie across 4 lanes.
@@ -384,18 +396,23 @@ __device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N /
     }
 }
 
-template <typename T, int DK, int LIMBS, int GROUPS>
-__global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
+template <typename T, int DK, int LIMBS>
+__global__ void __launch_bounds__(kScanThreads, 1)
     delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab, const uint8_t* __restrict__ images,
                       const uint8_t* __restrict__ images_t, int* err) {
     using I = Image<DK, LIMBS>;
-    using L = Split<DK, GROUPS>;
-    constexpr int ROWS = L::kRows, NT = ROWS / 8, KS = ROWS / 16, TILES = L::kTiles;
+    constexpr int HALF = DK / 2, NT = HALF / 8, KS = HALF / 16;
     constexpr int kStage = I::kBytes + kImageT;
     extern __shared__ __align__(16) uint8_t smem[];
-    float* ex = reinterpret_cast<float*>(smem + 2 * kStage);
+    __shared__ __align__(8) uint64_t arrived[kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = warp / L::kWarps, part = warp % L::kWarps;
+    // the warps of S first, then those of the outputs: one of each a scheduler
+    const bool holds = warp < 2 * kGroups;
+    const int group = (warp >> 1) % kGroups, half = warp & 1;
+    Handoff<DK>* const hands = reinterpret_cast<Handoff<DK>*>(smem + kStages * kStage) + group * 2;
+    // Barriers: two for chunks whose outputs are written, then a group's: halves
+    // of S^T K^T, S's limbs handed on, U handed on.
+    const int bar_done = 1, bar_y = 3 + group * 3, bar_s = bar_y + 1, bar_u = bar_y + 2;
     int b = blockIdx.x;
     const int cb = b % a.col_blocks;
     b /= a.col_blocks;
@@ -403,27 +420,126 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
     const Seq seq = sequence_at(tab, b / a.v_heads);
     const int hk = key_head(a, h);
     const int chunks = (seq.len + kChunk - 1) / kChunk;
-    const int j0 = cb * L::kCols + group * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
+    const int j0 = cb * kCols + group * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
     const bool in0 = j0 < a.v_dim, in1 = j1 < a.v_dim;
     const int tc = (lane & 3) * 2;
-    const int d0 = part * ROWS + tc;  // its first row of S
+    const int d0 = half * HALF + tc;  // its first row of S
 
-    __shared__ __align__(8) uint64_t arrived[2];
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kStages; ++i)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_addr(&arrived[i])) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     auto stage = [&](int c) {  // by one thread
         const int64_t tile = seq.tile0 + c;
-        const uint32_t dst = shared_addr(smem + (c & 1) * kStage), bar = shared_addr(&arrived[c & 1]);
+        const uint32_t dst = shared_addr(smem + (c % kStages) * kStage), bar = shared_addr(&arrived[c % kStages]);
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kStage) : "memory");
         bulk_copy(dst, images + (tile * a.k_heads + hk) * I::kBytes, I::kBytes, bar);
         bulk_copy(dst + I::kBytes, images_t + (tile * a.v_heads + h) * kImageT, kImageT, bar);
     };
     if (threadIdx.x == 0) stage(0);
+    // Waits for chunk c's copy. Where one does not come (a second is long past),
+    // the thread goes on without waiting, so that no other is left behind at a
+    // barrier, and the call is reported as timed out.
+    bool there = true;
+    auto wait = [&](int c) {
+        if (there) there = bulk_wait(shared_addr(&arrived[c % kStages]), (c / kStages) & 1);
+        if (!there) atomicExch(err, 1);
+    };
+    const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
+    const uint32_t half_b = ((lane >> 3) & 1) * 16;             // and its half of a row
 
+    if (!holds) {  // ---- outputs of tokens half * 16 .. + 15
+        T* O = static_cast<T*>(a.o) + (int64_t)seq.row * a.o_stride + (int64_t)h * a.v_dim;
+        for (int c = 0; c < chunks; ++c) {
+            wait(c);
+            const uint8_t* image = smem + (c % kStages) * kStage;
+            const Handoff<DK>& hand = hands[c & 1];
+            const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
+            const uint32_t q_at = shared_addr(image) + LIMBS * I::kLimb + (half * 16 + lane_b) * I::kPitch + half_b;
+            float out[2][4] = {};
+            group_sync(bar_s, 128);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // the two halves of k_dim, each with its own row factors
+                float o1[2][4] = {};
+                uint32_t hi[KS][4];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint4 h4 = hand.hi[k * KS + ks][lane], l4 = hand.lo[k * KS + ks][lane];
+                    const uint32_t lo[4] = {l4.x, l4.y, l4.z, l4.w};
+                    hi[ks][0] = h4.x, hi[ks][1] = h4.y, hi[ks][2] = h4.z, hi[ks][3] = h4.w;
+                    uint32_t bq[4];
+                    if (LIMBS == 2) {
+                        ldmatrix(bq, q_at + I::kLimb + (k * KS + ks) * 32);
+                        mma(o1[0], hi[ks], bq[0], bq[1]);
+                        mma(o1[1], hi[ks], bq[2], bq[3]);
+                    }
+                    ldmatrix(bq, q_at + (k * KS + ks) * 32);
+                    mma(o1[0], lo, bq[0], bq[1]);
+                    mma(o1[1], lo, bq[2], bq[3]);
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    uint32_t bq[4];
+                    ldmatrix(bq, q_at + (k * KS + ks) * 32);
+                    mma(o1[0], hi[ks], bq[0], bq[1]);
+                    mma(o1[1], hi[ks], bq[2], bq[3]);
+                }
+                const float2 down = hand.down[k][lane];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) out[t][r] = fmaf(o1[t][r], r < 2 ? down.x : down.y, out[t][r]);
+            }
+            group_sync(bar_u, 128);
+            float u[4][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float4 w = hand.u[t][lane];
+                u[t][0] = w.x, u[t][1] = w.y, u[t][2] = w.z, u[t][3] = w.w;
+            }
+            uint32_t hi[2][4], lo[2][4];
+            float down[2], c1[2][4] = {};
+            limbs<4>(u, hi, lo, down);
+            const uint32_t p_at =
+                shared_addr(image) + I::kBytes + 2 * kLimbT + (half * 16 + lane_b) * kPitchT + half_b;
+            uint32_t bh[2][4], bl[4];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {  // later tokens' columns of P are zero
+                ldmatrix(bh[ks], p_at + ks * 32);
+                ldmatrix(bl, p_at + kLimbT + ks * 32);
+                mma(c1[0], lo[ks], bh[ks][0], bh[ks][1]);
+                mma(c1[1], lo[ks], bh[ks][2], bh[ks][3]);
+                mma(c1[0], hi[ks], bl[0], bl[1]);
+                mma(c1[1], hi[ks], bl[2], bl[3]);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                mma(c1[0], hi[ks], bh[ks][0], bh[ks][1]);
+                mma(c1[1], hi[ks], bh[ks][2], bh[ks][3]);
+            }
+            T* row = O + (int64_t)(c * kChunk + half * 16 + tc) * a.o_stride;
+            const int left = seq.len - (c * kChunk + half * 16 + tc);  // tokens from the lane's first
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float2 sp = *reinterpret_cast<const float2*>(gate + kScaleP * kChunk + half * 16 + t * 8 + tc);
+                const float2 oq = *reinterpret_cast<const float2*>(gate + kOq * kChunk + half * 16 + t * 8 + tc);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float y1 = c1[t][r] * (down[r >> 1] * (r & 1 ? sp.y : sp.x));
+                    const float res = fmaf(r & 1 ? oq.y : oq.x, out[t][r], y1);
+                    if (t * 8 + (r & 1) < left && (r < 2 ? in0 : in1))
+                        from_f32(row[(t * 8 + (r & 1)) * a.o_stride + (r < 2 ? j0 : j1)], res);
+                }
+            }
+            // the stage and the handoff may be written again (two chunks on)
+            if (c + 2 < chunks) group_arrive(bar_done + (c & 1), kScanThreads);
+        }
+        return;
+    }
+
+    // ---- the state
     float* S = a.state + ((int64_t)seq.slot * a.v_heads + h) * a.k_dim * a.v_dim;
     float s[NT][4];
 #pragma unroll
@@ -434,194 +550,164 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
             s[t][r] = d < a.k_dim && j < a.v_dim ? S[(int64_t)d * a.v_dim + j] : 0.0f;
         }
     const T* V = static_cast<const T*>(a.v) + (int64_t)seq.row * a.v_stride + (int64_t)h * a.v_dim;
-    T* O = static_cast<T*>(a.o) + (int64_t)seq.row * a.o_stride + (int64_t)h * a.v_dim;
     float v[4][4];
+    V += (int64_t)tc * a.v_stride;
     auto fetch = [&](int c) {
+        const T* row = V + (int64_t)c * kChunk * a.v_stride;
+        const int left = seq.len - c * kChunk - tc;  // tokens from the lane's first
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = c * kChunk + t * 8 + tc + (r & 1);
-                const bool in = i < seq.len && (r < 2 ? in0 : in1);
-                v[t][r] = in ? to_f32(V[(int64_t)i * a.v_stride + (r < 2 ? j0 : j1)]) : 0.0f;
+                const bool in = t * 8 + (r & 1) < left && (r < 2 ? in0 : in1);
+                v[t][r] = in ? to_f32(row[(t * 8 + (r & 1)) * a.v_stride + (r < 2 ? j0 : j1)]) : 0.0f;
             }
     };
     fetch(0);
-
-    const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
     for (int c = 0; c < chunks; ++c) {
-        bool there = bulk_wait(shared_addr(&arrived[c & 1]), (c >> 1) & 1);
-        // the chunk is staged, and every warp is done with the one before
-        if (__syncthreads_or(!there)) {
-            // a copy that does not come: wait for it once more, report, leave the state as it was
-            if (!there) bulk_wait(shared_addr(&arrived[c & 1]), (c >> 1) & 1);
-            if (threadIdx.x == 0) atomicExch(err, 1);
-            return;
-        }
-        if (threadIdx.x == 0 && c + 1 < chunks) stage(c + 1);
-        const uint32_t base = shared_addr(smem + (c & 1) * kStage);
-        const float* gate = reinterpret_cast<const float*>(smem + (c & 1) * kStage + I::kBytes + kGates);
-
-        // this warp's part of S^T K^T and S^T Q^T
-        {
-            float y[4][4] = {}, o[4][4] = {};
-            float y2[4][4] = {}, o2[4][4] = {};
+        // chunk c - 2 is written out, so its stage can take chunk c + 1 and its handoff this chunk's
+        if (c >= 2) group_sync(bar_done + (c & 1), kScanThreads);
+        if (threadIdx.x == 0 && c + 1 < chunks && there) stage(c + 1);
+        wait(c);
+        Handoff<DK>& hand = hands[c & 1];
+        const uint8_t* image = smem + (c % kStages) * kStage;
+        const uint32_t base = shared_addr(image);
+        const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
+        float x[4][4];
+        {  // this half's part of S^T K^T
             uint32_t hi[KS][4], lo[KS][4];
-            float down[2];
+            float down[2], y[4][4] = {};
             limbs<NT>(s, hi, lo, down);
-            const uint32_t at = base + lane_b * I::kPitch + part * ROWS * 2 + ((lane >> 3) & 1) * 16;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                hand.hi[half * KS + ks][lane] = make_uint4(hi[ks][0], hi[ks][1], hi[ks][2], hi[ks][3]);
+                hand.lo[half * KS + ks][lane] = make_uint4(lo[ks][0], lo[ks][1], lo[ks][2], lo[ks][3]);
+            }
+            hand.down[half][lane] = make_float2(down[0], down[1]);
+            const uint32_t at = base + lane_b * I::kPitch + half * HALF * 2 + half_b;
+            uint32_t bk[KS][2][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    uint32_t bk[4], bq[4];
-                    const uint32_t k_at = at + p * 16 * I::kPitch + ks * 32, q_at = k_at + LIMBS * I::kLimb;
-                    ldmatrix(bk, k_at);
-                    ldmatrix(bq, q_at);
-                    mma(y[2 * p], hi[ks], bk[0], bk[1]);
-                    mma(y[2 * p + 1], hi[ks], bk[2], bk[3]);
-                    mma(o[2 * p], hi[ks], bq[0], bq[1]);
-                    mma(o[2 * p + 1], hi[ks], bq[2], bq[3]);
-                    mma(y2[2 * p], lo[ks], bk[0], bk[1]);
-                    mma(y2[2 * p + 1], lo[ks], bk[2], bk[3]);
-                    mma(o2[2 * p], lo[ks], bq[0], bq[1]);
-                    mma(o2[2 * p + 1], lo[ks], bq[2], bq[3]);
+                    const uint32_t k_at = at + p * 16 * I::kPitch + ks * 32;
+                    ldmatrix(bk[ks][p], k_at);
+                    mma(y[2 * p], lo[ks], bk[ks][p][0], bk[ks][p][1]);
+                    mma(y[2 * p + 1], lo[ks], bk[ks][p][2], bk[ks][p][3]);
                     if (LIMBS == 2) {
-                        ldmatrix(bk, k_at + I::kLimb);
-                        ldmatrix(bq, q_at + I::kLimb);
-                        mma(y2[2 * p], hi[ks], bk[0], bk[1]);
-                        mma(y2[2 * p + 1], hi[ks], bk[2], bk[3]);
-                        mma(o2[2 * p], hi[ks], bq[0], bq[1]);
-                        mma(o2[2 * p + 1], hi[ks], bq[2], bq[3]);
+                        uint32_t bl[4];
+                        ldmatrix(bl, k_at + I::kLimb);
+                        mma(y[2 * p], hi[ks], bl[0], bl[1]);
+                        mma(y[2 * p + 1], hi[ks], bl[2], bl[3]);
                     }
                 }
-            float* mine = ex + warp * L::kExchange * 32 + lane;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    mine[(t * 4 + r) * 32] = (y[t][r] + y2[t][r]) * down[r >> 1];
-                    mine[(16 + t * 4 + r) * 32] = (o[t][r] + o2[t][r]) * down[r >> 1];
+                for (int p = 0; p < 2; ++p) {
+                    mma(y[2 * p], hi[ks], bk[ks][p][0], bk[ks][p][1]);
+                    mma(y[2 * p + 1], hi[ks], bk[ks][p][2], bk[ks][p][3]);
                 }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[t][r] = y[t][r] * down[r >> 1];
+                hand.y[half][t][lane] = make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
+            }
         }
-        // the warps of the group only
-        asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(L::kWarps * 32) : "memory");
-        // all parts in the order of the warps, so that every warp has the same bits
-        const float* parts = ex + group * L::kWarps * L::kExchange * 32 + lane;
-        float x[4][4], out[TILES][4];
+        float2 beta[4], xk[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) {
+            beta[t] = *reinterpret_cast<const float2*>(gate + kBeta * kChunk + t * 8 + tc);
+            xk[t] = *reinterpret_cast<const float2*>(gate + kXk * kChunk + t * 8 + tc);
+        }
+        // S's limbs are handed on only now: the outputs' products take the tensor
+        // cores while this chain exchanges and scales, not before
+        group_arrive(bar_s, 128);
+        group_sync(bar_y, 64);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = t * 8 + tc + (r & 1);
-                float yy = parts[(t * 4 + r) * 32];
-#pragma unroll
-                for (int q = 1; q < L::kWarps; ++q) yy += parts[(q * L::kExchange + t * 4 + r) * 32];
-                x[t][r] = gate[kBeta * kChunk + i] * v[t][r] - gate[kXk * kChunk + i] * yy;
-            }
-#pragma unroll
-        for (int k = 0; k < TILES; ++k)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float* at = parts + (16 + (part * TILES + k) * 4 + r) * 32;
-                out[k][r] = at[0];
-#pragma unroll
-                for (int q = 1; q < L::kWarps; ++q) out[k][r] += at[q * L::kExchange * 32];
-            }
+        for (int t = 0; t < 4; ++t) {  // sums of two: the same bits in both warps
+            const float4 w = hand.y[half ^ 1][t][lane];
+            x[t][0] = beta[t].x * v[t][0] - xk[t].x * (x[t][0] + w.x);
+            x[t][1] = beta[t].y * v[t][1] - xk[t].y * (x[t][1] + w.y);
+            x[t][2] = beta[t].x * v[t][2] - xk[t].x * (x[t][2] + w.z);
+            x[t][3] = beta[t].y * v[t][3] - xk[t].y * (x[t][3] + w.w);
+        }
         if (c + 1 < chunks) fetch(c + 1);
 
-        const uint32_t t_at = base + I::kBytes + lane_b * kPitchT + ((lane >> 3) & 1) * 16;
         // U^T = X^T T^T: token i takes tokens j <= i, so the second half of j only reaches the second half of i
+        const uint32_t t_at = base + I::kBytes + lane_b * kPitchT + half_b;
         float u[4][4];
         {
             uint32_t hi[2][4], lo[2][4];
-            float down[2], c1[4][4] = {}, c2[4][4] = {};
+            float down[2], c1[4][4] = {};
             limbs<4>(x, hi, lo, down);
+            uint32_t bh[2][2][4];
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int p = ks; p < 2; ++p) {
-                    uint32_t bh[4], bl[4];
-                    ldmatrix(bh, t_at + p * 16 * kPitchT + ks * 32);
+                    uint32_t bl[4];
+                    ldmatrix(bh[ks][p], t_at + p * 16 * kPitchT + ks * 32);
                     ldmatrix(bl, t_at + kLimbT + p * 16 * kPitchT + ks * 32);
-                    mma(c1[2 * p], hi[ks], bh[0], bh[1]);
-                    mma(c1[2 * p + 1], hi[ks], bh[2], bh[3]);
-                    mma(c2[2 * p], lo[ks], bh[0], bh[1]);
-                    mma(c2[2 * p + 1], lo[ks], bh[2], bh[3]);
-                    mma(c2[2 * p], hi[ks], bl[0], bl[1]);
-                    mma(c2[2 * p + 1], hi[ks], bl[2], bl[3]);
+                    mma(c1[2 * p], lo[ks], bh[ks][p][0], bh[ks][p][1]);
+                    mma(c1[2 * p + 1], lo[ks], bh[ks][p][2], bh[ks][p][3]);
+                    mma(c1[2 * p], hi[ks], bl[0], bl[1]);
+                    mma(c1[2 * p + 1], hi[ks], bl[2], bl[3]);
                 }
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    u[t][r] = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleT * kChunk + t * 8 + tc + (r & 1)]);
+                for (int p = ks; p < 2; ++p) {
+                    mma(c1[2 * p], hi[ks], bh[ks][p][0], bh[ks][p][1]);
+                    mma(c1[2 * p + 1], hi[ks], bh[ks][p][2], bh[ks][p][3]);
+                }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float2 f = *reinterpret_cast<const float2*>(gate + kScaleT * kChunk + t * 8 + tc);
+                const float2 e = *reinterpret_cast<const float2*>(gate + kDown * kChunk + t * 8 + tc);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[t][r] = c1[t][r] * (down[r >> 1] * (r & 1 ? f.y : f.x));
+                if ((t >> 1) == half) hand.u[t][lane] = make_float4(u[t][0], u[t][1], u[t][2], u[t][3]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[t][r] *= r & 1 ? e.y : e.x;  // to the chunk's end
+            }
+            group_arrive(bar_u, 128);
         }
-        // S <- e^{G_C} S + (rows of U scaled to the chunk's end) K
+        // S <- e^{G_C} S + U^T K
         {
-            float e[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) e[t][r] = u[t][r] * gate[kDown * kChunk + t * 8 + tc + (r & 1)];
             uint32_t hi[2][4], lo[2][4];
             float down[2];
-            limbs<4>(e, hi, lo, down);
+            limbs<4>(u, hi, lo, down);
             const float total = gate[kTotal * kChunk];
-            const uint32_t at = base + (lane & 15) * I::kPitch + part * ROWS * 2 + (lane >> 4) * 16;
+            const uint32_t at = base + (lane & 15) * I::kPitch + half * HALF * 2 + (lane >> 4) * 16;
 #pragma unroll
             for (int p = 0; p < NT / 2; ++p) {
-                float c1[2][4] = {}, c2[2][4] = {};
+                float c1[2][4] = {};
+                uint32_t bh[2][4];
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    uint32_t bh[4], bl[4];
-                    ldmatrix_trans(bh, at + ks * 16 * I::kPitch + p * 32);
-                    mma(c1[0], hi[ks], bh[0], bh[1]);
-                    mma(c1[1], hi[ks], bh[2], bh[3]);
-                    mma(c2[0], lo[ks], bh[0], bh[1]);
-                    mma(c2[1], lo[ks], bh[2], bh[3]);
+                    ldmatrix_trans(bh[ks], at + ks * 16 * I::kPitch + p * 32);
+                    mma(c1[0], lo[ks], bh[ks][0], bh[ks][1]);
+                    mma(c1[1], lo[ks], bh[ks][2], bh[ks][3]);
                     if (LIMBS == 2) {
+                        uint32_t bl[4];
                         ldmatrix_trans(bl, at + I::kLimb + ks * 16 * I::kPitch + p * 32);
-                        mma(c2[0], hi[ks], bl[0], bl[1]);
-                        mma(c2[1], hi[ks], bl[2], bl[3]);
+                        mma(c1[0], hi[ks], bl[0], bl[1]);
+                        mma(c1[1], hi[ks], bl[2], bl[3]);
                     }
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    mma(c1[0], hi[ks], bh[ks][0], bh[ks][1]);
+                    mma(c1[1], hi[ks], bh[ks][2], bh[ks][3]);
                 }
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], (c1[t][r] + c2[t][r]) * down[r >> 1]);
+                        s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], c1[t][r] * down[r >> 1]);
             }
-        }
-        // the outputs of this warp's tokens (columns of P behind them are zero)
-        {
-            uint32_t hi[2][4], lo[2][4];
-            float down[2];
-            limbs<4>(u, hi, lo, down);
-            const uint32_t p_at = t_at + 2 * kLimbT + part * TILES * 8 * kPitchT;
-            float c1[2][4] = {}, c2[2][4] = {};
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                uint32_t bh[4], bl[4];  // two tiles of tokens; the second is another warp's where a warp has one
-                ldmatrix(bh, p_at + ks * 32);
-                ldmatrix(bl, p_at + kLimbT + ks * 32);
-#pragma unroll
-                for (int k = 0; k < TILES; ++k) {
-                    mma(c1[k], hi[ks], bh[2 * k], bh[2 * k + 1]);
-                    mma(c2[k], lo[ks], bh[2 * k], bh[2 * k + 1]);
-                    mma(c2[k], hi[ks], bl[2 * k], bl[2 * k + 1]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int k = (part * TILES + t) * 8 + tc + (r & 1), i = c * kChunk + k;
-                    const float y1 = (c1[t][r] + c2[t][r]) * (down[r >> 1] * gate[kScaleP * kChunk + k]);
-                    const float res = fmaf(gate[kOq * kChunk + k], out[t][r], y1);
-                    if (i < seq.len && (r < 2 ? in0 : in1))
-                        from_f32(O[(int64_t)i * a.o_stride + (r < 2 ? j0 : j1)], res);
-                }
         }
     }
 #pragma unroll
@@ -694,40 +780,24 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
     return STRATA_OK;
 }
 
-template <typename T, int DK, int LIMBS, int GROUPS>
-int enqueue_scan(strata_ctx* ctx, DeltaArgs a, const SeqTable& t, const uint8_t* images, const uint8_t* images_t,
-                 cudaStream_t s) {
-    using L = Split<DK, GROUPS>;
-    auto scan = delta_scan_kernel<T, DK, LIMBS, GROUPS>;
-    constexpr int smem = scan_smem<DK, LIMBS, GROUPS>();
-    const cudaError_t e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
-    a.col_blocks = (a.v_dim + L::kCols - 1) / L::kCols;
-    const int64_t grid = (int64_t)t.n * a.v_heads * a.col_blocks;
-    if (grid > kMaxTokens) return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %d sequences of %d heads", t.n, a.v_heads);
-    scan<<<(unsigned)grid, L::kThreads, smem, s>>>(a, t, images, images_t, ctx->err_dev);
-    return check_launch(ctx, "gated_delta scan kernel");
-}
-
 template <typename T, int DK, int LIMBS>
-int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
+int enqueue(strata_ctx* ctx, const strata_gated_delta& d, DeltaArgs a, uint8_t* work, cudaStream_t s) {
     auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
-    constexpr int smem = prepare_smem<DK, LIMBS>();
-    const cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    auto scan = delta_scan_kernel<T, DK, LIMBS>;
+    constexpr int sp = prepare_smem<DK, LIMBS>(), ss = scan_smem<DK, LIMBS>();
+    cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, sp);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ss);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
+    a.col_blocks = (a.v_dim + kCols - 1) / kCols;
     const uint64_t keys = chunk_bytes(d).keys;
     return plan_chunks(d, [&](const SeqTable& t, int64_t tiles) {
-        const int64_t grid = tiles * a.k_heads;
-        if (grid > kMaxTokens)
-            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.k_heads);
+        const int64_t gp = tiles * a.k_heads, gs = (int64_t)t.n * a.v_heads * a.col_blocks;
+        if (gp > kMaxTokens || gs > kMaxTokens)
+            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.v_heads);
         uint8_t* images_t = work + keys * (uint64_t)tiles;
-        prepare<<<(unsigned)grid, kThreads, smem, s>>>(a, t, work, images_t);
-        int rc = check_launch(ctx, "gated_delta prepare kernel");
-        if (rc) return rc;
-        // narrow blocks while they fit the multiprocessors side by side
-        const int64_t narrow = (int64_t)t.n * a.v_heads * ((a.v_dim + 31) / 32);
-        return narrow <= ctx->sm_count ? enqueue_scan<T, DK, LIMBS, 2>(ctx, a, t, work, images_t, s)
-                                       : enqueue_scan<T, DK, LIMBS, 4>(ctx, a, t, work, images_t, s);
+        prepare<<<(unsigned)gp, kThreads, sp, s>>>(a, t, work, images_t);
+        scan<<<(unsigned)gs, kScanThreads, ss, s>>>(a, t, work, images_t, ctx->err_dev);
+        return check_launch(ctx, "gated_delta chunk kernels");
     });
 }
 
