@@ -28,10 +28,11 @@
 // then, split into limbs, the left operand of the next product without leaving
 // the registers, and the right operands (keys, queries, T, P) are the same for
 // all columns: they are staged in shared memory by bulk copies one chunk ahead.
-// Two warps of a group hold S, half of k_dim each, and follow the chain from
-// chunk to chunk; they exchange their halves of S^T K^T through shared memory.
-// The other two take S's limbs and U from shared memory and compute half of the
-// chunk's outputs each, off the chain and on the other half of the tensor time.
+// Four warps of a group (two for small or odd k_dim) hold a part of S's rows
+// each and follow the chain from chunk to chunk; the sums over k_dim, X and U
+// go between them through shared memory, a part of the tokens each. Two more
+// take S's limbs and U from there and compute half of the chunk's outputs
+// each, off the chain, up to a chunk behind.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -340,18 +341,26 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
 
 // ------------------------------------------------------------------- scan
 
-// A scan block: kGroups groups of 16 columns of S, each with two warps for S
+// A scan block: kGroups groups of 16 columns of S, each with kParts warps for S
 // and two for the outputs.
-constexpr int kGroups = 2, kScanThreads = kGroups * 4 * 32, kCols = kGroups * 16;
+constexpr int kGroups = 2, kCols = kGroups * 16;
 constexpr int kStages = 3;  // the chunk being read, the next, and the one whose outputs are still to come
+template <int DK>
+struct Split {
+    static constexpr int kParts = DK % 64 ? 2 : 4;
+    static constexpr int kHolders = kGroups * kParts * 32, kThreads = kHolders + kGroups * 64;
+    static constexpr int kRows = DK / kParts;    // rows of S a warp holds
+    static constexpr int kTiles = 4 / kParts;    // tiles of 8 tokens whose X and U it computes
+};
 
-// What a group's warps hand on: halves of S^T K^T, S's limbs and their row
+// What a group's warps hand on: parts of S^T K^T, X, S's limbs and their row
 // factors, U.
 template <int DK>
 struct Handoff {
-    float4 y[2][4][32];
+    float4 y[Split<DK>::kParts][4][32];
+    float4 x[4][32];
     uint4 hi[DK / 16][32], lo[DK / 16][32];
-    float2 down[2][32];
+    float2 down[Split<DK>::kParts][32];
     float4 u[4][32];
 };
 
@@ -397,22 +406,28 @@ __device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N /
 }
 
 template <typename T, int DK, int LIMBS>
-__global__ void __launch_bounds__(kScanThreads, 1)
+__global__ void __launch_bounds__(Split<DK>::kThreads, 1)
     delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab, const uint8_t* __restrict__ images,
                       const uint8_t* __restrict__ images_t, int* err) {
     using I = Image<DK, LIMBS>;
-    constexpr int HALF = DK / 2, NT = HALF / 8, KS = HALF / 16;
+    using L = Split<DK>;
+    constexpr int PARTS = L::kParts, ROWS = L::kRows, NT = ROWS / 8, KS = ROWS / 16, TILES = L::kTiles;
     constexpr int kStage = I::kBytes + kImageT;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t arrived[kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the warps of S first, then those of the outputs: one of each a scheduler
-    const bool holds = warp < 2 * kGroups;
-    const int group = (warp >> 1) % kGroups, half = warp & 1;
+    // the warps of S first, then those of the outputs, spread evenly over the schedulers
+    const bool holds = threadIdx.x < L::kHolders;
+    const int group = holds ? warp / PARTS : (warp - kGroups * PARTS) / 2;
+    const int part = holds ? warp % PARTS : (warp - kGroups * PARTS) % 2;
     Handoff<DK>* const hands = reinterpret_cast<Handoff<DK>*>(smem + kStages * kStage) + group * 2;
-    // Barriers: two for chunks whose outputs are written, then a group's: halves
-    // of S^T K^T, S's limbs handed on, U handed on.
-    const int bar_done = 1, bar_y = 3 + group * 3, bar_s = bar_y + 1, bar_u = bar_y + 2;
+    // Barriers: chunk written out, then a group's: among the warps of S, S's
+    // limbs handed on, U handed on. The warps of S only arrive at the last two
+    // and may be a chunk ahead there, so that even and odd chunks have their own:
+    // one is used again two chunks on, behind the outputs' arrival at bar_done
+    // for the chunk that used it before.
+    const int bar_done = 1, bar_g = 3 + group * 5, bar_s = bar_g + 1, bar_u = bar_g + 3;
+    constexpr int kOfGroup = (PARTS + 2) * 32;
     int b = blockIdx.x;
     const int cb = b % a.col_blocks;
     b /= a.col_blocks;
@@ -423,7 +438,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     const int j0 = cb * kCols + group * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
     const bool in0 = j0 < a.v_dim, in1 = j1 < a.v_dim;
     const int tc = (lane & 3) * 2;
-    const int d0 = half * HALF + tc;  // its first row of S
+    const int d0 = part * ROWS + tc;  // its first row of S (warps of S)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i)
@@ -444,24 +459,28 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     // barrier, and the call is reported as timed out.
     bool there = true;
     auto wait = [&](int c) {
-        if (there) there = bulk_wait(shared_addr(&arrived[c % kStages]), (c / kStages) & 1);
-        if (!there) atomicExch(err, 1);
+        if (!there) return;
+        there = bulk_wait(shared_addr(&arrived[c % kStages]), (c / kStages) & 1);
+        if (!there) {
+            bulk_wait(shared_addr(&arrived[c % kStages]), (c / kStages) & 1);  // nothing in flight when the block ends
+            atomicExch(err, 1);
+        }
     };
     const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
     const uint32_t half_b = ((lane >> 3) & 1) * 16;             // and its half of a row
 
-    if (!holds) {  // ---- outputs of tokens half * 16 .. + 15
+    if (!holds) {  // ---- outputs of tokens part * 16 .. + 15
         T* O = static_cast<T*>(a.o) + (int64_t)seq.row * a.o_stride + (int64_t)h * a.v_dim;
         for (int c = 0; c < chunks; ++c) {
             wait(c);
             const uint8_t* image = smem + (c % kStages) * kStage;
             const Handoff<DK>& hand = hands[c & 1];
             const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
-            const uint32_t q_at = shared_addr(image) + LIMBS * I::kLimb + (half * 16 + lane_b) * I::kPitch + half_b;
+            const uint32_t q_at = shared_addr(image) + LIMBS * I::kLimb + (part * 16 + lane_b) * I::kPitch + half_b;
             float out[2][4] = {};
-            group_sync(bar_s, 128);
+            group_sync(bar_s + (c & 1), kOfGroup);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {  // the two halves of k_dim, each with its own row factors
+            for (int k = 0; k < PARTS; ++k) {  // the parts of k_dim, each with its own row factors
                 float o1[2][4] = {};
                 uint32_t hi[KS][4];
 #pragma unroll
@@ -492,7 +511,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) out[t][r] = fmaf(o1[t][r], r < 2 ? down.x : down.y, out[t][r]);
             }
-            group_sync(bar_u, 128);
+            group_sync(bar_u + (c & 1), kOfGroup);
             float u[4][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -503,7 +522,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
             float down[2], c1[2][4] = {};
             limbs<4>(u, hi, lo, down);
             const uint32_t p_at =
-                shared_addr(image) + I::kBytes + 2 * kLimbT + (half * 16 + lane_b) * kPitchT + half_b;
+                shared_addr(image) + I::kBytes + 2 * kLimbT + (part * 16 + lane_b) * kPitchT + half_b;
             uint32_t bh[2][4], bl[4];
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {  // later tokens' columns of P are zero
@@ -519,12 +538,12 @@ __global__ void __launch_bounds__(kScanThreads, 1)
                 mma(c1[0], hi[ks], bh[ks][0], bh[ks][1]);
                 mma(c1[1], hi[ks], bh[ks][2], bh[ks][3]);
             }
-            T* row = O + (int64_t)(c * kChunk + half * 16 + tc) * a.o_stride;
-            const int left = seq.len - (c * kChunk + half * 16 + tc);  // tokens from the lane's first
+            T* row = O + (int64_t)(c * kChunk + part * 16 + tc) * a.o_stride;
+            const int left = seq.len - (c * kChunk + part * 16 + tc);  // tokens from the lane's first
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float2 sp = *reinterpret_cast<const float2*>(gate + kScaleP * kChunk + half * 16 + t * 8 + tc);
-                const float2 oq = *reinterpret_cast<const float2*>(gate + kOq * kChunk + half * 16 + t * 8 + tc);
+                const float2 sp = *reinterpret_cast<const float2*>(gate + kScaleP * kChunk + part * 16 + t * 8 + tc);
+                const float2 oq = *reinterpret_cast<const float2*>(gate + kOq * kChunk + part * 16 + t * 8 + tc);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float y1 = c1[t][r] * (down[r >> 1] * (r & 1 ? sp.y : sp.x));
@@ -534,7 +553,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
                 }
             }
             // the stage and the handoff may be written again (two chunks on)
-            if (c + 2 < chunks) group_arrive(bar_done + (c & 1), kScanThreads);
+            if (c + 2 < chunks) group_arrive(bar_done + (c & 1), L::kThreads);
         }
         return;
     }
@@ -550,13 +569,13 @@ __global__ void __launch_bounds__(kScanThreads, 1)
             s[t][r] = d < a.k_dim && j < a.v_dim ? S[(int64_t)d * a.v_dim + j] : 0.0f;
         }
     const T* V = static_cast<const T*>(a.v) + (int64_t)seq.row * a.v_stride + (int64_t)h * a.v_dim;
-    float v[4][4];
-    V += (int64_t)tc * a.v_stride;
+    V += (int64_t)(part * TILES * 8 + tc) * a.v_stride;
+    float v[TILES][4];
     auto fetch = [&](int c) {
         const T* row = V + (int64_t)c * kChunk * a.v_stride;
-        const int left = seq.len - c * kChunk - tc;  // tokens from the lane's first
+        const int left = seq.len - c * kChunk - part * TILES * 8 - tc;  // tokens from the lane's first
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const bool in = t * 8 + (r & 1) < left && (r < 2 ? in0 : in1);
@@ -566,25 +585,24 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     fetch(0);
     for (int c = 0; c < chunks; ++c) {
         // chunk c - 2 is written out, so its stage can take chunk c + 1 and its handoff this chunk's
-        if (c >= 2) group_sync(bar_done + (c & 1), kScanThreads);
+        if (c >= 2) group_sync(bar_done + (c & 1), L::kThreads);
         if (threadIdx.x == 0 && c + 1 < chunks && there) stage(c + 1);
         wait(c);
         Handoff<DK>& hand = hands[c & 1];
         const uint8_t* image = smem + (c % kStages) * kStage;
         const uint32_t base = shared_addr(image);
         const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
-        float x[4][4];
-        {  // this half's part of S^T K^T
+        {  // this warp's part of S^T K^T
             uint32_t hi[KS][4], lo[KS][4];
             float down[2], y[4][4] = {};
             limbs<NT>(s, hi, lo, down);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                hand.hi[half * KS + ks][lane] = make_uint4(hi[ks][0], hi[ks][1], hi[ks][2], hi[ks][3]);
-                hand.lo[half * KS + ks][lane] = make_uint4(lo[ks][0], lo[ks][1], lo[ks][2], lo[ks][3]);
+                hand.hi[part * KS + ks][lane] = make_uint4(hi[ks][0], hi[ks][1], hi[ks][2], hi[ks][3]);
+                hand.lo[part * KS + ks][lane] = make_uint4(lo[ks][0], lo[ks][1], lo[ks][2], lo[ks][3]);
             }
-            hand.down[half][lane] = make_float2(down[0], down[1]);
-            const uint32_t at = base + lane_b * I::kPitch + half * HALF * 2 + half_b;
+            hand.down[part][lane] = make_float2(down[0], down[1]);
+            const uint32_t at = base + lane_b * I::kPitch + part * ROWS * 2 + half_b;
             uint32_t bk[KS][2][4];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
@@ -609,78 +627,79 @@ __global__ void __launch_bounds__(kScanThreads, 1)
                     mma(y[2 * p + 1], hi[ks], bk[ks][p][2], bk[ks][p][3]);
                 }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[t][r] = y[t][r] * down[r >> 1];
-                hand.y[half][t][lane] = make_float4(x[t][0], x[t][1], x[t][2], x[t][3]);
-            }
-        }
-        float2 beta[4], xk[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            beta[t] = *reinterpret_cast<const float2*>(gate + kBeta * kChunk + t * 8 + tc);
-            xk[t] = *reinterpret_cast<const float2*>(gate + kXk * kChunk + t * 8 + tc);
+            for (int t = 0; t < 4; ++t)
+                hand.y[part][t][lane] =
+                    make_float4(y[t][0] * down[0], y[t][1] * down[0], y[t][2] * down[1], y[t][3] * down[1]);
         }
         // S's limbs are handed on only now: the outputs' products take the tensor
         // cores while this chain exchanges and scales, not before
-        group_arrive(bar_s, 128);
-        group_sync(bar_y, 64);
+        group_arrive(bar_s + (c & 1), kOfGroup);
+        group_sync(bar_g, PARTS * 32);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {  // sums of two: the same bits in both warps
-            const float4 w = hand.y[half ^ 1][t][lane];
-            x[t][0] = beta[t].x * v[t][0] - xk[t].x * (x[t][0] + w.x);
-            x[t][1] = beta[t].y * v[t][1] - xk[t].y * (x[t][1] + w.y);
-            x[t][2] = beta[t].x * v[t][2] - xk[t].x * (x[t][2] + w.z);
-            x[t][3] = beta[t].y * v[t][3] - xk[t].y * (x[t][3] + w.w);
+        for (int k = 0; k < TILES; ++k) {  // X of this warp's tokens
+            const int t = part * TILES + k;
+            const float2 beta = *reinterpret_cast<const float2*>(gate + kBeta * kChunk + t * 8 + tc);
+            const float2 xk = *reinterpret_cast<const float2*>(gate + kXk * kChunk + t * 8 + tc);
+            float4 y = hand.y[0][t][lane];
+#pragma unroll
+            for (int q = 1; q < PARTS; ++q) {
+                const float4 w = hand.y[q][t][lane];
+                y.x += w.x, y.y += w.y, y.z += w.z, y.w += w.w;
+            }
+            hand.x[t][lane] = make_float4(beta.x * v[k][0] - xk.x * y.x, beta.y * v[k][1] - xk.y * y.y,
+                                          beta.x * v[k][2] - xk.x * y.z, beta.y * v[k][3] - xk.y * y.w);
         }
+        group_sync(bar_g, PARTS * 32);
         if (c + 1 < chunks) fetch(c + 1);
 
-        // U^T = X^T T^T: token i takes tokens j <= i, so the second half of j only reaches the second half of i
-        const uint32_t t_at = base + I::kBytes + lane_b * kPitchT + half_b;
-        float u[4][4];
+        // U^T = X^T T^T, this warp's tokens; columns of T behind them are zero
         {
-            uint32_t hi[2][4], lo[2][4];
-            float down[2], c1[4][4] = {};
-            limbs<4>(x, hi, lo, down);
-            uint32_t bh[2][2][4];
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int p = ks; p < 2; ++p) {
-                    uint32_t bl[4];
-                    ldmatrix(bh[ks][p], t_at + p * 16 * kPitchT + ks * 32);
-                    ldmatrix(bl, t_at + kLimbT + p * 16 * kPitchT + ks * 32);
-                    mma(c1[2 * p], lo[ks], bh[ks][p][0], bh[ks][p][1]);
-                    mma(c1[2 * p + 1], lo[ks], bh[ks][p][2], bh[ks][p][3]);
-                    mma(c1[2 * p], hi[ks], bl[0], bl[1]);
-                    mma(c1[2 * p + 1], hi[ks], bl[2], bl[3]);
-                }
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int p = ks; p < 2; ++p) {
-                    mma(c1[2 * p], hi[ks], bh[ks][p][0], bh[ks][p][1]);
-                    mma(c1[2 * p + 1], hi[ks], bh[ks][p][2], bh[ks][p][3]);
-                }
+            float x[4][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const float2 f = *reinterpret_cast<const float2*>(gate + kScaleT * kChunk + t * 8 + tc);
-                const float2 e = *reinterpret_cast<const float2*>(gate + kDown * kChunk + t * 8 + tc);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) u[t][r] = c1[t][r] * (down[r >> 1] * (r & 1 ? f.y : f.x));
-                if ((t >> 1) == half) hand.u[t][lane] = make_float4(u[t][0], u[t][1], u[t][2], u[t][3]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) u[t][r] *= r & 1 ? e.y : e.x;  // to the chunk's end
+                const float4 w = hand.x[t][lane];
+                x[t][0] = w.x, x[t][1] = w.y, x[t][2] = w.z, x[t][3] = w.w;
             }
-            group_arrive(bar_u, 128);
+            uint32_t hi[2][4], lo[2][4], bh[2][4], bl[2][4];
+            float down[2], c1[2][4] = {};
+            const uint32_t t_at = base + I::kBytes + (part * TILES * 8 + lane_b) * kPitchT + half_b;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {  // two tiles of tokens; the second is another warp's where a warp has one
+                ldmatrix(bh[ks], t_at + ks * 32);
+                ldmatrix(bl[ks], t_at + kLimbT + ks * 32);
+            }
+            limbs<4>(x, hi, lo, down);
+#pragma unroll
+            for (int k = 0; k < TILES; ++k) {
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    mma(c1[k], lo[ks], bh[ks][2 * k], bh[ks][2 * k + 1]);
+                    mma(c1[k], hi[ks], bl[ks][2 * k], bl[ks][2 * k + 1]);
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) mma(c1[k], hi[ks], bh[ks][2 * k], bh[ks][2 * k + 1]);
+                const int t = part * TILES + k;
+                const float2 f = *reinterpret_cast<const float2*>(gate + kScaleT * kChunk + t * 8 + tc);
+                hand.u[t][lane] = make_float4(c1[k][0] * (down[0] * f.x), c1[k][1] * (down[0] * f.y),
+                                              c1[k][2] * (down[1] * f.x), c1[k][3] * (down[1] * f.y));
+            }
         }
-        // S <- e^{G_C} S + U^T K
+        group_arrive(bar_u + (c & 1), kOfGroup);
+        group_sync(bar_g, PARTS * 32);
+        // S <- e^{G_C} S + U^T K, with U scaled to the chunk's end
         {
+            float u[4][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float2 e = *reinterpret_cast<const float2*>(gate + kDown * kChunk + t * 8 + tc);
+                const float4 w = hand.u[t][lane];
+                u[t][0] = w.x * e.x, u[t][1] = w.y * e.y, u[t][2] = w.z * e.x, u[t][3] = w.w * e.y;
+            }
             uint32_t hi[2][4], lo[2][4];
             float down[2];
             limbs<4>(u, hi, lo, down);
             const float total = gate[kTotal * kChunk];
-            const uint32_t at = base + (lane & 15) * I::kPitch + half * HALF * 2 + (lane >> 4) * 16;
+            const uint32_t at = base + (lane & 15) * I::kPitch + part * ROWS * 2 + (lane >> 4) * 16;
 #pragma unroll
             for (int p = 0; p < NT / 2; ++p) {
                 float c1[2][4] = {};
@@ -796,7 +815,7 @@ int enqueue(strata_ctx* ctx, const strata_gated_delta& d, DeltaArgs a, uint8_t* 
             return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.v_heads);
         uint8_t* images_t = work + keys * (uint64_t)tiles;
         prepare<<<(unsigned)gp, kThreads, sp, s>>>(a, t, work, images_t);
-        scan<<<(unsigned)gs, kScanThreads, ss, s>>>(a, t, work, images_t, ctx->err_dev);
+        scan<<<(unsigned)gs, Split<DK>::kThreads, ss, s>>>(a, t, work, images_t, ctx->err_dev);
         return check_launch(ctx, "gated_delta chunk kernels");
     });
 }
