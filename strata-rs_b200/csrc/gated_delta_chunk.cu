@@ -15,8 +15,10 @@
 // chunks of a sequence in order with S in registers.
 //
 // Precision. The products run on the tensor cores as f16 limbs: x 2^e = hi + lo
-// with the exponent e taken per row from the row's largest magnitude, so a
-// limb pair carries 22 bits of it, and lo hi + hi lo + hi hi is summed in f32,
+// with the exponent e taken per row from the row's largest magnitude or a bound
+// of it (X and U: from the chunk's norms, prepared with it, so that warps can
+// scale apart from each other). A limb pair carries 22 bits of what is within
+// 2^-18 of the bound, 2^-40 of the bound below that, and lo hi + hi lo + hi hi is summed in f32,
 // the two small products first. That keeps f32-like results at f16 rate; plain
 // tf32 would carry 11 bits. Keys and queries given
 // as bf16 are exact in one limb. The scan adds to S outside the tensor core,
@@ -46,7 +48,10 @@ constexpr int kThreads = 128;                  // of a prepare block
 constexpr int kPitchT = kChunk * 2 + 16;       // bytes of a row of T or P: 16-byte steps that no two of 8 rows share
 constexpr int kLimbT = kChunk * kPitchT;
 constexpr int kGates = 4 * kLimbT;             // T hi, T lo, P hi, P lo, then the gate rows
-enum { kBeta, kXk, kOq, kDown, kScaleT, kScaleP, kTotal, kGateRows };
+enum { kBeta, kXk, kOq, kDown, kScaleT, kScaleP, kChunkRow, kGateRows };
+// The last row: e^{G_C}, and what bounds X by the largest of S (kBoundS) and of
+// V (kBoundV), U by X, and U scaled to the chunk's end by U.
+enum { kTotal, kBoundS, kBoundV, kBoundU, kBoundEnd };
 constexpr int kImageT = kGates + kGateRows * kChunk * 4;
 constexpr uint64_t kMaxWork = uint64_t(256) << 20;
 
@@ -132,7 +137,21 @@ constexpr int kPitchA = kChunk + 4;  // floats of a row of A: 16-byte steps that
 template <int DK, int LIMBS>
 constexpr int prepare_smem() {
     constexpr int scratch = 4 * kChunk * kPitchA * 4, image = Image<DK, LIMBS>::kBytes;
-    return (image > scratch ? image : scratch) + (2 * kChunk * (kChunk + 1) + 2 * kChunk) * 4;
+    return (image > scratch ? image : scratch) + (2 * kChunk * (kChunk + 1) + 3 * kChunk) * 4;
+}
+
+// e^x for a sum of log decays: the argument's rounding is 2^-24 |x| of the
+// result, which is below 2^-25 of 1 for every x <= 0.
+__device__ __forceinline__ float decay(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
 }
 
 // 32 values of a row as two limbs of halves, scaled to the row's largest
@@ -165,10 +184,11 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
     constexpr int PER = DK / 32;  // elements of a row a lane holds
     extern __shared__ __align__(16) uint8_t smem[];
     float(*kk)[kChunk + 1] =
-        reinterpret_cast<float(*)[kChunk + 1]>(smem + prepare_smem<DK, LIMBS>() - (2 * kChunk * (kChunk + 1) + 2 * kChunk) * 4);
+        reinterpret_cast<float(*)[kChunk + 1]>(smem + prepare_smem<DK, LIMBS>() - (2 * kChunk * (kChunk + 1) + 3 * kChunk) * 4);
     float(*qk)[kChunk + 1] = kk + kChunk;
     float* fk = &qk[kChunk][0];  // what a row of limbs is to be multiplied with
     float* fq = fk + kChunk;
+    float* kn = fq + kChunk;      // a bound of the sum of a key's magnitudes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float(*A)[kPitchA] = reinterpret_cast<float(*)[kPitchA]>(smem) + warp * kChunk;
     const int tile = blockIdx.x / a.k_heads, hk = blockIdx.x - tile * a.k_heads;
@@ -220,8 +240,9 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             if (LIMBS == 2) reinterpret_cast<__half*>(at + I::kLimb)[e] = lo[e];
         }
         if (lane == 0) {
-            if (a.norm) down *= 1.0f / sqrtf(ss + a.eps);
-            (r < 8 ? fk : fq)[i] = i < n ? (r < 8 ? down : down * a.scale) : 0.0f;
+            const float f = a.norm ? 1.0f / sqrtf(ss + a.eps) : 1.0f;
+            (r < 8 ? fk : fq)[i] = i < n ? (r < 8 ? down * f : down * f * a.scale) : 0.0f;
+            if (r < 8) kn[i] = i < n ? sqrtf((float)DK * ss) * f : 0.0f;
         }
     }
     __syncthreads();
@@ -290,21 +311,29 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
         float v[kChunk];  // a row a lane: beta_i e^{G_i - G_j} k_i . k_j, or e^{G_i - G_j} q_i . k_j
         const float(*products)[kChunk + 1] = task & 1 ? qk : kk;
         const int diagonal = task & 1 ? lane : lane - 1;  // the row's last column
+        const float Gh = (float)G, Gl = (float)(G - (double)Gh);  // the sum in two floats
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
-            const double Gj = __shfl_sync(0xFFFFFFFFu, G, j);
-            v[j] = j <= diagonal ? expf((float)(G - Gj)) * products[lane][j] : 0.0f;
+            const float h = __shfl_sync(0xFFFFFFFFu, Gh, j), l = __shfl_sync(0xFFFFFFFFu, Gl, j);
+            v[j] = j <= diagonal ? decay((Gh - h) + (Gl - l)) * products[lane][j] : 0.0f;
         }
         if (task & 1) {
             const float down = store_row(v, image + 2 * kLimbT + lane * kPitchT, image + 3 * kLimbT + lane * kPitchT);
             out[kScaleP * kChunk] = down;
             const double end = __shfl_sync(0xFFFFFFFFu, G, 31);
             const float before = expf((float)G), after = expf((float)(end - G));
+            const float bs = warp_max(fabsf(beta) * before * kn[lane]), bv = warp_max(fabsf(beta));
+            const float be = warp_max(after * fabsf(fk[lane]));
+            if (lane == 0) {
+                out[kChunkRow * kChunk + kTotal] = expf((float)end);
+                out[kChunkRow * kChunk + kBoundS] = bs;
+                out[kChunkRow * kChunk + kBoundV] = bv;
+                out[kChunkRow * kChunk + kBoundEnd] = be;
+            }
             out[kBeta * kChunk] = beta;
             out[kXk * kChunk] = beta * before * fk[lane];
             out[kOq * kChunk] = before * fq[lane];
             out[kDown * kChunk] = after * fk[lane];
-            out[kTotal * kChunk] = expf((float)end);
             continue;
         }
         __syncwarp();
@@ -335,6 +364,11 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) v[j] = flat[lane * (kChunk + 1) + j];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) sum += fabsf(v[j]);
+        sum = warp_max(sum);
+        if (lane == 0) out[kChunkRow * kChunk + kBoundU] = sum;
         out[kScaleT * kChunk] = store_row(v, image + lane * kPitchT, image + kLimbT + lane * kPitchT);
     }
 }
@@ -353,20 +387,28 @@ struct Split {
     static constexpr int kTiles = 4 / kParts;    // tiles of 8 tokens whose X and U it computes
 };
 
-// What a group's warps hand on: parts of S^T K^T, X, S's limbs and their row
-// factors, U.
+// What a group's warps hand on to its outputs' (two, for even and odd chunks):
+// S's limbs and their row factors, U and what undoes its scale. Limbs lie as
+// left operands take them: two rows of hi, two of lo.
 template <int DK>
 struct Handoff {
-    float4 y[Split<DK>::kParts][4][32];
-    float4 x[4][32];
     uint4 hi[DK / 16][32], lo[DK / 16][32];
-    float2 down[Split<DK>::kParts][32];
-    float4 u[4][32];
+    float2 down[Split<DK>::kParts][32], scale[32];
+    uint4 u[4][32];
+};
+// And among each other, within a chunk: parts of S^T K^T with the largest
+// magnitudes of their rows of S and V, X, and U scaled to the chunk's end.
+template <int DK>
+struct Shared {
+    float4 y[Split<DK>::kParts][4][32];
+    float4 top[Split<DK>::kParts][8];  // S and V of a row, and of the row 8 on
+    uint4 x[4][32], e[4][32];
 };
 
 template <int DK, int LIMBS>
 constexpr int scan_smem() {
-    return kStages * (Image<DK, LIMBS>::kBytes + kImageT) + 2 * kGroups * (int)sizeof(Handoff<DK>);
+    return kStages * (Image<DK, LIMBS>::kBytes + kImageT) + 2 * kGroups * (int)sizeof(Handoff<DK>) +
+           kGroups * (int)sizeof(Shared<DK>);
 }
 
 // Named barriers of a group: `threads` of them arrive in all.
@@ -387,15 +429,16 @@ __device__ __forceinline__ float row_max(float m) {
 // down: what undoes the scale, for the two rows of a lane.
 template <int N>
 __device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N / 2][4], uint32_t (&lo)[N / 2][4],
-                                      float (&down)[2]) {
+                                      float (&down)[2], float (&most)[2]) {
     float m0 = 0.0f, m1 = 0.0f, up0, up1;
 #pragma unroll
     for (int t = 0; t < N; ++t) {
         m0 = fmaxf(m0, fmaxf(fabsf(x[t][0]), fabsf(x[t][1])));
         m1 = fmaxf(m1, fmaxf(fabsf(x[t][2]), fabsf(x[t][3])));
     }
-    power_for(row_max(m0), up0, down[0]);
-    power_for(row_max(m1), up1, down[1]);
+    most[0] = row_max(m0), most[1] = row_max(m1);
+    power_for(most[0], up0, down[0]);
+    power_for(most[1], up1, down[1]);
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) {
         split(x[2 * k][0] * up0, x[2 * k][1] * up0, hi[k][0], lo[k][0]);
@@ -403,6 +446,19 @@ __device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N /
         split(x[2 * k + 1][0] * up0, x[2 * k + 1][1] * up0, hi[k][2], lo[k][2]);
         split(x[2 * k + 1][2] * up1, x[2 * k + 1][3] * up1, hi[k][3], lo[k][3]);
     }
+}
+
+// A tile's four values of a lane (two of a row, two of the row 8 on) as limbs.
+__device__ __forceinline__ uint4 tile_limbs(float a, float b, float c, float d, float up0, float up1) {
+    uint4 w;
+    split(a * up0, b * up0, w.x, w.z);
+    split(c * up1, d * up1, w.y, w.w);
+    return w;
+}
+// Two tiles' limbs as a left operand.
+__device__ __forceinline__ void operand(const uint4& a, const uint4& b, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    hi[0] = a.x, hi[1] = a.y, hi[2] = b.x, hi[3] = b.y;
+    lo[0] = a.z, lo[1] = a.w, lo[2] = b.z, lo[3] = b.w;
 }
 
 template <typename T, int DK, int LIMBS>
@@ -421,6 +477,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
     const int group = holds ? warp / PARTS : (warp - kGroups * PARTS) / 2;
     const int part = holds ? warp % PARTS : (warp - kGroups * PARTS) % 2;
     Handoff<DK>* const hands = reinterpret_cast<Handoff<DK>*>(smem + kStages * kStage) + group * 2;
+    Shared<DK>& sh = reinterpret_cast<Shared<DK>*>(smem + kStages * kStage + 2 * kGroups * sizeof(Handoff<DK>))[group];
     // Barriers: chunk written out, then a group's: among the warps of S, S's
     // limbs handed on, U handed on. The warps of S only arrive at the last two
     // and may be a chunk ahead there, so that even and odd chunks have their own:
@@ -512,15 +569,11 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
                     for (int r = 0; r < 4; ++r) out[t][r] = fmaf(o1[t][r], r < 2 ? down.x : down.y, out[t][r]);
             }
             group_sync(bar_u + (c & 1), kOfGroup);
-            float u[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float4 w = hand.u[t][lane];
-                u[t][0] = w.x, u[t][1] = w.y, u[t][2] = w.z, u[t][3] = w.w;
-            }
             uint32_t hi[2][4], lo[2][4];
-            float down[2], c1[2][4] = {};
-            limbs<4>(u, hi, lo, down);
+            float c1[2][4] = {};
+            operand(hand.u[0][lane], hand.u[1][lane], hi[0], lo[0]);
+            operand(hand.u[2][lane], hand.u[3][lane], hi[1], lo[1]);
+            const float2 down = hand.scale[lane];
             const uint32_t p_at =
                 shared_addr(image) + I::kBytes + 2 * kLimbT + (part * 16 + lane_b) * kPitchT + half_b;
             uint32_t bh[2][4], bl[4];
@@ -546,7 +599,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
                 const float2 oq = *reinterpret_cast<const float2*>(gate + kOq * kChunk + part * 16 + t * 8 + tc);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float y1 = c1[t][r] * (down[r >> 1] * (r & 1 ? sp.y : sp.x));
+                    const float y1 = c1[t][r] * ((r < 2 ? down.x : down.y) * (r & 1 ? sp.y : sp.x));
                     const float res = fmaf(r & 1 ? oq.y : oq.x, out[t][r], y1);
                     if (t * 8 + (r & 1) < left && (r < 2 ? in0 : in1))
                         from_f32(row[(t * 8 + (r & 1)) * a.o_stride + (r < 2 ? j0 : j1)], res);
@@ -594,8 +647,16 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
         const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
         {  // this warp's part of S^T K^T
             uint32_t hi[KS][4], lo[KS][4];
-            float down[2], y[4][4] = {};
-            limbs<NT>(s, hi, lo, down);
+            float down[2], most[2], y[4][4] = {};
+            limbs<NT>(s, hi, lo, down, most);
+            float v0 = 0.0f, v1 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < TILES; ++k) {
+                v0 = fmaxf(v0, fmaxf(fabsf(v[k][0]), fabsf(v[k][1])));
+                v1 = fmaxf(v1, fmaxf(fabsf(v[k][2]), fabsf(v[k][3])));
+            }
+            v0 = row_max(v0), v1 = row_max(v1);
+            if (tc == 0) sh.top[part][lane >> 2] = make_float4(most[0], v0, most[1], v1);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 hand.hi[part * KS + ks][lane] = make_uint4(hi[ks][0], hi[ks][1], hi[ks][2], hi[ks][3]);
@@ -628,47 +689,67 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
                 }
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                hand.y[part][t][lane] =
+                sh.y[part][t][lane] =
                     make_float4(y[t][0] * down[0], y[t][1] * down[0], y[t][2] * down[1], y[t][3] * down[1]);
         }
         // S's limbs are handed on only now: the outputs' products take the tensor
         // cores while this chain exchanges and scales, not before
         group_arrive(bar_s + (c & 1), kOfGroup);
         group_sync(bar_g, PARTS * 32);
+        // the same bounds in every warp: no row of X or U is larger
+        float up[2], down[2];
+        float x_most[2];
+        {
+            float4 top = sh.top[0][lane >> 2];
+#pragma unroll
+            for (int q = 1; q < PARTS; ++q) {
+                const float4 w = sh.top[q][lane >> 2];
+                top.x = fmaxf(top.x, w.x), top.y = fmaxf(top.y, w.y);
+                top.z = fmaxf(top.z, w.z), top.w = fmaxf(top.w, w.w);
+            }
+            const float bs = gate[kChunkRow * kChunk + kBoundS], bv = gate[kChunkRow * kChunk + kBoundV];
+            x_most[0] = bs * top.x + bv * top.y, x_most[1] = bs * top.z + bv * top.w;
+            power_for(x_most[0], up[0], down[0]);
+            power_for(x_most[1], up[1], down[1]);
+        }
 #pragma unroll
         for (int k = 0; k < TILES; ++k) {  // X of this warp's tokens
             const int t = part * TILES + k;
             const float2 beta = *reinterpret_cast<const float2*>(gate + kBeta * kChunk + t * 8 + tc);
             const float2 xk = *reinterpret_cast<const float2*>(gate + kXk * kChunk + t * 8 + tc);
-            float4 y = hand.y[0][t][lane];
+            float4 y = sh.y[0][t][lane];
 #pragma unroll
             for (int q = 1; q < PARTS; ++q) {
-                const float4 w = hand.y[q][t][lane];
+                const float4 w = sh.y[q][t][lane];
                 y.x += w.x, y.y += w.y, y.z += w.z, y.w += w.w;
             }
-            hand.x[t][lane] = make_float4(beta.x * v[k][0] - xk.x * y.x, beta.y * v[k][1] - xk.y * y.y,
-                                          beta.x * v[k][2] - xk.x * y.z, beta.y * v[k][3] - xk.y * y.w);
+            sh.x[t][lane] = tile_limbs(beta.x * v[k][0] - xk.x * y.x, beta.y * v[k][1] - xk.y * y.y,
+                                         beta.x * v[k][2] - xk.x * y.z, beta.y * v[k][3] - xk.y * y.w, up[0], up[1]);
         }
         group_sync(bar_g, PARTS * 32);
         if (c + 1 < chunks) fetch(c + 1);
 
         // U^T = X^T T^T, this warp's tokens; columns of T behind them are zero
+        float e_down[2];
         {
-            float x[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float4 w = hand.x[t][lane];
-                x[t][0] = w.x, x[t][1] = w.y, x[t][2] = w.z, x[t][3] = w.w;
-            }
             uint32_t hi[2][4], lo[2][4], bh[2][4], bl[2][4];
-            float down[2], c1[2][4] = {};
+            float c1[2][4] = {};
+            operand(sh.x[0][lane], sh.x[1][lane], hi[0], lo[0]);
+            operand(sh.x[2][lane], sh.x[3][lane], hi[1], lo[1]);
+            const float bu = gate[kChunkRow * kChunk + kBoundU], be = gate[kChunkRow * kChunk + kBoundEnd];
+            float u_up[2], u_down[2], e_up[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                power_for(x_most[r] * bu, u_up[r], u_down[r]);
+                power_for(x_most[r] * bu * be, e_up[r], e_down[r]);
+            }
+            if (part == 0) hand.scale[lane] = make_float2(u_down[0], u_down[1]);
             const uint32_t t_at = base + I::kBytes + (part * TILES * 8 + lane_b) * kPitchT + half_b;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {  // two tiles of tokens; the second is another warp's where a warp has one
                 ldmatrix(bh[ks], t_at + ks * 32);
                 ldmatrix(bl[ks], t_at + kLimbT + ks * 32);
             }
-            limbs<4>(x, hi, lo, down);
 #pragma unroll
             for (int k = 0; k < TILES; ++k) {
 #pragma unroll
@@ -680,25 +761,21 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
                 for (int ks = 0; ks < 2; ++ks) mma(c1[k], hi[ks], bh[ks][2 * k], bh[ks][2 * k + 1]);
                 const int t = part * TILES + k;
                 const float2 f = *reinterpret_cast<const float2*>(gate + kScaleT * kChunk + t * 8 + tc);
-                hand.u[t][lane] = make_float4(c1[k][0] * (down[0] * f.x), c1[k][1] * (down[0] * f.y),
-                                              c1[k][2] * (down[1] * f.x), c1[k][3] * (down[1] * f.y));
+                const float2 e = *reinterpret_cast<const float2*>(gate + kDown * kChunk + t * 8 + tc);
+                const float u0 = c1[k][0] * (down[0] * f.x), u1 = c1[k][1] * (down[0] * f.y);
+                const float u2 = c1[k][2] * (down[1] * f.x), u3 = c1[k][3] * (down[1] * f.y);
+                hand.u[t][lane] = tile_limbs(u0, u1, u2, u3, u_up[0], u_up[1]);
+                sh.e[t][lane] = tile_limbs(u0 * e.x, u1 * e.y, u2 * e.x, u3 * e.y, e_up[0], e_up[1]);
             }
         }
         group_arrive(bar_u + (c & 1), kOfGroup);
         group_sync(bar_g, PARTS * 32);
         // S <- e^{G_C} S + U^T K, with U scaled to the chunk's end
         {
-            float u[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float2 e = *reinterpret_cast<const float2*>(gate + kDown * kChunk + t * 8 + tc);
-                const float4 w = hand.u[t][lane];
-                u[t][0] = w.x * e.x, u[t][1] = w.y * e.y, u[t][2] = w.z * e.x, u[t][3] = w.w * e.y;
-            }
             uint32_t hi[2][4], lo[2][4];
-            float down[2];
-            limbs<4>(u, hi, lo, down);
-            const float total = gate[kTotal * kChunk];
+            operand(sh.e[0][lane], sh.e[1][lane], hi[0], lo[0]);
+            operand(sh.e[2][lane], sh.e[3][lane], hi[1], lo[1]);
+            const float total = gate[kChunkRow * kChunk + kTotal];
             const uint32_t at = base + (lane & 15) * I::kPitch + part * ROWS * 2 + (lane >> 4) * 16;
 #pragma unroll
             for (int p = 0; p < NT / 2; ++p) {
@@ -725,7 +802,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], c1[t][r] * down[r >> 1]);
+                        s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], c1[t][r] * e_down[r >> 1]);
             }
         }
     }
