@@ -30,13 +30,18 @@
 // then, split into limbs, the left operand of the next product without leaving
 // the registers, and the right operands (keys, queries, T, P) are the same for
 // all columns: they are staged in shared memory by bulk copies one chunk ahead.
-// Four warps of a group (two for small or odd k_dim) hold a part of S's rows
-// each and follow the chain from chunk to chunk; the sums over k_dim, X and U
-// go between them through shared memory, a part of the tokens each. Two more
-// take S's limbs and U from there and compute half of the chunk's outputs
-// each, off the chain, up to a chunk behind.
+// Two warps of a group hold half of S's rows each and follow the chain from
+// chunk to chunk; the sums over k_dim, X and U go between them through shared
+// memory, half of the tokens each. Two more take S's limbs and U from there and
+// compute half of the chunk's outputs each, off the chain, up to a chunk behind.
+// One sequence is bound by that chain (about 3000 cycles a chunk of 32 tokens at
+// k_dim 128 and f32: a conversion, a product, an exchange, three times over); a
+// batch by how many groups share a multiprocessor, four where shared memory
+// allows.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "gated_delta.cuh"
 
@@ -375,14 +380,14 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
 
 // ------------------------------------------------------------------- scan
 
-// A scan block: kGroups groups of 16 columns of S, each with kParts warps for S
+// A scan block: GROUPS groups of 16 columns of S, each with kParts warps for S
 // and two for the outputs.
-constexpr int kGroups = 2, kCols = kGroups * 16;
 constexpr int kStages = 3;  // the chunk being read, the next, and the one whose outputs are still to come
-template <int DK>
+constexpr int kMaxShared = 227 * 1024;
+template <int DK, int GROUPS>
 struct Split {
-    static constexpr int kParts = DK % 64 ? 2 : 4;
-    static constexpr int kHolders = kGroups * kParts * 32, kThreads = kHolders + kGroups * 64;
+    static constexpr int kParts = 2, kCols = GROUPS * 16;
+    static constexpr int kHolders = GROUPS * kParts * 32, kThreads = kHolders + GROUPS * 64;
     static constexpr int kRows = DK / kParts;    // rows of S a warp holds
     static constexpr int kTiles = 4 / kParts;    // tiles of 8 tokens whose X and U it computes
 };
@@ -393,22 +398,22 @@ struct Split {
 template <int DK>
 struct Handoff {
     uint4 hi[DK / 16][32], lo[DK / 16][32];
-    float2 down[Split<DK>::kParts][32], scale[32];
+    float2 down[2][32], scale[32];
     uint4 u[4][32];
 };
 // And among each other, within a chunk: parts of S^T K^T with the largest
 // magnitudes of their rows of S and V, X, and U scaled to the chunk's end.
 template <int DK>
 struct Shared {
-    float4 y[Split<DK>::kParts][4][32];
-    float4 top[Split<DK>::kParts][8];  // S and V of a row, and of the row 8 on
+    float4 y[2][4][32];
+    float4 top[2][8];  // S and V of a row, and of the row 8 on
     uint4 x[4][32], e[4][32];
 };
 
-template <int DK, int LIMBS>
+template <int DK, int LIMBS, int GROUPS>
 constexpr int scan_smem() {
-    return kStages * (Image<DK, LIMBS>::kBytes + kImageT) + 2 * kGroups * (int)sizeof(Handoff<DK>) +
-           kGroups * (int)sizeof(Shared<DK>);
+    return kStages * (Image<DK, LIMBS>::kBytes + kImageT) + 2 * GROUPS * (int)sizeof(Handoff<DK>) +
+           GROUPS * (int)sizeof(Shared<DK>);
 }
 
 // Named barriers of a group: `threads` of them arrive in all.
@@ -461,30 +466,28 @@ __device__ __forceinline__ void operand(const uint4& a, const uint4& b, uint32_t
     lo[0] = a.z, lo[1] = a.w, lo[2] = b.z, lo[3] = b.w;
 }
 
-template <typename T, int DK, int LIMBS>
-__global__ void __launch_bounds__(Split<DK>::kThreads, 1)
+template <typename T, int DK, int LIMBS, int GROUPS>
+__global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
     delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab, const uint8_t* __restrict__ images,
                       const uint8_t* __restrict__ images_t, int* err) {
     using I = Image<DK, LIMBS>;
-    using L = Split<DK>;
+    using L = Split<DK, GROUPS>;
     constexpr int PARTS = L::kParts, ROWS = L::kRows, NT = ROWS / 8, KS = ROWS / 16, TILES = L::kTiles;
     constexpr int kStage = I::kBytes + kImageT;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(8) uint64_t arrived[kStages];
+    __shared__ __align__(8) uint64_t arrived[kStages], ready[GROUPS][2][2];  // ready: S's limbs, U; even and odd chunks
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the warps of S first, then those of the outputs, spread evenly over the schedulers
     const bool holds = threadIdx.x < L::kHolders;
-    const int group = holds ? warp / PARTS : (warp - kGroups * PARTS) / 2;
-    const int part = holds ? warp % PARTS : (warp - kGroups * PARTS) % 2;
+    const int group = holds ? warp / PARTS : (warp - GROUPS * PARTS) / 2;
+    const int part = holds ? warp % PARTS : (warp - GROUPS * PARTS) % 2;
     Handoff<DK>* const hands = reinterpret_cast<Handoff<DK>*>(smem + kStages * kStage) + group * 2;
-    Shared<DK>& sh = reinterpret_cast<Shared<DK>*>(smem + kStages * kStage + 2 * kGroups * sizeof(Handoff<DK>))[group];
-    // Barriers: chunk written out, then a group's: among the warps of S, S's
-    // limbs handed on, U handed on. The warps of S only arrive at the last two
-    // and may be a chunk ahead there, so that even and odd chunks have their own:
-    // one is used again two chunks on, behind the outputs' arrival at bar_done
-    // for the chunk that used it before.
-    const int bar_done = 1, bar_g = 3 + group * 5, bar_s = bar_g + 1, bar_u = bar_g + 3;
-    constexpr int kOfGroup = (PARTS + 2) * 32;
+    Shared<DK>& sh = reinterpret_cast<Shared<DK>*>(smem + kStages * kStage + 2 * GROUPS * sizeof(Handoff<DK>))[group];
+    // Named barriers: chunk written out (even, odd), and among a group's warps of
+    // S. Those only arrive at `ready` and may be a chunk ahead of the outputs
+    // there, so that even and odd chunks have their own: one is used again two
+    // chunks on, behind the outputs' arrival at bar_done for its last chunk.
+    const int bar_done = 1, bar_g = 3 + group;
     int b = blockIdx.x;
     const int cb = b % a.col_blocks;
     b /= a.col_blocks;
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
     const Seq seq = sequence_at(tab, b / a.v_heads);
     const int hk = key_head(a, h);
     const int chunks = (seq.len + kChunk - 1) / kChunk;
-    const int j0 = cb * kCols + group * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
+    const int j0 = cb * L::kCols + group * 16 + (lane >> 2), j1 = j0 + 8;  // the lane's two columns of S
     const bool in0 = j0 < a.v_dim, in1 = j1 < a.v_dim;
     const int tc = (lane & 3) * 2;
     const int d0 = part * ROWS + tc;  // its first row of S (warps of S)
@@ -500,6 +503,10 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_addr(&arrived[i])) : "memory");
+        for (int i = 0; i < GROUPS * 4; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_addr(&ready[i / 4][i / 2 % 2][i % 2])),
+                         "n"(PARTS)
+                         : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -511,17 +518,24 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
         bulk_copy(dst + I::kBytes, images_t + (tile * a.v_heads + h) * kImageT, kImageT, bar);
     };
     if (threadIdx.x == 0) stage(0);
-    // Waits for chunk c's copy. Where one does not come (a second is long past),
-    // the thread goes on without waiting, so that no other is left behind at a
+    // Waits for a phase. Where it does not come (a second is long past), the
+    // thread goes on without waiting, so that no other is left behind at a
     // barrier, and the call is reported as timed out.
     bool there = true;
-    auto wait = [&](int c) {
+    auto wait = [&](const uint64_t* bar, int parity) {
         if (!there) return;
-        there = bulk_wait(shared_addr(&arrived[c % kStages]), (c / kStages) & 1);
+        there = bulk_wait(shared_addr(bar), parity);
         if (!there) {
-            bulk_wait(shared_addr(&arrived[c % kStages]), (c / kStages) & 1);  // nothing in flight when the block ends
+            bulk_wait(shared_addr(bar), parity);  // no copy in flight when the block ends
             atomicExch(err, 1);
         }
+    };
+    auto wait_chunk = [&](int c) { wait(&arrived[c % kStages], (c / kStages) & 1); };
+    auto wait_ready = [&](int what, int c) { wait(&ready[group][what][c & 1], (c >> 1) & 1); };
+    auto set_ready = [&](int what, int c) {  // by every warp of S
+        __syncwarp();
+        if (lane == 0)
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_addr(&ready[group][what][c & 1])) : "memory");
     };
     const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
     const uint32_t half_b = ((lane >> 3) & 1) * 16;             // and its half of a row
@@ -529,13 +543,13 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
     if (!holds) {  // ---- outputs of tokens part * 16 .. + 15
         T* O = static_cast<T*>(a.o) + (int64_t)seq.row * a.o_stride + (int64_t)h * a.v_dim;
         for (int c = 0; c < chunks; ++c) {
-            wait(c);
+            wait_chunk(c);
             const uint8_t* image = smem + (c % kStages) * kStage;
             const Handoff<DK>& hand = hands[c & 1];
             const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
             const uint32_t q_at = shared_addr(image) + LIMBS * I::kLimb + (part * 16 + lane_b) * I::kPitch + half_b;
             float out[2][4] = {};
-            group_sync(bar_s + (c & 1), kOfGroup);
+            wait_ready(0, c);
 #pragma unroll
             for (int k = 0; k < PARTS; ++k) {  // the parts of k_dim, each with its own row factors
                 float o1[2][4] = {};
@@ -568,7 +582,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) out[t][r] = fmaf(o1[t][r], r < 2 ? down.x : down.y, out[t][r]);
             }
-            group_sync(bar_u + (c & 1), kOfGroup);
+            wait_ready(1, c);
             uint32_t hi[2][4], lo[2][4];
             float c1[2][4] = {};
             operand(hand.u[0][lane], hand.u[1][lane], hi[0], lo[0]);
@@ -623,7 +637,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
         }
     const T* V = static_cast<const T*>(a.v) + (int64_t)seq.row * a.v_stride + (int64_t)h * a.v_dim;
     V += (int64_t)(part * TILES * 8 + tc) * a.v_stride;
-    float v[TILES][4];
+    T coming[TILES][4];  // the next chunk's values, not touched before it begins
     auto fetch = [&](int c) {
         const T* row = V + (int64_t)c * kChunk * a.v_stride;
         const int left = seq.len - c * kChunk - part * TILES * 8 - tc;  // tokens from the lane's first
@@ -632,7 +646,8 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const bool in = t * 8 + (r & 1) < left && (r < 2 ? in0 : in1);
-                v[t][r] = in ? to_f32(row[(t * 8 + (r & 1)) * a.v_stride + (r < 2 ? j0 : j1)]) : 0.0f;
+                from_f32(coming[t][r], 0.0f);
+                if (in) coming[t][r] = row[(t * 8 + (r & 1)) * a.v_stride + (r < 2 ? j0 : j1)];
             }
     };
     fetch(0);
@@ -640,11 +655,12 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
         // chunk c - 2 is written out, so its stage can take chunk c + 1 and its handoff this chunk's
         if (c >= 2) group_sync(bar_done + (c & 1), L::kThreads);
         if (threadIdx.x == 0 && c + 1 < chunks && there) stage(c + 1);
-        wait(c);
+        wait_chunk(c);
         Handoff<DK>& hand = hands[c & 1];
         const uint8_t* image = smem + (c % kStages) * kStage;
         const uint32_t base = shared_addr(image);
         const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
+        float v[TILES][4];
         {  // this warp's part of S^T K^T
             uint32_t hi[KS][4], lo[KS][4];
             float down[2], most[2], y[4][4] = {};
@@ -652,6 +668,8 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
             float v0 = 0.0f, v1 = 0.0f;
 #pragma unroll
             for (int k = 0; k < TILES; ++k) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[k][r] = to_f32(coming[k][r]);
                 v0 = fmaxf(v0, fmaxf(fabsf(v[k][0]), fabsf(v[k][1])));
                 v1 = fmaxf(v1, fmaxf(fabsf(v[k][2]), fabsf(v[k][3])));
             }
@@ -694,7 +712,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
         }
         // S's limbs are handed on only now: the outputs' products take the tensor
         // cores while this chain exchanges and scales, not before
-        group_arrive(bar_s + (c & 1), kOfGroup);
+        set_ready(0, c);
         group_sync(bar_g, PARTS * 32);
         // the same bounds in every warp: no row of X or U is larger
         float up[2], down[2];
@@ -768,7 +786,7 @@ __global__ void __launch_bounds__(Split<DK>::kThreads, 1)
                 sh.e[t][lane] = tile_limbs(u0 * e.x, u1 * e.y, u2 * e.x, u3 * e.y, e_up[0], e_up[1]);
             }
         }
-        group_arrive(bar_u + (c & 1), kOfGroup);
+        set_ready(1, c);
         group_sync(bar_g, PARTS * 32);
         // S <- e^{G_C} S + U^T K, with U scaled to the chunk's end
         {
@@ -857,12 +875,28 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
         int64_t end = i, live = 0;  // sequences [i, end), `live` of them with tokens
         while (end < d.n_seq && live < group) live += off[end + 1] > off[end], ++end;
         for (int64_t t = 0; live > 0;) {
-            const int64_t step = per_sequence(live) * kChunk;
+            // the longest piece (in chunks, of every sequence that still has tokens) that fits
+            int64_t fits = 1, over = cap + 1;
+            while (over - fits > 1) {
+                const int64_t mid = (fits + over) / 2;
+                int64_t sum = 0;
+                for (int64_t k = i; k < end; ++k) {
+                    const int64_t left = (off[k + 1] - off[k] - t + kChunk - 1) / kChunk;
+                    sum += left <= 0 ? 0 : left < mid ? left : mid;
+                }
+                if (sum <= cap) fits = mid;
+                else over = mid;
+            }
+            const int64_t step = fits * kChunk;
+            // the longest first, so that no long one is left to start last
+            int64_t order[kSeqGroup], count = 0, left = 0;
+            for (int64_t k = i; k < end; ++k)
+                if (off[k + 1] - off[k] > t) order[count++] = k;
+            std::stable_sort(order, order + count,
+                             [&](int64_t x, int64_t y) { return off[x + 1] - off[x] > off[y + 1] - off[y]; });
             SeqTable tab = ragged_table();
-            int64_t left = 0;
-            for (int64_t k = i; k < end; ++k) {
-                const int64_t len = off[k + 1] - off[k] - t;
-                if (len <= 0) continue;
+            for (int64_t n = 0; n < count; ++n) {
+                const int64_t k = order[n], len = off[k + 1] - off[k] - t;
                 add_sequence(tab, k, off[k] + t, len < step ? len : step, kChunk);
                 left += len > step;
             }
@@ -876,24 +910,44 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
     return STRATA_OK;
 }
 
-template <typename T, int DK, int LIMBS>
-int enqueue(strata_ctx* ctx, const strata_gated_delta& d, DeltaArgs a, uint8_t* work, cudaStream_t s) {
-    auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
-    auto scan = delta_scan_kernel<T, DK, LIMBS>;
-    constexpr int sp = prepare_smem<DK, LIMBS>(), ss = scan_smem<DK, LIMBS>();
-    cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, sp);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ss);
+template <typename T, int DK, int LIMBS, int GROUPS>
+int enqueue_scan(strata_ctx* ctx, DeltaArgs a, const SeqTable& t, const uint8_t* images, const uint8_t* images_t,
+                 cudaStream_t s) {
+    using L = Split<DK, GROUPS>;
+    auto scan = delta_scan_kernel<T, DK, LIMBS, GROUPS>;
+    constexpr int smem = scan_smem<DK, LIMBS, GROUPS>();
+    static_assert(smem <= kMaxShared - 1024, "a block's shared memory");
+    const cudaError_t e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
-    a.col_blocks = (a.v_dim + kCols - 1) / kCols;
+    a.col_blocks = (a.v_dim + L::kCols - 1) / L::kCols;
+    const int64_t grid = (int64_t)t.n * a.v_heads * a.col_blocks;
+    if (grid > kMaxTokens) return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %d sequences of %d heads", t.n, a.v_heads);
+    scan<<<(unsigned)grid, L::kThreads, smem, s>>>(a, t, images, images_t, ctx->err_dev);
+    return check_launch(ctx, "gated_delta scan kernel");
+}
+
+template <typename T, int DK, int LIMBS>
+int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
+    auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
+    constexpr int smem = prepare_smem<DK, LIMBS>();
+    const cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
     const uint64_t keys = chunk_bytes(d).keys;
     return plan_chunks(d, [&](const SeqTable& t, int64_t tiles) {
-        const int64_t gp = tiles * a.k_heads, gs = (int64_t)t.n * a.v_heads * a.col_blocks;
-        if (gp > kMaxTokens || gs > kMaxTokens)
-            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.v_heads);
+        const int64_t grid = tiles * a.k_heads;
+        if (grid > kMaxTokens)
+            return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.k_heads);
         uint8_t* images_t = work + keys * (uint64_t)tiles;
-        prepare<<<(unsigned)gp, kThreads, sp, s>>>(a, t, work, images_t);
-        scan<<<(unsigned)gs, Split<DK>::kThreads, ss, s>>>(a, t, work, images_t, ctx->err_dev);
-        return check_launch(ctx, "gated_delta chunk kernels");
+        prepare<<<(unsigned)grid, kThreads, smem, s>>>(a, t, work, images_t);
+        const int rc = check_launch(ctx, "gated_delta prepare kernel");
+        if (rc) return rc;
+        // blocks of two groups while they all run side by side (the shortest
+        // chain), of four where there are more and four fit
+        if constexpr (scan_smem<DK, LIMBS, 4>() <= kMaxShared - 1024) {
+            if ((int64_t)t.n * a.v_heads * ((a.v_dim + 31) / 32) > ctx->sm_count && a.v_dim > 32)
+                return enqueue_scan<T, DK, LIMBS, 4>(ctx, a, t, work, images_t, s);
+        }
+        return enqueue_scan<T, DK, LIMBS, 2>(ctx, a, t, work, images_t, s);
     });
 }
 
