@@ -153,6 +153,20 @@ __device__ __forceinline__ float decay(float x) {
     return y;
 }
 
+// Reduces 16 values of a lane across the warp: v[0] becomes value lane / 2's.
+template <typename F>
+__device__ __forceinline__ void reduce_rows(float (&v)[16], F op) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 8, o = 16; n > 0; n >>= 1, o >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float keep = lane & o ? v[i + n] : v[i], send = lane & o ? v[i] : v[i + n];
+            v[i] = op(keep, __shfl_xor_sync(0xFFFFFFFFu, send, o));
+        }
+    v[0] = op(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 1));
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
@@ -219,35 +233,46 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             for (int e = 0; e < PER; ++e) x[r][e] = i < n && lane * PER + e < a.k_dim ? to_f32(p[e]) : 0.0f;
         }
     }
+    {
+        float most[16], squares[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int i = warp * 8 + (r & 7);
-        float m = 0.0f, ss = 0.0f;
+        for (int r = 0; r < 16; ++r) {
+            most[r] = squares[r] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) m = fmaxf(m, fabsf(x[r][e])), ss = fmaf(x[r][e], x[r][e], ss);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+            for (int e = 0; e < PER; ++e)
+                most[r] = fmaxf(most[r], fabsf(x[r][e])), squares[r] = fmaf(x[r][e], x[r][e], squares[r]);
         }
+        // lane 2 r (and the next) ends up with row r's
+        reduce_rows(most, [](float a, float b) { return fmaxf(a, b); });
+        reduce_rows(squares, [](float a, float b) { return a + b; });
         float up, down;
-        power_for(m, up, down);
-        __half hi[PER], lo[PER];
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            hi[e] = __float2half_rn(x[r][e] * up);
-            lo[e] = __float2half_rn(x[r][e] * up - __half2float(hi[e]));
-        }
-        uint8_t* at = smem + (r < 8 ? 0 : LIMBS * I::kLimb) + i * I::kPitch + lane * PER * 2;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            reinterpret_cast<__half*>(at)[e] = hi[e];
-            if (LIMBS == 2) reinterpret_cast<__half*>(at + I::kLimb)[e] = lo[e];
-        }
-        if (lane == 0) {
-            const float f = a.norm ? 1.0f / sqrtf(ss + a.eps) : 1.0f;
+        power_for(most[0], up, down);
+        if (!(lane & 1)) {
+            const int r = lane >> 1, i = warp * 8 + (r & 7);
+            const float f = a.norm ? 1.0f / sqrtf(squares[0] + a.eps) : 1.0f;
             (r < 8 ? fk : fq)[i] = i < n ? (r < 8 ? down * f : down * f * a.scale) : 0.0f;
-            if (r < 8) kn[i] = i < n ? sqrtf((float)DK * ss) * f : 0.0f;
+            if (r < 8) kn[i] = i < n ? sqrtf((float)DK * squares[0]) * f : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = warp * 8 + (r & 7);
+            const float scale = __shfl_sync(0xFFFFFFFFu, up, r * 2);
+            uint8_t* at = smem + (r < 8 ? 0 : LIMBS * I::kLimb) + i * I::kPitch + lane * PER * 2;
+            Pack<__half, PER> hi, lo;
+#pragma unroll
+            for (int e = 0; e + 1 < PER; e += 2) {
+                uint32_t h, l;
+                split(x[r][e] * scale, x[r][e + 1] * scale, h, l);
+                const __half2 h2 = *reinterpret_cast<const __half2*>(&h), l2 = *reinterpret_cast<const __half2*>(&l);
+                hi.v[e] = __low2half(h2), hi.v[e + 1] = __high2half(h2);
+                lo.v[e] = __low2half(l2), lo.v[e + 1] = __high2half(l2);
+            }
+            if (PER & 1) {
+                hi.v[PER - 1] = __float2half_rn(x[r][PER - 1] * scale);
+                lo.v[PER - 1] = __float2half_rn(x[r][PER - 1] * scale - __half2float(hi.v[PER - 1]));
+            }
+            *reinterpret_cast<Pack<__half, PER>*>(at) = hi;
+            if (LIMBS == 2) *reinterpret_cast<Pack<__half, PER>*>(at + I::kLimb) = lo;
         }
     }
     __syncthreads();
