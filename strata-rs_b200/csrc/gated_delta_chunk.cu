@@ -215,6 +215,15 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
     const int t0 = (tile - seq.tile0) * kChunk, n = min(kChunk, seq.len - t0);
     const int64_t row = (int64_t)seq.row + t0;
 
+    const int per = a.v_heads / a.k_heads;
+    auto value_head = [&](int task) { return a.tiled ? hk + (task >> 1) * a.k_heads : hk * per + (task >> 1); };
+    auto gate_of = [&](int h, float& g, float& beta) {
+        g = lane < n ? a.gate[(row + lane) * a.gate_stride + h] : 0.0f;
+        beta = lane < n ? a.beta[(row + lane) * a.beta_stride + h] : 0.0f;
+    };
+    float g_first = 0.0f, b_first = 0.0f;  // the warp's first task's, there by the time they are needed
+    if (warp < 2 * per) gate_of(value_head(warp), g_first, b_first);
+
     const T* K = static_cast<const T*>(a.k) + row * a.k_stride + (int64_t)hk * a.k_dim + lane * PER;
     const T* Q = static_cast<const T*>(a.q) + row * a.q_stride + (int64_t)hk * a.k_dim + lane * PER;
     const bool whole = a.k_dim == DK && PER * sizeof(T) >= 4 && a.k_stride % PER == 0 && a.q_stride % PER == 0 &&
@@ -275,10 +284,14 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             if (LIMBS == 2) *reinterpret_cast<Pack<__half, PER>*>(at + I::kLimb) = lo;
         }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the copy below reads what was just written
     __syncthreads();
-    {  // the image, as the scan will stage it
-        uint4* out = reinterpret_cast<uint4*>(images + (int64_t)blockIdx.x * I::kBytes);
-        for (int i = threadIdx.x; i < I::kBytes / 16; i += kThreads) out[i] = reinterpret_cast<const uint4*>(smem)[i];
+    if (threadIdx.x == 0) {  // the image, as the scan will stage it, on its way out
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                         images + (int64_t)blockIdx.x * I::kBytes),
+                     "r"(shared_addr(smem)), "r"(I::kBytes)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
     {  // warps 0, 1: K K^T; 2, 3: Q K^T; 16 rows each, up to the diagonal
         const int m0 = (warp & 1) * 16;
@@ -317,15 +330,14 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
                 out[i][j] = (c[t][r] + s[t][r]) * f[i] * fk[j];
             }
     }
+    // the image is out of shared memory before the scratch takes its place
+    if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncthreads();
-    const int per = a.v_heads / a.k_heads;
     for (int task = warp; task < 2 * per; task += kThreads / 32) {
-        const int m = task >> 1;
-        const int h = a.tiled ? hk + m * a.k_heads : hk * per + m;
-        float g = 0.0f, beta = 0.0f;
+        const int h = value_head(task);
+        float g = g_first, beta = b_first;
+        if (task != warp) gate_of(h, g, beta);
         if (lane < n) {
-            g = a.gate[(row + lane) * a.gate_stride + h];
-            beta = a.beta[(row + lane) * a.beta_stride + h];
             gates(a, h, g, beta);
             // e^-10000 is zero; a sum of these stays a number, so that differences do
             if (g < -1e4f) g = -1e4f;
