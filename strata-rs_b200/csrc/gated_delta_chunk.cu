@@ -954,7 +954,8 @@ int enqueue_scan(strata_ctx* ctx, DeltaArgs a, const SeqTable& t, const uint8_t*
     auto scan = delta_scan_kernel<T, DK, LIMBS, GROUPS>;
     constexpr int smem = scan_smem<DK, LIMBS, GROUPS>();
     static_assert(smem <= kMaxShared - 1024, "a block's shared memory");
-    const cudaError_t e = cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> asked;
+    const cudaError_t e = allow_shared(scan, smem, asked, ctx->device);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
     a.col_blocks = (a.v_dim + L::kCols - 1) / L::kCols;
     const int64_t grid = (int64_t)t.n * a.v_heads * a.col_blocks;
@@ -967,7 +968,8 @@ template <typename T, int DK, int LIMBS>
 int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
     auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
     constexpr int smem = prepare_smem<DK, LIMBS>();
-    const cudaError_t e = cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> asked;
+    const cudaError_t e = allow_shared(prepare, smem, asked, ctx->device);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
     const uint64_t keys = chunk_bytes(d).keys;
     return plan_chunks(d, [&](const SeqTable& t, int64_t tiles) {

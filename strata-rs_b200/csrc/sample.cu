@@ -1367,8 +1367,8 @@ extern "C" int strata_cuda_sample_dev(strata_ctx* ctx, const float* logits_dev, 
     SampleArgs a{logits_dev, stride, temperature_dev, top_k_dev, top_p_dev, min_p_dev, uniform_dev, ids_dev,
                  logprobs_dev, (int)vocab, (int)slice, resident, packs};
     auto kernel = packs ? sample_kernel<true> : sample_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kListBytes + kMaxSlice);
+    static std::atomic<uint64_t> asked[2];
+    cudaError_t e = allow_shared(kernel, kListBytes + kMaxSlice, asked[packs], ctx->device);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(sample)");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ranks));

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "runtime.cuh"
@@ -23,6 +24,17 @@ struct DeviceGuard {
         if (before >= 0) cudaSetDevice(before);
     }
 };
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device:
+// asked for once per device.
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t>& asked, int device) {
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (asked.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // The sequences of one launch, by value in the kernel's parameters: no copy
 // to wait for, nothing to allocate, and a captured graph holds its own. Empty

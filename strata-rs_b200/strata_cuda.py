@@ -217,6 +217,7 @@ class ShortConv:
         self._rows = _sequences(d, n_seq, seq_len, offsets)
         d.channels, d.taps, d.x_stride, d.y_stride = channels, taps, x_stride, y_stride
         d.dtype, d.silu = dtype, int(silu)
+        self.ref = C.byref(d)
 
 
 class GatedDelta:
@@ -235,12 +236,13 @@ class GatedDelta:
         d.gate_stride, d.beta_stride = gate_stride, beta_stride
         d.scale = max(k_dim, 1) ** -0.5 if scale is None else scale
         d.l2_eps, d.dtype, d.tiled, d.raw_gates = l2_eps, dtype, int(tiled), int(raw_gates)
+        self.ref = C.byref(d)
 
 
 def gated_delta_work_bytes(shape: GatedDelta) -> int:
     """Bytes of device workspace gated_delta_dev needs for this shape (0: none)."""
     v = C.c_uint64()
-    rc = lib().strata_cuda_gated_delta_work_bytes(C.byref(shape.desc), C.byref(v))
+    rc = lib().strata_cuda_gated_delta_work_bytes(shape.ref, C.byref(v))
     if rc != OK:
         raise BackendError(rc, "gated_delta: bad shape")
     return v.value
@@ -731,29 +733,31 @@ class Context:
         self.check(lib().strata_cuda_moe_ffn_ep_dev(self.h, layer.handle, x_ptr, logits_ptr or None, tokens, out_ptr,
                                                     stream or None))
 
-    # ---- the sequence operators (strata_sequence.h), on device pointers
+    # ---- the sequence operators (strata_sequence.h), on device pointers (0: NULL).
+    # One token of one sequence is a few microseconds on the device: nothing is
+    # converted here that ctypes does not convert anyway.
 
     def short_conv_dev(self, shape: ShortConv, x_ptr: int, w_ptr: int, bias_ptr: int, state_ptr: int, y_ptr: int,
                        stream: int = 0):
-        self.check(lib().strata_cuda_short_conv_dev(self.h, C.byref(shape.desc), x_ptr or None, w_ptr or None,
-                                                    bias_ptr or None, state_ptr or None, y_ptr or None,
-                                                    stream or None))
+        rc = _lib.strata_cuda_short_conv_dev(self.h, shape.ref, x_ptr, w_ptr, bias_ptr, state_ptr, y_ptr, stream)
+        if rc:
+            self.check(rc)
 
     def gated_delta_dev(self, shape: GatedDelta, q_ptr: int, k_ptr: int, v_ptr: int, gate_ptr: int, beta_ptr: int,
                         coef_ptr: int, shift_ptr: int, state_ptr: int, o_ptr: int, work_ptr: int = 0,
                         work_bytes: int = 0, stream: int = 0):
-        self.check(lib().strata_cuda_gated_delta_dev(self.h, C.byref(shape.desc), q_ptr or None, k_ptr or None,
-                                                     v_ptr or None, gate_ptr or None, beta_ptr or None,
-                                                     coef_ptr or None, shift_ptr or None, state_ptr or None,
-                                                     o_ptr or None, work_ptr or None, work_bytes, stream or None))
+        rc = _lib.strata_cuda_gated_delta_dev(self.h, shape.ref, q_ptr, k_ptr, v_ptr, gate_ptr, beta_ptr, coef_ptr,
+                                              shift_ptr, state_ptr, o_ptr, work_ptr, work_bytes, stream)
+        if rc:
+            self.check(rc)
 
     def sample_dev(self, logits_ptr: int, rows: int, vocab: int, uniform_ptr: int, ids_ptr: int,
                    logprobs_ptr: int = 0, temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0,
                    min_p_ptr: int = 0, stride: int = 0, stream: int = 0):
-        self.check(lib().strata_cuda_sample_dev(self.h, logits_ptr or None, rows, vocab, stride,
-                                                temperature_ptr or None, top_k_ptr or None, top_p_ptr or None,
-                                                min_p_ptr or None, uniform_ptr or None, ids_ptr or None,
-                                                logprobs_ptr or None, stream or None))
+        rc = _lib.strata_cuda_sample_dev(self.h, logits_ptr, rows, vocab, stride, temperature_ptr, top_k_ptr,
+                                         top_p_ptr, min_p_ptr, uniform_ptr, ids_ptr, logprobs_ptr, stream)
+        if rc:
+            self.check(rc)
 
     def set_gemm_terms(self, terms: int):
         self.check(lib().strata_cuda_set_gemm_terms(self.h, terms))
