@@ -122,8 +122,9 @@ struct Shared {
 struct Row {
     const SampleArgs& a;
     Shared& sh;
-    const float* x;  // this block's slice, in shared or global memory
-    int base, n;     // its first index and its number of elements
+    const float* x;    // this block's slice, in shared or global memory; or a list
+    const int* index;  // a list's indices (nullptr: x is a slice)
+    int base, n;       // its first index and its number of elements
     int seg;         // elements of a warp (contiguous)
     int rank, ranks;
     int turn, hturn;
@@ -138,12 +139,14 @@ struct Row {
         return ranks == 1 ? p : cluster.map_shared_rank(const_cast<T*>(p), k);
     }
 
+    __device__ __forceinline__ int at(int i) const { return index ? index[i] : base + i; }
+
     // every element of this warp's segment, 32 at a time: f(value, index)
     template <typename F>
     __device__ __forceinline__ void each(F f) {
         const int lo = (threadIdx.x >> 5) * seg, hi = min(lo + seg, n);
 #pragma unroll 4
-        for (int i = lo + (threadIdx.x & 31); i < hi; i += 32) f(x[i], base + i);
+        for (int i = lo + (threadIdx.x & 31); i < hi; i += 32) f(x[i], at(i));
     }
 
     // Sums (a, b, n) and bounds (lo, hi) over the cluster, the same in every thread.
@@ -268,7 +271,7 @@ struct Row {
                 const bool hit = i + lane < hi && key_of(x[i + lane]) == key;
                 const unsigned m = __ballot_sync(0xFFFFFFFFu, hit);
                 if (seen + __popc(m) >= want) {
-                    if (hit && seen + __popc(m & ((1u << lane) - 1u)) + 1 == want) found = (uint32_t)(base + i + lane);
+                    if (hit && seen + __popc(m & ((1u << lane) - 1u)) + 1 == want) found = (uint32_t)at(i + lane);
                     break;
                 }
                 seen += __popc(m);
@@ -330,7 +333,11 @@ __device__ Cut cut_top_k(Row& r, float top, uint32_t k) {
     }
 }
 
-__device__ Cut cut_top_p(Row& r, float top, double p, Cut cut) {
+// above: the mass of kept tokens larger than all of the view's; total: the kept
+// tokens' mass (0: above and the view's). Where the border lies outside the view
+// the cut stays as it was, and `holds` says so.
+__device__ Cut cut_top_p(Row& r, float top, double p, Cut cut, double above = 0.0, double total = 0.0,
+                         bool* holds = nullptr) {
     // the kept tokens' mass, and their histogram
     Part z{0.0, 0.0, 0u, 0u, 0};
     const uint32_t count = r.histogram([&](uint32_t* h) {
@@ -342,7 +349,12 @@ __device__ Cut cut_top_p(Row& r, float top, double p, Cut cut) {
             }
         });
     });
-    const double target = p * r.reduce(z).a;
+    const double mass = r.reduce(z).a;
+    const double target = p * (total > 0.0 ? total : above + mass) - above;
+    if (holds) {
+        *holds = target > 0.0 && target <= mass;
+        if (!*holds) return cut;
+    }
     const double guess = (double)count * exp(-((double)threadIdx.x + 0.5) / (double)kBinsPerNat);
     double before;
     int bin = r.border<double>(count, guess, target, before), way = 0;
@@ -753,7 +765,22 @@ __device__ bool settle_list(Shared& sh, const float* list, unsigned long long* o
         const int i = e * kThreads + threadIdx.x;
         mine[e] = i < listed ? (unsigned long long)~key_of(list[i]) << 32 | (unsigned)i : ~0ull;
     }
-    sort_block<PER>(mine, order);
+    if (PER == 1 && listed <= kThreads / 2) {
+        // few: every token counts those before it
+        order[threadIdx.x] = mine[0];
+        __syncthreads();
+        int rank = 0;
+        for (int j = 0; j < (listed + 1) / 2; ++j) {
+            const ulonglong2 w = reinterpret_cast<const ulonglong2*>(order)[j];
+            rank += (w.x < mine[0]) + (w.y < mine[0]);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < listed) order[rank] = mine[0];
+        __syncthreads();
+        if ((int)threadIdx.x < listed) mine[0] = order[threadIdx.x];
+    } else {
+        sort_block<PER>(mine, order);
+    }
     int kept = k > 0 && k < listed ? k : listed;
     bool holds = true;
     if (p < 1.0f) {
@@ -805,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const float* logits = a.logits + row * a.stride;
     const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
     const int seg = ((n + kWarps * 256 - 1) / (kWarps * 256)) * 256;
-    Row r{a, sh, a.resident ? held : logits + base, base, n, seg, rank, ranks, 0, 0, cluster};
+    Row r{a, sh, a.resident ? held : logits + base, nullptr, base, n, seg, rank, ranks, 0, 0, cluster};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int lo = min(warp * seg, n), hi = min(lo + seg, n);
     const int part = ((seg / 256 + kSub - 1) / kSub) * 256;  // elements of a part of the segment
@@ -1238,9 +1265,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                     return settle_list<decltype(per)::value>(sh, list, order, weight_of, listed, k, p, above, all, sure,
                                                              list_mass, kept_weight);
                 };
-                holds = listed <= kThreads       ? settle(std::integral_constant<int, 1>())
-                        : listed <= 2 * kThreads ? settle(std::integral_constant<int, 2>())
-                                                 : settle(std::integral_constant<int, kList / kThreads>());
+                if (listed <= kThreads) {
+                    holds = settle(std::integral_constant<int, 1>());
+                } else if (listed <= 2 * kThreads) {
+                    holds = settle(std::integral_constant<int, 2>());
+                } else {
+                    // too long to sort in time: the search by key ranges, on the list (17 us against 37 at 4096)
+                    Row l{a, sh, list, list_index, 0, listed, ((listed + kThreads - 1) / kThreads) * 32, 0, 1, 0, 0, cluster};
+                    Cut cut{1u, INT_MAX};
+                    if (k > 0 && k < listed) cut = cut_top_k(l, top, (uint32_t)k);
+                    if (p < 1.0f) {
+                        const double scale = sums_all ? exp(ref - (double)top) : 1.0;
+                        bool inside = true;
+                        cut = cut_top_p(l, top, (double)p, cut, above * scale, all * scale, sums_all ? &inside : nullptr);
+                        holds = inside || !sure;  // behind a list that ends at min-p it cuts nothing
+                    }
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < listed; i += kThreads)
+                        weight_of[i] = cut.keeps(key_of(list[i]), list_index[i]) ? kept_weight(list[i]) : 0.0;
+                    __syncthreads();
+                }
             }
             if (!holds) {
                 if (threadIdx.x == 0) sh.won = -2;
