@@ -80,14 +80,17 @@ int strata_cuda_short_conv_dev(strata_ctx *ctx, const strata_short_conv *desc, c
  * Where l2_eps >= 0, q and k are first divided by sqrt(sum of squares + l2_eps)
  * per head; a negative l2_eps takes them as they are. k_dim 1..256, v_dim 1..8192.
  *
- * Products and sums are f32 or carry at least f32's 24 bits less two (limb
- * products on the tensor cores), o is rounded once. Sequences of at least
- * strata_cuda_gated_delta_work_bytes' threshold are read in chunks of tokens,
- * which needs that many bytes of work_dev (16-byte aligned; its contents need
- * not be kept between calls, and two calls that may overlap need one each);
- * 0 bytes (NULL) where no sequence is read that way. A NaN or infinity among
- * a token's inputs reaches its own and later outputs of the sequence, and,
- * where it is read in chunks, earlier tokens of the same chunk. o may not
+ * Products and sums are f32, or carry 22 bits (limb products on the tensor
+ * cores, where a call is read in chunks of 32 tokens: k_dim up to 128 and a
+ * sequence of 16 tokens or more, 32 where there are few heads and sequences);
+ * o is rounded once. Chunks need strata_cuda_gated_delta_work_bytes bytes of
+ * work_dev (16-byte aligned; its contents need not be kept between calls, and
+ * calls that may overlap need one each); where that is 0 work_dev may be NULL.
+ * A NaN or infinity among a token's inputs reaches its own and later outputs of
+ * its sequence and head and, where it is read in chunks, earlier ones of the
+ * same chunk. A device wait that expires leaves o and the state undefined and
+ * is reported as STRATA_ERR_TIMEOUT by the context's next host wait
+ * (strata_cuda_synchronize). The state may not overlap an input, nor o
  * overlap any input. */
 typedef struct {
     int64_t n_seq;

@@ -26,7 +26,6 @@ __device__ __forceinline__ void load_pack(const T* p, float (&d)[VEC]) {
 }
 
 constexpr int kRows = 32;  // rows of S a thread holds
-constexpr int64_t kChunkFrom = 16;
 
 template <typename T, int WARPS, int VEC>
 __global__ void __launch_bounds__(WARPS * 32, VEC == 4 ? (WARPS == 8 ? 1 : 12 / WARPS) : 1)
@@ -151,21 +150,28 @@ void launch_step(const DeltaArgs& a, const SeqTable& t, unsigned grid, cudaStrea
 }
 
 // Columns a thread takes: 4 (16-byte state accesses) or 2 where rows and
-// pointers allow, 1 otherwise.
-int columns(const strata_gated_delta& d, const void* v, const float* state, const void* o) {
+// pointers allow, 1 otherwise; fewer where that many blocks would leave
+// multiprocessors without one.
+int columns(const strata_gated_delta& d, const void* v, const float* state, const void* o, int sm_count) {
     const int64_t b = dtype_bytes(d.dtype);
     for (int vec = 4; vec > 1; vec >>= 1) {
         if (d.v_dim % vec == 0 && d.v_stride % vec == 0 && d.o_stride % vec == 0 &&
             (uintptr_t)state % (4 * vec) == 0 && (uintptr_t)v % (b * vec) == 0 && (uintptr_t)o % (b * vec) == 0 &&
-            d.v_dim > 32 * (vec / 2))
+            d.v_dim > 32 * (vec / 2) && d.n_seq * d.n_v_head * ((d.v_dim + 32 * vec - 1) / (32 * vec)) >= sm_count)
             return vec;
     }
     return 1;
 }
 
 // Whether a call is read in chunks: k_dim as the chunk kernels hold it, and a
-// sequence long enough that chunks beat single tokens.
-bool in_chunks(const strata_gated_delta& d, int64_t longest) { return d.k_dim <= 128 && longest >= kChunkFrom; }
+// sequence long enough that chunks beat single tokens. Measured at 32 heads of
+// 128 x 128: one sequence takes 0.67 us a token against 24 us for up to 32 in
+// chunks (even at 32), 32 sequences 8 us a token against 122 us (at 16), because
+// few sequences leave the token kernel's blocks a multiprocessor each.
+bool in_chunks(const strata_gated_delta& d, int64_t longest) {
+    const bool few = d.n_seq * d.n_v_head * ((d.v_dim + 127) / 128) <= 128;
+    return d.k_dim <= 128 && longest >= (few ? 32 : 16);
+}
 
 uint64_t work_needed(const strata_gated_delta& d, int64_t longest) {
     return in_chunks(d, longest) ? delta_chunk_work(d) : 0;
@@ -206,7 +212,7 @@ int strata_cuda_gated_delta_dev(strata_ctx* ctx, const strata_gated_delta* desc,
                                        state_dev, o_dev, work_dev, work_bytes, work_needed(d, longest));
     if (rc) return fail(ctx, rc, "gated_delta: %s", why.text);
     if (longest == 0) return STRATA_OK;
-    const int vec = columns(d, v_dev, state_dev, o_dev);
+    const int vec = columns(d, v_dev, state_dev, o_dev, ctx->sm_count);
     const int64_t blocks = (d.v_dim + 32 * vec - 1) / (32 * vec);
     DeltaArgs a{q_dev, k_dev, v_dev, gate_dev, beta_dev, coef_dev, shift_dev, state_dev, o_dev, d.q_stride,
                 d.k_stride, d.v_stride, d.o_stride, d.gate_stride, d.beta_stride, (int)d.n_k_head, (int)d.n_v_head,
