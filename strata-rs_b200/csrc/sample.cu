@@ -19,8 +19,8 @@
 // over the whole slices, narrowing key ranges pass by pass.
 //
 // Bound by the logits' bytes for rows whose filters need no sum over the
-// vocabulary, and by the f64 pipe (one exponential a token, 8 products and
-// sums) where they do.
+// vocabulary, and by the f64 pipe (one exponential a token, ten operations of
+// two cycles a warp and a conversion of eight) where they do.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -59,7 +59,6 @@ struct SampleArgs {
     float* logprobs;
     int vocab, slice;
     int resident;  // the slice fits shared memory
-    int packs;     // rows and slices are whole 16-byte packs
 };
 
 // Larger key = larger logit; 0 for what is never taken (-inf, NaN). -0 and +0 are equal.
@@ -1025,7 +1024,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     // Which bins the list takes ([first, last]); bins before it are kept for sure.
     int first = 0, last = -1;
     // a range that the sample misjudged, or infinite logits
-    bool wide = sums_all && !(m.sum > 1e-250 && m.sum < 1e250 && top < center + 500.0f * fminf(t, 1.0f));
+    bool wide = sums_all && !(m.sum > 1e-100 && m.sum < 1e250 && top < center + 500.0f * fminf(t, 1.0f));
+    // Excluded tokens have weighed e^-600 each in the sums: nothing, unless the
+    // draw asks for the very first or last token with a weight.
+    if ((sure || draws_all) && !(u > 1e-100 && u < 1.0 - 1e-9)) wide = true;
     if (!draws_all && !wide) {
         uint32_t count[kPer] = {};
 #pragma unroll
@@ -1323,7 +1325,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 const int won = pick<PER>(sh, w, u, 0.0, total, weight);
                 if (threadIdx.x == 0) {
                     // a temperature that takes the weights out of range
-                    sh.won = total > 1e-250 && total < 1e250 ? won : -2;
+                    sh.won = total > 1e-100 && total < 1e250 ? won : -2;
                     sh.won_before = u * total - (sh.won_before - weight);  // the target within the segment
                     sh.total = total;
                 }
@@ -1409,7 +1411,7 @@ extern "C" int strata_cuda_sample_dev(strata_ctx* ctx, const float* logits_dev, 
     const bool resident = slice * 4 <= (rows * ranks > ctx->sm_count ? kPairSlice : kMaxSlice);
     const bool packs = stride % 4 == 0 && vocab % 4 == 0 && (uintptr_t)logits_dev % 16 == 0;
     SampleArgs a{logits_dev, stride, temperature_dev, top_k_dev, top_p_dev, min_p_dev, uniform_dev, ids_dev,
-                 logprobs_dev, (int)vocab, (int)slice, resident, packs};
+                 logprobs_dev, (int)vocab, (int)slice, resident};
     auto kernel = packs ? sample_kernel<true> : sample_kernel<false>;
     static std::atomic<uint64_t> asked[2];
     cudaError_t e = allow_shared(kernel, kListBytes + kMaxSlice, asked[packs], ctx->device);

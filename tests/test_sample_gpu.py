@@ -183,6 +183,65 @@ def test_random_numbers_outside_the_interval(ctx):
         assert draw(ctx, xd, [u])[0][0] == want
 
 
+@pytest.mark.parametrize("vocab", [9000, 60001])
+@pytest.mark.parametrize("kw", [dict(), dict(t=0.01), dict(p=0.9), dict(p=0.9, t=0.005), dict(p=0.99, t=3.0), dict(k=50), dict(m=0.1)], ids=str)
+def test_the_ends_of_the_interval_pass_over_masked_stretches(ctx, vocab, kw):
+    """The smallest and largest random numbers, with most of the row masked on the side that they point at."""
+    rng = np.random.default_rng(vocab)
+    near = 1 - 2.0 ** (-53 if kw.get("t", 1) >= 1 else -40)  # closer, and sums of tiny weights would decide by their order
+    u = [0.0, 2.0 ** -53, 1e-300, near, 1.0, 5.0, 0.5]
+    for masked in (slice(0, vocab * 3 // 4), slice(vocab // 4, vocab)):
+        for mask in (-np.inf, np.nan, np.finfo(np.float32).min, -1e4):
+            x = (rng.standard_normal((1, vocab)) * 2).astype(np.float32).repeat(len(u), 0)
+            x[:, masked] = mask
+            got = [int(v) for v in draw(ctx, torch.from_numpy(x).cuda(), u, **{a: [v] * len(u) for a, v in kw.items()})[0]]
+            f32 = {a: float(np.float32(v)) if a != "k" else v for a, v in kw.items()}
+            want = [expected(x[0].copy(), f32.get("t", 1.0), f32.get("k", 0), f32.get("p", 1.0), f32.get("m", 0.0), min(v, 1.0))[0] for v in u]
+            assert got == want
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 20000), (2, 120001), (40, 9001), (80, 5000), (150, 16384), (150, 16383)])
+@pytest.mark.parametrize("sigma", [0.02, 0.1, 0.5])
+def test_lists_of_every_length(ctx, rows, vocab, sigma):
+    """Nearly flat rows: a border's bins hold hundreds to tens of thousands of tokens, for each number of blocks a row takes."""
+    rng = np.random.default_rng(rows + vocab)
+    x = (rng.standard_normal((rows, vocab)) * sigma + 3).astype(np.float32)
+    u = list(rng.random(rows))
+    k = [int(v) for v in rng.choice([300, 900, 1500, 3900, 4500], rows)]
+    for kw in (dict(k=k), dict(k=k, p=[0.4] * rows), dict(p=list(rng.choice([0.01, 0.1, 0.5, 0.98], rows))),
+               dict(m=list(rng.choice([0.999, 0.9, 0.5], rows))), dict(k=k, p=[0.7] * rows, m=[0.8] * rows, t=[0.3] * rows)):
+        check(ctx, x, u, **kw)
+
+
+def test_a_nearly_flat_row_too_long_for_shared_memory(ctx):
+    rng = np.random.default_rng(21)
+    x = (rng.standard_normal((2, 700001)) * 0.1).astype(np.float32)
+    for kw in (dict(k=[300000, 2000]), dict(p=[0.5, 0.002]), dict(m=[0.9, 0.7])):
+        check(ctx, x, [0.2, 0.8], **kw)
+
+
+@pytest.mark.parametrize("center", [12345.0, -9990.0, -70000.0, 3e38])
+def test_logits_far_from_zero(ctx, center):
+    """f32 holds few steps between them: many tokens are equal, and all lie above or below the histogram's bins."""
+    rng = np.random.default_rng(5)
+    x = (rng.standard_normal((6, 9000)) * (3 if center < 1e30 else 1e31) + center).astype(np.float32)
+    u = list(rng.random(6))
+    for kw in (dict(), dict(k=[5, 50, 700, 1500, 5000, 8999]), dict(p=[0.05, 0.3, 0.5, 0.9, 0.99, 0.999]), dict(m=[0.5, 0.1, 0.01] * 2)):
+        check(ctx, x, u, **kw)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_rows_that_start_anywhere(ctx, shift):
+    rng = np.random.default_rng(shift)
+    x = (rng.standard_normal((3, 8192)) * 2).astype(np.float32)
+    whole = torch.full((shift + x.size,), 99.0, device="cuda")
+    view = whole[shift:].view(3, 8192)
+    view.copy_(torch.from_numpy(x))
+    u = list(rng.random(3))
+    ids, _ = draw(ctx, view, u, p=[0.9] * 3)
+    assert [expected(x[r].copy(), 1.0, 0, float(np.float32(0.9)), 0.0, u[r])[0] for r in range(3)] == list(ids)
+
+
 def test_every_random_number_lands_in_its_token(ctx):
     """The unit interval split by the cumulative probabilities: 4096 draws from one distribution."""
     w = np.array([1, 2, 0, 5, 3, 1, 4], np.float64)
