@@ -167,6 +167,54 @@ def test_a_long_prompt(ctx, dtype):
     check(ctx, [1500], hk=1, hv=2, dk=128, dv=128, raw=True, dtype=dtype)
 
 
+@pytest.mark.parametrize("dtype", [sc.F32, sc.BF16])
+@pytest.mark.parametrize("n,length,dk,dv", [(1, 16, 64, 64), (3, 17, 128, 36), (2, 32, 80, 52), (5, 40, 128, 128), (20, 33, 128, 130), (9, 64, 33, 40), (250, 35, 16, 24)])
+def test_uniform_lengths_without_offsets(ctx, n, length, dk, dv, dtype):
+    check(ctx, [length] * n, hk=1, hv=2, dk=dk, dv=dv, dtype=dtype, ragged=False, seed=length)
+
+
+@pytest.mark.parametrize("dtype", [sc.F32, sc.BF16])
+def test_many_sequences_in_chunks(ctx, dtype):
+    check(ctx, [33 + i % 40 for i in range(230)], hk=2, hv=4, dk=64, dv=100, dtype=dtype)
+
+
+@pytest.mark.parametrize("lens,ragged", [([10500], False), ([4900, 4900], False), ([5200, 0, 33, 4700, 1], True)])
+def test_prompts_beyond_one_filling_of_the_workspace(ctx, lens, ragged):
+    """What is computed ahead of the scan is bounded, so that the longest calls run in pieces."""
+    hk, hv, d = 16, 32, 128
+    g = torch.Generator(device="cuda").manual_seed(sum(lens))
+    rows, size = sum(lens), 2 * hk * d + hv * d
+    qkv = torch.randn(rows, size, generator=g, device="cuda")
+    gate, beta = -torch.rand(rows, hv, generator=g, device="cuda") * 0.2, torch.rand(rows, hv, generator=g, device="cuda")
+    state0 = torch.randn(len(lens), hv, d, d, generator=g, device="cuda") * 0.3
+    state, o = state0.clone(), torch.empty(rows, hv * d, device="cuda")
+    off = [0]
+    for n in lens:
+        off.append(off[-1] + n)
+    shape = sc.GatedDelta(len(lens), hk, hv, d, d, seq_len=lens[0], offsets=off if ragged else None, l2_eps=1e-6, q_stride=size, k_stride=size, v_stride=size)
+    need = sc.gated_delta_work_bytes(shape)
+    assert need <= 257 << 20
+    work = torch.full((need + 256,), 0xFF, dtype=torch.uint8, device="cuda")
+    p = qkv.data_ptr()
+    ctx.gated_delta_dev(shape, p, p + hk * d * 4, p + 2 * hk * d * 4, gate.data_ptr(), beta.data_ptr(), 0, 0, state.data_ptr(), o.data_ptr(), work.data_ptr(), need, stream())
+    spread = 8 * 2.0 ** -24 * np.sqrt(d * 256)
+    q, k, v = (x.reshape(rows, -1, d) for x in qkv.double().split([hk * d, hk * d, hv * d], 1))
+    q, k = (x / (x.square().sum(-1, keepdim=True) + 1e-6).sqrt() for x in (q, k))
+    q, k = (x.repeat_interleave(hv // hk, 1) for x in (q * d ** -0.5, k))
+    decay, beta = gate.double().exp(), beta.double()
+    want = torch.empty(rows, hv, d, dtype=torch.float64, device="cuda")
+    for i, (a, e) in enumerate(zip(off, off[1:])):
+        S = state0[i].double()
+        for t in range(a, e):
+            S *= decay[t, :, None, None]
+            u = beta[t, :, None] * (v[t] - torch.bmm(k[t, :, None], S)[:, 0])
+            S.baddbmm_(k[t, :, :, None], u[:, None])
+            want[t] = torch.bmm(q[t, :, None], S)[:, 0]
+        assert float((state[i].double() - S).abs().max()) <= spread * float(S.abs().max())
+    assert float((o.view(rows, hv, d).double() - want).abs().max()) <= spread * float(want.abs().max())
+    assert bool((work[need:] == 0xFF).all())
+
+
 def test_more_sequences_than_one_launch_holds(ctx):
     check(ctx, [(i * 7) % 5 for i in range(600)], hk=1, hv=2, dk=16, dv=8)
     check(ctx, [40 * (i % 3 == 0) for i in range(300)], hk=1, hv=1, dk=32, dv=16)
