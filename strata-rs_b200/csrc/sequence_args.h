@@ -25,6 +25,7 @@ struct Why {
 
 constexpr int64_t kMaxTokens = (int64_t(1) << 31) - 1;
 constexpr int64_t kMaxStride = int64_t(1) << 31;
+constexpr int64_t kMaxElements = int64_t(1) << 56;  // of a buffer, strides included: byte offsets stay far inside 64 bits
 
 // A buffer as the rows a call touches: `rows` rows of `row` bytes, `pitch`
 // bytes apart, from `base`.
@@ -87,13 +88,21 @@ inline int check_sequences(Why& why, int64_t n_seq, int64_t seq_len, const int64
     return STRATA_OK;
 }
 
-// 0 = packed; otherwise at least one row, and small enough that a row's byte
-// offset stays far inside 64 bits.
-inline int check_stride(Why& why, const char* what, int64_t& stride, int64_t packed) {
+// 0 = packed; otherwise at least one row. `rows` rows of it are a buffer.
+inline int check_stride(Why& why, const char* what, int64_t& stride, int64_t packed, int64_t rows) {
     if (stride == 0) stride = packed;
     if (stride < packed || stride > kMaxStride)
         return why.refuse(STRATA_ERR_INVALID, "%s is %lld for rows of %lld", what, (long long)stride,
                           (long long)packed);
+    if (rows > kMaxElements / stride)
+        return why.refuse(STRATA_ERR_INVALID, "%s is %lld for %lld rows", what, (long long)stride, (long long)rows);
+    return STRATA_OK;
+}
+
+// The states of n sequences, `each` elements long (below 2^40).
+inline int check_states(Why& why, int64_t n, int64_t each) {
+    if (each > 0 && n > kMaxElements / each)
+        return why.refuse(STRATA_ERR_INVALID, "%lld states of %lld elements", (long long)n, (long long)each);
     return STRATA_OK;
 }
 
@@ -111,8 +120,10 @@ inline int check_short_conv(Why& why, strata_short_conv& d, int64_t* tokens, int
     if (d.channels < 1 || d.channels > (int64_t(1) << 30))
         return why.refuse(STRATA_ERR_INVALID, "bad channels %lld", (long long)d.channels);
     if (d.taps < 1 || d.taps > 8) return why.refuse(STRATA_ERR_INVALID, "taps %lld (1 to 8)", (long long)d.taps);
-    if ((rc = check_stride(why, "x_stride", d.x_stride, d.channels))) return rc;
-    return check_stride(why, "y_stride", d.y_stride, d.channels);
+    if ((rc = check_stride(why, "x_stride", d.x_stride, d.channels, *tokens)) ||
+        (rc = check_stride(why, "y_stride", d.y_stride, d.channels, *tokens)))
+        return rc;
+    return check_states(why, d.n_seq, (d.taps - 1) * d.channels);
 }
 
 // `d` and `tokens` as check_short_conv left them.
@@ -145,15 +156,16 @@ inline int check_gated_delta(Why& why, strata_gated_delta& d, int64_t* tokens, i
     if (d.k_dim < 1 || d.k_dim > 256 || d.v_dim < 1 || d.v_dim > 8192)
         return why.refuse(STRATA_ERR_INVALID, "head sizes %lld x %lld (k_dim 1 to 256, v_dim 1 to 8192)",
                           (long long)d.k_dim, (long long)d.v_dim);
-    if (!std::isfinite(d.scale)) return why.refuse(STRATA_ERR_INVALID, "scale is not finite");
+    if (!std::isfinite((float)d.scale)) return why.refuse(STRATA_ERR_INVALID, "scale is not finite");
     if (std::isnan(d.l2_eps) || d.l2_eps > 1e30) return why.refuse(STRATA_ERR_INVALID, "bad l2_eps");
-    if ((rc = check_stride(why, "q_stride", d.q_stride, d.n_k_head * d.k_dim)) ||
-        (rc = check_stride(why, "k_stride", d.k_stride, d.n_k_head * d.k_dim)) ||
-        (rc = check_stride(why, "v_stride", d.v_stride, d.n_v_head * d.v_dim)) ||
-        (rc = check_stride(why, "o_stride", d.o_stride, d.n_v_head * d.v_dim)) ||
-        (rc = check_stride(why, "gate_stride", d.gate_stride, d.n_v_head)))
+    if ((rc = check_stride(why, "q_stride", d.q_stride, d.n_k_head * d.k_dim, *tokens)) ||
+        (rc = check_stride(why, "k_stride", d.k_stride, d.n_k_head * d.k_dim, *tokens)) ||
+        (rc = check_stride(why, "v_stride", d.v_stride, d.n_v_head * d.v_dim, *tokens)) ||
+        (rc = check_stride(why, "o_stride", d.o_stride, d.n_v_head * d.v_dim, *tokens)) ||
+        (rc = check_stride(why, "gate_stride", d.gate_stride, d.n_v_head, *tokens)) ||
+        (rc = check_stride(why, "beta_stride", d.beta_stride, d.n_v_head, *tokens)))
         return rc;
-    return check_stride(why, "beta_stride", d.beta_stride, d.n_v_head);
+    return check_states(why, d.n_seq, d.n_v_head * d.k_dim * d.v_dim);
 }
 
 inline int check_gated_delta_buffers(Why& why, const strata_gated_delta& d, int64_t tokens, const void* q,
@@ -203,7 +215,7 @@ inline int check_sample(Why& why, const float* logits, int64_t rows, int64_t voc
     if (vocab < 1 || vocab > (int64_t(1) << 22))
         return why.refuse(STRATA_ERR_INVALID, "vocab %lld (1 to 2^22)", (long long)vocab);
     int rc;
-    if ((rc = check_stride(why, "stride", stride, vocab)) || (rc = check_aligned(why, "logits", logits, 4)) ||
+    if ((rc = check_stride(why, "stride", stride, vocab, rows)) || (rc = check_aligned(why, "logits", logits, 4)) ||
         (rc = check_aligned(why, "temperature", temperature, 4)) || (rc = check_aligned(why, "top_k", top_k, 4)) ||
         (rc = check_aligned(why, "top_p", top_p, 4)) || (rc = check_aligned(why, "min_p", min_p, 4)) ||
         (rc = check_aligned(why, "uniform", uniform, 8)) || (rc = check_aligned(why, "ids", ids, 4)) ||

@@ -100,6 +100,10 @@ static void short_conv() {
     EXPECT(conv_with([](auto& d) { d.x_stride = 63; }) == STRATA_ERR_INVALID);
     EXPECT(conv_with([](auto& d) { d.y_stride = -64; }) == STRATA_ERR_INVALID);
     EXPECT(conv_with([](auto& d) { d.x_stride = INT64_MAX; }) == STRATA_ERR_INVALID);
+    // rows and states whose byte offsets would pass 64 bits
+    EXPECT(conv_with([](auto& d) { d.seq_len = 1 << 26, d.x_stride = int64_t(1) << 30; }) == STRATA_ERR_INVALID);
+    EXPECT(conv_with([](auto& d) { d.seq_len = 1 << 24, d.x_stride = int64_t(1) << 30; }) == STRATA_OK);
+    EXPECT(conv_with([](auto& d) { d.n_seq = 1 << 28, d.seq_len = 0, d.channels = 1 << 27; }) == STRATA_ERR_INVALID);
     EXPECT(conv_with([](auto& d) { d.dtype = STRATA_QUANT_F16; }) == STRATA_ERR_UNSUPPORTED_QUANT);
     EXPECT(conv_with([](auto& d) { d.dtype = STRATA_QUANT_Q8_0; }) == STRATA_ERR_UNSUPPORTED_QUANT);
     EXPECT(conv_with([](auto& d) { d.dtype = STRATA_QUANT_BF16; }) == STRATA_OK);
@@ -144,6 +148,11 @@ static void gated_delta() {
     EXPECT(delta_with([](auto& d) { d.v_stride = 31; }) == STRATA_ERR_INVALID);
     EXPECT(delta_with([](auto& d) { d.gate_stride = 3; }) == STRATA_ERR_INVALID);
     EXPECT(delta_with([](auto& d) { d.o_stride = -1; }) == STRATA_ERR_INVALID);
+    EXPECT(delta_with([](auto& d) { d.seq_len = 1 << 28, d.v_stride = int64_t(1) << 28; }) == STRATA_ERR_INVALID);
+    EXPECT(delta_with([](auto& d) {
+               d.n_seq = 1 << 24, d.seq_len = 1, d.n_k_head = 1, d.n_v_head = 65536, d.k_dim = 256, d.v_dim = 8192;
+           }) == STRATA_ERR_INVALID);
+    EXPECT(delta_with([](auto& d) { d.scale = 1e39; }) == STRATA_ERR_INVALID);
     EXPECT(delta_with([](auto& d) { d.dtype = STRATA_QUANT_F16; }) == STRATA_ERR_UNSUPPORTED_QUANT);
 
     strata_gated_delta d = delta();
