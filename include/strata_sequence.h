@@ -81,9 +81,10 @@ int strata_cuda_short_conv_dev(strata_ctx *ctx, const strata_short_conv *desc, c
  * per head; a negative l2_eps takes them as they are. k_dim 1..256, v_dim 1..8192.
  *
  * Products and sums are f32, or carry 22 bits (limb products on the tensor
- * cores, where a call is read in chunks of 32 tokens: k_dim up to 128 and a
- * sequence of 16 tokens or more, 32 where there are few heads and sequences);
- * o is rounded once. Chunks need strata_cuda_gated_delta_work_bytes bytes of
+ * cores, where sequences are read in chunks of 32 tokens: k_dim up to 128 and a
+ * sequence of 16 tokens or more in the call, 32 where there are few heads and
+ * sequences; many shorter ones beside it are still read token by token); o is
+ * rounded once. Chunks need strata_cuda_gated_delta_work_bytes bytes of
  * work_dev (16-byte aligned; its contents need not be kept between calls, and
  * calls that may overlap need one each); where that is 0 work_dev may be NULL.
  * A NaN or infinity among a token's inputs reaches its own and later outputs of

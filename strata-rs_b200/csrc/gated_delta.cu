@@ -10,7 +10,10 @@
 // first token to the last: the state is read and written once a call. One pass
 // over the registers gives both S^T k and S^T q, because
 // S_new^T q = e^g S^T q + (k . q) u, so a token costs one reduction across the
-// warps. For one token per sequence it is bound by the state's bytes.
+// warps. For one token per sequence it is bound by the state's bytes: 128
+// sequences of 32 heads of 128 x 128 take 88 us, 537 MB at 6.2 TB/s. One
+// sequence is bound by latency (3.7 us, with a column a thread: four columns,
+// a quarter of the blocks, took 5.6).
 #include <cuda_runtime.h>
 
 #include "gated_delta.cuh"
@@ -163,18 +166,29 @@ int columns(const strata_gated_delta& d, const void* v, const float* state, cons
     return 1;
 }
 
-// Whether a call is read in chunks: k_dim as the chunk kernels hold it, and a
-// sequence long enough that chunks beat single tokens. Measured at 32 heads of
-// 128 x 128: one sequence takes 0.67 us a token against 24 us for up to 32 in
-// chunks (even at 32), 32 sequences 8 us a token against 122 us (at 16), because
-// few sequences leave the token kernel's blocks a multiprocessor each.
-bool in_chunks(const strata_gated_delta& d, int64_t longest) {
-    const bool few = d.n_seq * d.n_v_head * ((d.v_dim + 127) / 128) <= 128;
-    return d.k_dim <= 128 && longest >= (few ? 32 : 16);
+// The tokens from which on a sequence of the call is read in chunks (more than
+// `longest`: none is). Measured at 32 heads of 128 x 128: one sequence takes
+// 0.67 us a token against 24 us for up to 32 in chunks (even at 32), 32
+// sequences 8 us a token against 122 us (at 16), because few sequences leave the
+// token kernel's blocks a multiprocessor each. Beside long sequences a short
+// one costs 3.7 us as a chunk against 0.5 us and 0.18 us a token, unless there
+// are so few that they run alongside: 31 single tokens and 500 take 72 us, not
+// 160, apart; 3 sequences of 12 tokens and 500 take 53 us, not 59, together.
+int64_t chunks_from(const strata_gated_delta& d, int64_t longest) {
+    const int64_t blocks = d.n_v_head * ((d.v_dim + 127) / 128), few = 128 / blocks;  // sequences
+    if (d.k_dim > 128 || longest < (d.n_seq <= few ? 32 : 16)) return longest + 1;
+    if (!d.seq_offsets) return 1;
+    int64_t n = 0;
+    for (int64_t i = 0; i < d.n_seq; ++i) {
+        const int64_t len = d.seq_offsets[i + 1] - d.seq_offsets[i];
+        n += len > 0 && len < 16;
+    }
+    return n > few ? 16 : 1;
 }
 
 uint64_t work_needed(const strata_gated_delta& d, int64_t longest) {
-    return in_chunks(d, longest) ? delta_chunk_work(d) : 0;
+    const int64_t from = chunks_from(d, longest);
+    return from <= longest ? delta_chunk_work(d, from) : 0;
 }
 
 }  // namespace
@@ -220,8 +234,12 @@ int strata_cuda_gated_delta_dev(strata_ctx* ctx, const strata_gated_delta* desc,
                 (float)d.l2_eps};
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    if (in_chunks(d, longest)) return delta_chunk_enqueue(ctx, d, a, work_dev, s);
-    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kMaxTokens, [&](const SeqTable& t, int64_t) {
+    const int64_t from = chunks_from(d, longest);
+    if (from <= longest) {
+        rc = delta_chunk_enqueue(ctx, d, a, work_dev, from, s);
+        if (rc || from == 1) return rc;
+    }
+    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, kMaxTokens, from, [&](const SeqTable& t, int64_t) {
         if (t.n * blocks * d.n_v_head > kMaxTokens)
             return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %d sequences of %lld heads", t.n,
                         (long long)d.n_v_head);

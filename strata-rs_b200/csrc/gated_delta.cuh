@@ -29,8 +29,9 @@ __device__ __forceinline__ void gates(const DeltaArgs& a, int h, float& g, float
     beta = 1.0f / (1.0f + expf(-beta));
 }
 
-// gated_delta_chunk.cu
-uint64_t delta_chunk_work(const strata_gated_delta& d);
-int delta_chunk_enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, void* work, cudaStream_t s);
+// gated_delta_chunk.cu: the call's sequences of `from` tokens (1 at least) and more.
+uint64_t delta_chunk_work(const strata_gated_delta& d, int64_t from);
+int delta_chunk_enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, void* work, int64_t from,
+                        cudaStream_t s);
 
 }  // namespace strata

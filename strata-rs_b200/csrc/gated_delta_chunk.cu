@@ -801,7 +801,7 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
             if (part == 0) hand.scale[lane] = make_float2(u_down[0], u_down[1]);
             const uint32_t t_at = base + I::kBytes + (part * TILES * 8 + lane_b) * kPitchT + half_b;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {  // two tiles of tokens; the second is another warp's where a warp has one
+            for (int ks = 0; ks < 2; ++ks) {
                 ldmatrix(bh[ks], t_at + ks * 32);
                 ldmatrix(bl[ks], t_at + kLimbT + ks * 32);
             }
@@ -887,9 +887,9 @@ ChunkBytes chunk_bytes(const strata_gated_delta& d) {
 
 // The launches of a call: groups of sequences, each read in pieces of as many
 // chunks as the workspace bound allows (one per sequence at least). Calls
-// launch(table, tiles) in order.
+// launch(table, tiles) in order. Sequences below `from` tokens are left out.
 template <typename F>
-int plan_chunks(const strata_gated_delta& d, F launch) {
+int plan_chunks(const strata_gated_delta& d, int64_t from, F launch) {
     const uint64_t fit = kMaxWork / chunk_bytes(d).all();
     const int64_t cap = fit < 1 ? 1 : (int64_t)fit;
     auto per_sequence = [&](int64_t n) { return cap / n > 1 ? cap / n : int64_t(1); };
@@ -907,10 +907,13 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
         return STRATA_OK;
     }
     const int64_t group = cap < kSeqGroup ? cap : kSeqGroup;
-    const int64_t* off = d.seq_offsets;
+    auto length = [&](int64_t i) {
+        const int64_t len = d.seq_offsets[i + 1] - d.seq_offsets[i];
+        return len < from ? int64_t(0) : len;
+    };
     for (int64_t i = 0; i < d.n_seq;) {
         int64_t end = i, live = 0;  // sequences [i, end), `live` of them with tokens
-        while (end < d.n_seq && live < group) live += off[end + 1] > off[end], ++end;
+        while (end < d.n_seq && live < group) live += length(end) > 0, ++end;
         for (int64_t t = 0; live > 0;) {
             // the longest piece (in chunks, of every sequence that still has tokens) that fits
             int64_t fits = 1, over = cap + 1;
@@ -918,7 +921,7 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
                 const int64_t mid = (fits + over) / 2;
                 int64_t sum = 0;
                 for (int64_t k = i; k < end; ++k) {
-                    const int64_t left = (off[k + 1] - off[k] - t + kChunk - 1) / kChunk;
+                    const int64_t left = (length(k) - t + kChunk - 1) / kChunk;
                     sum += left <= 0 ? 0 : left < mid ? left : mid;
                 }
                 if (sum <= cap) fits = mid;
@@ -928,13 +931,12 @@ int plan_chunks(const strata_gated_delta& d, F launch) {
             // the longest first, so that no long one is left to start last
             int64_t order[kSeqGroup], count = 0, left = 0;
             for (int64_t k = i; k < end; ++k)
-                if (off[k + 1] - off[k] > t) order[count++] = k;
-            std::stable_sort(order, order + count,
-                             [&](int64_t x, int64_t y) { return off[x + 1] - off[x] > off[y + 1] - off[y]; });
+                if (length(k) > t) order[count++] = k;
+            std::stable_sort(order, order + count, [&](int64_t x, int64_t y) { return length(x) > length(y); });
             SeqTable tab = ragged_table();
             for (int64_t n = 0; n < count; ++n) {
-                const int64_t k = order[n], len = off[k + 1] - off[k] - t;
-                add_sequence(tab, k, off[k] + t, len < step ? len : step, kChunk);
+                const int64_t k = order[n], len = length(k) - t;
+                add_sequence(tab, k, d.seq_offsets[k] + t, len < step ? len : step, kChunk);
                 left += len > step;
             }
             const int rc = launch(tab, (int64_t)tab.tile[tab.n]);
@@ -965,14 +967,15 @@ int enqueue_scan(strata_ctx* ctx, DeltaArgs a, const SeqTable& t, const uint8_t*
 }
 
 template <typename T, int DK, int LIMBS>
-int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
+int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, int64_t from,
+            cudaStream_t s) {
     auto prepare = delta_prepare_kernel<T, DK, LIMBS>;
     constexpr int smem = prepare_smem<DK, LIMBS>();
     static std::atomic<uint64_t> asked;
     const cudaError_t e = allow_shared(prepare, smem, asked, ctx->device);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(gated_delta)");
     const uint64_t keys = chunk_bytes(d).keys;
-    return plan_chunks(d, [&](const SeqTable& t, int64_t tiles) {
+    return plan_chunks(d, from, [&](const SeqTable& t, int64_t tiles) {
         const int64_t grid = tiles * a.k_heads;
         if (grid > kMaxTokens)
             return fail(ctx, STRATA_ERR_INVALID, "gated_delta: %lld chunks of %d heads", (long long)tiles, a.k_heads);
@@ -991,30 +994,32 @@ int enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, ui
 }
 
 template <typename T, int LIMBS>
-int enqueue_dim(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, cudaStream_t s) {
+int enqueue_dim(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, uint8_t* work, int64_t from,
+                cudaStream_t s) {
     switch (padded_dim(d.k_dim)) {
-        case 32: return enqueue<T, 32, LIMBS>(ctx, d, a, work, s);
-        case 64: return enqueue<T, 64, LIMBS>(ctx, d, a, work, s);
-        case 96: return enqueue<T, 96, LIMBS>(ctx, d, a, work, s);
-        default: return enqueue<T, 128, LIMBS>(ctx, d, a, work, s);
+        case 32: return enqueue<T, 32, LIMBS>(ctx, d, a, work, from, s);
+        case 64: return enqueue<T, 64, LIMBS>(ctx, d, a, work, from, s);
+        case 96: return enqueue<T, 96, LIMBS>(ctx, d, a, work, from, s);
+        default: return enqueue<T, 128, LIMBS>(ctx, d, a, work, from, s);
     }
 }
 
 }  // namespace
 
-uint64_t delta_chunk_work(const strata_gated_delta& d) {
+uint64_t delta_chunk_work(const strata_gated_delta& d, int64_t from) {
     int64_t most = 0;
-    plan_chunks(d, [&](const SeqTable&, int64_t tiles) {
+    plan_chunks(d, from, [&](const SeqTable&, int64_t tiles) {
         if (tiles > most) most = tiles;
         return (int)STRATA_OK;
     });
     return (uint64_t)most * chunk_bytes(d).all();
 }
 
-int delta_chunk_enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, void* work, cudaStream_t s) {
+int delta_chunk_enqueue(strata_ctx* ctx, const strata_gated_delta& d, const DeltaArgs& a, void* work, int64_t from,
+                        cudaStream_t s) {
     uint8_t* w = static_cast<uint8_t*>(work);
-    if (d.dtype == STRATA_QUANT_BF16) return enqueue_dim<__nv_bfloat16, 1>(ctx, d, a, w, s);
-    return enqueue_dim<float, 2>(ctx, d, a, w, s);
+    if (d.dtype == STRATA_QUANT_BF16) return enqueue_dim<__nv_bfloat16, 1>(ctx, d, a, w, from, s);
+    return enqueue_dim<float, 2>(ctx, d, a, w, from, s);
 }
 
 }  // namespace strata

@@ -100,9 +100,10 @@ inline void add_sequence(SeqTable& t, int64_t slot, int64_t row, int64_t len, in
     ++t.n;
 }
 
-// Calls launch(table, tiles) for each group of sequences, cut into tiles of `rows` rows.
+// Calls launch(table, tiles) for each group of sequences, cut into tiles of
+// `rows` rows. Of ragged ones those below `below` rows only.
 template <typename F>
-int for_sequence_groups(int64_t n_seq, int64_t seq_len, const int64_t* off, int64_t rows, F launch) {
+int for_sequence_groups(int64_t n_seq, int64_t seq_len, const int64_t* off, int64_t rows, int64_t below, F launch) {
     if (!off) {
         if (seq_len == 0) return STRATA_OK;
         const SeqTable t = uniform_table(n_seq, 0, seq_len, 0, seq_len, rows);
@@ -110,7 +111,8 @@ int for_sequence_groups(int64_t n_seq, int64_t seq_len, const int64_t* off, int6
     }
     SeqTable t = ragged_table();
     for (int64_t i = 0; i < n_seq; ++i) {
-        if (off[i + 1] > off[i]) add_sequence(t, i, off[i], off[i + 1] - off[i], rows);
+        const int64_t len = off[i + 1] - off[i];
+        if (len > 0 && len < below) add_sequence(t, i, off[i], len, rows);
         if (t.n == kSeqGroup || (i + 1 == n_seq && t.n)) {
             const int rc = launch(t, (int64_t)t.tile[t.n]);
             if (rc) return rc;

@@ -235,7 +235,7 @@ extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_co
                      (int)tile, d.silu, (uintptr_t)w_dev % 16 == 0};
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, tile, [&](const SeqTable& t, int64_t tiles) {
+    return for_sequence_groups(d.n_seq, d.seq_len, d.seq_offsets, tile, tokens + 1, [&](const SeqTable& t, int64_t tiles) {
         if (tiles * a.blocks > kMaxTokens)
             return fail(ctx, STRATA_ERR_INVALID, "short_conv: %lld tiles of %d channel blocks", (long long)tiles,
                         a.blocks);

@@ -178,6 +178,14 @@ def test_many_sequences_in_chunks(ctx, dtype):
     check(ctx, [33 + i % 40 for i in range(230)], hk=2, hv=4, dk=64, dv=100, dtype=dtype)
 
 
+@pytest.mark.parametrize("dtype", [sc.F32, sc.BF16])
+def test_single_tokens_beside_prompts(ctx, dtype):
+    """Many short sequences in a call with long ones are read token by token, the others in chunks."""
+    check(ctx, [1, 0, 3, 15] * 12 + [70, 0, 16, 33, 14], dk=64, dv=64, dtype=dtype, first=2)
+    check(ctx, [200] + [1] * 40 + [0] + [17], hk=2, hv=4, dk=128, dv=36, raw=True, dtype=dtype, gap=3)
+    check(ctx, [1 + (i % 9 == 0) * 40 for i in range(600)], hk=1, hv=2, dk=16, dv=8, dtype=dtype)
+
+
 @pytest.mark.parametrize("lens,ragged", [([10500], False), ([4900, 4900], False), ([5200, 0, 33, 4700, 1], True)])
 def test_prompts_beyond_one_filling_of_the_workspace(ctx, lens, ragged):
     """What is computed ahead of the scan is bounded, so that the longest calls run in pieces."""
