@@ -38,6 +38,13 @@
 // k_dim 128 and f32: a conversion, a product, an exchange, three times over); a
 // batch by how many groups share a multiprocessor, four where shared memory
 // allows.
+//
+// Measured at 32 value and 16 key heads of 128 x 128: one sequence of 8192 f32
+// tokens 619 us, 98 of it prepare (368 MB, 3.8 TB/s; warps wait for loads and
+// for their row sums) and 520 the scan (2.0 us a chunk, 128 blocks; 1.7 us
+// without outputs). The tensor cores are a third busy: chunks of 64 would halve
+// the steps of the chain, but their images do not fit shared memory three deep.
+// Eight bf16 sequences of 1 to 2049 tokens, 7036 in all, 423 us (92 and 333).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

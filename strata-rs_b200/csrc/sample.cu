@@ -18,9 +18,15 @@
 // hold (nearly flat or clustered rows with a far cut), the same search runs
 // over the whole slices, narrowing key ranges pass by pass.
 //
-// Bound by the logits' bytes for rows whose filters need no sum over the
-// vocabulary, and by the f64 pipe (one exponential a token, ten operations of
-// two cycles a warp and a conversion of eight) where they do.
+// What it measured, and what bounds it: 256 rows of 151,936 logits with top-p
+// take 209 us (155 MB from DRAM in each pass). Of the 190,000 cycles of the first
+// pass on a multiprocessor with two rows, 87,000 are its exponentials (37 a warp
+// for 32 tokens; ten f64 operations of two and a conversion of eight are 28),
+// 11,000 the histogram; of the second's 180,000, 37,000 the exponentials of what
+// lies above the border, 50,000 queueing them, 30,000 the list. Instruction
+// issue is the limit in both. Without a filter 256 rows take 84 us, greedy ones
+// 39 us (4.0 TB/s). Few rows are bound by the fixed steps, which wait on each
+// other: one row 26 us, of which the passes over the logits take 7.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -15,6 +15,13 @@
 // (their weights and halo are then a small part), one token where sequences
 // have one.
 //
+// Measured: 8192 tokens of 8192 bf16 channels, 4 taps, 49 us, 5.5 TB/s (the
+// asynchronous copies took it from 111 to 65, tiles for two whole rounds of
+// blocks from there; SiLU's exponential and reciprocal keep the special-function
+// unit 58% busy); 64
+// sequences of one token 5.1 us, launch and latency; 3537
+// tokens of 8 sequences, 2571 f32 channels element by element, 18 us.
+//
 // The state of a sequence is read and replaced by the same thread (the one
 // that has its first tile; the new state is the sequence's last K - 1 inputs,
 // read again from x), so no other block has to be waited for.
