@@ -19,14 +19,15 @@
 // over the whole slices, narrowing key ranges pass by pass.
 //
 // What it measured, and what bounds it: 256 rows of 151,936 logits with top-p
-// take 209 us (155 MB from DRAM in each pass). Of the 190,000 cycles of the first
+// take 205 us (155 MB from DRAM in each pass). Of the 172,000 cycles of the first
 // pass on a multiprocessor with two rows, 87,000 are its exponentials (37 a warp
 // for 32 tokens; ten f64 operations of two and a conversion of eight are 28),
-// 11,000 the histogram; of the second's 180,000, 37,000 the exponentials of what
-// lies above the border, 50,000 queueing them, 30,000 the list. Instruction
+// 11,000 the histogram; of the second's 182,000, 37,000 the exponentials of what
+// lies above the border, 49,000 queueing them, 30,000 the list. Instruction
 // issue is the limit in both. Without a filter 256 rows take 84 us, greedy ones
-// 39 us (4.0 TB/s). Few rows are bound by the fixed steps, which wait on each
-// other: one row 26 us, of which the passes over the logits take 7.
+// 39 us (4.0 TB/s). Few rows are bound by steps that wait for each other, most of
+// them for another block's shared memory (700 cycles a read): one row 7 us greedy,
+// 18 with a top-k of 20, 30 with top-p.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -102,7 +103,7 @@ struct Shared {
     First first;                   // exchanged
     double above;                  // exchanged: mass above the list
     double seg[kWarps * kSub];     // exchanged: weights of the tokens above the list, by part of the slice
-    int listed[kWarps];            // exchanged: tokens each warp put into the list,
+    int listed[kWarps];            // exchanged: tokens each warp put into the list (then: crowded bins),
     int listed_part[kWarps * kSub];  // and how many of them by the end of each part
     int block_listed;              // exchanged: their sum
     uint8_t chain[kWarps][kList / 32];  // the pool's groups of 32 that hold them, in order
@@ -111,7 +112,7 @@ struct Shared {
     int part_end[kMaxCluster * kWarps * kSub];  // and the list's length by the end of each part
     double exp2_table[kExpTable][32];  // a copy a lane: no two lanes meet in a bank
     alignas(16) uint32_t fine[kFine + 32];              // exchanged: the first pass's histogram
-    double segment[kMaxCluster * kWarps * kSub];
+    alignas(16) uint32_t share[kFine / 2];  // exchanged: the block's share of the bins, summed over the row (then: the list's counts)
     int won, id;                   // the draw: its segment (-1: id is the token)
     double won_before, total, weight;
     Part part[2];                  // exchanged, alternating
@@ -571,75 +572,178 @@ __device__ int pick(Shared& sh, const double (&w)[PER], double u, double offset,
     return at;
 }
 
-// The bins of the first pass, kPer a thread: the first whose running sum
-// reaches `target`; kFine, for what has no bin, if none does.
+// Sums of two values over the block's threads.
+__device__ __forceinline__ void block_sums(Shared& sh, double& a, double& b) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+    }
+    __syncthreads();
+    if (lane == 0) sh.wsum[0][warp] = a, sh.wsum[1][warp] = b;
+    __syncthreads();
+    a = sh.wsum[0][lane % kWarps], b = sh.wsum[1][lane % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+    }
+}
+
+// The bins of the first pass, kPer a thread: the first ones whose running sums
+// reach `low` and `high`; kFine, for what has no bin, if none does.
 template <typename W>
-__device__ int fine_border(Shared& sh, const W (&weight)[kPer], W target) {
+__device__ int2 fine_borders(Shared& sh, const W (&weight)[kPer], W low, W high) {
     double own = 0.0, total;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) own += (double)weight[e];
     double run = block_scan(sh, own, total) - own;
-    if (threadIdx.x == 0) sh.pick_bin = kFine;
+    if (threadIdx.x == 0) sh.pick_bin = sh.found = kFine;
     __syncthreads();
-    int reached = kFine;
+    int at_low = kFine, at_high = kFine;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         run += (double)weight[e];
-        if (weight[e] > 0 && run >= (double)target) reached = min(reached, (int)threadIdx.x * kPer + e);
+        const int bin = (int)threadIdx.x * kPer + e;
+        if (weight[e] > 0 && run >= (double)low) at_low = min(at_low, bin);
+        if (weight[e] > 0 && run >= (double)high) at_high = min(at_high, bin);
     }
-    reached = __reduce_min_sync(0xFFFFFFFFu, reached);
-    if ((threadIdx.x & 31) == 0) atomicMin(&sh.pick_bin, reached);
+    at_low = __reduce_min_sync(0xFFFFFFFFu, at_low), at_high = __reduce_min_sync(0xFFFFFFFFu, at_high);
+    if ((threadIdx.x & 31) == 0) {
+        if (at_low < kFine) atomicMin(&sh.pick_bin, at_low);
+        if (at_high < kFine) atomicMin(&sh.found, at_high);
+    }
     __syncthreads();
-    const int bin = sh.pick_bin;
-    __syncthreads();
-    return bin;
+    return make_int2(sh.pick_bin, sh.found);
 }
 
-// Sorts the block's kThreads * PER values x[e] (place threadIdx.x * PER + e),
-// rising: a bitonic network whose short strides stay within a thread or a
-// warp's registers; `buffer` holds kThreads * PER values.
+// Puts the list's tokens in falling order (equal ones by place): mine[e] is
+// token threadIdx.x + e * kThreads on entry and the one of place
+// threadIdx.x * PER + e on return; the words order[0 .. listed) are scratch. A
+// key is ~key_of(value) << 32 | place, ~0 behind the list. The values' range is
+// cut into kFine bins, every token takes a place in its bin, and counts those of
+// its bin that precede it. Where a bin has too many for that to be quick they
+// are mostly one value (rounded logits), and stay in the list's order. False
+// where they are several. (A list of 1000 takes 2 us so; 9 with a bitonic sort.)
 template <int PER>
-__device__ void sort_block(unsigned long long (&x)[PER], unsigned long long* buffer) {
-    constexpr int N = kThreads * PER;
-    const int first = threadIdx.x * PER;
-#pragma unroll 1
-    for (int size = 2; size <= N; size <<= 1) {
-        int stride = size >> 1;
-#pragma unroll 1
-        for (; stride >= 32 * PER; stride >>= 1) {
-            __syncthreads();
+__device__ bool order_list(Shared& sh, unsigned long long (&mine)[PER], const float* list, unsigned long long* order,
+                           int listed) {
+    constexpr uint32_t kCrowd = 256;
+    static_assert(PER * kThreads / kCrowd <= kWarps, "room for the crowded bins' numbers");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t first = 0xFFFFFFFFu, last = 0u;  // keys
 #pragma unroll
-            for (int e = 0; e < PER; ++e) buffer[e * kThreads + threadIdx.x] = x[e];
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                const unsigned long long y = buffer[e * kThreads + (threadIdx.x ^ (stride / PER))];
-                const bool low = (((first + e) & stride) == 0) == (((first + e) & size) == 0);
-                x[e] = low ? min(x[e], y) : max(x[e], y);
-            }
-        }
-#pragma unroll 1
-        for (; stride >= PER; stride >>= 1) {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                const unsigned long long y = __shfl_xor_sync(0xFFFFFFFFu, x[e], stride / PER);
-                const bool low = (((first + e) & stride) == 0) == (((first + e) & size) == 0);
-                x[e] = low ? min(x[e], y) : max(x[e], y);
-            }
-        }
-#pragma unroll
-        for (int s = PER / 2; s > 0; s >>= 1) {
-            if (s >= size) continue;
-#pragma unroll
-            for (int e = 0; e < PER; ++e)
-                if (!(e & s)) {
-                    const unsigned long long a = x[e], b = x[e | s];
-                    const bool rising = ((first + e) & size) == 0;
-                    x[e] = rising ? min(a, b) : max(a, b);
-                    x[e | s] = rising ? max(a, b) : min(a, b);
-                }
-        }
+    for (int e = 0; e < PER; ++e) {
+        const uint32_t key = ~(uint32_t)(mine[e] >> 32);
+        if (e * kThreads + (int)threadIdx.x < listed) first = min(first, key), last = max(last, key);
     }
+    first = __reduce_min_sync(0xFFFFFFFFu, first), last = __reduce_max_sync(0xFFFFFFFFu, last);
+    if (lane == 0) sh.wlo[warp] = first, sh.whi[warp] = last;
+    reinterpret_cast<uint4*>(sh.fine)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const float low = logit_of(__reduce_min_sync(0xFFFFFFFFu, sh.wlo[lane % kWarps]));
+    const float high = logit_of(__reduce_max_sync(0xFFFFFFFFu, sh.whi[lane % kWarps]));
+    // monotone, whatever the range: infinite ones make it one bin
+    const float scale = high > low ? (float)(kFine - 1) / (high - low) : 0.0f;
+    auto bin_of = [&](uint32_t key) {
+        return (uint32_t)fminf(fmaxf((high - logit_of(key)) * scale, 0.0f), (float)(kFine - 1));
+    };
+    uint32_t bin[PER], at[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        bin[e] = bin_of(~(uint32_t)(mine[e] >> 32));
+        if (e * kThreads + (int)threadIdx.x < listed) at[e] = atomicAdd(&sh.fine[bin[e]], 1u);
+    }
+    __syncthreads();
+    const uint4 c = reinterpret_cast<const uint4*>(sh.fine)[threadIdx.x];
+    if (threadIdx.x == 0) sh.pick_bin = 0;
+    const bool crowded = __syncthreads_or(max(max(c.x, c.y), max(c.z, c.w)) > kCrowd);
+    if (crowded) {
+        const uint32_t n[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n[e] > kCrowd) sh.listed[atomicAdd(&sh.pick_bin, 1)] = (int)threadIdx.x * 4 + e;
+    }
+    const uint32_t own = c.x + c.y + c.z + c.w;
+    uint32_t incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) sh.wn[warp] = (int)incl;
+    __syncthreads();
+    const uint32_t before = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? (uint32_t)sh.wn[lane % kWarps] : 0u) + incl - own;
+    reinterpret_cast<uint4*>(sh.fine)[threadIdx.x] =
+        make_uint4(before, before + c.x, before + c.x + c.y, before + c.x + c.y + c.z);
+    if (threadIdx.x == 0) sh.fine[kFine] = (uint32_t)listed;
+    __syncthreads();
+    uint32_t lone = 0;  // tokens in bins that are not crowded
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const uint32_t from = sh.fine[bin[e]], to = sh.fine[bin[e] + 1];
+        if (e * kThreads + (int)threadIdx.x >= listed || to - from > kCrowd) continue;
+        lone |= 1u << e;
+        order[from + at[e]] = mine[e];
+    }
+    if (crowded) {
+        // every warp has a stretch of the list and counts what it holds of each
+        // crowded bin (lane q of bin q), then puts these behind earlier warps'
+        const int crowds = sh.pick_bin, stretch = (listed + kWarps * 32 - 1) / (kWarps * 32) * 32;
+        const int lo = warp * stretch, hi = min(lo + stretch, listed);
+        const uint32_t own_crowd = lane < crowds ? (uint32_t)sh.listed[lane] : kFine;
+        uint32_t to = 0;
+        for (int i = lo + lane; i - lane < hi; i += 32) {
+            const uint32_t b = i < hi ? bin_of(key_of(list[i])) : kFine;
+            for (int q = 0; q < crowds; ++q) {
+                const unsigned votes = __ballot_sync(0xFFFFFFFFu, b == __shfl_sync(0xFFFFFFFFu, own_crowd, q));
+                if (lane == q) to += __popc(votes);
+            }
+        }
+        sh.share[warp * 32 + lane] = to;
+        __syncthreads();
+        to = lane < crowds ? sh.fine[own_crowd] : 0;
+        for (int w = 0; w < warp; ++w) to += sh.share[w * 32 + lane];
+        for (int i = lo + lane; i - lane < hi; i += 32) {
+            const uint32_t key = i < hi ? key_of(list[i]) : 0u, b = i < hi ? bin_of(key) : kFine;
+            for (int q = 0; q < crowds; ++q) {
+                const bool in = b == __shfl_sync(0xFFFFFFFFu, own_crowd, q);
+                const unsigned votes = __ballot_sync(0xFFFFFFFFu, in);
+                const uint32_t start = __shfl_sync(0xFFFFFFFFu, to, q);
+                if (in) order[start + __popc(votes & ((1u << lane) - 1u))] = (unsigned long long)~key << 32 | (unsigned)i;
+                if (lane == q) to += __popc(votes);
+            }
+        }
+        __syncthreads();
+        bool mixed = false;
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (e * kThreads + (int)threadIdx.x < listed && !(lone >> e & 1))
+                mixed |= (uint32_t)(order[sh.fine[bin[e]]] >> 32) != (uint32_t)(mine[e] >> 32);
+        if (__syncthreads_or(mixed)) return false;
+    } else {
+        __syncthreads();
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        if (!(lone >> e & 1)) continue;
+        const uint32_t from = sh.fine[bin[e]], to = sh.fine[bin[e] + 1];
+        at[e] = from;
+#pragma unroll 4
+        for (uint32_t i = from; i < to; ++i) at[e] += order[i] < mine[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        if (lone >> e & 1) order[at[e]] = mine[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = (int)threadIdx.x * PER + e;
+        mine[e] = i < listed ? order[i] : ~0ull;
+    }
+    return true;
 }
 
 // The search over whole slices: for rows whose cut no list holds.
@@ -759,33 +863,19 @@ __device__ int locate(Row& r, int lo, int hi, double target, double& weight_out,
 // The list's order and cut. On entry list holds `listed` tokens in index order;
 // on return out[i] is token i's weight in the draw (0 where it is not kept).
 // above: mass of larger tokens outside the list; all: mass that p refers to
-// (0: that of the first k). False where the border of p lies outside a list
-// that has tokens above it. A thread holds PER neighbours of the order.
+// (0: that of the first k). 0 where the border of p lies outside a list that has
+// tokens above it, -1 where too many are nearly equal to be put in order, else 1.
+// A thread holds PER neighbours of the order.
 template <int PER, typename M, typename D>
-__device__ bool settle_list(Shared& sh, const float* list, unsigned long long* order, double* out, int listed, int k,
-                            float p, double above, double all, bool sure, M mass, D draw) {
+__device__ int settle_list(Shared& sh, const float* list, unsigned long long* order, double* out, int listed, int k,
+                           float p, double above, double all, bool sure, M mass, D draw) {
     unsigned long long mine[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int i = e * kThreads + threadIdx.x;
         mine[e] = i < listed ? (unsigned long long)~key_of(list[i]) << 32 | (unsigned)i : ~0ull;
     }
-    if (PER == 1 && listed <= kThreads / 2) {
-        // few: every token counts those before it
-        order[threadIdx.x] = mine[0];
-        __syncthreads();
-        int rank = 0;
-        for (int j = 0; j < (listed + 1) / 2; ++j) {
-            const ulonglong2 w = reinterpret_cast<const ulonglong2*>(order)[j];
-            rank += (w.x < mine[0]) + (w.y < mine[0]);
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < listed) order[rank] = mine[0];
-        __syncthreads();
-        if ((int)threadIdx.x < listed) mine[0] = order[threadIdx.x];
-    } else {
-        sort_block<PER>(mine, order);
-    }
+    if (!order_list<PER>(sh, mine, list, order, listed)) return -1;
     int kept = k > 0 && k < listed ? k : listed;
     bool holds = true;
     if (p < 1.0f) {
@@ -859,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     // Where the histogram lies and what the sums refer to: the largest of a
     // sample of the row, the same for all its blocks.
     const bool exps = !greedy && (sums_all || p < 1.0f);
-    if (exps && threadIdx.x < kExpTable) sh.segment[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
+    if (exps && threadIdx.x < kExpTable) reinterpret_cast<double*>(sh.share)[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
     if (threadIdx.x == 0) sh.pool_used = 0;
     if (threadIdx.x < kWarps * kSub) sh.seg[threadIdx.x] = 0.0, sh.listed_part[threadIdx.x] = 0;
 #pragma unroll
@@ -877,7 +967,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     if (exps) {
 #pragma unroll
         for (int i = 0; i < kExpTable / kWarps; ++i)
-            sh.exp2_table[i * kWarps + warp][lane] = sh.segment[i * kWarps + warp];
+            sh.exp2_table[i * kWarps + warp][lane] = reinterpret_cast<const double*>(sh.share)[i * kWarps + warp];
     }
     center = __uint_as_float(sh.wlo[lane % kWarps]);
     // the fourth largest of the warps' maxima: six in a thousand tokens or so are above it
@@ -891,6 +981,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) center = fmaxf(center, __shfl_xor_sync(0xFFFFFFFFu, center, o));
     __syncthreads();
+    reinterpret_cast<uint2*>(sh.share)[threadIdx.x] = make_uint2(0, 0);
     // a masked sample, or values too large for the bins
     if (!(fabsf(center) < 1e4f)) center = upper = 0.0f;
     if (!(fabsf(upper) < 1e4f)) upper = center;
@@ -1035,20 +1126,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     // draw asks for the very first or last token with a weight.
     if ((sure || draws_all) && !(u > 1e-100 && u < 1.0 - 1e-9)) wide = true;
     if (!draws_all && !wide) {
-        uint32_t count[kPer] = {};
-#pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i) {
-            if (i >= ranks) break;
-            const uint4 c = *reinterpret_cast<const uint4*>(r.of(sh.fine, i) + threadIdx.x * kPer);
-            count[0] += c.x, count[1] += c.y, count[2] += c.z, count[3] += c.w;
+        uint4 c;
+        if (ranks == 1) {
+            c = reinterpret_cast<const uint4*>(sh.fine)[threadIdx.x];
+        } else {
+            // Each block sums its share of the bins over all blocks, then all
+            // read the sums: what crosses between multiprocessors (10 bytes a
+            // cycle) is a quarter of all histograms read by all.
+            const int quads = kFine / 4 / ranks;  // of a share; as many threads read from each block
+            const int quad = threadIdx.x % quads, from = threadIdx.x / quads;
+            const uint4 part = reinterpret_cast<const uint4*>(r.of(sh.fine, from))[rank * quads + quad];
+            atomicAdd(&sh.share[quad * 4], part.x), atomicAdd(&sh.share[quad * 4 + 1], part.y);
+            atomicAdd(&sh.share[quad * 4 + 2], part.z), atomicAdd(&sh.share[quad * 4 + 3], part.w);
+            cluster.sync();
+            c = reinterpret_cast<const uint4*>(r.of(sh.share, from))[quad];
         }
+        const uint32_t count[kPer] = {c.x, c.y, c.z, c.w};
         if (!sure) {
             // top-p behind top-k needs the mass of all k; otherwise nothing below min-p's bin matters
             last = mp > 0.0f && !(k > 0 && p < 1.0f)
                        ? bin_of(__double2float_rd((double)top + log((double)mp) - 1e-4))
                        : kFine;
             if (k > 0) {
-                const int by_k = fine_border<uint32_t>(sh, count, (uint32_t)k);
+                const int by_k = fine_borders<uint32_t>(sh, count, (uint32_t)k, (uint32_t)k).x;
                 if (by_k > last) k = 0;  // what min-p keeps is less than k
                 else last = by_k;
             }
@@ -1060,22 +1160,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             // The first bin takes what the sum has beyond the others. Where
             // that is not enough, the list does not hold the border and the
             // wide search settles the row.
-            double guess[kPer], own = 0.0, squares = 0.0, others, spread;
+            double guess[kPer], others = 0.0, spread = 0.0;
             double one = exp(((double)bin_of.high - 8388608.0 - (double)(threadIdx.x * kPer)) / kFinePerNat - ref);
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
                 guess[e] = threadIdx.x * kPer + e ? (double)count[e] * one : 0.0;
-                own += guess[e], squares += guess[e] * one;
+                others += guess[e], spread += guess[e] * one;
                 one *= 0.98449643700540845;  // exp(-1 / kFinePerNat)
             }
-            block_scan(sh, own, others);
-            block_scan(sh, squares, spread);
+            block_sums(sh, others, spread);
             if (threadIdx.x == 0) guess[0] = fmax(m.sum - others, 0.0);
             const double border = (double)p * m.sum;
             const double none = 3.8e-11 * (double)a.vocab;
             const double off = fmin(m.sum / 125.0, 6.0 / 222.0 * sqrt(spread) + 1e-4 * m.sum) + none;
-            first = fine_border<double>(sh, guess, border - off);
-            last = fine_border<double>(sh, guess, border + off);
+            const int2 at = fine_borders<double>(sh, guess, border - off, border + off);
+            first = at.x, last = at.y;
         }
     }
 
@@ -1224,16 +1323,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             if (threadIdx.x == 0) sh.won = -1;
             if (!draws_all) {
                 if (warp == 0) {  // where each warp's tokens start in the list
-                    int before = 0;
-                    for (int g = 0; g < segs; g += 32) {
-                        const int c = g + lane < segs ? r.of(sh.listed, (g + lane) / kWarps)[(g + lane) % kWarps] : 0;
-                        int incl = c;
+                    int before = 0, c[kMaxCluster * kWarps / 32];
+#pragma unroll
+                    for (int q = 0; q < kMaxCluster * kWarps / 32; ++q) {
+                        const int g = min(q * 32 + lane, segs - 1);
+                        c[q] = r.of(sh.listed, g / kWarps)[g % kWarps];
+                    }
+#pragma unroll
+                    for (int q = 0; q < kMaxCluster * kWarps / 32; ++q) {
+                        const int g = q * 32 + lane, own = g < segs ? c[q] : 0;
+                        int incl = own;
 #pragma unroll
                         for (int o = 1; o < 32; o <<= 1) {
                             const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
                             if (lane >= o) incl += up;
                         }
-                        if (g + lane < segs) sh.offset[g + lane] = before + incl - c;
+                        if (g < segs) sh.offset[g] = before + incl - own;
                         before += __shfl_sync(0xFFFFFFFFu, incl, 31);
                     }
                     if (lane == 0) sh.offset[segs] = before;
@@ -1273,12 +1378,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                     return settle_list<decltype(per)::value>(sh, list, order, weight_of, listed, k, p, above, all, sure,
                                                              list_mass, kept_weight);
                 };
-                if (listed <= kThreads) {
-                    holds = settle(std::integral_constant<int, 1>());
-                } else if (listed <= 2 * kThreads) {
-                    holds = settle(std::integral_constant<int, 2>());
-                } else {
-                    // too long to sort in time: the search by key ranges, on the list (17 us against 37 at 4096)
+                int settled = -1;
+                if (listed <= kThreads) settled = settle(std::integral_constant<int, 1>());
+                else if (listed <= 2 * kThreads) settled = settle(std::integral_constant<int, 2>());
+                else if (listed <= 4 * kThreads) settled = settle(std::integral_constant<int, 4>());
+                else settled = settle(std::integral_constant<int, 8>());
+                holds = settled != 0;
+                if (settled < 0) {  // the search by key ranges, on the list
                     Row l{a, sh, list, list_index, 0, listed, ((listed + kThreads - 1) / kThreads) * 32, 0, 1, 0, 0, cluster};
                     Cut cut{1u, INT_MAX};
                     if (k > 0 && k < listed) cut = cut_top_k(l, top, (uint32_t)k);
@@ -1396,6 +1502,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
 using namespace strata;
 
+// How many clusters of `ranks` blocks the context's device (the current one)
+// runs at once with a block a multiprocessor: fewer than its multiprocessors
+// divided by `ranks` (15 of 8 on 148), as a cluster stays within a part of them.
+static int64_t clusters_at_once(strata_ctx* ctx, int ranks) {
+    static std::atomic<int> known[64][4];
+    std::atomic<int>* slot = ctx->device < 64 ? &known[ctx->device][ranks == 8 ? 3 : ranks / 2] : nullptr;
+    int n = slot ? slot->load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ranks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)(kListBytes + kMaxSlice);
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<true>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = ctx->sm_count / ranks;
+    }
+    if (slot) slot->store(n, std::memory_order_relaxed);
+    return n;
+}
+
 extern "C" int strata_cuda_sample_dev(strata_ctx* ctx, const float* logits_dev, int64_t rows, int64_t vocab,
                                       int64_t stride, const float* temperature_dev, const int32_t* top_k_dev,
                                       const float* top_p_dev, const float* min_p_dev, const double* uniform_dev,
@@ -1408,20 +1540,24 @@ extern "C" int strata_cuda_sample_dev(strata_ctx* ctx, const float* logits_dev, 
                                 uniform_dev, ids_dev, logprobs_dev);
     if (rc) return fail(ctx, rc, "sample: %s", why.text);
     DeviceGuard dev(ctx->device);
-    // blocks a row takes: as many as keep the GPU busy with two a multiprocessor
-    // (eight are the portable cluster), each with at least 2048 logits
-    int ranks = 1;
-    while (ranks < kMaxCluster && vocab > (int64_t)ranks * 2048 && rows * ranks * 2 <= 2 * (int64_t)ctx->sm_count)
-        ranks *= 2;
+    static std::atomic<uint64_t> asked[2];
+    cudaError_t e = allow_shared(sample_kernel<true>, kListBytes + kMaxSlice, asked[0], ctx->device);
+    if (e == cudaSuccess) e = allow_shared(sample_kernel<false>, kListBytes + kMaxSlice, asked[1], ctx->device);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(sample)");
+    // Blocks a row takes: as many as let all rows run at once with a block a
+    // multiprocessor (eight are the portable cluster), each with at least 1024
+    // logits; one where there are more rows, two a multiprocessor then. Two
+    // blocks that share one wait for each other's issue slots in every step: 32
+    // rows of 151,936 logits with top-k take 24 us in clusters of 4, 30 in
+    // clusters of 8 two a multiprocessor, 17 rows of 32,003 17 us against 22.
+    int ranks = kMaxCluster;
+    while (ranks > 1 && (vocab <= (int64_t)ranks * 1024 || rows > clusters_at_once(ctx, ranks))) ranks /= 2;
     const int64_t slice = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
     const bool resident = slice * 4 <= (rows * ranks > ctx->sm_count ? kPairSlice : kMaxSlice);
     const bool packs = stride % 4 == 0 && vocab % 4 == 0 && (uintptr_t)logits_dev % 16 == 0;
     SampleArgs a{logits_dev, stride, temperature_dev, top_k_dev, top_p_dev, min_p_dev, uniform_dev, ids_dev,
                  logprobs_dev, (int)vocab, (int)slice, resident};
     auto kernel = packs ? sample_kernel<true> : sample_kernel<false>;
-    static std::atomic<uint64_t> asked[2];
-    cudaError_t e = allow_shared(kernel, kListBytes + kMaxSlice, asked[packs], ctx->device);
-    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(sample)");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ranks));
     cfg.blockDim = dim3(kThreads);

@@ -213,6 +213,22 @@ def test_lists_of_every_length(ctx, rows, vocab, sigma):
         check(ctx, x, u, **kw)
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 3500), (3, 20000), (40, 3999), (160, 3600)])
+def test_crowds_of_equal_and_nearly_equal_logits(ctx, rows, vocab):
+    """Rounded logits (hundreds of one value), and thousands of different ones within a hair beside a few far above."""
+    rng = np.random.default_rng(rows)
+    u = list(rng.random(rows))
+    k = [int(v) for v in rng.choice([100, 300, 700, 1500, 2500, 3400], rows)]
+    p = list(rng.choice([0.2, 0.6, 0.9, 0.97], rows))
+    rounded = np.round(rng.standard_normal((rows, vocab)) * 1.5 * 8) / 8
+    close = rng.standard_normal((rows, vocab)) * 1e-5
+    close[:, rng.integers(0, vocab, 3)] = 11.0
+    halves = np.where(rng.random((rows, vocab)) < 0.1, rng.standard_normal((rows, vocab)), np.round(rng.standard_normal((rows, vocab))))
+    for x in (rounded, close, halves):
+        for kw in (dict(k=k), dict(p=p), dict(k=k, p=p), dict(k=k, p=p, m=[0.001] * rows, t=[1.7] * rows), dict(p=p, t=[0.5] * rows)):
+            check(ctx, x.astype(np.float32), u, **kw)
+
+
 def test_a_nearly_flat_row_too_long_for_shared_memory(ctx):
     rng = np.random.default_rng(21)
     x = (rng.standard_normal((2, 700001)) * 0.1).astype(np.float32)
