@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             const int r = lane >> 1, i = warp * 8 + (r & 7);
             const float f = a.norm ? 1.0f / sqrtf(squares[0] + a.eps) : 1.0f;
             (r < 8 ? fk : fq)[i] = i < n ? (r < 8 ? down * f : down * f * a.scale) : 0.0f;
-            if (r < 8) kn[i] = i < n ? sqrtf((float)DK * squares[0]) * f : 0.0f;
+            // DK times the squares may leave f32 where they do not
+            if (r < 8) kn[i] = i < n ? sqrtf((float)DK) * (sqrtf(squares[0]) * f) : 0.0f;
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
