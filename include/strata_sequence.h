@@ -80,11 +80,17 @@ int strata_cuda_short_conv_dev(strata_ctx *ctx, const strata_short_conv *desc, c
  * Where l2_eps >= 0, q and k are first divided by sqrt(sum of squares + l2_eps)
  * per head; a negative l2_eps takes them as they are. k_dim 1..256, v_dim 1..8192.
  *
- * Products and sums are f32, or carry 22 bits (limb products on the tensor
- * cores, where sequences are read in chunks of 32 tokens: k_dim up to 128 and a
- * sequence of 16 tokens or more in the call, 32 where there are few heads and
- * sequences; many shorter ones beside it are still read token by token); o is
- * rounded once. Chunks need strata_cuda_gated_delta_work_bytes bytes of
+ * Products and sums are f32; o is rounded once. Sequences are read in chunks of
+ * 32 tokens on the tensor cores where k_dim is up to 128 and a sequence of the
+ * call has 16 tokens or more, 32 where there are few heads and sequences (many
+ * shorter ones beside it are still read token by token). There, products over
+ * k_dim carry 22 bits of the norms of their vectors (a key, a query, a column of
+ * the state), all others 22 bits of themselves: however the sizes of tokens and
+ * columns differ, none costs another, nor an earlier token, precision. Either
+ * way, squares of q and k are summed in f32, so normalised ones have norms below
+ * 1.8e19, and in chunks the decay from one token to another within 32 is one f32
+ * factor: gates above 0 may add up to 88 there, and below e^-88 it counts as 0.
+ * Chunks need strata_cuda_gated_delta_work_bytes bytes of
  * work_dev (16-byte aligned; its contents need not be kept between calls, and
  * calls that may overlap need one each); where that is 0 work_dev may be NULL.
  * A NaN or infinity among a token's inputs reaches its own and later outputs of

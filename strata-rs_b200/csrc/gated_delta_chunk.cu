@@ -14,22 +14,28 @@
 // no second product with the keys). delta_scan_kernel then goes through the
 // chunks of a sequence in order with S in registers.
 //
-// Precision. The products run on the tensor cores as f16 limbs: x 2^e = hi + lo
-// with the exponent e taken per row from the row's largest magnitude or a bound
-// of it (X and U: from the chunk's norms, prepared with it, so that warps can
-// scale apart from each other). A limb pair carries 22 bits of what is within
-// 2^-18 of the bound, 2^-40 of the bound below that, and lo hi + hi lo + hi hi is summed in f32,
-// the two small products first. That keeps f32-like results at f16 rate; plain
-// tf32 would carry 11 bits. Keys and queries given
-// as bf16 are exact in one limb. The scan adds to S outside the tensor core,
-// where the addition rounds to nearest.
+// Precision. Products over k_dim run on the tensor cores as f16 limbs: x 2^e =
+// hi + lo with the exponent e taken per vector (a key, a query, a column of S)
+// from its largest magnitude. A limb pair carries 22 bits of what is within 2^-18
+// of that, 2^-40 of it below, and lo hi + hi lo + hi hi is summed in f32, the two
+// small products first. That keeps f32-like results at f16 rate; plain tf32 would
+// carry 11 bits. Keys and queries given as bf16 are exact in one limb.
+// The two triangular products over a chunk's tokens, T X and P U, take tf32 limbs
+// instead, which have f32's exponents: tokens of one column may differ by any
+// factor (outliers, states that grow), and a scale shared by a chunk would let
+// later ones take bits from earlier ones. hi is rounded, so that lo lacks the last
+// of f32's bits at most. (In plain f32 on the CUDA cores these two cost 0.38 us a
+// chunk: reading the operands for a dot product a lane fills shared memory's
+// bandwidth.) Only what is added to S at the chunk's end, a sum over its tokens
+// anyway, shares a scale per column and 16 tokens. The scan adds to S outside the
+// tensor core, where the addition rounds to nearest.
 //
 // Layout of the scan. The columns of S are independent, and products are
 // written transposed: a group of warps has 16 columns of S as the 16 rows of
-// m16n8k16 products, S^T K^T, X^T T^T, U^T P^T, U^T K. An accumulator tile is
-// then, split into limbs, the left operand of the next product without leaving
-// the registers, and the right operands (keys, queries, T, P) are the same for
-// all columns: they are staged in shared memory by bulk copies one chunk ahead.
+// m16n8k16 (k8 in tf32) products, S^T K^T, X^T T^T, U^T P^T, U^T K. An accumulator
+// tile is then, split into limbs, the left operand of the next product as it lies,
+// and the right operands (keys, queries, T, P) are the same for all columns: they
+// are staged in shared memory by bulk copies one chunk ahead.
 // Two warps of a group hold half of S's rows each and follow the chain from
 // chunk to chunk; the sums over k_dim, X and U go between them through shared
 // memory, half of the tokens each. Two more take S's limbs and U from there and
@@ -40,11 +46,11 @@
 // allows.
 //
 // Measured at 32 value and 16 key heads of 128 x 128: one sequence of 8192 f32
-// tokens 619 us, 98 of it prepare (368 MB, 3.8 TB/s; warps wait for loads and
-// for their row sums) and 520 the scan (2.0 us a chunk, 128 blocks; 1.7 us
-// without outputs). The tensor cores are a third busy: chunks of 64 would halve
-// the steps of the chain, but their images do not fit shared memory three deep.
-// Eight bf16 sequences of 1 to 2049 tokens, 7036 in all, 423 us (92 and 333).
+// tokens 623 us, 86 of it prepare (366 MB, 4.3 TB/s; warps wait for loads and
+// for their row sums) and 535 the scan (2.1 us a chunk, 128 blocks). The tensor
+// pipe is busy for 36% of the scan's cycles: chunks of 64 would halve the steps
+// of the chain, but their images do not fit shared memory three deep. Eight bf16
+// sequences of 1 to 2049 tokens, 7036 in all, 416 us (84 and 327).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -57,18 +63,15 @@ namespace {
 
 constexpr int kChunk = 32;
 constexpr int kThreads = 128;                  // of a prepare block
-constexpr int kPitchT = kChunk * 2 + 16;       // bytes of a row of T or P: 16-byte steps that no two of 8 rows share
-constexpr int kLimbT = kChunk * kPitchT;
-constexpr int kGates = 4 * kLimbT;             // T hi, T lo, P hi, P lo, then the gate rows
-enum { kBeta, kXk, kOq, kDown, kScaleT, kScaleP, kChunkRow, kGateRows };
-// The last row: e^{G_C}, and what bounds X by the largest of S (kBoundS) and of
-// V (kBoundV), U by X, and U scaled to the chunk's end by U.
-enum { kTotal, kBoundS, kBoundV, kBoundU, kBoundEnd };
+constexpr int kPitchT = kChunk + 8;            // floats of a row of T or P: 32-byte steps that no two of 4 rows share
+constexpr int kMatT = kChunk * kPitchT * 4;
+constexpr int kGates = 2 * kMatT;              // T, P, then the gate rows; the last one starts with e^{G_C}
+enum { kBeta, kXk, kOq, kDown, kTotal, kGateRows };
 constexpr int kImageT = kGates + kGateRows * kChunk * 4;
 constexpr uint64_t kMaxWork = uint64_t(256) << 20;
 
 // The image of a chunk's keys and queries: K limbs, then Q limbs, rows of
-// DK halves padded as T's.
+// DK halves padded to 16-byte steps that no two of 8 rows share.
 template <int DK, int LIMBS>
 struct Image {
     static constexpr int kPitch = DK * 2 + 16;
@@ -76,12 +79,16 @@ struct Image {
     static constexpr int kBytes = 2 * LIMBS * kLimb;
 };
 
-// The power of two that brings m to [2^14, 2^15), and its inverse. Both stay normal numbers.
-__device__ __forceinline__ void power_for(float m, float& up, float& down) {
-    int f = 268 - (int)((__float_as_uint(m) >> 23) & 255u);
+// The power of two that brings a number of this (biased) exponent to [2^14, 2^15),
+// and its inverse. Both stay normal numbers.
+__device__ __forceinline__ void power_of(uint32_t exponent, float& up, float& down) {
+    int f = 268 - (int)exponent;
     f = f < 2 ? 2 : f > 252 ? 252 : f;
     up = __uint_as_float((uint32_t)f << 23);
     down = __uint_as_float((uint32_t)(254 - f) << 23);
+}
+__device__ __forceinline__ void power_for(float m, float& up, float& down) {
+    power_of((__float_as_uint(m) >> 23) & 255u, up, down);
 }
 
 // (x, y) as two f16 limbs, packed with x in the low half.
@@ -98,6 +105,17 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same of 8 products, tf32: what a register holds beyond 11 bits is not read.
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// x as two tf32 limbs. A NaN whose bits carry into the sign is still one in lo.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
@@ -149,15 +167,19 @@ constexpr int kPitchA = kChunk + 4;  // floats of a row of A: 16-byte steps that
 template <int DK, int LIMBS>
 constexpr int prepare_smem() {
     constexpr int scratch = 4 * kChunk * kPitchA * 4, image = Image<DK, LIMBS>::kBytes;
-    return (image > scratch ? image : scratch) + (2 * kChunk * (kChunk + 1) + 3 * kChunk) * 4;
+    return (image > scratch ? image : scratch) + (2 * kChunk * (kChunk + 1) + 2 * kChunk) * 4;
 }
 
-// e^x for a sum of log decays: the argument's rounding is 2^-24 |x| of the
-// result, which is below 2^-25 of 1 for every x <= 0.
-__device__ __forceinline__ float decay(float x) {
+// 2^(i + f) for |f| <= 1, good to 2^-22 of itself: a decay between two tokens as
+// the exact difference of the whole parts of their sums and the rounded one of
+// the rest, so that its precision does not depend on its size. From 2^-127 down it
+// is zero, from i = 128 up infinite (a second factor would reach further, for 25%
+// of the prepare kernel's time).
+__device__ __forceinline__ float power(int i, float f) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
-    return y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(f));
+    i = min(max(i, -127), 128);
+    return y * __int_as_float((i + 127) << 23);
 }
 
 // Reduces 16 values of a lane across the warp: v[0] becomes value lane / 2's.
@@ -174,32 +196,6 @@ __device__ __forceinline__ void reduce_rows(float (&v)[16], F op) {
     v[0] = op(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 1));
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    return v;
-}
-
-// 32 values of a row as two limbs of halves, scaled to the row's largest
-// magnitude; returns what undoes the scale.
-__device__ __forceinline__ float store_row(const float (&v)[kChunk], uint8_t* hi_at, uint8_t* lo_at) {
-    float m = 0.0f, up, down;
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) m = fmaxf(m, fabsf(v[j]));
-    power_for(m, up, down);
-#pragma unroll
-    for (int j = 0; j < kChunk; j += 8) {
-        uint4 hi, lo;
-        split(v[j] * up, v[j + 1] * up, hi.x, lo.x);
-        split(v[j + 2] * up, v[j + 3] * up, hi.y, lo.y);
-        split(v[j + 4] * up, v[j + 5] * up, hi.z, lo.z);
-        split(v[j + 6] * up, v[j + 7] * up, hi.w, lo.w);
-        *reinterpret_cast<uint4*>(hi_at + j * 2) = hi;
-        *reinterpret_cast<uint4*>(lo_at + j * 2) = lo;
-    }
-    return down;
-}
-
 // One block per chunk and key head: limbs of K and Q, K K^T and Q K^T; then,
 // for each value head of that key head, one warp for T and one for P.
 template <typename T, int DK, int LIMBS>
@@ -210,11 +206,10 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
     constexpr int PER = DK / 32;  // elements of a row a lane holds
     extern __shared__ __align__(16) uint8_t smem[];
     float(*kk)[kChunk + 1] =
-        reinterpret_cast<float(*)[kChunk + 1]>(smem + prepare_smem<DK, LIMBS>() - (2 * kChunk * (kChunk + 1) + 3 * kChunk) * 4);
+        reinterpret_cast<float(*)[kChunk + 1]>(smem + prepare_smem<DK, LIMBS>() - (2 * kChunk * (kChunk + 1) + 2 * kChunk) * 4);
     float(*qk)[kChunk + 1] = kk + kChunk;
     float* fk = &qk[kChunk][0];  // what a row of limbs is to be multiplied with
     float* fq = fk + kChunk;
-    float* kn = fq + kChunk;      // a bound of the sum of a key's magnitudes
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float(*A)[kPitchA] = reinterpret_cast<float(*)[kPitchA]>(smem) + warp * kChunk;
     const int tile = blockIdx.x / a.k_heads, hk = blockIdx.x - tile * a.k_heads;
@@ -267,8 +262,6 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             const int r = lane >> 1, i = warp * 8 + (r & 7);
             const float f = a.norm ? 1.0f / sqrtf(squares[0] + a.eps) : 1.0f;
             (r < 8 ? fk : fq)[i] = i < n ? (r < 8 ? down * f : down * f * a.scale) : 0.0f;
-            // DK times the squares may leave f32 where they do not
-            if (r < 8) kn[i] = i < n ? sqrtf((float)DK) * (sqrtf(squares[0]) * f) : 0.0f;
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -347,10 +340,11 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
         if (task != warp) gate_of(h, g, beta);
         if (lane < n) {
             gates(a, h, g, beta);
-            // e^-10000 is zero; a sum of these stays a number, so that differences do
+            // e^-10000 is zero and e^10000 infinite; a sum of these stays a number, so that differences do
             if (g < -1e4f) g = -1e4f;
+            if (g > 1e4f) g = 1e4f;
         }
-        double G = (double)g;  // differences of the sums must keep f32's precision
+        double G = (double)g * 1.4426950408889634;  // in powers of two
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double up = __shfl_up_sync(0xFFFFFFFFu, G, o);
@@ -361,25 +355,22 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
         float v[kChunk];  // a row a lane: beta_i e^{G_i - G_j} k_i . k_j, or e^{G_i - G_j} q_i . k_j
         const float(*products)[kChunk + 1] = task & 1 ? qk : kk;
         const int diagonal = task & 1 ? lane : lane - 1;  // the row's last column
-        const float Gh = (float)G, Gl = (float)(G - (double)Gh);  // the sum in two floats
+        const int Gi = __double2int_rn(G);  // whole (at most 32 * 1e4 log2 e; a NaN is the rest's) and rest
+        const float Gf = (float)(G - (double)Gi);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
-            const float h = __shfl_sync(0xFFFFFFFFu, Gh, j), l = __shfl_sync(0xFFFFFFFFu, Gl, j);
-            v[j] = j <= diagonal ? decay((Gh - h) + (Gl - l)) * products[lane][j] : 0.0f;
+            const int i = __shfl_sync(0xFFFFFFFFu, Gi, j);
+            const float f = __shfl_sync(0xFFFFFFFFu, Gf, j);
+            v[j] = j <= diagonal ? power(Gi - i, Gf - f) * products[lane][j] : 0.0f;
         }
         if (task & 1) {
-            const float down = store_row(v, image + 2 * kLimbT + lane * kPitchT, image + 3 * kLimbT + lane * kPitchT);
-            out[kScaleP * kChunk] = down;
-            const double end = __shfl_sync(0xFFFFFFFFu, G, 31);
-            const float before = expf((float)G), after = expf((float)(end - G));
-            const float bs = warp_max(fabsf(beta) * before * kn[lane]), bv = warp_max(fabsf(beta));
-            const float be = warp_max(after * fabsf(fk[lane]));
-            if (lane == 0) {
-                out[kChunkRow * kChunk + kTotal] = expf((float)end);
-                out[kChunkRow * kChunk + kBoundS] = bs;
-                out[kChunkRow * kChunk + kBoundV] = bv;
-                out[kChunkRow * kChunk + kBoundEnd] = be;
-            }
+            float4* row = reinterpret_cast<float4*>(image + kMatT) + lane * (kPitchT / 4);
+#pragma unroll
+            for (int j = 0; j < kChunk; j += 4) row[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            const int end_i = __shfl_sync(0xFFFFFFFFu, Gi, 31);
+            const float end_f = __shfl_sync(0xFFFFFFFFu, Gf, 31);
+            const float before = power(Gi, Gf), after = power(end_i - Gi, end_f - Gf);
+            if (lane == 0) out[kTotal * kChunk] = power(end_i, end_f);
             out[kBeta * kChunk] = beta;
             out[kXk * kChunk] = beta * before * fk[lane];
             out[kOq * kChunk] = before * fq[lane];
@@ -406,20 +397,8 @@ __global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaArgs
             for (int j = i & ~3; j < i; ++j) acc[j & 1] = fmaf(A[i][j], v[j], acc[j & 1]);
             v[i] = acc[0] + acc[1];
         }
-        // and back to a row a lane
-        __syncwarp();
-        float* flat = &A[0][0];
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) flat[i * (kChunk + 1) + lane] = v[i];
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[j] = flat[lane * (kChunk + 1) + j];
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) sum += fabsf(v[j]);
-        sum = warp_max(sum);
-        if (lane == 0) out[kChunkRow * kChunk + kBoundU] = sum;
-        out[kScaleT * kChunk] = store_row(v, image + lane * kPitchT, image + kLimbT + lane * kPitchT);
+        for (int i = 0; i < kChunk; ++i) reinterpret_cast<float*>(image)[i * kPitchT + lane] = v[i];
     }
 }
 
@@ -434,31 +413,33 @@ struct Split {
     static constexpr int kParts = 2, kCols = GROUPS * 16;
     static constexpr int kHolders = GROUPS * kParts * 32, kThreads = kHolders + GROUPS * 64;
     static constexpr int kRows = DK / kParts;    // rows of S a warp holds
-    static constexpr int kTiles = 4 / kParts;    // tiles of 8 tokens whose X and U it computes
 };
 
 // What a group's warps hand on to its outputs' (two, for even and odd chunks):
-// S's limbs and their row factors, U and what undoes its scale. Limbs lie as
-// left operands take them: two rows of hi, two of lo.
+// S's limbs and their row factors, and U. Limbs lie as left operands take them:
+// two rows of hi, two of lo. Tiles of U, X and S^T K^T lie as accumulators do.
 template <int DK>
 struct Handoff {
     uint4 hi[DK / 16][32], lo[DK / 16][32];
-    float2 down[2][32], scale[32];
-    uint4 u[4][32];
+    float2 down[2][32];
+    float4 u[4][32];
 };
-// And among each other, within a chunk: parts of S^T K^T with the largest
-// magnitudes of their rows of S and V, X, and U scaled to the chunk's end.
-template <int DK>
+// And among each other, within a chunk: parts of S^T K^T, X, and the limbs of U
+// scaled to the chunk's end with what undoes their scale.
 struct Shared {
-    float4 y[2][4][32];
-    float4 top[2][8];  // S and V of a row, and of the row 8 on
-    uint4 x[4][32], e[4][32];
+    float4 y[2][4][32], x[4][32];
+    uint4 e[4][32];
+    float2 e_down[2][32];
 };
+
+// Of the four tiles of 8 tokens of a chunk, those (k = 0, 1) that the warp `part`
+// of a pair takes: together as long as the other's in a triangular product.
+__device__ __forceinline__ int tile_of(int part, int k) { return k ? 3 - part : part; }
 
 template <int DK, int LIMBS, int GROUPS>
 constexpr int scan_smem() {
     return kStages * (Image<DK, LIMBS>::kBytes + kImageT) + 2 * GROUPS * (int)sizeof(Handoff<DK>) +
-           GROUPS * (int)sizeof(Shared<DK>);
+           GROUPS * (int)sizeof(Shared);
 }
 
 // Named barriers of a group: `threads` of them arrive in all.
@@ -469,32 +450,34 @@ __device__ __forceinline__ void group_arrive(int id, int threads) {
     asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
 }
 
-// The largest magnitude of a row of the warp's tile: rows lie across 4 lanes.
-__device__ __forceinline__ float row_max(float m) {
-    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    return fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+// Powers for two rows of the warp's tile from a lane's largest magnitudes of each:
+// rows lie across 4 lanes. The exponents of both go through one exchange.
+__device__ __forceinline__ void row_powers(float m0, float m1, float (&up)[2], float (&down)[2]) {
+    uint32_t e = __byte_perm(__float_as_uint(m0) << 1, __float_as_uint(m1) << 1, 0x7733) & 0x00FF00FFu;
+    e = __vmaxu2(e, __shfl_xor_sync(0xFFFFFFFFu, e, 1));
+    e = __vmaxu2(e, __shfl_xor_sync(0xFFFFFFFFu, e, 2));
+    power_of(e & 255u, up[0], down[0]);
+    power_of(e >> 16, up[1], down[1]);
 }
 
 // Tiles x (16 rows by 8 N columns) as limbs of a left operand, scaled by row;
 // down: what undoes the scale, for the two rows of a lane.
 template <int N>
 __device__ __forceinline__ void limbs(const float (&x)[N][4], uint32_t (&hi)[N / 2][4], uint32_t (&lo)[N / 2][4],
-                                      float (&down)[2], float (&most)[2]) {
-    float m0 = 0.0f, m1 = 0.0f, up0, up1;
+                                      float (&down)[2]) {
+    float m0 = 0.0f, m1 = 0.0f, up[2];
 #pragma unroll
     for (int t = 0; t < N; ++t) {
         m0 = fmaxf(m0, fmaxf(fabsf(x[t][0]), fabsf(x[t][1])));
         m1 = fmaxf(m1, fmaxf(fabsf(x[t][2]), fabsf(x[t][3])));
     }
-    most[0] = row_max(m0), most[1] = row_max(m1);
-    power_for(most[0], up0, down[0]);
-    power_for(most[1], up1, down[1]);
+    row_powers(m0, m1, up, down);
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) {
-        split(x[2 * k][0] * up0, x[2 * k][1] * up0, hi[k][0], lo[k][0]);
-        split(x[2 * k][2] * up1, x[2 * k][3] * up1, hi[k][1], lo[k][1]);
-        split(x[2 * k + 1][0] * up0, x[2 * k + 1][1] * up0, hi[k][2], lo[k][2]);
-        split(x[2 * k + 1][2] * up1, x[2 * k + 1][3] * up1, hi[k][3], lo[k][3]);
+        split(x[2 * k][0] * up[0], x[2 * k][1] * up[0], hi[k][0], lo[k][0]);
+        split(x[2 * k][2] * up[1], x[2 * k][3] * up[1], hi[k][1], lo[k][1]);
+        split(x[2 * k + 1][0] * up[0], x[2 * k + 1][1] * up[0], hi[k][2], lo[k][2]);
+        split(x[2 * k + 1][2] * up[1], x[2 * k + 1][3] * up[1], hi[k][3], lo[k][3]);
     }
 }
 
@@ -511,13 +494,49 @@ __device__ __forceinline__ void operand(const uint4& a, const uint4& b, uint32_t
     lo[0] = a.z, lo[1] = a.w, lo[2] = b.z, lo[3] = b.w;
 }
 
+// The tiles of X^T M^T of the warp PART of a pair, M lower triangular. A lane holds
+// tokens 2 c and 2 c + 1 of a tile of X where a product's left operand has its
+// terms c and c + 4: the right one is read in the same order.
+template <int PART>
+__device__ __forceinline__ void triangular(const float* M, const float4 (&X)[4][32], float (&acc)[2][4]) {
+    const int lane = threadIdx.x & 31;
+    const float* m = M + (lane >> 2) * kPitchT + (lane & 3) * 2;
+    float hl[2][4] = {}, lh[2][4] = {};  // apart: a product waits for the last one into its sum
+#pragma unroll
+    for (int t = 0; t <= 3 - PART; ++t) {
+        const float4 x = X[t][lane];
+        uint32_t ah[4], al[4];
+        split_tf32(x.x, ah[0], al[0]), split_tf32(x.z, ah[1], al[1]);
+        split_tf32(x.y, ah[2], al[2]), split_tf32(x.w, ah[3], al[3]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int out = k ? 3 - PART : PART;
+            if (t > out) continue;  // later tokens' columns of M are zero
+            const float2 w = *reinterpret_cast<const float2*>(m + out * 8 * kPitchT + t * 8);
+            uint32_t bh[2], bl[2];
+            split_tf32(w.x, bh[0], bl[0]), split_tf32(w.y, bh[1], bl[1]);
+            mma_tf32(hl[k], ah, bl);
+            mma_tf32(lh[k], al, bh);
+            mma_tf32(acc[k], ah, bh);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[k][r] += hl[k][r] + lh[k][r];
+}
+__device__ __forceinline__ void triangular(int part, const float* M, const float4 (&X)[4][32], float (&acc)[2][4]) {
+    if (part == 0) triangular<0>(M, X, acc);
+    else triangular<1>(M, X, acc);
+}
+
 template <typename T, int DK, int LIMBS, int GROUPS>
 __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
     delta_scan_kernel(const DeltaArgs a, const __grid_constant__ SeqTable tab, const uint8_t* __restrict__ images,
                       const uint8_t* __restrict__ images_t, int* err) {
     using I = Image<DK, LIMBS>;
     using L = Split<DK, GROUPS>;
-    constexpr int PARTS = L::kParts, ROWS = L::kRows, NT = ROWS / 8, KS = ROWS / 16, TILES = L::kTiles;
+    constexpr int PARTS = L::kParts, ROWS = L::kRows, NT = ROWS / 8, KS = ROWS / 16;
     constexpr int kStage = I::kBytes + kImageT;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t arrived[kStages], ready[GROUPS][2][2];  // ready: S's limbs, U; even and odd chunks
@@ -527,7 +546,7 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
     const int group = holds ? warp / PARTS : (warp - GROUPS * PARTS) / 2;
     const int part = holds ? warp % PARTS : (warp - GROUPS * PARTS) % 2;
     Handoff<DK>* const hands = reinterpret_cast<Handoff<DK>*>(smem + kStages * kStage) + group * 2;
-    Shared<DK>& sh = reinterpret_cast<Shared<DK>*>(smem + kStages * kStage + 2 * GROUPS * sizeof(Handoff<DK>))[group];
+    Shared& sh = reinterpret_cast<Shared*>(smem + kStages * kStage + 2 * GROUPS * sizeof(Handoff<DK>))[group];
     // Named barriers: chunk written out (even, odd), and among a group's warps of
     // S. Those only arrive at `ready` and may be a chunk ahead of the outputs
     // there, so that even and odd chunks have their own: one is used again two
@@ -585,14 +604,15 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
     const uint32_t lane_b = ((lane & 7) + ((lane >> 4) << 3));  // row of a right operand's pair of tiles
     const uint32_t half_b = ((lane >> 3) & 1) * 16;             // and its half of a row
 
-    if (!holds) {  // ---- outputs of tokens part * 16 .. + 15
+    if (!holds) {  // ---- outputs of the tokens of two tiles
         T* O = static_cast<T*>(a.o) + (int64_t)seq.row * a.o_stride + (int64_t)h * a.v_dim;
         for (int c = 0; c < chunks; ++c) {
             wait_chunk(c);
             const uint8_t* image = smem + (c % kStages) * kStage;
             const Handoff<DK>& hand = hands[c & 1];
             const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
-            const uint32_t q_at = shared_addr(image) + LIMBS * I::kLimb + (part * 16 + lane_b) * I::kPitch + half_b;
+            const uint32_t q_at = shared_addr(image) + LIMBS * I::kLimb +
+                                  (tile_of(part, lane >> 4) * 8 + (lane & 7)) * I::kPitch + half_b;
             float out[2][4] = {};
             wait_ready(0, c);
 #pragma unroll
@@ -628,40 +648,19 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
                     for (int r = 0; r < 4; ++r) out[t][r] = fmaf(o1[t][r], r < 2 ? down.x : down.y, out[t][r]);
             }
             wait_ready(1, c);
-            uint32_t hi[2][4], lo[2][4];
-            float c1[2][4] = {};
-            operand(hand.u[0][lane], hand.u[1][lane], hi[0], lo[0]);
-            operand(hand.u[2][lane], hand.u[3][lane], hi[1], lo[1]);
-            const float2 down = hand.scale[lane];
-            const uint32_t p_at =
-                shared_addr(image) + I::kBytes + 2 * kLimbT + (part * 16 + lane_b) * kPitchT + half_b;
-            uint32_t bh[2][4], bl[4];
+            float y[2][4] = {};
+            triangular(part, reinterpret_cast<const float*>(image + I::kBytes + kMatT), hand.u, y);
+            T* row = O + (int64_t)(c * kChunk + tc) * a.o_stride;
+            const int left = seq.len - (c * kChunk + tc);  // tokens from the lane's first
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {  // later tokens' columns of P are zero
-                ldmatrix(bh[ks], p_at + ks * 32);
-                ldmatrix(bl, p_at + kLimbT + ks * 32);
-                mma(c1[0], lo[ks], bh[ks][0], bh[ks][1]);
-                mma(c1[1], lo[ks], bh[ks][2], bh[ks][3]);
-                mma(c1[0], hi[ks], bl[0], bl[1]);
-                mma(c1[1], hi[ks], bl[2], bl[3]);
-            }
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                mma(c1[0], hi[ks], bh[ks][0], bh[ks][1]);
-                mma(c1[1], hi[ks], bh[ks][2], bh[ks][3]);
-            }
-            T* row = O + (int64_t)(c * kChunk + part * 16 + tc) * a.o_stride;
-            const int left = seq.len - (c * kChunk + part * 16 + tc);  // tokens from the lane's first
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const float2 sp = *reinterpret_cast<const float2*>(gate + kScaleP * kChunk + part * 16 + t * 8 + tc);
-                const float2 oq = *reinterpret_cast<const float2*>(gate + kOq * kChunk + part * 16 + t * 8 + tc);
+            for (int k = 0; k < 2; ++k) {
+                const int t = tile_of(part, k) * 8;
+                const float2 oq = *reinterpret_cast<const float2*>(gate + kOq * kChunk + t + tc);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float y1 = c1[t][r] * ((r < 2 ? down.x : down.y) * (r & 1 ? sp.y : sp.x));
-                    const float res = fmaf(r & 1 ? oq.y : oq.x, out[t][r], y1);
-                    if (t * 8 + (r & 1) < left && (r < 2 ? in0 : in1))
-                        from_f32(row[(t * 8 + (r & 1)) * a.o_stride + (r < 2 ? j0 : j1)], res);
+                    const float res = fmaf(r & 1 ? oq.y : oq.x, out[k][r], y[k][r]);
+                    if (t + (r & 1) < left && (r < 2 ? in0 : in1))
+                        from_f32(row[(t + (r & 1)) * a.o_stride + (r < 2 ? j0 : j1)], res);
                 }
             }
             // the stage and the handoff may be written again (two chunks on)
@@ -681,18 +680,19 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
             s[t][r] = d < a.k_dim && j < a.v_dim ? S[(int64_t)d * a.v_dim + j] : 0.0f;
         }
     const T* V = static_cast<const T*>(a.v) + (int64_t)seq.row * a.v_stride + (int64_t)h * a.v_dim;
-    V += (int64_t)(part * TILES * 8 + tc) * a.v_stride;
-    T coming[TILES][4];  // the next chunk's values, not touched before it begins
+    V += (int64_t)tc * a.v_stride;
+    T coming[2][4];  // the next chunk's values, not touched before it begins
     auto fetch = [&](int c) {
         const T* row = V + (int64_t)c * kChunk * a.v_stride;
-        const int left = seq.len - c * kChunk - part * TILES * 8 - tc;  // tokens from the lane's first
+        const int left = seq.len - c * kChunk - tc;  // tokens from the lane's first
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const bool in = t * 8 + (r & 1) < left && (r < 2 ? in0 : in1);
-                from_f32(coming[t][r], 0.0f);
-                if (in) coming[t][r] = row[(t * 8 + (r & 1)) * a.v_stride + (r < 2 ? j0 : j1)];
+                const int t = tile_of(part, k) * 8 + (r & 1);
+                const bool in = t < left && (r < 2 ? in0 : in1);
+                from_f32(coming[k][r], 0.0f);
+                if (in) coming[k][r] = row[t * a.v_stride + (r < 2 ? j0 : j1)];
             }
     };
     fetch(0);
@@ -705,21 +705,15 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
         const uint8_t* image = smem + (c % kStages) * kStage;
         const uint32_t base = shared_addr(image);
         const float* gate = reinterpret_cast<const float*>(image + I::kBytes + kGates);
-        float v[TILES][4];
+        float v[2][4];
         {  // this warp's part of S^T K^T
             uint32_t hi[KS][4], lo[KS][4];
-            float down[2], most[2], y[4][4] = {};
-            limbs<NT>(s, hi, lo, down, most);
-            float v0 = 0.0f, v1 = 0.0f;
+            float down[2], y[4][4] = {};
+            limbs<NT>(s, hi, lo, down);
 #pragma unroll
-            for (int k = 0; k < TILES; ++k) {
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[k][r] = to_f32(coming[k][r]);
-                v0 = fmaxf(v0, fmaxf(fabsf(v[k][0]), fabsf(v[k][1])));
-                v1 = fmaxf(v1, fmaxf(fabsf(v[k][2]), fabsf(v[k][3])));
-            }
-            v0 = row_max(v0), v1 = row_max(v1);
-            if (tc == 0) sh.top[part][lane >> 2] = make_float4(most[0], v0, most[1], v1);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 hand.hi[part * KS + ks][lane] = make_uint4(hi[ks][0], hi[ks][1], hi[ks][2], hi[ks][3]);
@@ -759,25 +753,9 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
         // cores while this chain exchanges and scales, not before
         set_ready(0, c);
         group_sync(bar_g, PARTS * 32);
-        // the same bounds in every warp: no row of X or U is larger
-        float up[2], down[2];
-        float x_most[2];
-        {
-            float4 top = sh.top[0][lane >> 2];
 #pragma unroll
-            for (int q = 1; q < PARTS; ++q) {
-                const float4 w = sh.top[q][lane >> 2];
-                top.x = fmaxf(top.x, w.x), top.y = fmaxf(top.y, w.y);
-                top.z = fmaxf(top.z, w.z), top.w = fmaxf(top.w, w.w);
-            }
-            const float bs = gate[kChunkRow * kChunk + kBoundS], bv = gate[kChunkRow * kChunk + kBoundV];
-            x_most[0] = bs * top.x + bv * top.y, x_most[1] = bs * top.z + bv * top.w;
-            power_for(x_most[0], up[0], down[0]);
-            power_for(x_most[1], up[1], down[1]);
-        }
-#pragma unroll
-        for (int k = 0; k < TILES; ++k) {  // X of this warp's tokens
-            const int t = part * TILES + k;
+        for (int k = 0; k < 2; ++k) {  // X of this warp's tokens
+            const int t = tile_of(part, k);
             const float2 beta = *reinterpret_cast<const float2*>(gate + kBeta * kChunk + t * 8 + tc);
             const float2 xk = *reinterpret_cast<const float2*>(gate + kXk * kChunk + t * 8 + tc);
             float4 y = sh.y[0][t][lane];
@@ -786,86 +764,67 @@ __global__ void __launch_bounds__((Split<DK, GROUPS>::kThreads), 1)
                 const float4 w = sh.y[q][t][lane];
                 y.x += w.x, y.y += w.y, y.z += w.z, y.w += w.w;
             }
-            sh.x[t][lane] = tile_limbs(beta.x * v[k][0] - xk.x * y.x, beta.y * v[k][1] - xk.y * y.y,
-                                         beta.x * v[k][2] - xk.x * y.z, beta.y * v[k][3] - xk.y * y.w, up[0], up[1]);
+            sh.x[t][lane] = make_float4(beta.x * v[k][0] - xk.x * y.x, beta.y * v[k][1] - xk.y * y.y,
+                                        beta.x * v[k][2] - xk.x * y.z, beta.y * v[k][3] - xk.y * y.w);
         }
         group_sync(bar_g, PARTS * 32);
         if (c + 1 < chunks) fetch(c + 1);
 
-        // U^T = X^T T^T, this warp's tokens; columns of T behind them are zero
-        float e_down[2];
-        {
-            uint32_t hi[2][4], lo[2][4], bh[2][4], bl[2][4];
-            float c1[2][4] = {};
-            operand(sh.x[0][lane], sh.x[1][lane], hi[0], lo[0]);
-            operand(sh.x[2][lane], sh.x[3][lane], hi[1], lo[1]);
-            const float bu = gate[kChunkRow * kChunk + kBoundU], be = gate[kChunkRow * kChunk + kBoundEnd];
-            float u_up[2], u_down[2], e_up[2];
+        {  // U = T X, this warp's tokens, and its limbs scaled to the chunk's end
+            float u[2][4] = {}, m0 = 0.0f, m1 = 0.0f, up[2], down[2];
+            triangular(part, reinterpret_cast<const float*>(image + I::kBytes), sh.x, u);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                power_for(x_most[r] * bu, u_up[r], u_down[r]);
-                power_for(x_most[r] * bu * be, e_up[r], e_down[r]);
-            }
-            if (part == 0) hand.scale[lane] = make_float2(u_down[0], u_down[1]);
-            const uint32_t t_at = base + I::kBytes + (part * TILES * 8 + lane_b) * kPitchT + half_b;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                ldmatrix(bh[ks], t_at + ks * 32);
-                ldmatrix(bl[ks], t_at + kLimbT + ks * 32);
-            }
-#pragma unroll
-            for (int k = 0; k < TILES; ++k) {
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    mma(c1[k], lo[ks], bh[ks][2 * k], bh[ks][2 * k + 1]);
-                    mma(c1[k], hi[ks], bl[ks][2 * k], bl[ks][2 * k + 1]);
-                }
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) mma(c1[k], hi[ks], bh[ks][2 * k], bh[ks][2 * k + 1]);
-                const int t = part * TILES + k;
-                const float2 f = *reinterpret_cast<const float2*>(gate + kScaleT * kChunk + t * 8 + tc);
+            for (int k = 0; k < 2; ++k) {
+                const int t = tile_of(part, k);
+                hand.u[t][lane] = make_float4(u[k][0], u[k][1], u[k][2], u[k][3]);
                 const float2 e = *reinterpret_cast<const float2*>(gate + kDown * kChunk + t * 8 + tc);
-                const float u0 = c1[k][0] * (down[0] * f.x), u1 = c1[k][1] * (down[0] * f.y);
-                const float u2 = c1[k][2] * (down[1] * f.x), u3 = c1[k][3] * (down[1] * f.y);
-                hand.u[t][lane] = tile_limbs(u0, u1, u2, u3, u_up[0], u_up[1]);
-                sh.e[t][lane] = tile_limbs(u0 * e.x, u1 * e.y, u2 * e.x, u3 * e.y, e_up[0], e_up[1]);
+                u[k][0] *= e.x, u[k][1] *= e.y, u[k][2] *= e.x, u[k][3] *= e.y;
+                m0 = fmaxf(m0, fmaxf(fabsf(u[k][0]), fabsf(u[k][1])));
+                m1 = fmaxf(m1, fmaxf(fabsf(u[k][2]), fabsf(u[k][3])));
             }
+            row_powers(m0, m1, up, down);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                sh.e[tile_of(part, k)][lane] = tile_limbs(u[k][0], u[k][1], u[k][2], u[k][3], up[0], up[1]);
+            sh.e_down[part][lane] = make_float2(down[0], down[1]);
         }
         set_ready(1, c);
         group_sync(bar_g, PARTS * 32);
-        // S <- e^{G_C} S + U^T K, with U scaled to the chunk's end
+        // S <- e^{G_C} S + U^T K, with U scaled to the chunk's end; each warp's tokens have their own scale
         {
-            uint32_t hi[2][4], lo[2][4];
-            operand(sh.e[0][lane], sh.e[1][lane], hi[0], lo[0]);
-            operand(sh.e[2][lane], sh.e[3][lane], hi[1], lo[1]);
-            const float total = gate[kChunkRow * kChunk + kTotal];
-            const uint32_t at = base + (lane & 15) * I::kPitch + part * ROWS * 2 + (lane >> 4) * 16;
+            uint32_t hi[2][4], lo[2][4], at[2];
+            float2 down[2];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                operand(sh.e[tile_of(ks, 0)][lane], sh.e[tile_of(ks, 1)][lane], hi[ks], lo[ks]);
+                down[ks] = sh.e_down[ks][lane];
+                at[ks] = base + (tile_of(ks, lane >> 3 & 1) * 8 + (lane & 7)) * I::kPitch + part * ROWS * 2 + (lane >> 4) * 16;
+            }
+            const float total = gate[kTotal * kChunk];
 #pragma unroll
             for (int p = 0; p < NT / 2; ++p) {
-                float c1[2][4] = {};
-                uint32_t bh[2][4];
+                float c1[2][2][4] = {};
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    ldmatrix_trans(bh[ks], at + ks * 16 * I::kPitch + p * 32);
-                    mma(c1[0], lo[ks], bh[ks][0], bh[ks][1]);
-                    mma(c1[1], lo[ks], bh[ks][2], bh[ks][3]);
+                    uint32_t bh[4], bl[4];
+                    ldmatrix_trans(bh, at[ks] + p * 32);
+                    mma(c1[ks][0], lo[ks], bh[0], bh[1]);
+                    mma(c1[ks][1], lo[ks], bh[2], bh[3]);
                     if (LIMBS == 2) {
-                        uint32_t bl[4];
-                        ldmatrix_trans(bl, at + I::kLimb + ks * 16 * I::kPitch + p * 32);
-                        mma(c1[0], hi[ks], bl[0], bl[1]);
-                        mma(c1[1], hi[ks], bl[2], bl[3]);
+                        ldmatrix_trans(bl, at[ks] + I::kLimb + p * 32);
+                        mma(c1[ks][0], hi[ks], bl[0], bl[1]);
+                        mma(c1[ks][1], hi[ks], bl[2], bl[3]);
                     }
-                }
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    mma(c1[0], hi[ks], bh[ks][0], bh[ks][1]);
-                    mma(c1[1], hi[ks], bh[ks][2], bh[ks][3]);
+                    mma(c1[ks][0], hi[ks], bh[0], bh[1]);
+                    mma(c1[ks][1], hi[ks], bh[2], bh[3]);
                 }
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        s[2 * p + t][r] = fmaf(total, s[2 * p + t][r], c1[t][r] * e_down[r >> 1]);
+                    for (int r = 0; r < 4; ++r) {
+                        const float first = fmaf(total, s[2 * p + t][r], c1[0][t][r] * (r < 2 ? down[0].x : down[0].y));
+                        s[2 * p + t][r] = fmaf(c1[1][t][r], r < 2 ? down[1].x : down[1].y, first);
+                    }
             }
         }
     }

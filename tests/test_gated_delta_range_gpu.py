@@ -92,6 +92,41 @@ DTYPES = pytest.mark.parametrize("dtype", [sc.F32, sc.BF16], ids=["f32", "bf16"]
 
 
 @DTYPES
+@pytest.mark.parametrize("g,length", [(0.05, 15), (0.05, 200), (0.3, 64), (0.3, 200), (0.5, 150), (1.0, 64), (2.0, 15), (2.0, 40)])
+def test_growing_states(ctx, g, length, dtype):
+    """Gates above zero, as far as f32 holds what they grow (e^80)."""
+    c = Case([length], dk=128, dv=64, dtype=dtype, seed=length)
+    c.gate.fill_(g)
+    check(ctx, c)
+
+
+@DTYPES
+@pytest.mark.parametrize("power", [20, 30, 40, 60])
+@pytest.mark.parametrize("at", [31, 20, 63, 16])
+def test_one_value_far_above_the_others(ctx, at, power, dtype):
+    """What comes later costs earlier tokens nothing, nor does a column its neighbours."""
+    c = Case([70], dk=64, dv=64, dtype=dtype, seed=at)
+    c.parts()[2][at] *= 2.0 ** power
+    check(ctx, c)
+    c = Case([40, 1, 70], dk=128, dv=128, hk=1, hv=2, dtype=dtype, seed=at)
+    c.parts()[2][at, 5::17] *= 2.0 ** power
+    check(ctx, c)
+
+
+@DTYPES
+@pytest.mark.parametrize("power", [-60, -30, 30, 60])
+def test_values_that_rise_and_fall_within_a_chunk(ctx, power, dtype):
+    """From 1 to 2^power over 32 tokens, with decays that forget about as fast."""
+    c = Case([96], dk=64, dv=48, dtype=dtype)
+    steps = torch.arange(c.rows) % 32 * (power / 31)
+    c.parts()[2].mul_((2.0 ** steps)[:, None].cuda())
+    check(ctx, c)
+    c.state.copy_(c.state0)
+    c.gate.fill_(-abs(power) / 31 * 0.7)
+    check(ctx, c)
+
+
+@DTYPES
 @pytest.mark.parametrize("power", [-40, -12, 12, 40, 62])
 def test_normalised_keys_of_any_norm(ctx, power, dtype):
     """The norm of a key passes 2^power, its square stays within f32, and the update does not depend on either."""
@@ -100,3 +135,38 @@ def test_normalised_keys_of_any_norm(ctx, power, dtype):
     for x, p in ((k, power), (q, -abs(power) // 4)):
         x.copy_((x.float() / x.float().reshape(c.rows, c.hk, c.dk).norm(dim=-1).repeat_interleave(c.dk, 1) * 2.0 ** p).to(c.dt))
     check(ctx, c)
+
+
+@DTYPES
+@pytest.mark.parametrize("power", [10, 25, 40])
+def test_one_key_far_above_the_others(ctx, power, dtype):
+    """Keys as they are, one of them long, with a step short enough for it."""
+    c = Case([70], dk=64, dv=64, dtype=dtype, norm=False, seed=power)
+    _, k, _ = c.parts()
+    k[25] *= 2.0 ** power
+    c.beta[25] *= 2.0 ** (-2 * power)
+    check(ctx, c)
+
+
+@DTYPES
+@pytest.mark.parametrize("g", [-3.0, -0.5, 0.7, 2.7])
+def test_one_token_seen_from_every_later_one(ctx, g, dtype):
+    """o_t = scale e^{t g} beta (q_t . k_0) v_0 where nothing else is learnt: the decay of up to 31 tokens as one factor.
+    Its own error is a few roundings (2^-21 in all, 2^-24 |g| a token where tokens multiply theirs); q . k carries 22 bits
+    and a limb's 2^-40, f32 sums of 128 products another 2^-21 of the norms. Below f32's normal numbers (2^-126) that is absolute."""
+    c = Case([32], hk=1, hv=1, dk=128, dv=32, dtype=dtype, norm=False)
+    c.state0.zero_()
+    c.state.zero_()
+    q, k, v = c.parts()
+    q.copy_(k[0:1].expand_as(q))
+    v[1:] = 0
+    c.beta[1:] = 0
+    c.gate.fill_(g)
+    c.run(ctx)
+    torch.cuda.synchronize()
+    q, k, v = (x.cpu().double().numpy() for x in (q, k, v))
+    b, gate = float(c.beta[0, 0]), float(c.gate[0, 0])
+    want = c.scale * np.exp(gate * np.arange(32))[:, None] * b * (k[0] @ k[0]) * v[0]
+    got = c.o[:32, :32].float().cpu().double().numpy()
+    rel = 2.0 ** -21 + 2.0 ** -21 + (2.0 ** -8 if dtype == sc.BF16 else 0)
+    assert (np.abs(got - want) <= rel * np.abs(want) + 1e-37).all(), float((np.abs(got - want) / np.abs(want)).max())
