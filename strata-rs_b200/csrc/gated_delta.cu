@@ -152,15 +152,24 @@ void launch_step(const DeltaArgs& a, const SeqTable& t, unsigned grid, cudaStrea
     else delta_step_kernel<T, 8, VEC><<<grid, 256, 0, s>>>(a, t);
 }
 
+// The sequences that have tokens: empty ones launch nothing, so no rule counts them.
+int64_t live_sequences(const strata_gated_delta& d) {
+    if (!d.seq_offsets) return d.n_seq;
+    int64_t n = 0;
+    for (int64_t i = 0; i < d.n_seq; ++i) n += d.seq_offsets[i + 1] > d.seq_offsets[i];
+    return n;
+}
+
 // Columns a thread takes: 4 (16-byte state accesses) or 2 where rows and
 // pointers allow, 1 otherwise; fewer where that many blocks would leave
 // multiprocessors without one.
 int columns(const strata_gated_delta& d, const void* v, const float* state, const void* o, int sm_count) {
+    const int64_t live = live_sequences(d);
     const int64_t b = dtype_bytes(d.dtype);
     for (int vec = 4; vec > 1; vec >>= 1) {
         if (d.v_dim % vec == 0 && d.v_stride % vec == 0 && d.o_stride % vec == 0 &&
             (uintptr_t)state % (4 * vec) == 0 && (uintptr_t)v % (b * vec) == 0 && (uintptr_t)o % (b * vec) == 0 &&
-            d.v_dim > 32 * (vec / 2) && d.n_seq * d.n_v_head * ((d.v_dim + 32 * vec - 1) / (32 * vec)) >= sm_count)
+            d.v_dim > 32 * (vec / 2) && live * d.n_v_head * ((d.v_dim + 32 * vec - 1) / (32 * vec)) >= sm_count)
             return vec;
     }
     return 1;
@@ -176,7 +185,7 @@ int columns(const strata_gated_delta& d, const void* v, const float* state, cons
 // 160, apart; 3 sequences of 12 tokens and 500 take 53 us, not 59, together.
 int64_t chunks_from(const strata_gated_delta& d, int64_t longest) {
     const int64_t blocks = d.n_v_head * ((d.v_dim + 127) / 128), few = 128 / blocks;  // sequences
-    if (d.k_dim > 128 || longest < (d.n_seq <= few ? 32 : 16)) return longest + 1;
+    if (d.k_dim > 128 || longest < 16 || (longest < 32 && live_sequences(d) <= few)) return longest + 1;
     if (!d.seq_offsets) return 1;
     int64_t n = 0;
     for (int64_t i = 0; i < d.n_seq; ++i) {
