@@ -442,21 +442,18 @@ __device__ Cut cut_top_p(Row& r, float top, double p, Cut cut, double above = 0.
 
 // exp by the table method (Tang, 1989): v f + c = (64 m + j) ln2 / 64 + r,
 // exp = 2^m 2^(j/64) exp(r), |r| <= ln2 / 128, four terms of exp(r) - 1. Good
-// to 4e-14 of the result while |v f + c| < 700.
+// to 4e-14 of the result while |v f + c| < 700. (The whole steps are those of the
+// rounded v f + c: from v and c apart they would be off by one where c lies
+// between two, and r^5 / 120 thirty times larger.)
 struct Exp {
     const double (*table)[32];
-    double f, c, tf, tc;  // the argument, and 64 / ln2 times it plus the rounding constant
-    __device__ Exp(const double (*t)[32], double f_, double c_) : table(t), f(f_), c(c_) {
-        constexpr double kLn2 = 0.69314718055994530942, kMagic = 6755399441055744.0;  // 1.5 * 2^52
-        tf = f * (kExpTable / kLn2);
-        tc = c * (kExpTable / kLn2) + kMagic;
-    }
+    double f, c;
+    __device__ Exp(const double (*t)[32], double f_, double c_) : table(t), f(f_), c(c_) {}
     __device__ __forceinline__ double operator()(float v) const {
-        constexpr double kLn2 = 0.69314718055994530942, kMagic = 6755399441055744.0;
-        const double x = (double)v;
-        const double t = fma(x, tf, tc);
+        constexpr double kLn2 = 0.69314718055994530942, kMagic = 6755399441055744.0;  // 1.5 * 2^52
+        const double d = fma((double)v, f, c), t = fma(d, kExpTable / kLn2, kMagic);
         const int n = __double2loint(t);
-        const double r = fma(t - kMagic, -kLn2 / kExpTable, fma(x, f, c));
+        const double r = fma(t - kMagic, -kLn2 / kExpTable, d);
         const double b = table[n & (kExpTable - 1)][threadIdx.x & 31];
         const double q = fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0);
         const double y = fma(b * r, q, b);
