@@ -1119,6 +1119,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     int first = 0, last = -1;
     // a range that the sample misjudged, or infinite logits
     bool wide = sums_all && !(m.sum > 1e-100 && m.sum < 1e250 && top < center + 500.0f * fminf(t, 1.0f));
+    // or a temperature so small that the rounded floor lies outside the exponential's range, or so large that none is left
+    wide |= sums_all && !((ref - (double)draw_floor) * inv_t < 700.0);
     // Excluded tokens have weighed e^-600 each in the sums: nothing, unless the
     // draw asks for the very first or last token with a weight.
     if ((sure || draws_all) && !(u > 1e-100 && u < 1.0 - 1e-9)) wide = true;

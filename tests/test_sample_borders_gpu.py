@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import strata_cuda as sc
-from test_sample_gpu import draw
+from test_sample_gpu import check, draw
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -37,3 +37,15 @@ def test_random_numbers_next_to_a_border(ctx, vocab, t):
         off = np.nonzero(ids != want)[0]
         sure = (u < 1 - 1e-9) & (np.abs(u - border) > 1e-13)  # a border next to 0 or 1 leaves no room beside it
         assert not sure[off].any(), (len(off), x[off[0]], u[off[0]])
+
+
+@pytest.mark.parametrize("center", [0.0, 10.0, -300.0, 9000.0])
+def test_temperatures_that_leave_the_table(ctx, center):
+    """A temperature times 600 within a few steps of the largest logit, where the weights' floor rounds; and very large ones."""
+    rng = np.random.default_rng(7)
+    for t in (1e-12, 1e-9, 1.7e-9, 2e-9, 3e-9, 1e-8, 1e-6, 3e-6, 1e-5, 1e-3, 1e5, 1e34, 4e35, 6e35, 1e38):
+        x = (rng.standard_normal((6, 700)) * 2 + center).astype(np.float32)
+        x[2:4] = np.round(x[2:4])  # several largest ones
+        x[4:, ::3] = -np.inf
+        for kw in ({}, dict(p=[0.9] * 6), dict(p=[0.3] * 6, m=[0.01] * 6)):
+            check(ctx, x, list(rng.random(6)), t=[t] * 6, **kw)
