@@ -1,8 +1,8 @@
 //! `extern "C"` declarations of `include/strata_sequence.h`: the sequence
 //! operators (short convolution, gated delta rule, sampling) on device buffers.
-//! Contexts and status codes are [`crate::ffi`]'s.
+//! Contexts and status codes are [`crate::ffi`]'s; [`crate::sequence`] calls them.
 
-#![allow(non_camel_case_types, dead_code)] // an engine's device-resident step calls these; the trait does not
+#![allow(non_camel_case_types)]
 
 use std::os::raw::{c_int, c_void};
 

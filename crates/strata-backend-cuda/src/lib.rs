@@ -12,8 +12,9 @@
 //! Beyond the trait: [`CudaBackend::gemm`] (a whole prompt through one
 //! projection — the bf16-staged tensor-core GEMM), [`CudaBackend::moe_layer`]
 //! / [`CudaBackend::moe_ffn`] (route, experts, shared expert and combine in
-//! one device call) and [`CudaBackend::preload`] (every tensor resident before
-//! the first token, in one staged pass).
+//! one device call), [`CudaBackend::preload`] (every tensor resident before
+//! the first token, in one staged pass) and [`sequence`] (a recurrent layer's
+//! steps and sampling, on device buffers).
 //!
 //! There is no CPU fallback: a type the device does not take is
 //! [`Error::UnsupportedQuant`], any device failure is [`Error::Backend`] with
@@ -21,6 +22,7 @@
 
 mod ffi;
 mod ffi_sequence;
+pub mod sequence;
 
 use std::collections::HashMap;
 use std::ffi::CStr;
