@@ -25,8 +25,9 @@
  * [i * seq_len, (i + 1) * seq_len)), or seq_offsets gives n_seq + 1
  * non-decreasing row numbers in HOST memory, read during the call (sequence i
  * holds rows [seq_offsets[i], seq_offsets[i + 1])). A sequence may be empty:
- * its state stays as it is. Rows outside every sequence are neither read nor
- * written. Below 2^31 rows.
+ * its state stays as it is; where all are, a call does nothing and its buffers
+ * may be NULL. Rows outside every sequence are neither read nor written. Below
+ * 2^31 rows.
  */
 #ifndef STRATA_SEQUENCE_H
 #define STRATA_SEQUENCE_H

@@ -230,7 +230,7 @@ int strata_cuda_gated_delta_dev(strata_ctx* ctx, const strata_gated_delta* desc,
     Why why;
     int64_t tokens = 0, longest = 0;
     int rc = check_gated_delta(why, d, &tokens, &longest);
-    if (!rc)
+    if (!rc && longest > 0)
         rc = check_gated_delta_buffers(why, d, tokens, q_dev, k_dev, v_dev, gate_dev, beta_dev, coef_dev, shift_dev,
                                        state_dev, o_dev, work_dev, work_bytes, work_needed(d, longest));
     if (rc) return fail(ctx, rc, "gated_delta: %s", why.text);

@@ -226,7 +226,7 @@ extern "C" int strata_cuda_short_conv_dev(strata_ctx* ctx, const strata_short_co
     Why why;
     int64_t tokens = 0, longest = 0;
     int rc = check_short_conv(why, d, &tokens, &longest);
-    if (!rc) rc = check_short_conv_buffers(why, d, tokens, x_dev, w_dev, bias_dev, state_dev, y_dev);
+    if (!rc && longest > 0) rc = check_short_conv_buffers(why, d, tokens, x_dev, w_dev, bias_dev, state_dev, y_dev);
     if (rc) return fail(ctx, rc, "short_conv: %s", why.text);
     if (longest == 0) return STRATA_OK;
     const bool bf16 = d.dtype == STRATA_QUANT_BF16, vec = packs(d, x_dev, y_dev, bias_dev, state_dev);
