@@ -83,7 +83,7 @@ int strata_cuda_short_conv_dev(strata_ctx *ctx, const strata_short_conv *desc, c
  *
  * Products and sums are f32; o is rounded once. Sequences are read in chunks of
  * 32 tokens on the tensor cores where k_dim is up to 128 and a sequence of the
- * call has 16 tokens or more, 32 where there are few heads and sequences (many
+ * call has 16 tokens or more, 20 where there are few heads and sequences (many
  * shorter ones beside it are still read token by token). There, products over
  * k_dim carry 22 bits of the norms of their vectors (a key, a query, a column of
  * the state), all others 22 bits of themselves: however the sizes of tokens and

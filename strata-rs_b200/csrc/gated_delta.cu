@@ -176,16 +176,21 @@ int columns(const strata_gated_delta& d, const void* v, const float* state, cons
 }
 
 // The tokens from which on a sequence of the call is read in chunks (more than
-// `longest`: none is). Measured at 32 heads of 128 x 128: one sequence takes
-// 0.67 us a token against 24 us for up to 32 in chunks (even at 32), 32
-// sequences 8 us a token against 122 us (at 16), because few sequences leave the
-// token kernel's blocks a multiprocessor each. Beside long sequences a short
+// `longest`: none is). A chunk takes as long with 16 tokens as with 32; measured
+// in replayed graphs, tokens one after another against a chunk:
+//   heads   32 of 128 x 128   16 of 64 x 64   64 of 96 x 128   2 of 32 x 32
+//   1 seq.  0.70 a token, 12  0.61, 10        0.84, 14         0.61, 9.4 us
+//   4       1.0, 24           0.62, 10        1.8, 30          0.61, 9.4
+//   64      13, 254           2.1, 41         25, 358          0.63, 9.6
+// (and 2 us a call), so they meet at 12 to 19 tokens, or at 21 where a few
+// sequences' blocks have a multiprocessor each one way but share it the other.
+// Beside long sequences a short
 // one costs 3.7 us as a chunk against 0.5 us and 0.18 us a token, unless there
 // are so few that they run alongside: 31 single tokens and 500 take 72 us, not
 // 160, apart; 3 sequences of 12 tokens and 500 take 53 us, not 59, together.
 int64_t chunks_from(const strata_gated_delta& d, int64_t longest) {
     const int64_t blocks = d.n_v_head * ((d.v_dim + 127) / 128), few = 128 / blocks;  // sequences
-    if (d.k_dim > 128 || longest < 16 || (longest < 32 && live_sequences(d) <= few)) return longest + 1;
+    if (d.k_dim > 128 || longest < 16 || (longest < 20 && live_sequences(d) <= few)) return longest + 1;
     if (!d.seq_offsets) return 1;
     int64_t n = 0;
     for (int64_t i = 0; i < d.n_seq; ++i) {
