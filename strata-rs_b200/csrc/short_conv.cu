@@ -65,8 +65,11 @@ __device__ __forceinline__ float silu(float z) {
     return __fdividef(z, 1.0f + expf(-z));
 }
 
-// Blocks a multiprocessor runs side by side (up to four taps), as their registers allow.
-constexpr int resident(int vec, bool few) { return few ? (vec == 8 ? 5 : 8) : vec == 8 ? 4 : vec == 4 ? 6 : 8; }
+// Blocks a multiprocessor runs side by side (up to four taps), as their registers
+// allow without spilling: a fifth of eight channels for a few tokens costs 128
+// bytes of them a thread (64 single bf16 tokens of 8192 channels 8.1 us, not 7.4,
+// 512 of them 45, not 40).
+constexpr int resident(int vec, bool few) { return vec == 8 ? 4 : vec == 4 && !few ? 6 : 8; }
 
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&d)[VEC]) {
