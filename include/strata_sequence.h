@@ -121,7 +121,9 @@ int strata_cuda_gated_delta_dev(strata_ctx *ctx, const strata_gated_delta *desc,
 /* ---------------------------------------------------------------- sampling */
 
 /* One token for every row of logits (rows x vocab f32, rows `stride` floats
- * apart, 0 = vocab; vocab up to 2^22). Per row, in this order:
+ * apart, 0 = vocab; vocab up to 2^22). The reference's sampler applies its
+ * penalties first (they need the tokens so far); a caller that has some changes
+ * the logits before the call. Per row, in this order:
  *   top_k        keeps the k largest logits; k <= 0 keeps all
  *   top_p        with the kept tokens' softmax in falling order, keeps the
  *                shortest prefix whose sum reaches p (one token at least);
@@ -132,7 +134,9 @@ int strata_cuda_gated_delta_dev(strata_ctx *ctx, const strata_gated_delta *desc,
  *                the largest logit
  *   uniform      u in [0, 1): the first kept token, in index order, whose
  *                cumulative probability exceeds u (u outside is clamped)
- * Equal logits rank by index, the lowest first. Sums and exponentials are f64.
+ * Equal logits rank by index, the lowest first. Sums and exponentials are f64:
+ * a p or u that falls on a border between two tokens to within 1e-13 of the
+ * total may be taken to either side of it.
  * A logit of -inf or NaN is never taken; infinite ones share everything; a row
  * with nothing left gives id -1 and log-probability -inf. ids_dev receives
  * int32, logprobs_dev (or NULL) the natural log of the taken token's final

@@ -19,7 +19,7 @@
 // over the whole slices, narrowing key ranges pass by pass.
 //
 // What it measured, and what bounds it: 256 rows of 151,936 logits with top-p
-// take 205 us (155 MB from DRAM in each pass). Of the 172,000 cycles of the first
+// take 203 us (155 MB from DRAM in each pass). Of the 172,000 cycles of the first
 // pass on a multiprocessor with two rows, 87,000 are its exponentials (37 a warp
 // for 32 tokens; ten f64 operations of two and a conversion of eight are 28),
 // 11,000 the histogram; of the second's 182,000, 37,000 the exponentials of what
