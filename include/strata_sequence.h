@@ -86,9 +86,10 @@ int strata_cuda_short_conv_dev(strata_ctx *ctx, const strata_short_conv *desc, c
  * call has 16 tokens or more, 20 where there are few heads and sequences (many
  * shorter ones beside it are still read token by token). There, products over
  * k_dim carry 22 bits of the norms of their vectors (a key, a query, a column of
- * the state), all others 22 bits of themselves: however the sizes of tokens and
- * columns differ, none costs another, nor an earlier token, precision. Either
- * way, squares of q and k are summed in f32, so normalised ones have norms below
+ * the state; the elements of one that lie 2^18 below its largest carry fewer of
+ * their own), and all others 22 bits of themselves: however sizes differ, no
+ * column costs another, and no token an earlier one, precision. Either way,
+ * squares of q and k are summed in f32, so normalised ones have norms below
  * 1.8e19, and in chunks the decay from one token to another within 32 is one f32
  * factor: gates above 0 may add up to 88 there, and below e^-88 it counts as 0.
  * Chunks need strata_cuda_gated_delta_work_bytes bytes of
