@@ -13,15 +13,18 @@
 //! projection — the bf16-staged tensor-core GEMM), [`CudaBackend::moe_layer`]
 //! / [`CudaBackend::moe_ffn`] (route, experts, shared expert and combine in
 //! one device call), [`CudaBackend::preload`] (every tensor resident before
-//! the first token, in one staged pass) and [`sequence`] (a recurrent layer's
-//! steps and sampling, on device buffers).
+//! the first token, in one staged pass), [`sequence`] (a recurrent layer's
+//! steps and sampling, on device buffers) and [`attention`] (an attention layer's
+//! steps over a paged cache and the scoring of tokens, likewise).
 //!
 //! There is no CPU fallback: a type the device does not take is
 //! [`Error::UnsupportedQuant`], any device failure is [`Error::Backend`] with
 //! the library's message.
 
 mod ffi;
+mod ffi_attention;
 mod ffi_sequence;
+pub mod attention;
 pub mod sequence;
 
 use std::collections::HashMap;

@@ -30,7 +30,7 @@ pub enum Activations {
 }
 
 impl Activations {
-    fn id(self) -> u32 {
+    pub(crate) fn id(self) -> u32 {
         match self {
             Self::F32 => 0,   // STRATA_QUANT_F32
             Self::Bf16 => 30, // STRATA_QUANT_BF16
@@ -54,7 +54,7 @@ pub enum Sequences<'a> {
 
 impl Sequences<'_> {
     /// `n_seq`, `seq_len` and `seq_offsets` of a call.
-    fn parts(&self) -> (i64, i64, *const i64) {
+    pub(crate) fn parts(&self) -> (i64, i64, *const i64) {
         match *self {
             Self::Uniform { count, len } => (count, len, std::ptr::null()),
             // no offsets at all are no sequences, which the library refuses

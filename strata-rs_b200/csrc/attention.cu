@@ -1,0 +1,573 @@
+// attention.cu — attention of new tokens over a paged cache: the call, and the
+// kernel for few rows a key head (single tokens, short chunks, f32 queries).
+//
+//   o = sum_j softmax_j(scale q . k_j) v_j,  j over what the row sees
+//
+// in one pass over the keys, with the running maximum m and sum l of the
+// weights: a tile of scores s gives m' = max(m, s), and l and o are scaled by
+// exp(m - m') before its weights exp(s - m') are added.
+//
+// Rows: the r query heads of a key head share its keys, so 16 rows (tokens x r
+// heads) are one tile of the tensor cores and every key is read once for them.
+// A single token's work is then its keys and values: bound by memory, 16 to 64
+// operations a byte.
+//
+// The keys of all blocks of rows together (tiles of 64) are cut evenly over as
+// many blocks as run at once, however the sequences' lengths differ: a block
+// takes a contiguous range of tiles, of one block of rows or of several, and a
+// block of rows that falls to more than one thread block leaves (o, m, l) a
+// piece in the workspace, which a second kernel joins. The cut follows from the
+// lengths on the device, so that a captured call follows them.
+//
+// Each warp goes through keys of its own (16 of a tile's 64) with its own ring
+// of asynchronous copies, and no warp waits for another before its block's
+// range ends.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace strata {
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kRows = 16;  // rows of a block
+constexpr int kUnit = 16;  // keys a warp takes of a tile
+static_assert(kWarps * kUnit == kTile, "a tile's keys are the warps' units");
+
+// DP: head_dim rounded up to 64, 128 or 256. Stages and blocks side by side fill
+// the shared memory, so that about 128 KB a multiprocessor are under way.
+template <int DP, int LIMBS>
+struct Cfg {
+    static constexpr int kStages = DP == 64 ? 4 : 3;
+    static constexpr int kBlocks = DP == 256 ? 1 : DP == 128 ? 2 : 3;
+    static constexpr int kUnitBytes = kUnit * DP * 2;  // of keys; as much of values
+    static constexpr int kQBytes = LIMBS * kRows * DP * 2;
+    static constexpr int kRing = kWarps * kStages * 2 * kUnitBytes;
+    static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;
+    static constexpr int kSmem = kQBytes + (kRing > kJoin ? kRing : kJoin);
+    static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024, "blocks do not fit side by side");
+};
+constexpr int kMaxGrid = 148 * 3;  // blocks of a launch at most; the workspace is for as many
+
+// The workspace: what each block leaves of its first and its last block of rows
+// where other blocks have the rest, and which blocks of rows are to be joined.
+struct Split {
+    int item_entry, item_head;  // block of rows, key head
+    int pieces;                 // 0: none
+    int first_slot;             // of the first piece (the others are their blocks' slot 0)
+};
+struct Work {
+    Split* split;  // [kMaxGrid]
+    float* ml;     // [kMaxGrid][2][2][kRows]
+    float* o;      // [kMaxGrid][2][kRows][DP]
+};
+constexpr int64_t kSplitBytes = kMaxGrid * sizeof(Split), kMlBytes = (int64_t)kMaxGrid * 2 * 2 * kRows * 4;
+constexpr int64_t work_bytes_for(int dp) { return kSplitBytes + kMlBytes + (int64_t)kMaxGrid * 2 * kRows * dp * 4; }
+inline Work work_of(void* p) {
+    char* b = static_cast<char*>(p);
+    return {reinterpret_cast<Split*>(b), reinterpret_cast<float*>(b + kSplitBytes), reinterpret_cast<float*>(b + kSplitBytes + kMlBytes)};
+}
+
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two floats as bf16 pairs, the largest limb first: x = limb 0 + limb 1 + ..., each
+// rounding leaves 2^-9 of what it rounds, so three limbs keep f32's 24 bits.
+template <int LIMBS>
+__device__ __forceinline__ void limbs(float x, float y, uint32_t (&out)[LIMBS]) {
+#pragma unroll
+    for (int i = 0; i < LIMBS; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        out[i] = *reinterpret_cast<const uint32_t*>(&h);
+        x -= __uint_as_float(out[i] << 16), y -= __uint_as_float(out[i] & 0xFFFF0000u);
+    }
+}
+// Byte offset of 16-byte chunk c of row r in a tile of rows of DP elements: chunks
+// are permuted within a row so that 8 rows' same chunk lie in different banks.
+template <int DP>
+__device__ __forceinline__ int chunk_at(int r, int c) { return r * DP * 2 + ((c ^ (r & 7)) << 4); }
+
+// The tiles of a block of rows; one at least, so that rows that see nothing are written.
+__device__ __forceinline__ int cost_of(const AttnArgs& a, const SeqTable& tab, int entry) {
+    const int n = key_range(a, row_block(a, sequence_of_tile(tab, entry), entry, kRows)).tiles;
+    return n > 0 ? n : 1;
+}
+
+// Sums over blocks of rows, for all threads. chunk[t]: prefix of thread t's entry.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t x = v;
+    for (int w = 1; w < 32; w <<= 1) {
+        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, w);
+        if (lane >= w) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) before += sh[i];
+        total += sh[i];
+    }
+    return before + x - v;
+}
+
+template <int DP, int LIMBS, typename T>
+__global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
+    split_kernel(const AttnArgs a, const Work work, int entries, const __grid_constant__ SeqTable tab) {
+    using C = Cfg<DP, LIMBS>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* const qs = smem;
+    uint8_t* const ring = smem + C::kQBytes;
+    __shared__ int64_t scan[kWarps];
+    __shared__ int64_t start_entry_before;
+    __shared__ int start_entry;
+    __shared__ int odd_rows[kRows];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int heads = a.c.n_kv_head, d = a.c.head_dim;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- this block's range of the call's tiles
+    int64_t total = 0, mine = 0;
+    for (int e0 = 0; e0 < entries; e0 += kThreads) {
+        const int e = e0 + threadIdx.x;
+        mine += e < entries ? cost_of(a, tab, e) : 0;
+    }
+    block_scan(mine, scan, total);
+    total *= heads;
+    const int64_t grid = total < gridDim.x ? total : (int64_t)gridDim.x;
+    if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
+    if (blockIdx.x >= grid) return;
+    int64_t pos = total * blockIdx.x / grid;
+    const int64_t end = total * (blockIdx.x + 1) / grid;
+    {
+        int64_t base = 0;
+        for (int e0 = 0; e0 < entries; e0 += kThreads) {
+            const int e = e0 + threadIdx.x;
+            const int64_t cost = e < entries ? (int64_t)cost_of(a, tab, e) * heads : 0;
+            int64_t sum;
+            const int64_t before = base + block_scan(cost, scan, sum);
+            if (cost && pos >= before && pos < before + cost) start_entry = e, start_entry_before = before;
+            base += sum;
+            if (base > pos) break;
+        }
+        __syncthreads();
+    }
+    int entry = start_entry;
+    int64_t entry_at = start_entry_before;
+    const int64_t range_begin = pos;
+
+    while (pos < end) {
+        const RowBlock b = row_block(a, sequence_of_tile(tab, entry), entry, kRows);
+        const KeyRange kr = key_range(a, b);
+        const int cost = kr.tiles > 0 ? kr.tiles : 1;
+        const int head = (int)((pos - entry_at) / cost);
+        const int64_t item_at = entry_at + (int64_t)head * cost;
+        const int tile0 = (int)(pos - item_at);
+        const int tile1 = (int)((end - item_at < cost ? end - item_at : cost));
+        const int steps = (kr.tiles < tile1 ? kr.tiles : tile1) - tile0;  // none where the rows see nothing
+
+        // ---- this warp's keys, kStages - 1 units ahead
+        int pages = -1;      // of unit (step & ~31) + lane
+        uint32_t none = 0;   // bit step & 31: the unit has no page
+        auto load = [&](int step) {
+            if (step < steps) {
+                if ((step & 31) == 0) {
+                    const int at = step + lane;
+                    const int j = at < steps ? kr.key(tile0 + at) + warp * kUnit : kr.hi;
+                    pages = j < kr.hi ? page_of(a.c, b.slot, j) : -1;
+                }
+                const int j0 = kr.key(tile0 + step) + warp * kUnit;
+                const int page = __shfl_sync(0xFFFFFFFFu, pages, step & 31);
+                none = (none & ~(1u << (step & 31))) | (page < 0 ? 1u << (step & 31) : 0u);
+                uint8_t* const stage = ring + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes;
+                const int64_t at = page >= 0 ? place(a.c, page, j0, head) : 0;
+                constexpr int kChunks = DP / 8;
+#pragma unroll
+                for (int i = 0; i < kUnit * kChunks / 32; ++i) {
+                    const int row = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks, j = j0 + row;
+                    const bool ok = page >= 0 && c * 8 < d && j < kr.hi && (j >= kr.lo || j < a.sinks);
+                    const int64_t src = ok ? at + row * a.c.token_stride + c * 8 : 0;
+                    const int n = ok ? 16 : 0;  // the rest is zeros: what no row sees meets weights of zero
+                    const uint32_t dst = shared_at(stage) + chunk_at<DP>(row, c);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(a.c.k + src), "r"(n) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + C::kUnitBytes), "l"(a.c.v + src), "r"(n) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < C::kStages - 1; ++i) load(i);
+
+        // ---- the rows' queries, as limbs
+        for (int i = threadIdx.x; i < kRows * (DP / 8); i += kThreads) {
+            const int row = i / (DP / 8), c = i % (DP / 8), packed = b.row0 + row;
+            float x[8] = {};
+            if (row < b.rows && c * 8 < d) {
+                const int64_t at = (int64_t)(b.first_row + packed / a.r) * a.q_stride + (int64_t)(head * a.r + packed % a.r) * d + c * 8;
+                if (a.wide) {
+                    using P = Pack<T, 16 / sizeof(T)>;
+#pragma unroll
+                    for (int w = 0; w < 8; w += 16 / sizeof(T)) {
+                        const P p = *reinterpret_cast<const P*>(static_cast<const T*>(a.q) + at + w);
+#pragma unroll
+                        for (int u = 0; u < (int)(16 / sizeof(T)); ++u) x[w + u] = to_f32(p.v[u]);
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) x[u] = load_f32<T>(a.q, at + u);
+                }
+            }
+            uint32_t w[4][LIMBS];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) limbs<LIMBS>(x[2 * u], x[2 * u + 1], w[u]);
+#pragma unroll
+            for (int l = 0; l < LIMBS; ++l)
+                *reinterpret_cast<uint4*>(qs + l * kRows * DP * 2 + chunk_at<DP>(row, c)) = make_uint4(w[0][l], w[1][l], w[2][l], w[3][l]);
+        }
+        if (threadIdx.x < kRows) odd_rows[threadIdx.x] = 0;
+        __syncthreads();
+
+        float o[DP / 8][4] = {};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+        int p[2];  // positions of this lane's rows; rows that are none are zeros and go nowhere
+#pragma unroll
+        for (int i = 0; i < 2; ++i) p[i] = g + 8 * i < b.rows ? b.p0 + (b.row0 + g + 8 * i) / a.r : -1;
+        const int p_min = b.p0 + b.row0 / a.r, p_max = b.p0 + (b.row0 + b.rows - 1) / a.r;
+
+        for (int step = 0; step < steps; ++step) {
+            load(step + C::kStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+            __syncwarp();
+            const int j0 = kr.key(tile0 + step) + warp * kUnit;
+            const uint32_t ks = shared_at(ring) + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes, vs = ks + C::kUnitBytes;
+            if (!(none >> (step & 31) & 1) && j0 < kr.hi && (j0 + kUnit > kr.lo || j0 < a.sinks)) {
+                float s[LIMBS > 1 ? 2 : 1][2][4] = {};  // the small limbs' sums apart
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    uint32_t kb[4];
+                    ldsm4(kb, ks + chunk_at<DP>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int u = 0; u < LIMBS; ++u) {
+                        uint32_t qa[4];
+                        ldsm4(qa, shared_at(qs) + u * kRows * DP * 2 + chunk_at<DP>(lane & 15, 2 * k + (lane >> 4)));
+                        mma(s[u > 0][0], qa, kb[0], kb[1]);
+                        mma(s[u > 0][1], qa, kb[2], kb[3]);
+                    }
+                }
+                if (LIMBS > 1)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[0][n][i] += s[LIMBS > 1 ? 1 : 0][n][i];
+                if (j0 + kUnit - 1 > p_min || (a.window && j0 <= p_max - a.window) || j0 + kUnit > kr.hi) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = j0 + n * 8 + 2 * t4 + (i & 1);
+                            if (j >= kr.hi || !sees(a, p[i >> 1], j)) s[0][n][i] = -INFINITY;
+                        }
+                }
+                float w[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float top = fmaxf(fmaxf(s[0][0][2 * i], s[0][0][2 * i + 1]), fmaxf(s[0][1][2 * i], s[0][1][2 * i + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                    const float next = fmaxf(m[i], top * a.scale2), base = next == -INFINITY ? 0.0f : next;
+                    if (next != m[i]) {
+                        const float alpha = exp2_approx(m[i] - base);
+                        l[i] *= alpha;
+#pragma unroll
+                        for (int n = 0; n < DP / 8; ++n) o[n][2 * i] *= alpha, o[n][2 * i + 1] *= alpha;
+                        m[i] = next;
+                    }
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const float e = exp2_approx(fmaf(s[0][n][2 * i + u], a.scale2, -base));
+                            w[n][2 * i + u] = e;
+                            l[i] += e;
+                        }
+                }
+                // weights as the left operand: its 16 keys are the two tiles' columns
+                uint32_t wa[LIMBS][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t x[LIMBS];
+                        limbs<LIMBS>(w[n][2 * i], w[n][2 * i + 1], x);
+#pragma unroll
+                        for (int u = 0; u < LIMBS; ++u) wa[u][2 * n + i] = x[u];
+                    }
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n) {
+                    uint32_t vb[4];
+                    ldsm4_t(vb, vs + chunk_at<DP>(lane & 15, 2 * n + (lane >> 4)));
+                    if (LIMBS == 1) {
+                        mma(o[2 * n], wa[0], vb[0], vb[1]);
+                        mma(o[2 * n + 1], wa[0], vb[2], vb[3]);
+                    } else {
+                        // the tensor cores round a long running sum towards zero: a unit's
+                        // products by themselves, added to it in f32
+                        float x[2][4] = {};
+#pragma unroll
+                        for (int u = LIMBS - 1; u >= 0; --u) {
+                            mma(x[0], wa[u], vb[0], vb[1]);
+                            mma(x[1], wa[u], vb[2], vb[3]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[2 * n][i] += x[0][i], o[2 * n + 1][i] += x[1][i];
+                    }
+                }
+            }
+            __syncwarp();  // before the stage is written again
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+
+        // ---- the warps' sums joined, in the ring's memory
+        __syncthreads();
+        float* const jo = reinterpret_cast<float*>(ring);          // [kWarps][kRows][DP]
+        float* const jm = jo + kWarps * kRows * DP;                // [kWarps][2][kRows]
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
+            if (t4 == 0) jm[(warp * 2) * kRows + g + 8 * i] = m[i], jm[(warp * 2 + 1) * kRows + g + 8 * i] = l[i];
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+                *reinterpret_cast<float2*>(jo + (warp * kRows + g + 8 * i) * DP + n * 8 + 2 * t4) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        }
+        __syncthreads();
+        const bool whole = tile0 == 0 && tile1 == cost;
+        const int slot = pos == range_begin ? 0 : 1;
+        const int64_t wslot = (int64_t)blockIdx.x * 2 + slot;
+        for (int i = threadIdx.x; i < b.rows * (DP / 4); i += kThreads) {
+            const int row = i / (DP / 4), c = (i % (DP / 4)) * 4;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[(w * 2) * kRows + row]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f, x[4] = {};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = exp2_approx(jm[(w * 2) * kRows + row] - base);
+                const float4 v = *reinterpret_cast<const float4*>(jo + (w * kRows + row) * DP + c);
+                sum = fmaf(f, jm[(w * 2 + 1) * kRows + row], sum);
+                x[0] = fmaf(f, v.x, x[0]), x[1] = fmaf(f, v.y, x[1]), x[2] = fmaf(f, v.z, x[2]), x[3] = fmaf(f, v.w, x[3]);
+            }
+            if (!whole) {
+                *reinterpret_cast<float4*>(work.o + (wslot * kRows + row) * DP + c) = make_float4(x[0], x[1], x[2], x[3]);
+                if (c == 0) work.ml[(wslot * 2) * kRows + row] = top, work.ml[(wslot * 2 + 1) * kRows + row] = sum;
+                continue;
+            }
+            const float inv = 1.0f / sum;  // 0: the row sees nothing, or only scores of -inf
+            bool odd = !(sum > 0.0f);
+            const int packed = b.row0 + row;
+            const int64_t at = (int64_t)(b.first_row + packed / a.r) * a.o_stride + (int64_t)(head * a.r + packed % a.r) * d + c;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                x[u] *= inv;
+                if (c + u < d) {
+                    odd |= !isfinite(x[u]);
+                    from_f32(static_cast<T*>(a.o)[at + u], x[u]);
+                }
+            }
+            if (odd) odd_rows[row] = 1;
+        }
+        __syncthreads();
+        if (whole) {
+            for (int row = warp; row < b.rows; row += kWarps)
+                if (odd_rows[row]) {
+                    const int token = (b.row0 + row) / a.r;
+                    careful_row<T>(a, b.slot, b.first_row + token, b.p0 + token, head * a.r + (b.row0 + row) % a.r, head);
+                }
+        } else if (tile0 == 0 && threadIdx.x == 0) {
+            // the block that has the item's last tile: the last to begin at or before it
+            const int64_t last = item_at + cost - 1;
+            const int64_t holder = ((last + 1) * grid - 1) / total;
+            work.split[blockIdx.x] = Split{entry, head, (int)(holder - blockIdx.x) + 1, slot};
+        }
+        __syncthreads();
+        pos = item_at + tile1;
+        if (pos >= entry_at + (int64_t)cost * heads) {
+            entry_at += (int64_t)cost * heads;
+            ++entry;
+        }
+    }
+}
+
+// Block b joins the block of rows whose first piece thread block b left.
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const Work work, const __grid_constant__ SeqTable tab) {
+    __shared__ int odd_rows[kRows];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Split s = work.split[blockIdx.x];
+    if (!s.pieces) return;
+    const RowBlock b = row_block(a, sequence_of_tile(tab, s.item_entry), s.item_entry, kRows);
+    const int head = s.item_head, d = a.c.head_dim;
+    if (threadIdx.x < kRows) odd_rows[threadIdx.x] = 0;
+    __syncthreads();
+    auto slot = [&](int i) { return i == 0 ? (int64_t)blockIdx.x * 2 + s.first_slot : (int64_t)(blockIdx.x + i) * 2; };
+    for (int i = threadIdx.x; i < b.rows * (DP / 4); i += kThreads) {
+        const int row = i / (DP / 4), c = (i % (DP / 4)) * 4;
+        float top = -INFINITY;
+        for (int n = 0; n < s.pieces; ++n) top = fmaxf(top, work.ml[(slot(n) * 2) * kRows + row]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f, x[4] = {};
+#pragma unroll 4
+        for (int n = 0; n < s.pieces; ++n) {
+            const float f = exp2_approx(work.ml[(slot(n) * 2) * kRows + row] - base);
+            const float4 v = *reinterpret_cast<const float4*>(work.o + (slot(n) * kRows + row) * DP + c);
+            sum = fmaf(f, work.ml[(slot(n) * 2 + 1) * kRows + row], sum);
+            x[0] = fmaf(f, v.x, x[0]), x[1] = fmaf(f, v.y, x[1]), x[2] = fmaf(f, v.z, x[2]), x[3] = fmaf(f, v.w, x[3]);
+        }
+        const float inv = 1.0f / sum;
+        bool odd = !(sum > 0.0f);
+        const int packed = b.row0 + row;
+        const int64_t at = (int64_t)(b.first_row + packed / a.r) * a.o_stride + (int64_t)(head * a.r + packed % a.r) * d + c;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            x[u] *= inv;
+            if (c + u < d) {
+                odd |= !isfinite(x[u]);
+                from_f32(static_cast<T*>(a.o)[at + u], x[u]);
+            }
+        }
+        if (odd) odd_rows[row] = 1;
+    }
+    __syncthreads();
+    for (int row = threadIdx.x >> 5; row < b.rows; row += kWarps)
+        if (odd_rows[row]) {
+            const int token = (b.row0 + row) / a.r;
+            careful_row<T>(a, b.slot, b.first_row + token, b.p0 + token, head * a.r + (b.row0 + row) % a.r, head);
+        }
+}
+
+template <int DP, int LIMBS, typename T>
+int launch_split(strata_ctx* ctx, const AttnArgs& a, void* work, const SeqTable& tab, int64_t entries, cudaStream_t s) {
+    using C = Cfg<DP, LIMBS>;
+    static std::atomic<uint64_t> asked{0};
+    cudaError_t e = allow_shared(split_kernel<DP, LIMBS, T>, C::kSmem, asked, ctx->device);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(attention)");
+    const int grid = std::min(ctx->sm_count * C::kBlocks, kMaxGrid);
+    const Work w = work_of(work);
+    split_kernel<DP, LIMBS, T><<<grid, kThreads, C::kSmem, s>>>(a, w, (int)entries, tab);
+    int rc = check_launch(ctx, "attention kernel");
+    if (rc) return rc;
+    // launched while the first one still runs; it waits for that one's end itself
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kThreads), cfg.stream = s, cfg.attrs = &at, cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, join_kernel<DP, T>, a, w, tab);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join");
+    return STRATA_OK;
+}
+
+template <int DP>
+int launch_split(strata_ctx* ctx, bool bf16, const AttnArgs& a, void* work, const SeqTable& tab, int64_t entries, cudaStream_t s) {
+    if (bf16) return launch_split<DP, 1, __nv_bfloat16>(ctx, a, work, tab, entries, s);
+    return launch_split<DP, 3, float>(ctx, a, work, tab, entries, s);
+}
+
+// Calls launch(table, entries) for each group of sequences, cut into blocks of `per` rows.
+template <typename F>
+int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, F launch) {
+    auto blocks = [&](int64_t n) { return (n * r + per - 1) / per; };
+    if (!d.seq_offsets) {
+        if (d.n_seq > kMaxTokens / blocks(d.seq_len)) return fail(ctx, STRATA_ERR_INVALID, "attention: %lld sequences of %lld tokens", (long long)d.n_seq, (long long)d.seq_len);
+        SeqTable t = uniform_table(d.n_seq, 0, d.seq_len, 0, d.seq_len, 1);
+        t.tiles_all = (int)blocks(d.seq_len);
+        return launch(t, d.n_seq * t.tiles_all);
+    }
+    SeqTable t = ragged_table();
+    int64_t entries = 0;
+    for (int64_t i = 0; i < d.n_seq; ++i) {
+        const int64_t n = d.seq_offsets[i + 1] - d.seq_offsets[i];
+        if (n > 0) {
+            if (t.n == kSeqGroup || entries + blocks(n) > kMaxTokens) {
+                const int rc = launch(t, entries);
+                if (rc) return rc;
+                t = ragged_table();
+                entries = 0;
+            }
+            add_sequence(t, i, d.seq_offsets[i], n, 1);
+            entries += blocks(n);
+            t.tile[t.n] = (int)entries;
+        }
+    }
+    return t.n ? launch(t, entries) : STRATA_OK;
+}
+
+int padded(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+}  // namespace
+}  // namespace strata
+
+using namespace strata;
+
+extern "C" int strata_cuda_attention_work_bytes(const strata_attention* desc, const strata_kv_cache* cache, uint64_t* bytes) {
+    if (!desc || !cache || !bytes) return STRATA_ERR_INVALID;
+    strata_attention d = *desc;
+    strata_kv_cache c = *cache;
+    Why why;
+    int64_t tokens = 0, longest = 0;
+    const int rc = check_attention(why, d, c, &tokens, &longest);
+    if (rc) return rc;
+    *bytes = longest ? (uint64_t)work_bytes_for(padded(c.head_dim)) : 0;
+    return STRATA_OK;
+}
+
+extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention* desc, const strata_kv_cache* cache,
+                                         const void* q_dev, void* o_dev, void* work_dev, uint64_t work_bytes, void* stream) {
+    if (!ctx || !desc || !cache) return STRATA_ERR_INVALID;
+    STRATA_CALL_RANGE();
+    std::lock_guard<std::mutex> g(ctx->mu);
+    strata_attention d = *desc;
+    strata_kv_cache c = *cache;
+    Why why;
+    int64_t tokens = 0, longest = 0;
+    int rc = check_attention(why, d, c, &tokens, &longest);
+    const int dp = padded(c.head_dim);
+    if (!rc && longest) rc = check_attention_buffers(why, d, c, tokens, q_dev, o_dev, work_dev, work_bytes, (uint64_t)work_bytes_for(dp));
+    if (rc) return fail(ctx, rc, "attention: %s", why.text);
+    if (!longest) return STRATA_OK;
+    const bool bf16 = d.dtype == STRATA_QUANT_BF16;
+    const int64_t size = dtype_bytes(d.dtype);
+    AttnArgs a = {};
+    a.c = cache_args(c);
+    a.q = q_dev, a.o = o_dev, a.q_stride = d.q_stride, a.o_stride = d.o_stride;
+    a.r = (int)(d.n_head / c.n_kv_head);
+    a.window = (int)std::min(d.window, kMaxTokens), a.sinks = d.window ? (int)std::min(d.sinks, kMaxTokens) : 0;
+    a.scale = (float)d.scale, a.scale2 = (float)(d.scale * 1.4426950408889634);
+    a.wide = ((uintptr_t)q_dev | (uintptr_t)o_dev) % 16 == 0 && (d.q_stride * size) % 16 == 0 && (d.o_stride * size) % 16 == 0;
+    DeviceGuard dev(ctx->device);
+    const cudaStream_t s = pick_stream(ctx, stream);
+    return for_row_groups(ctx, d, a.r, kRows, [&](const SeqTable& t, int64_t entries) {
+        if (dp == 64) return launch_split<64>(ctx, bf16, a, work_dev, t, entries, s);
+        if (dp == 128) return launch_split<128>(ctx, bf16, a, work_dev, t, entries, s);
+        return launch_split<256>(ctx, bf16, a, work_dev, t, entries, s);
+    });
+}

@@ -135,6 +135,10 @@ def lib() -> C.CDLL:
             "strata_cuda_gated_delta_dev": (i32, [vp, C.POINTER(GatedDeltaDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                                   u64, vp]),
             "strata_cuda_sample_dev": (i32, [vp, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp]),
+            "strata_cuda_kv_append_dev": (i32, [vp, C.POINTER(KvAppendDesc), C.POINTER(KvCacheDesc), vp, vp, vp, vp, vp]),
+            "strata_cuda_attention_work_bytes": (i32, [C.POINTER(AttentionDesc), C.POINTER(KvCacheDesc), C.POINTER(u64)]),
+            "strata_cuda_attention_dev": (i32, [vp, C.POINTER(AttentionDesc), C.POINTER(KvCacheDesc), vp, vp, vp, u64, vp]),
+            "strata_cuda_logprobs_dev": (i32, [vp, vp, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp]),
         }
         for name, (res, args) in sig.items():
             if not hasattr(L, name):
@@ -195,6 +199,27 @@ class GatedDeltaDesc(C.Structure):
                  ("raw_gates", C.c_int)]
 
 
+class KvCacheDesc(C.Structure):
+    """strata_kv_cache (strata_attention.h)."""
+    _fields_ = [(nm, C.c_void_p) for nm in ("k_dev", "v_dev", "table_dev", "len_dev")]
+    _fields_ += [(nm, C.c_int64) for nm in ("n_pages", "page_size", "n_kv_head", "head_dim", "page_stride",
+                                            "token_stride", "head_stride", "max_pages", "table_stride")]
+
+
+class KvAppendDesc(C.Structure):
+    """strata_kv_append (strata_attention.h)."""
+    _fields_ = [("n_seq", C.c_int64), ("seq_len", C.c_int64), ("seq_offsets", C.POINTER(C.c_int64))]
+    _fields_ += [(nm, C.c_int64) for nm in ("n_head", "n_rot", "q_stride", "k_stride", "v_stride", "q_out_stride")]
+    _fields_ += [("freq_base", C.c_double), ("dtype", C.c_uint32), ("q_dtype", C.c_uint32), ("neighbours", C.c_int)]
+
+
+class AttentionDesc(C.Structure):
+    """strata_attention (strata_attention.h)."""
+    _fields_ = [("n_seq", C.c_int64), ("seq_len", C.c_int64), ("seq_offsets", C.POINTER(C.c_int64))]
+    _fields_ += [(nm, C.c_int64) for nm in ("n_head", "q_stride", "o_stride", "window", "sinks")]
+    _fields_ += [("scale", C.c_double), ("dtype", C.c_uint32)]
+
+
 def _sequences(desc, n_seq: int, seq_len: int, offsets):
     """Fills a desc's sequences; returns the host array its pointer needs alive."""
     desc.n_seq, desc.seq_len = n_seq, seq_len
@@ -245,6 +270,60 @@ def gated_delta_work_bytes(shape: GatedDelta) -> int:
     rc = lib().strata_cuda_gated_delta_work_bytes(shape.ref, C.byref(v))
     if rc != OK:
         raise BackendError(rc, "gated_delta: bad shape")
+    return v.value
+
+
+class KvCache:
+    """A paged cache of one layer's keys and values (strata_kv_cache) by its device addresses: two bf16 pools
+    of n_pages pages of page_size tokens, the sequences' rows of page numbers (max_pages int32 each) and their
+    lengths (int32, the tokens of the call included). Strides of 0 are packed: [page][token][head][dim]."""
+
+    def __init__(self, k_ptr: int, v_ptr: int, table_ptr: int, len_ptr: int, n_pages: int, page_size: int,
+                 n_kv_head: int, head_dim: int, max_pages: int, page_stride: int = 0, token_stride: int = 0,
+                 head_stride: int = 0, table_stride: int = 0):
+        d = self.desc = KvCacheDesc()
+        d.k_dev, d.v_dev, d.table_dev, d.len_dev = k_ptr, v_ptr, table_ptr, len_ptr
+        d.n_pages, d.page_size, d.n_kv_head, d.head_dim = n_pages, page_size, n_kv_head, head_dim
+        d.page_stride, d.token_stride, d.head_stride = page_stride, token_stride, head_stride
+        d.max_pages, d.table_stride = max_pages, table_stride
+        self.ref = C.byref(d)
+
+
+class KvAppend:
+    """The shape of an append to a cache (strata_kv_append): sequences as in ShortConv, n_head query heads
+    beside the cache's key heads, n_rot elements of a head turned (pairs of halves, or of neighbours)."""
+
+    def __init__(self, n_seq: int, n_head: int, n_rot: int, freq_base: float = 10000.0, seq_len: int = 1,
+                 offsets=None, dtype: int = F32, q_dtype: int | None = None, neighbours: bool = False,
+                 q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, q_out_stride: int = 0):
+        d = self.desc = KvAppendDesc()
+        self._rows = _sequences(d, n_seq, seq_len, offsets)
+        d.n_head, d.n_rot, d.freq_base = n_head, n_rot, freq_base
+        d.q_stride, d.k_stride, d.v_stride, d.q_out_stride = q_stride, k_stride, v_stride, q_out_stride
+        d.dtype, d.q_dtype, d.neighbours = dtype, dtype if q_dtype is None else q_dtype, int(neighbours)
+        self.ref = C.byref(d)
+
+
+class Attention:
+    """The shape of an attention call (strata_attention): sequences as in ShortConv, n_head query heads over
+    the cache's key heads; window 0 sees everything up to the token itself, else `window` tokens and the
+    first `sinks`."""
+
+    def __init__(self, n_seq: int, n_head: int, scale: float, seq_len: int = 1, offsets=None, dtype: int = F32,
+                 window: int = 0, sinks: int = 0, q_stride: int = 0, o_stride: int = 0):
+        d = self.desc = AttentionDesc()
+        self._rows = _sequences(d, n_seq, seq_len, offsets)
+        d.n_head, d.q_stride, d.o_stride, d.window, d.sinks = n_head, q_stride, o_stride, window, sinks
+        d.scale, d.dtype = scale, dtype
+        self.ref = C.byref(d)
+
+
+def attention_work_bytes(shape: Attention, cache: KvCache) -> int:
+    """Bytes of device workspace attention_dev needs for this shape (0: none)."""
+    v = C.c_uint64()
+    rc = lib().strata_cuda_attention_work_bytes(shape.ref, cache.ref, C.byref(v))
+    if rc != OK:
+        raise BackendError(rc, "attention: bad shape")
     return v.value
 
 
@@ -756,6 +835,28 @@ class Context:
                    min_p_ptr: int = 0, stride: int = 0, stream: int = 0):
         rc = _lib.strata_cuda_sample_dev(self.h, logits_ptr, rows, vocab, stride, temperature_ptr, top_k_ptr,
                                          top_p_ptr, min_p_ptr, uniform_ptr, ids_ptr, logprobs_ptr, stream)
+        if rc:
+            self.check(rc)
+
+    # ---- attention over a paged cache and the scoring of tokens (strata_attention.h)
+
+    def kv_append_dev(self, shape: KvAppend, cache: KvCache, q_ptr: int, k_ptr: int, v_ptr: int, q_out_ptr: int,
+                      stream: int = 0):
+        rc = _lib.strata_cuda_kv_append_dev(self.h, shape.ref, cache.ref, q_ptr, k_ptr, v_ptr, q_out_ptr, stream)
+        if rc:
+            self.check(rc)
+
+    def attention_dev(self, shape: Attention, cache: KvCache, q_ptr: int, o_ptr: int, work_ptr: int = 0,
+                      work_bytes: int = 0, stream: int = 0):
+        rc = _lib.strata_cuda_attention_dev(self.h, shape.ref, cache.ref, q_ptr, o_ptr, work_ptr, work_bytes, stream)
+        if rc:
+            self.check(rc)
+
+    def logprobs_dev(self, logits_ptr: int, rows: int, vocab: int, targets_ptr: int = 0, logprobs_ptr: int = 0,
+                     entropy_ptr: int = 0, top: int = 0, top_ids_ptr: int = 0, top_logprobs_ptr: int = 0,
+                     stride: int = 0, stream: int = 0):
+        rc = _lib.strata_cuda_logprobs_dev(self.h, logits_ptr, rows, vocab, stride, targets_ptr, logprobs_ptr,
+                                           entropy_ptr, top, top_ids_ptr, top_logprobs_ptr, stream)
         if rc:
             self.check(rc)
 
