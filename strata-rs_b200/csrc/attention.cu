@@ -34,7 +34,9 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kRows = 16;  // rows of a block
 constexpr int kUnit = 16;  // keys a warp takes of a tile
-static_assert(kWarps * kUnit == kTile, "a tile's keys are the warps' units");
+constexpr int kTile = kWarps * kUnit;
+constexpr int kOver = 1;   // what a block of rows costs besides its tiles, in tiles
+static_assert(kTile == 64, "a tile's keys are the warps' units");
 
 // DP: head_dim rounded up to 64, 128 or 256. Stages and blocks side by side fill
 // the shared memory, so that about 128 KB a multiprocessor are under way.
@@ -53,11 +55,6 @@ constexpr int kMaxGrid = 148 * 3;  // blocks of a launch at most; the workspace 
 
 // The workspace: what each block leaves of its first and its last block of rows
 // where other blocks have the rest, and which blocks of rows are to be joined.
-struct Split {
-    int item_entry, item_head;  // block of rows, key head
-    int pieces;                 // 0: none
-    int first_slot;             // of the first piece (the others are their blocks' slot 0)
-};
 struct Work {
     Split* split;  // [kMaxGrid]
     float* ml;     // [kMaxGrid][2][2][kRows]
@@ -103,32 +100,6 @@ __device__ __forceinline__ void limbs(float x, float y, uint32_t (&out)[LIMBS]) 
 template <int DP>
 __device__ __forceinline__ int chunk_at(int r, int c) { return r * DP * 2 + ((c ^ (r & 7)) << 4); }
 
-// The tiles of a block of rows; one at least, so that rows that see nothing are written.
-__device__ __forceinline__ int cost_of(const AttnArgs& a, const SeqTable& tab, int entry) {
-    const int n = key_range(a, row_block(a, sequence_of_tile(tab, entry), entry, kRows)).tiles;
-    return n > 0 ? n : 1;
-}
-
-// Sums over blocks of rows, for all threads. chunk[t]: prefix of thread t's entry.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int64_t x = v;
-    for (int w = 1; w < 32; w <<= 1) {
-        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, w);
-        if (lane >= w) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) sh[warp] = x;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
-    for (int i = 0; i < kWarps; ++i) {
-        if (i < warp) before += sh[i];
-        total += sh[i];
-    }
-    return before + x - v;
-}
-
 template <int DP, int LIMBS, typename T>
 __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
     split_kernel(const AttnArgs a, const Work work, int entries, const __grid_constant__ SeqTable tab) {
@@ -136,53 +107,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const qs = smem;
     uint8_t* const ring = smem + C::kQBytes;
-    __shared__ int64_t scan[kWarps];
-    __shared__ int64_t start_entry_before;
-    __shared__ int start_entry;
+    __shared__ int64_t scan[kWarps + 2];
     __shared__ int odd_rows[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int heads = a.c.n_kv_head, d = a.c.head_dim;
+    const int d = a.c.head_dim;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    // ---- this block's range of the call's tiles
-    int64_t total = 0, mine = 0;
-    for (int e0 = 0; e0 < entries; e0 += kThreads) {
-        const int e = e0 + threadIdx.x;
-        mine += e < entries ? cost_of(a, tab, e) : 0;
-    }
-    block_scan(mine, scan, total);
-    total *= heads;
-    const int64_t grid = total < gridDim.x ? total : (int64_t)gridDim.x;
+    Cut cut = cut_range<kThreads, kRows, kTile, kOver>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
-    if (blockIdx.x >= grid) return;
-    int64_t pos = total * blockIdx.x / grid;
-    const int64_t end = total * (blockIdx.x + 1) / grid;
-    {
-        int64_t base = 0;
-        for (int e0 = 0; e0 < entries; e0 += kThreads) {
-            const int e = e0 + threadIdx.x;
-            const int64_t cost = e < entries ? (int64_t)cost_of(a, tab, e) * heads : 0;
-            int64_t sum;
-            const int64_t before = base + block_scan(cost, scan, sum);
-            if (cost && pos >= before && pos < before + cost) start_entry = e, start_entry_before = before;
-            base += sum;
-            if (base > pos) break;
-        }
-        __syncthreads();
-    }
-    int entry = start_entry;
-    int64_t entry_at = start_entry_before;
-    const int64_t range_begin = pos;
+    if (blockIdx.x >= cut.grid) return;
+    const int64_t range_begin = cut.pos;
 
-    while (pos < end) {
-        const RowBlock b = row_block(a, sequence_of_tile(tab, entry), entry, kRows);
-        const KeyRange kr = key_range(a, b);
-        const int cost = kr.tiles > 0 ? kr.tiles : 1;
-        const int head = (int)((pos - entry_at) / cost);
-        const int64_t item_at = entry_at + (int64_t)head * cost;
-        const int tile0 = (int)(pos - item_at);
-        const int tile1 = (int)((end - item_at < cost ? end - item_at : cost));
-        const int steps = (kr.tiles < tile1 ? kr.tiles : tile1) - tile0;  // none where the rows see nothing
+    Piece<kTile> pc;
+    while (next_piece<kRows, kTile, kOver>(a, tab, cut, pc)) {
+        const RowBlock& b = pc.b;
+        const KeyRange<kTile>& kr = pc.kr;
+        const int head = pc.head, steps = pc.steps;
 
         // ---- this warp's keys, kStages - 1 units ahead
         int pages = -1;      // of unit (step & ~31) + lane
@@ -191,10 +130,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
             if (step < steps) {
                 if ((step & 31) == 0) {
                     const int at = step + lane;
-                    const int j = at < steps ? kr.key(tile0 + at) + warp * kUnit : kr.hi;
+                    const int j = at < steps ? pc.key(at) + warp * kUnit : kr.hi;
                     pages = j < kr.hi ? page_of(a.c, b.slot, j) : -1;
                 }
-                const int j0 = kr.key(tile0 + step) + warp * kUnit;
+                const int j0 = pc.key(step) + warp * kUnit;
                 const int page = __shfl_sync(0xFFFFFFFFu, pages, step & 31);
                 none = (none & ~(1u << (step & 31))) | (page < 0 ? 1u << (step & 31) : 0u);
                 uint8_t* const stage = ring + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes;
@@ -256,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
             load(step + C::kStages - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
             __syncwarp();
-            const int j0 = kr.key(tile0 + step) + warp * kUnit;
+            const int j0 = pc.key(step) + warp * kUnit;
             const uint32_t ks = shared_at(ring) + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes, vs = ks + C::kUnitBytes;
             if (!(none >> (step & 31) & 1) && j0 < kr.hi && (j0 + kUnit > kr.lo || j0 < a.sinks)) {
                 float s[LIMBS > 1 ? 2 : 1][2][4] = {};  // the small limbs' sums apart
@@ -359,8 +298,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
                 *reinterpret_cast<float2*>(jo + (warp * kRows + g + 8 * i) * DP + n * 8 + 2 * t4) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
         }
         __syncthreads();
-        const bool whole = tile0 == 0 && tile1 == cost;
-        const int slot = pos == range_begin ? 0 : 1;
+        const bool whole = pc.whole();
+        const int slot = slot_of(pc, range_begin);
         const int64_t wslot = (int64_t)blockIdx.x * 2 + slot;
         for (int i = threadIdx.x; i < b.rows * (DP / 4); i += kThreads) {
             const int row = i / (DP / 4), c = (i % (DP / 4)) * 4;
@@ -402,18 +341,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
                     const int token = (b.row0 + row) / a.r;
                     careful_row<T>(a, b.slot, b.first_row + token, b.p0 + token, head * a.r + (b.row0 + row) % a.r, head);
                 }
-        } else if (tile0 == 0 && threadIdx.x == 0) {
-            // the block that has the item's last tile: the last to begin at or before it
-            const int64_t last = item_at + cost - 1;
-            const int64_t holder = ((last + 1) * grid - 1) / total;
-            work.split[blockIdx.x] = Split{entry, head, (int)(holder - blockIdx.x) + 1, slot};
+        } else if (pc.tile0 == 0 && threadIdx.x == 0) {
+            work.split[blockIdx.x] = Split{pc.entry, head, pieces_of(cut, pc), slot};
         }
         __syncthreads();
-        pos = item_at + tile1;
-        if (pos >= entry_at + (int64_t)cost * heads) {
-            entry_at += (int64_t)cost * heads;
-            ++entry;
-        }
     }
 }
 
@@ -424,8 +355,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Split s = work.split[blockIdx.x];
     if (!s.pieces) return;
-    const RowBlock b = row_block(a, sequence_of_tile(tab, s.item_entry), s.item_entry, kRows);
-    const int head = s.item_head, d = a.c.head_dim;
+    const RowBlock b = row_block(a, sequence_of_tile(tab, s.entry), s.entry, kRows);
+    const int head = s.head, d = a.c.head_dim;
     if (threadIdx.x < kRows) odd_rows[threadIdx.x] = 0;
     __syncthreads();
     auto slot = [&](int i) { return i == 0 ? (int64_t)blockIdx.x * 2 + s.first_slot : (int64_t)(blockIdx.x + i) * 2; };
@@ -492,11 +423,13 @@ int launch_split(strata_ctx* ctx, bool bf16, const AttnArgs& a, void* work, cons
     return launch_split<DP, 3, float>(ctx, a, work, tab, entries, s);
 }
 
-// Calls launch(table, entries) for each group of sequences, cut into blocks of `per` rows.
+// Calls launch(table, entries) for each group of the sequences of `from` tokens or
+// more but below `below`, cut into blocks of `per` rows.
 template <typename F>
-int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, F launch) {
+int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, int64_t from, int64_t below, F launch) {
     auto blocks = [&](int64_t n) { return (n * r + per - 1) / per; };
     if (!d.seq_offsets) {
+        if (d.seq_len < from || d.seq_len >= below) return STRATA_OK;
         if (d.n_seq > kMaxTokens / blocks(d.seq_len)) return fail(ctx, STRATA_ERR_INVALID, "attention: %lld sequences of %lld tokens", (long long)d.n_seq, (long long)d.seq_len);
         SeqTable t = uniform_table(d.n_seq, 0, d.seq_len, 0, d.seq_len, 1);
         t.tiles_all = (int)blocks(d.seq_len);
@@ -506,7 +439,7 @@ int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, F
     int64_t entries = 0;
     for (int64_t i = 0; i < d.n_seq; ++i) {
         const int64_t n = d.seq_offsets[i + 1] - d.seq_offsets[i];
-        if (n > 0) {
+        if (n > 0 && n >= from && n < below) {
             if (t.n == kSeqGroup || entries + blocks(n) > kMaxTokens) {
                 const int rc = launch(t, entries);
                 if (rc) return rc;
@@ -521,7 +454,16 @@ int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, F
     return t.n ? launch(t, entries) : STRATA_OK;
 }
 
+// Rows a key head from which a sequence goes to the tensor cores' tiles of 128.
+constexpr int64_t kTcRows = 64;
+
+bool tiles(const strata_attention& d, const strata_kv_cache& c) { return d.dtype == STRATA_QUANT_BF16 && c.head_dim <= 128; }
 int padded(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+uint64_t needed(const strata_attention& d, const strata_kv_cache& c) {
+    const int dp = padded(c.head_dim);
+    return (uint64_t)std::max(work_bytes_for(dp), tiles(d, c) ? attention_tc_work_bytes(dp) : 0);
+}
 
 }  // namespace
 }  // namespace strata
@@ -536,7 +478,7 @@ extern "C" int strata_cuda_attention_work_bytes(const strata_attention* desc, co
     int64_t tokens = 0, longest = 0;
     const int rc = check_attention(why, d, c, &tokens, &longest);
     if (rc) return rc;
-    *bytes = longest ? (uint64_t)work_bytes_for(padded(c.head_dim)) : 0;
+    *bytes = longest ? needed(d, c) : 0;
     return STRATA_OK;
 }
 
@@ -551,7 +493,7 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     int64_t tokens = 0, longest = 0;
     int rc = check_attention(why, d, c, &tokens, &longest);
     const int dp = padded(c.head_dim);
-    if (!rc && longest) rc = check_attention_buffers(why, d, c, tokens, q_dev, o_dev, work_dev, work_bytes, (uint64_t)work_bytes_for(dp));
+    if (!rc && longest) rc = check_attention_buffers(why, d, c, tokens, q_dev, o_dev, work_dev, work_bytes, needed(d, c));
     if (rc) return fail(ctx, rc, "attention: %s", why.text);
     if (!longest) return STRATA_OK;
     const bool bf16 = d.dtype == STRATA_QUANT_BF16;
@@ -565,7 +507,16 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     a.wide = ((uintptr_t)q_dev | (uintptr_t)o_dev) % 16 == 0 && (d.q_stride * size) % 16 == 0 && (d.o_stride * size) % 16 == 0;
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    return for_row_groups(ctx, d, a.r, kRows, [&](const SeqTable& t, int64_t entries) {
+    int64_t many = kMaxTokens;  // tokens from which a sequence is read in tiles
+    TcMaps maps;
+    if (tiles(d, c) && longest * a.r >= kTcRows && attention_tc_maps(a.c, &maps)) {
+        many = (kTcRows + a.r - 1) / a.r;
+        rc = for_row_groups(ctx, d, a.r, attention_tc_rows(), many, kMaxTokens + 1, [&](const SeqTable& t, int64_t entries) {
+            return launch_attention_tc(ctx, dp, a, work_dev, t, entries, maps, s);
+        });
+        if (rc) return rc;
+    }
+    return for_row_groups(ctx, d, a.r, kRows, 1, many, [&](const SeqTable& t, int64_t entries) {
         if (dp == 64) return launch_split<64>(ctx, bf16, a, work_dev, t, entries, s);
         if (dp == 128) return launch_split<128>(ctx, bf16, a, work_dev, t, entries, s);
         return launch_split<256>(ctx, bf16, a, work_dev, t, entries, s);

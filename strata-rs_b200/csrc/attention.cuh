@@ -52,29 +52,31 @@ __device__ __forceinline__ RowBlock row_block(const AttnArgs& a, const Seq& s, i
 }
 
 // The keys that some row of a block sees: [0, sink) and [lo, hi); in tiles of
-// kTile keys, first those of the sinks, then those from lo on.
-constexpr int kTile = 64;
+// TILE keys, first those of the sinks, then those from lo on.
+template <int TILE>
 struct KeyRange {
     int lo, hi, sink_tiles, tiles;
     __device__ __forceinline__ int key(int tile) const {
-        return (tile < sink_tiles ? tile : lo / kTile + (tile - sink_tiles)) * kTile;
+        return (tile < sink_tiles ? tile : lo / TILE + (tile - sink_tiles)) * TILE;
     }
 };
-__device__ __forceinline__ KeyRange key_range(const AttnArgs& a, int p_min, int p_max) {
-    KeyRange k;
+template <int TILE>
+__device__ __forceinline__ KeyRange<TILE> key_range(const AttnArgs& a, int p_min, int p_max) {
+    KeyRange<TILE> k;
     const int cap = a.c.max_pages * a.c.page_size;  // below 2^31
     k.hi = p_max < cap ? p_max + 1 : cap;
     if (k.hi < 0) k.hi = 0;
     k.lo = a.window && p_min >= a.window ? p_min - a.window + 1 : 0;
     if (k.lo > k.hi) k.lo = k.hi;
-    const int sink = a.sinks < k.lo ? a.sinks : k.lo, first = k.lo / kTile;
-    k.sink_tiles = (sink + kTile - 1) / kTile;
+    const int sink = a.sinks < k.lo ? a.sinks : k.lo, first = k.lo / TILE;
+    k.sink_tiles = (sink + TILE - 1) / TILE;
     if (k.sink_tiles > first) k.sink_tiles = first;  // the rest lies in lo's own tile
-    k.tiles = k.sink_tiles + (k.hi + kTile - 1) / kTile - first;
+    k.tiles = k.sink_tiles + (k.hi + TILE - 1) / TILE - first;
     return k;
 }
-__device__ __forceinline__ KeyRange key_range(const AttnArgs& a, const RowBlock& b) {
-    return key_range(a, b.p0 + b.row0 / a.r, b.p0 + (b.row0 + b.rows - 1) / a.r);
+template <int TILE>
+__device__ __forceinline__ KeyRange<TILE> key_range(const AttnArgs& a, const RowBlock& b) {
+    return key_range<TILE>(a, b.p0 + b.row0 / a.r, b.p0 + (b.row0 + b.rows - 1) / a.r);
 }
 __device__ __forceinline__ bool sees(const AttnArgs& a, int p, int j) {
     return j <= p && (!a.window || j > p - a.window || j < a.sinks);
@@ -92,6 +94,128 @@ __device__ __forceinline__ int64_t place(const CacheArgs& c, int page, int j, in
 template <typename T>
 __device__ __forceinline__ float load_f32(const void* base, int64_t i) { return to_f32(static_cast<const T*>(base)[i]); }
 
+// The work of all blocks of rows and key heads of a launch, cut evenly over its
+// thread blocks: this one's contiguous range of units. A block of rows costs OVER
+// units for its queries and outputs, then one a tile (one at least, so that rows
+// that see nothing are written).
+struct Cut {
+    int64_t total, grid;    // units, and thread blocks that get some
+    int64_t pos, end;       // this one's
+    int entry;              // block of rows that `pos` lies in,
+    int64_t entry_at;       // and its first unit
+};
+template <int ROWS, int TILE, int OVER>
+__device__ __forceinline__ int cost_of(const AttnArgs& a, const SeqTable& tab, int entry) {
+    const int n = key_range<TILE>(a, row_block(a, sequence_of_tile(tab, entry), entry, ROWS)).tiles;
+    return OVER + (n > 0 ? n : 1);
+}
+// Prefix of v over the block's threads, and its total. `sh`: a number a warp.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t x = v;
+    for (int w = 1; w < 32; w <<= 1) {
+        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, w);
+        if (lane >= w) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int i = 0; i < THREADS / 32; ++i) {
+        if (i < warp) before += sh[i];
+        total += sh[i];
+    }
+    return before + x - v;
+}
+// By all THREADS threads; blocks from c.grid on have none. `sh`: THREADS / 32 + 2 numbers.
+template <int THREADS, int ROWS, int TILE, int OVER>
+__device__ __forceinline__ Cut cut_range(const AttnArgs& a, const SeqTable& tab, int entries, int64_t* sh) {
+    Cut c;
+    const int heads = a.c.n_kv_head;
+    int64_t mine = 0, first = 0;
+    for (int e0 = 0; e0 < entries; e0 += THREADS) {
+        const int e = e0 + threadIdx.x;
+        const int64_t cost = e < entries ? (int64_t)cost_of<ROWS, TILE, OVER>(a, tab, e) * heads : 0;
+        if (e0 == 0) first = cost;
+        mine += cost;
+    }
+    block_scan<THREADS>(mine, sh, c.total);
+    c.grid = c.total < gridDim.x ? c.total : (int64_t)gridDim.x;
+    if (blockIdx.x >= c.grid) return c;
+    c.pos = c.total * blockIdx.x / c.grid;
+    c.end = c.total * (blockIdx.x + 1) / c.grid;
+    int64_t base = 0;
+    for (int e0 = 0; e0 < entries; e0 += THREADS) {
+        const int e = e0 + threadIdx.x;
+        const int64_t cost = e0 == 0 ? first : e < entries ? (int64_t)cost_of<ROWS, TILE, OVER>(a, tab, e) * heads : 0;
+        int64_t sum;
+        const int64_t before = base + block_scan<THREADS>(cost, sh, sum);
+        if (cost && c.pos >= before && c.pos < before + cost) sh[THREADS / 32] = e, sh[THREADS / 32 + 1] = before;
+        base += sum;
+        if (base > c.pos) break;
+    }
+    __syncthreads();
+    c.entry = (int)sh[THREADS / 32];
+    c.entry_at = sh[THREADS / 32 + 1];
+    return c;
+}
+// The piece of one block of rows and key head that begins at `c.pos`: tiles
+// [tile0, tile1) of its `tiles`.
+template <int TILE>
+struct Piece {
+    RowBlock b;
+    KeyRange<TILE> kr;
+    int head, cost;
+    int64_t at;             // the first unit of the block of rows and head
+    int64_t begin;          // this piece's
+    int entry;
+    int tiles, tile0, tile1;
+    int steps;              // tiles with keys
+    __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == tiles; }
+    __device__ __forceinline__ int key(int step) const { return kr.key(tile0 + step); }
+};
+// The next piece of the thread block's range, from c.pos on; false at its end.
+template <int ROWS, int TILE, int OVER>
+__device__ __forceinline__ bool next_piece(const AttnArgs& a, const SeqTable& tab, Cut& c, Piece<TILE>& p) {
+    while (c.pos < c.end) {
+        p.b = row_block(a, sequence_of_tile(tab, c.entry), c.entry, ROWS);
+        p.kr = key_range<TILE>(a, p.b);
+        p.tiles = p.kr.tiles > 0 ? p.kr.tiles : 1;
+        p.cost = OVER + p.tiles;
+        p.entry = c.entry;
+        p.head = (int)((c.pos - c.entry_at) / p.cost);
+        p.at = c.entry_at + (int64_t)p.head * p.cost;
+        p.begin = c.pos;
+        const int u0 = (int)(c.pos - p.at), u1 = (int)(c.end - p.at < p.cost ? c.end - p.at : p.cost);
+        p.tile0 = u0 > OVER ? u0 - OVER : 0;
+        p.tile1 = u1 > OVER ? u1 - OVER : 0;
+        p.steps = (p.kr.tiles < p.tile1 ? p.kr.tiles : p.tile1) - p.tile0;
+        c.pos = p.at + u1;
+        const int64_t all = (int64_t)p.cost * a.c.n_kv_head;
+        if (c.pos >= c.entry_at + all) c.entry_at += all, ++c.entry;
+        if (p.tile1 > p.tile0) return true;  // else the range ends within the block's first OVER units
+    }
+    return false;
+}
+// Which of a thread block's two places a piece's sums go to, where others have the rest.
+template <int TILE>
+__device__ __forceinline__ int slot_of(const Piece<TILE>& p, int64_t range_begin) { return p.begin == range_begin ? 0 : 1; }
+// Thread blocks that have pieces of `p`, of which this one has the first: the
+// last of them is the last that begins at or before its last unit.
+template <int TILE>
+__device__ __forceinline__ int pieces_of(const Cut& c, const Piece<TILE>& p) {
+    return (int)(((p.at + p.cost) * c.grid - 1) / c.total - blockIdx.x) + 1;
+}
+
+// What a thread block leaves for the join: which block of rows it has the first piece of.
+struct Split {
+    int entry, head;
+    int pieces;      // 0: none
+    int first_slot;  // of the first piece; the others are their thread blocks' slot 0
+};
+
 // One row, by a warp, key by key and leaving out what it does not see: for rows
 // whose result is not finite, since in a product of tiles a NaN or an infinity
 // that a row does not see meets its weight of zero (and gives a NaN).
@@ -102,9 +226,9 @@ __device__ __noinline__ void careful_row(const AttnArgs& a, int slot, int token,
     const int64_t q = (int64_t)token * a.q_stride + (int64_t)head * d;
     float m = -INFINITY, l = 0.0f, o[8] = {};
     bool seen = false;
-    const KeyRange kr = key_range(a, p, p);
+    const KeyRange<64> kr = key_range<64>(a, p, p);
     for (int tile = 0; tile < kr.tiles; ++tile)
-        for (int half = 0; half < kTile; half += 32) {
+        for (int half = 0; half < 64; half += 32) {
             const int j0 = kr.key(tile) + half, j = j0 + lane;
             float s = -INFINITY;
             bool live = j < kr.hi && sees(a, p, j);
@@ -145,5 +269,18 @@ __device__ __noinline__ void careful_row(const AttnArgs& a, int slot, int token,
     for (int i = 0; i < 8; ++i)
         if (lane + 32 * i < d) from_f32(out[lane + 32 * i], seen ? o[i] / l : 0.0f);
 }
+
+// attention_tc.cu: bf16 chunks with heads of up to 128 on the tensor cores, in
+// blocks of attention_tc_rows() rows. The maps describe the pools to the copies;
+// they fail where a stride is outside what a map can hold.
+struct TcMaps {
+    alignas(64) unsigned char k[128], v[128];
+    int box_rows, inside;
+};
+int attention_tc_rows();
+int64_t attention_tc_work_bytes(int dp);
+bool attention_tc_maps(const CacheArgs& c, TcMaps* maps);
+int launch_attention_tc(strata_ctx* ctx, int dp, const AttnArgs& a, void* work, const SeqTable& tab, int64_t entries, const TcMaps& maps,
+                        cudaStream_t s);
 
 }  // namespace strata
