@@ -509,7 +509,7 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     const cudaStream_t s = pick_stream(ctx, stream);
     int64_t many = kMaxTokens;  // tokens from which a sequence is read in tiles
     TcMaps maps;
-    if (tiles(d, c) && longest * a.r >= kTcRows && attention_tc_maps(a.c, &maps)) {
+    if (tiles(d, c) && a.wide && longest * a.r >= kTcRows && attention_tc_maps(a.c, &maps)) {
         many = (kTcRows + a.r - 1) / a.r;
         rc = for_row_groups(ctx, d, a.r, attention_tc_rows(), many, kMaxTokens + 1, [&](const SeqTable& t, int64_t entries) {
             return launch_attention_tc(ctx, dp, a, work_dev, t, entries, maps, s);
