@@ -37,7 +37,7 @@ constexpr int kRowTile = 128, kKeyTile = 128;
 constexpr int kRows = 2 * kRowTile;
 constexpr int kThreads = 384;  // three warpgroups, which registers are shared out by
 constexpr int kRegs = 208, kRegsRest = 88;  // 2 x 208 + 88 = 3 x 168, what the block is launched with
-constexpr int kOver = 4;       // what a block of rows costs besides its tiles, in tiles
+constexpr int kOver = 6;       // what a block of rows costs besides its tiles, in tiles (8 or 4: a prompt of 8192 501, 519 us, not 488)
 constexpr int kMaxGrid = 148;
 constexpr int kMasks = 8;   // tiles whose masks are kept
 constexpr int kPieces = 8;  // pieces that are known ahead
@@ -252,8 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t done = 0, tiles = 0;  // products into O so far, tiles
         bool live = true;
         // A tile's rows of queries and outputs are moved by the warps that own them, DP / 8
-        // lanes a row, so that lines are read and written whole. Queries come to registers
-        // first: while they are under way the last piece's outputs still use their place.
+        // lanes a row, so that lines are read and written whole; outputs pass through the
+        // queries' place in shared memory.
         constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes;
         const int unit = lane % kLanes, sub = lane / kLanes;
         uint8_t* const mine_at = qs + t * C::kTileBytes + (warp & 3) * 32 * 128;  // this warp's rows of the tile's first column
@@ -262,24 +262,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto known_at = [&](uint32_t i) { return live && __all_sync(0xFFFFFFFFu, bar_wait(shared_at(&known_full[i % kPieces]), (i / kPieces) & 1, err)); };
         float m = 0.0f, l = 0.0f;
         for (uint32_t i = 0;; ++i) {
-            // ---- piece i's queries to registers, piece i - 1's outputs out, then the queries to their place
+            // ---- piece i - 1's outputs, then piece i's queries
             const Known& kn = known[i % kPieces];
             live = known_at(i);
             if (!live) break;
             const bool last = kn.last, active = !last && has_rows(kn.piece);
-            uint4 ahead[kLanes];
-            if (active) {
-                const RowBlock& b = kn.piece.b;
-                const int in_block = t * kRowTile + row, packed = b.row0 + in_block;
-                // where this thread's own row lies (divisions: once a row)
-                const int64_t own = in_block < b.rows ? (int64_t)(b.first_row + packed / a.r) * a.q_stride + (int64_t)(kn.piece.head * a.r + packed % a.r) * a.c.head_dim : -1;
-#pragma unroll
-                for (int u = 0; u < kLanes; ++u) {
-                    const int64_t at = __shfl_sync(0xFFFFFFFFu, own, u * kAtOnce + sub);
-                    ahead[u] = make_uint4(0, 0, 0, 0);
-                    if (at >= 0 && unit * 8 < a.c.head_dim) ahead[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at + unit * 8);
-                }
-            }
             const Piece<kKeyTile>& pc = known[(i + kPieces - 1) % kPieces].piece;
             if (i > 0 && t * kRowTile < pc.b.rows) {
                 const RowBlock& b = pc.b;
@@ -348,6 +335,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!active) {
                 tiles += kn.piece.steps;
                 continue;
+            }
+            uint4 ahead[kLanes];
+            if (active) {
+                const RowBlock& b = kn.piece.b;
+                const int in_block = t * kRowTile + row, packed = b.row0 + in_block;
+                // where this thread's own row lies (divisions: once a row)
+                const int64_t own = in_block < b.rows ? (int64_t)(b.first_row + packed / a.r) * a.q_stride + (int64_t)(kn.piece.head * a.r + packed % a.r) * a.c.head_dim : -1;
+#pragma unroll
+                for (int u = 0; u < kLanes; ++u) {
+                    const int64_t at = __shfl_sync(0xFFFFFFFFu, own, u * kAtOnce + sub);
+                    ahead[u] = make_uint4(0, 0, 0, 0);
+                    if (at >= 0 && unit * 8 < a.c.head_dim) ahead[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at + unit * 8);
+                }
             }
 #pragma unroll
             for (int u = 0; u < kLanes; ++u) *reinterpret_cast<uint4*>(place_of(u * kAtOnce + sub, unit)) = ahead[u];
