@@ -4,15 +4,20 @@
 //   Z = sum_j exp(x_j - M), log p_i = x_i - M - log Z, H = log Z - sum_j e_j (x_j - M) / Z
 //
 // One pass over the row for M, Z and sum e_j (x_j - M), each thread with a
-// running maximum of its own; Z is summed in f64, because next to a certain
-// token it is 1 and a little, and log Z is that little. The threads' maxima are
-// what the likeliest tokens are found by: the n-th largest of them, T, is a lower
-// bound of the n-th largest logit, and only threads whose maximum reaches T can
-// have seen one of the n: their logits (one in kThreads each) are read again, and
-// those that reach T are ordered by counting.
+// running maximum of its own. Next to a certain token Z is 1 and a little, and
+// log Z is that little: so a batch's maximum is found by a tournament, whose
+// losers (which never hold the 1) are summed in f32 and whose winner apart, and
+// both go to an f64 sum. The threads' maxima are what the likeliest tokens are
+// found by: a bound T that at least n of them reach is a lower bound of the n-th
+// largest logit, only threads whose maximum reaches T can have seen one of the n,
+// and their logits (one in kThreads each) are read again, a warp a thread's. What
+// reaches T is ordered by counting.
 //
-// Bound by memory where rows are many (one block a row); few rows are cut over a
-// cluster of blocks, whose results the first one joins.
+// Bound by memory where rows are many (one block a row): 1024 rows of 151936 118 us,
+// 5.3 TB/s. Few rows are cut over a cluster, whose results the first block joins: 32 rows
+// 11 us, one row 14 (the pass 4, the rest steps that wait on each other). Before the
+// tournament each exponential went to the f64 sum by itself and maxima moved with f64
+// exponentials: 264 us for the 1024 rows.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -28,8 +33,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kTop = (int)kMaxTop;
 constexpr int kCand = 1024;     // candidates that are ordered at once
-constexpr int kMaxCluster = 8;
-constexpr int kAhead = 4;       // 16-byte packs a thread has under way
+constexpr int kMaxCluster = 4;
 
 struct LogprobArgs {
     const float* logits;
@@ -45,51 +49,62 @@ struct LogprobArgs {
 // What a thread, a block or a row has seen: the largest logit, sum e^(x - max) and sum e^(x - max) (x - max).
 struct Sum {
     float max;
-    double z, zd;
+    float zd;
+    double z;
 };
 __device__ __forceinline__ void rescale(Sum& s, float max) {  // max >= s.max
-    if (s.max == max) return;
-    if (s.max == -INFINITY) {
-        s.z = s.zd = 0.0;
-    } else {
-        const double down = (double)s.max - (double)max, f = exp(down);
-        s.zd = f * (s.zd + down * s.z);
-        s.z *= f;
-    }
+    const float down = fmaxf(s.max - max, -200.0f), f = expf(down);  // below e^-200 is nothing
+    const bool none = s.max == -INFINITY, same = s.max == max;
+    s.zd = none ? 0.0f : same ? s.zd : f * fmaf(down, (float)s.z, s.zd);
+    s.z = none ? 0.0 : same ? s.z : s.z * (double)f;
     s.max = max;
 }
-__device__ __forceinline__ void join(Sum& a, Sum b) {
-    const float max = fmaxf(a.max, b.max);
-    rescale(a, max), rescale(b, max);
-    a.z += b.z, a.zd += b.zd;
-}
-__device__ __forceinline__ Sum shuffled(const Sum& s, int w) {
-    return {__shfl_xor_sync(0xFFFFFFFFu, s.max, w), __shfl_xor_sync(0xFFFFFFFFu, s.z, w), __shfl_xor_sync(0xFFFFFFFFu, s.zd, w)};
+// The sums of a warp's lanes, for all of them.
+__device__ __forceinline__ Sum warp_sum(Sum s) {
+    float max = s.max;
+    for (int w = 16; w; w >>= 1) max = fmaxf(max, __shfl_xor_sync(0xFFFFFFFFu, max, w));
+    rescale(s, max);
+    for (int w = 16; w; w >>= 1) {
+        s.z += __shfl_xor_sync(0xFFFFFFFFu, s.z, w);
+        s.zd += __shfl_xor_sync(0xFFFFFFFFu, s.zd, w);
+    }
+    return s;
 }
 
 __device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }  // a NaN counts as -inf
-__device__ __forceinline__ float exp_of(float d) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.4426950408889634f));
-    return y;
+__device__ __forceinline__ float2 exp_of(float2 d) {
+    const float2 t = __fmul2_rn(d, make_float2(1.4426950408889634f, 1.4426950408889634f));
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    return e;
 }
-// N logits more. zd is summed in f32 within them: its terms never meet the 1 of the largest.
-template <int N>
-__device__ __forceinline__ void add(Sum& s, const float (&x)[N]) {
-    float max = x[0];
+// 16 logits more (-inf where there are fewer).
+__device__ __forceinline__ void add(Sum& s, float (&x)[16]) {
+    // after this x[0] is the largest, the others are what lost on the way
 #pragma unroll
-    for (int i = 1; i < N; ++i) max = fmaxf(max, x[i]);
-    if (max > s.max) rescale(s, max);
-    if (s.max == -INFINITY) return;
-    float zd = 0.0f;
+    for (int half = 8; half; half /= 2)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = fmaxf(x[i] - s.max, -200.0f);  // below e^-200 is nothing, and -inf * 0 is none
-        const float e = exp_of(d);
-        s.z += (double)e;
-        zd = fmaf(e, d, zd);
+        for (int i = 0; i < half; ++i) {
+            const float a = x[i], b = x[i + half];
+            x[i] = fmaxf(a, b), x[i + half] = fminf(a, b);
+        }
+    if (x[0] > s.max) rescale(s, x[0]);
+    const float m = s.max == -INFINITY ? 0.0f : -s.max;
+    float2 z = make_float2(0.0f, 0.0f), zd = z;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(m, m));
+        d = make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));  // below e^-200 is nothing, and -inf * 0 is none
+        float2 e = exp_of(d);
+        zd = __ffma2_rn(e, d, zd);
+        if (i == 0) top = e.x, e.x = 0.0f;
+        z = __fadd2_rn(z, e);
     }
-    s.zd += (double)zd;
+    s.z += (double)(z.x + z.y);
+    s.z += (double)top;
+    s.zd += zd.x + zd.y;
 }
 
 struct Cand {
@@ -98,106 +113,125 @@ struct Cand {
 };
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.x > b.x || (a.x == b.x && a.id < b.id); }
 
-// The first n of m candidates in order, into out (all threads; m up to kCand).
-__device__ void order_by_counting(const Cand* in, int m, int n, Cand* out) {
-    for (int i = threadIdx.x; i < m; i += kThreads) {
+// The first n of m candidates in order, into out (all threads; a warp a candidate).
+// Blanks (-inf) are left out.
+__device__ __forceinline__ void order_by_counting(const Cand* in, int m, int n, Cand* out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = warp; i < m; i += kWarps) {
         const Cand c = in[i];
+        if (c.x == -INFINITY) continue;
         int rank = 0;
-        for (int j = 0; j < m; ++j) rank += before(in[j], c);
-        if (rank < n) out[rank] = c;
+        for (int j = lane; j - lane < m; j += 32) rank += __popc(__ballot_sync(0xFFFFFFFFu, j < m && before(in[j], c)));
+        if (lane == 0 && rank < n) out[rank] = c;
     }
 }
 
 // PACKS: rows are 16-byte aligned and read in packs of four.
 template <bool PACKS>
 __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobArgs a, int cluster) {
-    __shared__ float maxima[kThreads];
+    __shared__ float seconds[kWarps];
+    __shared__ short reach[kThreads];       // threads whose maximum reaches T
     __shared__ Cand cand[kCand];
     __shared__ Cand best[kTop];             // of this block
     __shared__ Cand all[kMaxCluster * kTop], final[kTop];
-    __shared__ Sum part[kWarps], sums[kMaxCluster];
-    __shared__ int n_cand, infinite;
+    __shared__ Sum part[kWarps], sums[kMaxCluster], result;
+    __shared__ int n_cand, n_reach, infinite;
     __shared__ unsigned long long pick[kWarps];
     const int rank = cluster > 1 ? blockIdx.x % cluster : 0;
     const int64_t row = blockIdx.x / cluster;
     const float* x = a.logits + row * a.stride;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // this block's share, in whole rounds of the block's packs
-    constexpr int kStep = kThreads * (PACKS ? 4 : 1);
+    constexpr int kPack = PACKS ? 4 : 1, kStep = kThreads * kPack, kBatch = 16 / kPack;
     const int rounds = (a.vocab + kStep - 1) / kStep;
     const int r0 = (int)((int64_t)rounds * rank / cluster), r1 = (int)((int64_t)rounds * (rank + 1) / cluster);
     const int begin = r0 * kStep, end = min(r1 * kStep, a.vocab);
     // arrive here, wait before the first remote write: the first block then runs
     if (cluster > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-    if (threadIdx.x == 0) n_cand = 0, infinite = 0;
+    if (threadIdx.x == 0) n_cand = n_reach = infinite = 0;
     if (threadIdx.x < kTop) best[threadIdx.x] = Cand{-INFINITY, -1}, final[threadIdx.x] = Cand{-INFINITY, -1};
 
     // ---- the pass
-    Sum s = {-INFINITY, 0.0, 0.0};
-    if (PACKS) {
-        const int whole = end - (end & 3);
-        int i = begin + threadIdx.x * 4;
-        for (; i + (kAhead - 1) * kStep < whole; i += kAhead * kStep) {
-            float v[4 * kAhead];
+    Sum s = {-INFINITY, 0.0f, 0.0};
+    auto load = [&](int i, float (&v)[16]) {  // a batch: kBatch packs, kStep apart
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const float4 p = __ldcs(reinterpret_cast<const float4*>(x + i + u * kStep));
-                v[4 * u] = clean(p.x), v[4 * u + 1] = clean(p.y), v[4 * u + 2] = clean(p.z), v[4 * u + 3] = clean(p.w);
+        for (int u = 0; u < kBatch; ++u) {
+            const int at = i + u * kStep;
+            if (PACKS) {
+                float4 p = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (at + 4 <= end) {
+                    p = __ldcs(reinterpret_cast<const float4*>(x + at));
+                } else {  // the row's end in a pack
+                    if (at < end) p.x = x[at];
+                    if (at + 1 < end) p.y = x[at + 1];
+                    if (at + 2 < end) p.z = x[at + 2];
+                }
+                v[4 * (u % 4)] = p.x, v[4 * (u % 4) + 1] = p.y, v[4 * (u % 4) + 2] = p.z, v[4 * (u % 4) + 3] = p.w;
+            } else {
+                v[u] = at < end ? __ldcs(x + at) : -INFINITY;
             }
-            add(s, v);
         }
-        for (; i < whole; i += kStep) {
-            const float4 p = __ldcs(reinterpret_cast<const float4*>(x + i));
-            const float v[4] = {clean(p.x), clean(p.y), clean(p.z), clean(p.w)};
-            add(s, v);
-        }
-        if (threadIdx.x < end - whole) {  // what is no pack, by the threads of lowest number
-            const float v[1] = {clean(x[whole + threadIdx.x])};
-            add(s, v);
-        }
-    } else {
-        for (int i = begin + threadIdx.x; i < end; i += kAhead * kStep) {
-            float v[kAhead];
+    };
+    float now[16], next[16];
+    const int first = begin + threadIdx.x * kPack;
+    load(first, now);
+    for (int i = first; i < end; i += kBatch * kStep) {
+        load(i + kBatch * kStep, next);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) v[u] = i + u * kStep < end ? clean(__ldcs(x + i + u * kStep)) : -INFINITY;
-            add(s, v);
-        }
+        for (int u = 0; u < 16; ++u) now[u] = clean(now[u]);
+        add(s, now);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) now[u] = next[u];
     }
-    maxima[threadIdx.x] = s.max;
     const float own = s.max;
-    for (int w = 16; w; w >>= 1) join(s, shuffled(s, w));
-    if (lane == 0) part[warp] = s;
+    const Sum w_sum = warp_sum(s);
+    if (lane == 0) part[warp] = w_sum;
+    // T: of the warps' largest maxima the n-th, or where n is above their number the
+    // n/2-th of their second largest (two of a warp's lanes reach it)
+    {
+        float v = own;
+        if (a.top > kWarps) {
+            const unsigned at = __ballot_sync(0xFFFFFFFFu, own == w_sum.max);
+            if (lane == __ffs(at) - 1) v = -INFINITY;
+            for (int w = 16; w; w >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, w));
+        } else {
+            v = w_sum.max;
+        }
+        if (lane == 0) seconds[warp] = v;
+    }
     __syncthreads();
 
     // ---- this block's likeliest
     if (a.top && begin < end) {
-        // how many threads' maxima come before this one's, threads' numbers settling ties
-        int ahead = 0;
-        for (int j = 0; j < kThreads; ++j) {
-            const float m = maxima[j];
-            ahead += m > own || (m == own && j < (int)threadIdx.x);
+        const int nth = a.top > kWarps ? (a.top + 1) / 2 : a.top;
+        float t;
+        {
+            const float v = seconds[lane % kWarps];
+            int ahead = 0;
+#pragma unroll
+            for (int j = 0; j < kWarps; ++j) {
+                const float other = __shfl_sync(0xFFFFFFFFu, v, j);
+                ahead += other > v || (other == v && j < lane % kWarps);
+            }
+            t = __shfl_sync(0xFFFFFFFFu, v, __ffs(__ballot_sync(0xFFFFFFFFu, ahead == nth - 1)) - 1);
         }
-        __shared__ float bound;
-        if (ahead == a.top - 1) bound = own;
+        if (own >= t && own > -INFINITY) reach[atomicAdd(&n_reach, 1)] = (short)threadIdx.x;
         __syncthreads();
-        const float t = bound;
-        auto offer = [&](int i) {
-            const float v = clean(x[i]);
-            if (v >= t && v > -INFINITY) {
+        auto offer = [&](int i, float v) {
+            if (v >= t && v > -INFINITY) {  // not of a NaN
                 const int at = atomicAdd(&n_cand, 1);
                 if (at < kCand) cand[at] = Cand{v, i};
             }
         };
-        if (own >= t && own > -INFINITY) {
-            if (PACKS) {
-                const int whole = end - (end & 3);
-                for (int i = begin + threadIdx.x * 4; i < whole; i += kStep)
-                    for (int u = 0; u < 4; ++u) offer(i + u);
-                if (threadIdx.x < end - whole) offer(whole + threadIdx.x);
-            } else {
-                for (int i = begin + threadIdx.x; i < end; i += kStep) offer(i);
+        for (int n = warp; n < n_reach; n += kWarps)  // a warp a thread's logits
+            for (int i = begin + reach[n] * kPack + lane * kStep; i < end; i += 32 * kStep) {
+                if (PACKS && i + 4 <= end) {
+                    const float4 p = *reinterpret_cast<const float4*>(x + i);
+                    offer(i, p.x), offer(i + 1, p.y), offer(i + 2, p.z), offer(i + 3, p.w);
+                } else {
+                    for (int u = 0; u < kPack && i + u < end; ++u) offer(i + u, x[i + u]);
+                }
             }
-        }
         __syncthreads();
         if (n_cand <= kCand) {
             order_by_counting(cand, n_cand, a.top, best);
@@ -232,12 +266,8 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobArgs
     }
 
     // ---- the blocks of the row joined by the first
-    Sum total = {-INFINITY, 0.0, 0.0};
-    if (warp == 0) {
-        Sum v = lane < kWarps ? part[lane] : Sum{-INFINITY, 0.0, 0.0};
-        for (int w = 16; w; w >>= 1) join(v, shuffled(v, w));
-        total = v;
-    }
+    Sum total = {-INFINITY, 0.0f, 0.0};
+    if (warp == 0) total = warp_sum(lane < kWarps ? part[lane] : total);
     const Cand* list = best;
     if (cluster > 1) {
         cg::cluster_group cl = cg::this_cluster();
@@ -246,24 +276,13 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobArgs
         if ((int)threadIdx.x < a.top) cl.map_shared_rank(all, 0)[rank * a.top + threadIdx.x] = best[threadIdx.x];
         cl.sync();
         if (rank) return;
-        if (warp == 0) {
-            Sum v = lane < cluster ? sums[lane] : Sum{-INFINITY, 0.0, 0.0};
-            for (int w = 16; w; w >>= 1) join(v, shuffled(v, w));
-            total = v;
-        }
-        // the blanks' ids of -1 would come first among equals: none of -inf is taken
+        if (warp == 0) total = warp_sum(lane < cluster ? sums[lane] : Sum{-INFINITY, 0.0f, 0.0});
         if (a.top) {
-            for (int i = threadIdx.x; i < cluster * a.top; i += kThreads) {
-                const Cand c = all[i];
-                int place = 0;
-                for (int j = 0; j < cluster * a.top; ++j) place += before(all[j], c);
-                if (place < a.top && c.x > -INFINITY) final[place] = c;
-            }
+            order_by_counting(all, cluster * a.top, a.top, final);
             list = final;
         }
         __syncthreads();
     }
-    __shared__ Sum result;
     if (threadIdx.x == 0) result = total;
     __syncthreads();
     total = result;
@@ -272,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobArgs
         for (int i = threadIdx.x; i < a.vocab; i += kThreads) n += x[i] == INFINITY;
         atomicAdd(&infinite, n);
         __syncthreads();
-        total.z = infinite, total.zd = 0.0;
+        total.z = infinite, total.zd = 0.0f;
     }
     const double logz = total.z > 0.0 ? log(total.z) : 0.0;
     auto log_p = [&](float v) -> float {
@@ -285,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobArgs
             const int id = a.targets[row];
             a.logprobs[row] = id >= 0 && id < a.vocab ? log_p(clean(x[id])) : 0.0f;
         }
-        if (a.entropy) a.entropy[row] = total.max == -INFINITY ? 0.0f : (float)(logz - total.zd / total.z);
+        if (a.entropy) a.entropy[row] = total.max == -INFINITY ? 0.0f : (float)(logz - (double)total.zd / total.z);
     }
     if ((int)threadIdx.x < a.top) {
         const Cand c = list[threadIdx.x];
@@ -312,9 +331,11 @@ extern "C" int strata_cuda_logprobs_dev(strata_ctx* ctx, const float* logits_dev
     if (rows == 0) return STRATA_OK;
     const LogprobArgs a{logits_dev, stride, (int)vocab, (int)top, targets_dev, logprobs_dev, entropy_dev, top_ids_dev, top_logprobs_dev};
     const bool packs = (uintptr_t)logits_dev % 16 == 0 && stride % 4 == 0;
-    // a cluster a row while that leaves multiprocessors to every block, and a share worth a block
+    // Blocks a row: two or four while every block has a multiprocessor for itself and a
+    // share that is worth it (32 rows of 151936: 18.9, 14.3 and 11.0 us with 1, 2 and 4 blocks,
+    // 13.2 with 8; 128 rows: 19.9, 21.4 and 27.6; one row of 32000: 8.4, 8.2 and 7.9)
     int cluster = 1;
-    while (cluster < kMaxCluster && rows * cluster * 2 <= ctx->sm_count && vocab >= (int64_t)cluster * 2 * kThreads * 4) cluster *= 2;
+    while (cluster < kMaxCluster && rows * cluster * 2 <= ctx->sm_count && vocab >= (int64_t)cluster * 2 * 16384) cluster *= 2;
     DeviceGuard dev(ctx->device);
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;

@@ -1,7 +1,8 @@
 """Log-probabilities, entropies and likeliest tokens (strata_cuda_logprobs_dev) against their formulas in 64 bits.
 
 Ids must be equal. Tolerances, before any run: with d = x - max (rounded at 2^-24 of itself), an f32 weight e^d is off by
-2^-22 + 2 |d| 2^-24 of itself, and what is below e^-30 of the largest does not count here: t = 2^-22 + 2^-18. Z = 1 + R:
+2^-22 + 2 |d| 2^-24 of itself, and what is below e^-30 of the largest does not count here: t = 2^-22 + 2^-18 (at the |d| of 15
+and less that sums are made of, this leaves 2^-19 for eight maxima that moved, at 2^-22 each). Z = 1 + R:
 log Z is off by t R / (1 + R), a log-probability by that and half a step of f32; the entropy is log Z - sum e d / Z, whose
 sum is off by t and 16 roundings of 2^-24: t R / (1 + R) + (2 t + 2^-20) |sum e d| / Z and half a step. Z itself is an f64 sum of
 1 and R: a thread that holds the 1 adds at most n / 512 + 4 more numbers to it and takes part in 9 joins, a rounding of 2^-53
