@@ -123,31 +123,38 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
         const KeyRange<kTile>& kr = pc.kr;
         const int head = pc.head, steps = pc.steps;
 
-        // ---- this warp's keys, kStages - 1 units ahead
-        int pages = -1;      // of unit (step & ~31) + lane
-        uint32_t none = 0;   // bit step & 31: the unit has no page
+        // ---- this warp's keys, kStages - 1 units ahead. A lane copies the same 16 bytes of
+        // every kRowsAtOnce-th row.
+        constexpr int kChunks = DP / 8, kRowsAtOnce = 32 / kChunks;
+        static_assert(kChunks <= 32, "a row is at most 32 lanes");
+        const int my_row = lane / kChunks, my_chunk = lane % kChunks;
+        const int64_t my_at = (int64_t)head * a.c.head_stride + (int64_t)my_row * a.c.token_stride + my_chunk * 8;
+        const bool my_column = my_chunk * 8 < d;
+        int64_t places = -1;  // of the first key of unit (step & ~31) + lane, its page and row there; -1: none, or not needed
+        uint32_t none = 0;    // bit step & 31: the unit has no page, or no key that a row sees
         auto load = [&](int step) {
             if (step < steps) {
                 if ((step & 31) == 0) {
-                    const int at = step + lane;
-                    const int j = at < steps ? pc.key(at) + warp * kUnit : kr.hi;
-                    pages = j < kr.hi ? page_of(a.c, b.slot, j) : -1;
+                    const int at = step + lane, j = at < steps ? pc.key(at) + warp * kUnit : kr.hi;
+                    const int page = j < kr.hi && (j + kUnit > kr.lo || j < a.sinks) ? page_of(a.c, b.slot, j) : -1;
+                    places = page >= 0 ? place(a.c, page, j, 0) : -1;
                 }
-                const int j0 = pc.key(step) + warp * kUnit;
-                const int page = __shfl_sync(0xFFFFFFFFu, pages, step & 31);
-                none = (none & ~(1u << (step & 31))) | (page < 0 ? 1u << (step & 31) : 0u);
-                uint8_t* const stage = ring + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes;
-                const int64_t at = page >= 0 ? place(a.c, page, j0, head) : 0;
-                constexpr int kChunks = DP / 8;
+                const int64_t at = __shfl_sync(0xFFFFFFFFu, places, step & 31);
+                none = (none & ~(1u << (step & 31))) | (at < 0 ? 1u << (step & 31) : 0u);
+                if (at >= 0) {
+                    const int rows = kr.hi - (pc.key(step) + warp * kUnit);  // that any row may see: behind them may be anything
+                    const __nv_bfloat16* k = a.c.k + at + my_at;
+                    const __nv_bfloat16* v = a.c.v + at + my_at;
+                    const uint32_t stage = shared_at(ring) + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes;
 #pragma unroll
-                for (int i = 0; i < kUnit * kChunks / 32; ++i) {
-                    const int row = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks, j = j0 + row;
-                    const bool ok = page >= 0 && c * 8 < d && j < kr.hi && (j >= kr.lo || j < a.sinks);
-                    const int64_t src = ok ? at + row * a.c.token_stride + c * 8 : 0;
-                    const int n = ok ? 16 : 0;  // the rest is zeros: what no row sees meets weights of zero
-                    const uint32_t dst = shared_at(stage) + chunk_at<DP>(row, c);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(a.c.k + src), "r"(n) : "memory");
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + C::kUnitBytes), "l"(a.c.v + src), "r"(n) : "memory");
+                    for (int i = 0; i < kUnit / kRowsAtOnce; ++i) {
+                        const int row = i * kRowsAtOnce + my_row;
+                        const int n = my_column && row < rows ? 16 : 0;  // the rest is zeros
+                        const uint32_t dst = stage + chunk_at<DP>(row, my_chunk);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(n ? k : a.c.k), "r"(n) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + C::kUnitBytes), "l"(n ? v : a.c.v), "r"(n) : "memory");
+                        k += kRowsAtOnce * a.c.token_stride, v += kRowsAtOnce * a.c.token_stride;
+                    }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
             __syncwarp();
             const int j0 = pc.key(step) + warp * kUnit;
             const uint32_t ks = shared_at(ring) + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes, vs = ks + C::kUnitBytes;
-            if (!(none >> (step & 31) & 1) && j0 < kr.hi && (j0 + kUnit > kr.lo || j0 < a.sinks)) {
+            if (!(none >> (step & 31) & 1)) {
                 float s[LIMBS > 1 ? 2 : 1][2][4] = {};  // the small limbs' sums apart
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
