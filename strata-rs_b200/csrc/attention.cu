@@ -35,7 +35,10 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kRows = 16;  // rows of a block
 constexpr int kUnit = 16;  // keys a warp takes of a tile
 constexpr int kTile = kWarps * kUnit;
-constexpr int kOver = 1;   // what a block of rows costs besides its tiles, in tiles
+// What a block of rows costs besides its tiles, in tiles (64 single tokens over 100 to 16000 keys
+// 165, 147, 143 and 144 us with 1, 3, 4 and 6).
+constexpr int kOver = 4;
+constexpr int kLeast = 4;  // units of a thread block at least: fewer pieces to join where there is little to read
 static_assert(kTile == 64, "a tile's keys are the warps' units");
 
 // DP: head_dim rounded up to 64, 128 or 256. Stages and blocks side by side fill
@@ -112,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int d = a.c.head_dim;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    Cut cut = cut_range<kThreads, kRows, kTile, kOver>(a, tab, entries, scan);
+    Cut cut = cut_range<kThreads, kRows, kTile, kOver, kLeast>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
     if (blockIdx.x >= cut.grid) return;
     const int64_t range_begin = cut.pos;
@@ -358,26 +361,52 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
 // Block b joins the block of rows whose first piece thread block b left.
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const Work work, const __grid_constant__ SeqTable tab) {
+    __shared__ float weight[kMaxGrid][kRows];  // of a piece's sums
+    __shared__ float part[kThreads / kRows][kRows];
     __shared__ int odd_rows[kRows];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Split s = work.split[blockIdx.x];
     if (!s.pieces) return;
     const RowBlock b = row_block(a, sequence_of_tile(tab, s.entry), s.entry, kRows);
     const int head = s.head, d = a.c.head_dim;
-    if (threadIdx.x < kRows) odd_rows[threadIdx.x] = 0;
-    __syncthreads();
     auto slot = [&](int i) { return i == 0 ? (int64_t)blockIdx.x * 2 + s.first_slot : (int64_t)(blockIdx.x + i) * 2; };
+    {
+        constexpr int kGroups = kThreads / kRows;
+        const int row = threadIdx.x % kRows, group = threadIdx.x / kRows;
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int n = group; n < s.pieces; n += kGroups) {
+            const float m = work.ml[(slot(n) * 2) * kRows + row];
+            weight[n][row] = m;
+            top = fmaxf(top, m);
+        }
+        part[group][row] = top;
+        if (threadIdx.x < kRows) odd_rows[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) top = fmaxf(top, part[i][row]);
+        __syncthreads();
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int n = group; n < s.pieces; n += kGroups) {
+            const float f = exp2_approx(weight[n][row] - base);
+            weight[n][row] = f;
+            sum = fmaf(f, work.ml[(slot(n) * 2 + 1) * kRows + row], sum);
+        }
+        part[group][row] = sum;
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < b.rows * (DP / 4); i += kThreads) {
         const int row = i / (DP / 4), c = (i % (DP / 4)) * 4;
-        float top = -INFINITY;
-        for (int n = 0; n < s.pieces; ++n) top = fmaxf(top, work.ml[(slot(n) * 2) * kRows + row]);
-        const float base = top == -INFINITY ? 0.0f : top;
+        if (c >= d) continue;
         float sum = 0.0f, x[4] = {};
-#pragma unroll 4
+#pragma unroll
+        for (int g = 0; g < kThreads / kRows; ++g) sum += part[g][row];
+#pragma unroll 8
         for (int n = 0; n < s.pieces; ++n) {
-            const float f = exp2_approx(work.ml[(slot(n) * 2) * kRows + row] - base);
+            const float f = weight[n][row];
             const float4 v = *reinterpret_cast<const float4*>(work.o + (slot(n) * kRows + row) * DP + c);
-            sum = fmaf(f, work.ml[(slot(n) * 2 + 1) * kRows + row], sum);
             x[0] = fmaf(f, v.x, x[0]), x[1] = fmaf(f, v.y, x[1]), x[2] = fmaf(f, v.z, x[2]), x[3] = fmaf(f, v.w, x[3]);
         }
         const float inv = 1.0f / sum;
@@ -387,10 +416,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const 
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             x[u] *= inv;
-            if (c + u < d) {
-                odd |= !isfinite(x[u]);
-                from_f32(static_cast<T*>(a.o)[at + u], x[u]);
-            }
+            odd |= !isfinite(x[u]);
+            from_f32(static_cast<T*>(a.o)[at + u], x[u]);
         }
         if (odd) odd_rows[row] = 1;
     }

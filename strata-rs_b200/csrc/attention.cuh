@@ -129,8 +129,8 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
     }
     return before + x - v;
 }
-// By all THREADS threads; blocks from c.grid on have none. `sh`: THREADS / 32 + 2 numbers.
-template <int THREADS, int ROWS, int TILE, int OVER>
+// By all THREADS threads; blocks from c.grid on have none, the others LEAST units or more. `sh`: THREADS / 32 + 2 numbers.
+template <int THREADS, int ROWS, int TILE, int OVER, int LEAST>
 __device__ __forceinline__ Cut cut_range(const AttnArgs& a, const SeqTable& tab, int entries, int64_t* sh) {
     Cut c;
     const int heads = a.c.n_kv_head;
@@ -142,7 +142,7 @@ __device__ __forceinline__ Cut cut_range(const AttnArgs& a, const SeqTable& tab,
         mine += cost;
     }
     block_scan<THREADS>(mine, sh, c.total);
-    c.grid = c.total < gridDim.x ? c.total : (int64_t)gridDim.x;
+    c.grid = (c.total + LEAST - 1) / LEAST < gridDim.x ? (c.total + LEAST - 1) / LEAST : (int64_t)gridDim.x;
     if (blockIdx.x >= c.grid) return c;
     c.pos = c.total * blockIdx.x / c.grid;
     c.end = c.total * (blockIdx.x + 1) / c.grid;
@@ -243,6 +243,7 @@ __device__ __noinline__ void careful_row(const AttnArgs& a, int slot, int token,
                 for (int i = 0; i < d; ++i) sum = fmaf(load_f32<T>(a.q, q + i), __bfloat162float(a.c.k[at + i]), sum);
                 s = sum * a.scale2;
             }
+            if (l != l) break;  // a NaN stays one
             const unsigned any = __ballot_sync(0xFFFFFFFFu, live);
             if (!any) continue;
             float top = s;

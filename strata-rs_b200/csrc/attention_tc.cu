@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(8) uint64_t known_full[kPieces], known_empty[kPieces];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    Cut cut = cut_range<kThreads, kRows, kKeyTile, kOver>(a, tab, entries, scan);
+    Cut cut = cut_range<kThreads, kRows, kKeyTile, kOver, 1>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
     if (blockIdx.x >= cut.grid) return;
     const int64_t range_begin = cut.pos;
