@@ -10,7 +10,9 @@
 // Rows: the r query heads of a key head share its keys, so 16 rows (tokens x r
 // heads) are one tile of the tensor cores and every key is read once for them.
 // A single token's work is then its keys and values: bound by memory, 16 to 64
-// operations a byte.
+// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 136 us, 6.2 TB/s,
+// 95% of the copy rate; one token over 4100: 16 us, launches and loads that wait on each
+// other (lengths, pages, keys, sums to join).
 //
 // The keys of all blocks of rows together (tiles of 64) are cut evenly over as
 // many blocks as run at once, however the sequences' lengths differ: a block
@@ -19,7 +21,7 @@
 // piece in the workspace, which a second kernel joins. The cut follows from the
 // lengths on the device, so that a captured call follows them.
 //
-// Each warp goes through keys of its own (16 of a tile's 64) with its own ring
+// Each group of warps (one or two) goes through keys of its own (16 of a tile's 64) with its own ring
 // of asynchronous copies, and no warp waits for another before its block's
 // range ends.
 #include <cuda_runtime.h>
@@ -31,15 +33,14 @@
 namespace strata {
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kGroups = 4;  // of warps: each goes through keys of its own
 constexpr int kRows = 16;  // rows of a block
 constexpr int kUnit = 16;  // keys a warp takes of a tile
-constexpr int kTile = kWarps * kUnit;
+constexpr int kTile = kGroups * kUnit;
 // What a block of rows costs besides its tiles, in tiles (64 single tokens over 100 to 16000 keys
-// 165, 147, 143 and 144 us with 1, 3, 4 and 6).
+// took 165, 147, 143 and 144 us with 1, 3, 4 and 6).
 constexpr int kOver = 4;
 constexpr int kLeast = 4;  // units of a thread block at least: fewer pieces to join where there is little to read
-static_assert(kTile == 64, "a tile's keys are the warps' units");
 
 // DP: head_dim rounded up to 64, 128 or 256. Stages and blocks side by side fill
 // the shared memory, so that about 128 KB a multiprocessor are under way.
@@ -47,11 +48,17 @@ template <int DP, int LIMBS>
 struct Cfg {
     static constexpr int kStages = DP == 64 ? 4 : 3;
     static constexpr int kBlocks = DP == 256 ? 1 : DP == 128 ? 2 : 3;
+    // Two warps a group share its keys where a row is long: each has half of a row's
+    // products, and the scores' halves are added through shared memory (32 single tokens
+    // of 2 key heads of 256 in f32, a window of 4096: 74 us with one warp a group, 69 with
+    // two; 64 of bf16 131, 128).
+    static constexpr int kParts = DP == 256 ? 2 : 1, kWarps = kGroups * kParts, kThreads = kWarps * 32;
     static constexpr int kUnitBytes = kUnit * DP * 2;  // of keys; as much of values
     static constexpr int kQBytes = LIMBS * kRows * DP * 2;
-    static constexpr int kRing = kWarps * kStages * 2 * kUnitBytes;
-    static constexpr int kJoin = kWarps * kRows * (DP + 2) * 4;
-    static constexpr int kSmem = kQBytes + (kRing > kJoin ? kRing : kJoin);
+    static constexpr int kRing = kGroups * kStages * 2 * kUnitBytes;
+    static constexpr int kJoin = kGroups * kRows * (DP + 2) * 4;
+    static constexpr int kHalves = kParts > 1 ? kWarps * kRows * kUnit * 4 : 0;  // scores' halves
+    static constexpr int kSmem = kQBytes + (kRing > kJoin ? kRing : kJoin) + kHalves;
     static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024, "blocks do not fit side by side");
 };
 constexpr int kMaxGrid = 148 * 3;  // blocks of a launch at most; the workspace is for as many
@@ -104,16 +111,24 @@ template <int DP>
 __device__ __forceinline__ int chunk_at(int r, int c) { return r * DP * 2 + ((c ^ (r & 7)) << 4); }
 
 template <int DP, int LIMBS, typename T>
-__global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
+__global__ void __launch_bounds__(Cfg<DP, LIMBS>::kThreads, Cfg<DP, LIMBS>::kBlocks)
     split_kernel(const AttnArgs a, const Work work, int entries, const __grid_constant__ SeqTable tab) {
     using C = Cfg<DP, LIMBS>;
+    constexpr int kWarps = C::kWarps, kThreads = C::kThreads, DH = DP / C::kParts;  // a warp's columns of a row
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const qs = smem;
     uint8_t* const ring = smem + C::kQBytes;
+    float* const halves = reinterpret_cast<float*>(smem + C::kSmem - C::kHalves);
     __shared__ int64_t scan[kWarps + 2];
     __shared__ int odd_rows[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int group = warp / C::kParts, part = warp % C::kParts;
     const int d = a.c.head_dim;
+    // the warps of a group meet
+    auto meet = [&] {
+        if (C::kParts > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(C::kParts * 32) : "memory");
+        else __syncwarp();
+    };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     Cut cut = cut_range<kThreads, kRows, kTile, kOver, kLeast>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
@@ -131,27 +146,27 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
         constexpr int kChunks = DP / 8, kRowsAtOnce = 32 / kChunks;
         static_assert(kChunks <= 32, "a row is at most 32 lanes");
         const int my_row = lane / kChunks, my_chunk = lane % kChunks;
-        const int64_t my_at = (int64_t)head * a.c.head_stride + (int64_t)my_row * a.c.token_stride + my_chunk * 8;
+        const int64_t my_at = (int64_t)head * a.c.head_stride + (int64_t)(part * (kUnit / C::kParts) + my_row) * a.c.token_stride + my_chunk * 8;
         const bool my_column = my_chunk * 8 < d;
         int64_t places = -1;  // of the first key of unit (step & ~31) + lane, its page and row there; -1: none, or not needed
         uint32_t none = 0;    // bit step & 31: the unit has no page, or no key that a row sees
         auto load = [&](int step) {
             if (step < steps) {
                 if ((step & 31) == 0) {
-                    const int at = step + lane, j = at < steps ? pc.key(at) + warp * kUnit : kr.hi;
+                    const int at = step + lane, j = at < steps ? pc.key(at) + group * kUnit : kr.hi;
                     const int page = j < kr.hi && (j + kUnit > kr.lo || j < a.sinks) ? page_of(a.c, b.slot, j) : -1;
                     places = page >= 0 ? place(a.c, page, j, 0) : -1;
                 }
                 const int64_t at = __shfl_sync(0xFFFFFFFFu, places, step & 31);
                 none = (none & ~(1u << (step & 31))) | (at < 0 ? 1u << (step & 31) : 0u);
                 if (at >= 0) {
-                    const int rows = kr.hi - (pc.key(step) + warp * kUnit);  // that any row may see: behind them may be anything
+                    const int rows = kr.hi - (pc.key(step) + group * kUnit);  // that any row may see: behind them may be anything
                     const __nv_bfloat16* k = a.c.k + at + my_at;
                     const __nv_bfloat16* v = a.c.v + at + my_at;
-                    const uint32_t stage = shared_at(ring) + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes;
+                    const uint32_t stage = shared_at(ring) + (group * C::kStages + step % C::kStages) * 2 * C::kUnitBytes;
 #pragma unroll
-                    for (int i = 0; i < kUnit / kRowsAtOnce; ++i) {
-                        const int row = i * kRowsAtOnce + my_row;
+                    for (int i = 0; i < kUnit / kRowsAtOnce / C::kParts; ++i) {
+                        const int row = (part * (kUnit / kRowsAtOnce / C::kParts) + i) * kRowsAtOnce + my_row;
                         const int n = my_column && row < rows ? 16 : 0;  // the rest is zeros
                         const uint32_t dst = stage + chunk_at<DP>(row, my_chunk);
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(n ? k : a.c.k), "r"(n) : "memory");
@@ -194,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
         if (threadIdx.x < kRows) odd_rows[threadIdx.x] = 0;
         __syncthreads();
 
-        float o[DP / 8][4] = {};
+        float o[DH / 8][4] = {};
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {};
         int p[2];  // positions of this lane's rows; rows that are none are zeros and go nowhere
 #pragma unroll
@@ -202,15 +217,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
         const int p_min = b.p0 + b.row0 / a.r, p_max = b.p0 + (b.row0 + b.rows - 1) / a.r;
 
         for (int step = 0; step < steps; ++step) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
+            meet();  // the unit is there, and the last one has been read
             load(step + C::kStages - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
-            __syncwarp();
-            const int j0 = pc.key(step) + warp * kUnit;
-            const uint32_t ks = shared_at(ring) + (warp * C::kStages + step % C::kStages) * 2 * C::kUnitBytes, vs = ks + C::kUnitBytes;
+            const int j0 = pc.key(step) + group * kUnit;
+            const uint32_t ks = shared_at(ring) + (group * C::kStages + step % C::kStages) * 2 * C::kUnitBytes, vs = ks + C::kUnitBytes;
             if (!(none >> (step & 31) & 1)) {
                 float s[LIMBS > 1 ? 2 : 1][2][4] = {};  // the small limbs' sums apart
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
+                for (int k0 = 0; k0 < DH / 16; ++k0) {
+                    const int k = part * (DH / 16) + k0;
                     uint32_t kb[4];
                     ldsm4(kb, ks + chunk_at<DP>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
 #pragma unroll
@@ -226,6 +242,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[0][n][i] += s[LIMBS > 1 ? 1 : 0][n][i];
+                if (C::kParts > 1) {  // the other half of the row's products
+                    float4* const mine = reinterpret_cast<float4*>(halves) + warp * 64 + lane;
+                    mine[0] = make_float4(s[0][0][0], s[0][0][1], s[0][0][2], s[0][0][3]);
+                    mine[32] = make_float4(s[0][1][0], s[0][1][1], s[0][1][2], s[0][1][3]);
+                    meet();  // and again before the next step's are written
+                    const float4* const other = reinterpret_cast<const float4*>(halves) + (warp ^ 1) * 64 + lane;
+                    const float4 x = other[0], y = other[32];
+                    s[0][0][0] += x.x, s[0][0][1] += x.y, s[0][0][2] += x.z, s[0][0][3] += x.w;
+                    s[0][1][0] += y.x, s[0][1][1] += y.y, s[0][1][2] += y.z, s[0][1][3] += y.w;
+                }
                 if (j0 + kUnit - 1 > p_min || (a.window && j0 <= p_max - a.window) || j0 + kUnit > kr.hi) {
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
@@ -246,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
                         const float alpha = exp2_approx(m[i] - base);
                         l[i] *= alpha;
 #pragma unroll
-                        for (int n = 0; n < DP / 8; ++n) o[n][2 * i] *= alpha, o[n][2 * i + 1] *= alpha;
+                        for (int n = 0; n < DH / 8; ++n) o[n][2 * i] *= alpha, o[n][2 * i + 1] *= alpha;
                         m[i] = next;
                     }
 #pragma unroll
@@ -270,9 +296,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
                         for (int u = 0; u < LIMBS; ++u) wa[u][2 * n + i] = x[u];
                     }
 #pragma unroll
-                for (int n = 0; n < DP / 16; ++n) {
+                for (int n = 0; n < DH / 16; ++n) {
                     uint32_t vb[4];
-                    ldsm4_t(vb, vs + chunk_at<DP>(lane & 15, 2 * n + (lane >> 4)));
+                    ldsm4_t(vb, vs + chunk_at<DP>(lane & 15, part * (DH / 8) + 2 * n + (lane >> 4)));
                     if (LIMBS == 1) {
                         mma(o[2 * n], wa[0], vb[0], vb[1]);
                         mma(o[2 * n + 1], wa[0], vb[2], vb[3]);
@@ -290,22 +316,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
                     }
                 }
             }
-            __syncwarp();  // before the stage is written again
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
 
         // ---- the warps' sums joined, in the ring's memory
         __syncthreads();
-        float* const jo = reinterpret_cast<float*>(ring);          // [kWarps][kRows][DP]
-        float* const jm = jo + kWarps * kRows * DP;                // [kWarps][2][kRows]
+        float* const jo = reinterpret_cast<float*>(ring);          // [kGroups][kRows][DP]
+        float* const jm = jo + kGroups * kRows * DP;               // [kGroups][2][kRows]
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-            if (t4 == 0) jm[(warp * 2) * kRows + g + 8 * i] = m[i], jm[(warp * 2 + 1) * kRows + g + 8 * i] = l[i];
+            if (t4 == 0 && part == 0) jm[(group * 2) * kRows + g + 8 * i] = m[i], jm[(group * 2 + 1) * kRows + g + 8 * i] = l[i];
 #pragma unroll
-            for (int n = 0; n < DP / 8; ++n)
-                *reinterpret_cast<float2*>(jo + (warp * kRows + g + 8 * i) * DP + n * 8 + 2 * t4) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            for (int n = 0; n < DH / 8; ++n)
+                *reinterpret_cast<float2*>(jo + (group * kRows + g + 8 * i) * DP + part * DH + n * 8 + 2 * t4) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
         }
         __syncthreads();
         const bool whole = pc.whole();
@@ -315,11 +340,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
             const int row = i / (DP / 4), c = (i % (DP / 4)) * 4;
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, jm[(w * 2) * kRows + row]);
+            for (int w = 0; w < kGroups; ++w) top = fmaxf(top, jm[(w * 2) * kRows + row]);
             const float base = top == -INFINITY ? 0.0f : top;
             float sum = 0.0f, x[4] = {};
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < kGroups; ++w) {
                 const float f = exp2_approx(jm[(w * 2) * kRows + row] - base);
                 const float4 v = *reinterpret_cast<const float4*>(jo + (w * kRows + row) * DP + c);
                 sum = fmaf(f, jm[(w * 2 + 1) * kRows + row], sum);
@@ -358,11 +383,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, LIMBS>::kBlocks)
     }
 }
 
+constexpr int kJoiners = 128;  // threads
+
 // Block b joins the block of rows whose first piece thread block b left.
 template <int DP, typename T>
-__global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const Work work, const __grid_constant__ SeqTable tab) {
+__global__ void __launch_bounds__(kJoiners) join_kernel(const AttnArgs a, const Work work, const __grid_constant__ SeqTable tab) {
     __shared__ float weight[kMaxGrid][kRows];  // of a piece's sums
-    __shared__ float part[kThreads / kRows][kRows];
+    __shared__ float part[kJoiners / kRows][kRows];
     __shared__ int odd_rows[kRows];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Split s = work.split[blockIdx.x];
@@ -371,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const 
     const int head = s.head, d = a.c.head_dim;
     auto slot = [&](int i) { return i == 0 ? (int64_t)blockIdx.x * 2 + s.first_slot : (int64_t)(blockIdx.x + i) * 2; };
     {
-        constexpr int kGroups = kThreads / kRows;
+        constexpr int kGroups = kJoiners / kRows;
         const int row = threadIdx.x % kRows, group = threadIdx.x / kRows;
         float top = -INFINITY;
 #pragma unroll 4
@@ -397,12 +424,12 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const 
         part[group][row] = sum;
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < b.rows * (DP / 4); i += kThreads) {
+    for (int i = threadIdx.x; i < b.rows * (DP / 4); i += kJoiners) {
         const int row = i / (DP / 4), c = (i % (DP / 4)) * 4;
         if (c >= d) continue;
         float sum = 0.0f, x[4] = {};
 #pragma unroll
-        for (int g = 0; g < kThreads / kRows; ++g) sum += part[g][row];
+        for (int g = 0; g < kJoiners / kRows; ++g) sum += part[g][row];
 #pragma unroll 8
         for (int n = 0; n < s.pieces; ++n) {
             const float f = weight[n][row];
@@ -422,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a, const 
         if (odd) odd_rows[row] = 1;
     }
     __syncthreads();
-    for (int row = threadIdx.x >> 5; row < b.rows; row += kWarps)
+    for (int row = threadIdx.x >> 5; row < b.rows; row += kJoiners / 32)
         if (odd_rows[row]) {
             const int token = (b.row0 + row) / a.r;
             careful_row<T>(a, b.slot, b.first_row + token, b.p0 + token, head * a.r + (b.row0 + row) % a.r, head);
@@ -437,7 +464,7 @@ int launch_split(strata_ctx* ctx, const AttnArgs& a, void* work, const SeqTable&
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(attention)");
     const int grid = std::min(ctx->sm_count * C::kBlocks, kMaxGrid);
     const Work w = work_of(work);
-    split_kernel<DP, LIMBS, T><<<grid, kThreads, C::kSmem, s>>>(a, w, (int)entries, tab);
+    split_kernel<DP, LIMBS, T><<<grid, C::kThreads, C::kSmem, s>>>(a, w, (int)entries, tab);
     int rc = check_launch(ctx, "attention kernel");
     if (rc) return rc;
     // launched while the first one still runs; it waits for that one's end itself
@@ -445,7 +472,7 @@ int launch_split(strata_ctx* ctx, const AttnArgs& a, void* work, const SeqTable&
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kThreads), cfg.stream = s, cfg.attrs = &at, cfg.numAttrs = 1;
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kJoiners), cfg.stream = s, cfg.attrs = &at, cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, join_kernel<DP, T>, a, w, tab);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join");
     return STRATA_OK;
@@ -536,7 +563,8 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     a.c = cache_args(c);
     a.q = q_dev, a.o = o_dev, a.q_stride = d.q_stride, a.o_stride = d.o_stride;
     a.r = (int)(d.n_head / c.n_kv_head);
-    a.window = (int)std::min(d.window, kMaxTokens), a.sinks = d.window ? (int)std::min(d.sinks, kMaxTokens) : 0;
+    a.window = d.window < c.max_pages * c.page_size ? (int)d.window : 0;  // a window over the whole table is none
+    a.sinks = a.window ? (int)std::min(d.sinks, kMaxTokens) : 0;
     a.scale = (float)d.scale, a.scale2 = (float)(d.scale * 1.4426950408889634);
     a.wide = ((uintptr_t)q_dev | (uintptr_t)o_dev) % 16 == 0 && (d.q_stride * size) % 16 == 0 && (d.o_stride * size) % 16 == 0;
     DeviceGuard dev(ctx->device);

@@ -141,7 +141,7 @@ __device__ __forceinline__ Cut cut_range(const AttnArgs& a, const SeqTable& tab,
         if (e0 == 0) first = cost;
         mine += cost;
     }
-    block_scan<THREADS>(mine, sh, c.total);
+    const int64_t prefix = block_scan<THREADS>(mine, sh, c.total);
     c.grid = (c.total + LEAST - 1) / LEAST < gridDim.x ? (c.total + LEAST - 1) / LEAST : (int64_t)gridDim.x;
     if (blockIdx.x >= c.grid) return c;
     c.pos = c.total * blockIdx.x / c.grid;
@@ -150,8 +150,8 @@ __device__ __forceinline__ Cut cut_range(const AttnArgs& a, const SeqTable& tab,
     for (int e0 = 0; e0 < entries; e0 += THREADS) {
         const int e = e0 + threadIdx.x;
         const int64_t cost = e0 == 0 ? first : e < entries ? (int64_t)cost_of<ROWS, TILE, OVER>(a, tab, e) * heads : 0;
-        int64_t sum;
-        const int64_t before = base + block_scan<THREADS>(cost, sh, sum);
+        int64_t sum = c.total, before = prefix;  // an entry a thread at most: known already
+        if (entries > THREADS) before = base + block_scan<THREADS>(cost, sh, sum);
         if (cost && c.pos >= before && c.pos < before + cost) sh[THREADS / 32] = e, sh[THREADS / 32 + 1] = before;
         base += sum;
         if (base > c.pos) break;

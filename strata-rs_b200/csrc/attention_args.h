@@ -107,7 +107,8 @@ inline int check_attention(Why& why, strata_attention& d, strata_kv_cache& c, in
         return why.refuse(STRATA_ERR_INVALID, "%lld heads on %lld key heads", (long long)d.n_head, (long long)c.n_kv_head);
     if (*longest > kMaxTokens / d.n_head) return why.refuse(STRATA_ERR_INVALID, "%lld tokens of %lld heads", (long long)*longest, (long long)d.n_head);
     if (d.window < 0 || d.sinks < 0) return why.refuse(STRATA_ERR_INVALID, "bad window %lld or sinks %lld", (long long)d.window, (long long)d.sinks);
-    if (!(std::isfinite((float)d.scale) && (float)d.scale > 0)) return why.refuse(STRATA_ERR_INVALID, "scale is not above 0");
+    if (!(std::isfinite((float)(d.scale * 1.5)) && (float)d.scale > 0))  // in powers of two it is larger
+        return why.refuse(STRATA_ERR_INVALID, "scale is not above 0, or too large");
     const int64_t row = d.n_head * c.head_dim;
     if ((rc = check_stride(why, "q_stride", d.q_stride, row, *tokens)) || (rc = check_stride(why, "o_stride", d.o_stride, row, *tokens))) return rc;
     return STRATA_OK;

@@ -172,6 +172,8 @@ static void attentions() {
     EXPECT(attention_with([](auto& d) { d.scale = -1; }) == STRATA_ERR_INVALID);
     EXPECT(attention_with([](auto& d) { d.scale = NAN; }) == STRATA_ERR_INVALID);
     EXPECT(attention_with([](auto& d) { d.scale = 1e39; }) == STRATA_ERR_INVALID);
+    EXPECT(attention_with([](auto& d) { d.scale = 3e38; }) == STRATA_ERR_INVALID);  // times log2(e) it is infinite
+    EXPECT(attention_with([](auto& d) { d.scale = 2e38; }) == STRATA_OK);
     EXPECT(attention_with([](auto& d) { d.q_stride = 100; }) == STRATA_ERR_INVALID);
     EXPECT(attention_with([](auto& d) { d.o_stride = 100; }) == STRATA_ERR_INVALID);
     EXPECT(attention_with([](auto& d) { d.dtype = STRATA_QUANT_F16; }) == STRATA_ERR_UNSUPPORTED_QUANT);
