@@ -257,10 +257,11 @@ __device__ __noinline__ void careful_row(const AttnArgs& a, int slot, int token,
             m = next;
             l *= alpha;
             for (int i = 0; i < 8; ++i) o[i] *= alpha;
-            for (unsigned left = any; left; left &= left - 1) {
-                const int from = __ffs(left) - 1;
+#pragma unroll 8
+            for (int from = 0; from < 32; ++from) {
                 const float w = __shfl_sync(0xFFFFFFFFu, e, from);
                 const int64_t row = __shfl_sync(0xFFFFFFFFu, at, from);
+                if (!(any >> from & 1)) continue;
                 l += w;
                 for (int i = 0; i < 8; ++i)
                     if (lane + 32 * i < d) o[i] = fmaf(w, __bfloat162float(a.c.v[row + lane + 32 * i]), o[i]);

@@ -97,7 +97,8 @@ __device__ __forceinline__ bool bar_try(uint32_t b, uint32_t par) {
     asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(b), "r"(par) : "memory");
     return ok != 0;
 }
-// Waits for the phase of parity `par`; false, and *err set, after about a second.
+// Waits for the phase of parity `par`; false, and *err set, after about 20 seconds: warps
+// wait while others compute rows again that are not finite, over contexts of any length.
 // (In line: a call would keep the compiler from giving warps registers of others.)
 __device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t par, int* err) {
     uint64_t t0 = 0;
@@ -107,7 +108,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t par, int* err) {
         if ((i & 15) == 15) {
             const uint64_t t = now_ns();
             if (!t0) t0 = t;
-            else if (t - t0 > 1000000000ull) break;
+            else if (t - t0 > 20000000000ull) break;
         }
     }
     atomicExch(err, 1);

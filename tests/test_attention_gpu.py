@@ -182,6 +182,37 @@ def test_many_sequences(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_chunks(ctx, dtype):
+    """More sequences than a launch holds, each long enough for tiles of rows; and as many of one length."""
+    n = 260
+    Case([16 + i % 9 for i in range(n)], [(i * 53) % 150 for i in range(n)], 4, 1, 64, 16, dtype).check(ctx)
+    Case([50] * 7, [0, 1, 77, 78, 200, 300, 13], 8, 2, 128, 32, dtype, uniform=50).check(ctx)
+
+
+@pytest.mark.parametrize("heads", [(20, 1, 72), (64, 1, 16), (7, 7, 104), (3, 1, 128)], ids=str)
+def test_chunks_of_other_heads(ctx, heads):
+    hq, hkv, d = heads
+    Case([40, 1, 200], [100, 5, 0], hq, hkv, d, 16, "bf16").check(ctx)
+    Case([40, 1, 200], [100, 5, 0], hq, hkv, d, 64, "bf16", window=77, sinks=20).check(ctx)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 3.3e38])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(ctx, value, dtype):
+    for n in (1, 150):
+        c = Case([n, n], [30, 200], 4, 2, 64, 16, dtype)
+        want, tol = c.want()
+        c.q[n - 1, 1, 5] = value
+        c.run(ctx)
+        torch.cuda.synchronize()
+        got = c.obuf[: c.total].unflatten(1, (4, 64)).double()
+        others = torch.ones(c.total, 4, dtype=torch.bool, device="cuda")
+        others[n - 1, 1] = False
+        assert ((got - want).abs() <= tol)[others].all()
+        assert torch.isnan(got[n - 1, 1]).all() or math.isfinite(value)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_rows_between_and_behind_the_sequences_stay(ctx, dtype):
     Case([2, 3, 1], [4, 0, 9], 2, 2, 32, 16, dtype, offsets=[5, 7, 10, 11]).check(ctx)
 
