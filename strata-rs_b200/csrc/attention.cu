@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(Cfg<DP, LIMBS>::kThreads, Cfg<DP, LIMBS>::kBlo
         if (C::kParts > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(C::kParts * 32) : "memory");
         else __syncwarp();
     };
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    after_previous();
     Cut cut = cut_range<kThreads, kRows, kTile, kOver, kLeast>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
     if (blockIdx.x >= cut.grid) return;
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kJoiners) join_kernel(const AttnArgs a, const 
     __shared__ float weight[kMaxGrid][kRows];  // of a piece's sums
     __shared__ float part[kJoiners / kRows][kRows];
     __shared__ int odd_rows[kRows];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous(false);
     const Split s = work.split[blockIdx.x];
     if (!s.pieces) return;
     const RowBlock b = row_block(a, sequence_of_tile(tab, s.entry), s.entry, kRows);
@@ -464,18 +464,10 @@ int launch_split(strata_ctx* ctx, const AttnArgs& a, void* work, const SeqTable&
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaFuncSetAttribute(attention)");
     const int grid = std::min(ctx->sm_count * C::kBlocks, kMaxGrid);
     const Work w = work_of(work);
-    split_kernel<DP, LIMBS, T><<<grid, C::kThreads, C::kSmem, s>>>(a, w, (int)entries, tab);
-    int rc = check_launch(ctx, "attention kernel");
-    if (rc) return rc;
-    // launched while the first one still runs; it waits for that one's end itself
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kJoiners), cfg.stream = s, cfg.attrs = &at, cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, join_kernel<DP, T>, a, w, tab);
-    if (e != cudaSuccess) return cuda_fail(ctx, e, "attention join");
-    return STRATA_OK;
+    e = launch_early(split_kernel<DP, LIMBS, T>, dim3(grid), C::kThreads, C::kSmem, s, a, w, (int)entries, tab);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "attention kernel");
+    e = launch_early(join_kernel<DP, T>, dim3(grid), kJoiners, 0, s, a, w, tab);
+    return e == cudaSuccess ? STRATA_OK : cuda_fail(ctx, e, "attention join");
 }
 
 template <int DP>

@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Known known[kPieces];
     __shared__ __align__(8) uint64_t known_full[kPieces], known_empty[kPieces];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    after_previous();
     Cut cut = cut_range<kThreads, kRows, kKeyTile, kOver, 1>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
     if (blockIdx.x >= cut.grid) return;
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int DP>
 __global__ void __launch_bounds__(128) tc_join_kernel(const AttnArgs a, const TcWork work, const __grid_constant__ SeqTable tab) {
     __shared__ int odd_rows[32];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous(false);
     const Split s = work.split[blockIdx.x];
     if (!s.pieces) return;
     const RowBlock b = row_block(a, sequence_of_tile(tab, s.entry), s.entry, kRows);
@@ -725,15 +725,9 @@ int launch(strata_ctx* ctx, const AttnArgs& a, void* work, const SeqTable& tab, 
     const TcWork w = work_of(work);
     CUtensorMap k, v;
     memcpy(&k, maps.k, sizeof k), memcpy(&v, maps.v, sizeof v);
-    tc_kernel<DP><<<grid, kThreads, Cfg<DP>::kSmem, s>>>(a, w, (int)entries, ctx->err_dev, Boxes{maps.box_rows, maps.inside}, k, v, tab);
-    const int rc = check_launch(ctx, "attention kernel");
-    if (rc) return rc;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, kRows / 32), cfg.blockDim = dim3(128), cfg.stream = s, cfg.attrs = &at, cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, tc_join_kernel<DP>, a, w, tab);
+    e = launch_early(tc_kernel<DP>, dim3(grid), kThreads, Cfg<DP>::kSmem, s, a, w, (int)entries, ctx->err_dev, Boxes{maps.box_rows, maps.inside}, k, v, tab);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "attention kernel");
+    e = launch_early(tc_join_kernel<DP>, dim3(grid, kRows / 32), 128, 0, s, a, w, tab);
     return e == cudaSuccess ? STRATA_OK : cuda_fail(ctx, e, "attention join");
 }
 

@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(const AppendArgs a,
     __shared__ float2 turn[kMaxTable];
     __shared__ int64_t places[kMaxTokensABlock];  // of the tokens in the pools, head 0; -1: none
     const Seq seq = sequence_of_tile(tab, blockIdx.x);
+    after_previous();
     const int t0 = (blockIdx.x - seq.tile0) * a.tokens, n = min(a.tokens, seq.len - t0);
     const int raw = a.c.len[seq.slot], p0 = (raw > 0 ? raw : 0) - seq.len + t0;  // the first token's position
     const int d = a.c.head_dim, kv = a.c.n_kv_head, reach = a.c.max_pages * a.c.page_size;
@@ -142,15 +143,15 @@ __global__ void __launch_bounds__(kThreads, 5) append_kernel(const AppendArgs a,
 }
 
 template <typename TI, typename TQ, int VEC>
-void launch(dim3 grid, const AppendArgs& a, const SeqTable& t, cudaStream_t s) {
-    if (a.neighbours) append_kernel<TI, TQ, VEC, true><<<grid, kThreads, 0, s>>>(a, t);
-    else append_kernel<TI, TQ, VEC, false><<<grid, kThreads, 0, s>>>(a, t);
+cudaError_t launch(dim3 grid, const AppendArgs& a, const SeqTable& t, cudaStream_t s) {
+    if (a.neighbours) return launch_early(append_kernel<TI, TQ, VEC, true>, grid, kThreads, 0, s, a, t);
+    return launch_early(append_kernel<TI, TQ, VEC, false>, grid, kThreads, 0, s, a, t);
 }
 template <typename TI, typename TQ>
-void launch(int vec, dim3 grid, const AppendArgs& a, const SeqTable& t, cudaStream_t s) {
-    if (vec == 8) launch<TI, TQ, 8>(grid, a, t, s);
-    else if (vec == 4) launch<TI, TQ, 4>(grid, a, t, s);
-    else launch<TI, TQ, 1>(grid, a, t, s);
+cudaError_t launch(int vec, dim3 grid, const AppendArgs& a, const SeqTable& t, cudaStream_t s) {
+    if (vec == 8) return launch<TI, TQ, 8>(grid, a, t, s);
+    if (vec == 4) return launch<TI, TQ, 4>(grid, a, t, s);
+    return launch<TI, TQ, 1>(grid, a, t, s);
 }
 
 }  // namespace
@@ -193,10 +194,10 @@ extern "C" int strata_cuda_kv_append_dev(strata_ctx* ctx, const strata_kv_append
         if (tiles > kMaxTokens) return fail(ctx, STRATA_ERR_INVALID, "kv_append: %lld tiles", (long long)tiles);
         const int64_t share = std::max<int64_t>(1, std::min<int64_t>(4, fill / tiles));
         const dim3 grid((unsigned)tiles, (unsigned)share);
-        if (bi && bq) launch<__nv_bfloat16, __nv_bfloat16>(vec, grid, a, t, s);
-        else if (bi) launch<__nv_bfloat16, float>(vec, grid, a, t, s);
-        else if (bq) launch<float, __nv_bfloat16>(vec, grid, a, t, s);
-        else launch<float, float>(vec, grid, a, t, s);
-        return check_launch(ctx, "kv_append kernel");
+        const cudaError_t e = bi && bq ? launch<__nv_bfloat16, __nv_bfloat16>(vec, grid, a, t, s)
+                              : bi     ? launch<__nv_bfloat16, float>(vec, grid, a, t, s)
+                              : bq     ? launch<float, __nv_bfloat16>(vec, grid, a, t, s)
+                                       : launch<float, float>(vec, grid, a, t, s);
+        return e == cudaSuccess ? STRATA_OK : cuda_fail(ctx, e, "kv_append kernel");
     });
 }

@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const LogprobArgs
     if (threadIdx.x == 0) n_cand = n_reach = infinite = 0;
     if (threadIdx.x < kTop) best[threadIdx.x] = Cand{-INFINITY, -1}, final[threadIdx.x] = Cand{-INFINITY, -1};
 
+    after_previous();
+
     // ---- the pass
     Sum s = {-INFINITY, 0.0f, 0.0};
     auto load = [&](int i, float (&v)[16]) {  // a batch: kBatch packs, kStep apart
@@ -337,12 +339,14 @@ extern "C" int strata_cuda_logprobs_dev(strata_ctx* ctx, const float* logits_dev
     int cluster = 1;
     while (cluster < kMaxCluster && rows * cluster * 2 <= ctx->sm_count && vocab >= (int64_t)cluster * 2 * 16384) cluster *= 2;
     DeviceGuard dev(ctx->device);
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = cluster, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster)), cfg.blockDim = dim3(kThreads), cfg.stream = pick_stream(ctx, stream);
-    cfg.attrs = &at, cfg.numAttrs = cluster > 1 ? 1 : 0;
+    cfg.attrs = at, cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = packs ? cudaLaunchKernelEx(&cfg, logprobs_kernel<true>, a, cluster) : cudaLaunchKernelEx(&cfg, logprobs_kernel<false>, a, cluster);
     return e == cudaSuccess ? STRATA_OK : cuda_fail(ctx, e, "logprobs kernel");
 }
