@@ -10,8 +10,8 @@
 // Rows: the r query heads of a key head share its keys, so 16 rows (tokens x r
 // heads) are one tile of the tensor cores and every key is read once for them.
 // A single token's work is then its keys and values: bound by memory, 16 to 64
-// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 136 us, 6.2 TB/s,
-// 95% of the copy rate; one token over 4100: 16 us, launches and loads that wait on each
+// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 136 to 140 us,
+// 6.0 to 6.2 TB/s, 92 to 95% of the copy rate; one token over 4100: 16 us, launches and loads that wait on each
 // other (lengths, pages, keys, sums to join).
 //
 // The keys of all blocks of rows together (tiles of 64) are cut evenly over as
