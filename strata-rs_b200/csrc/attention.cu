@@ -507,8 +507,14 @@ int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, i
     return t.n ? launch(t, entries) : STRATA_OK;
 }
 
-// Rows a key head from which a sequence goes to the tensor cores' tiles of 128.
-constexpr int64_t kTcRows = 64;
+// A sequence of kTcRows rows a key head goes to the tiles of 128 rows where the call has
+// kTcAll such rows and key heads together. Measured, tiles against 16 rows at a time (us,
+// heads of 128 behind 8000 keys, 4 query heads a key head): 16 sequences on 8 key heads
+// with 16 rows 128, 101, with 32 rows 130, 179, with 256 rows 154, 1200; one sequence
+// with 64 rows (512 in all) 65, 33, with 128 (1024) 67, 47, with 256 (2048) 72, 69; 16 sequences
+// of 8 query heads on one key head with 64 rows (1024) 58, 47, with 128 (2048) 60, 69; one
+// sequence of those with 512 rows 165, 32.
+constexpr int64_t kTcRows = 32, kTcAll = 2048;
 
 bool tiles(const strata_attention& d, const strata_kv_cache& c) { return d.dtype == STRATA_QUANT_BF16 && c.head_dim <= 128; }
 int padded(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -561,14 +567,22 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     a.wide = ((uintptr_t)q_dev | (uintptr_t)o_dev) % 16 == 0 && (d.q_stride * size) % 16 == 0 && (d.o_stride * size) % 16 == 0;
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);
-    int64_t many = kMaxTokens;  // tokens from which a sequence is read in tiles
+    int64_t many = kMaxTokens + 1;  // tokens from which a sequence is read in tiles
     TcMaps maps;
-    if (tiles(d, c) && a.wide && longest * a.r >= kTcRows && attention_tc_maps(a.c, &maps)) {
-        many = (kTcRows + a.r - 1) / a.r;
-        rc = for_row_groups(ctx, d, a.r, attention_tc_rows(), many, kMaxTokens + 1, [&](const SeqTable& t, int64_t entries) {
-            return launch_attention_tc(ctx, dp, a, work_dev, t, entries, maps, s);
-        });
-        if (rc) return rc;
+    const int64_t enough = (kTcRows + a.r - 1) / a.r;
+    if (tiles(d, c) && a.wide && longest >= enough) {
+        int64_t all = d.seq_offsets ? 0 : d.n_seq * d.seq_len;
+        for (int64_t i = 0; d.seq_offsets && i < d.n_seq && all < kTcAll; ++i) {
+            const int64_t n = d.seq_offsets[i + 1] - d.seq_offsets[i];
+            if (n >= enough) all += n;
+        }
+        if (all * d.n_head >= kTcAll && attention_tc_maps(a.c, &maps)) {
+            many = enough;
+            rc = for_row_groups(ctx, d, a.r, attention_tc_rows(), many, kMaxTokens + 1, [&](const SeqTable& t, int64_t entries) {
+                return launch_attention_tc(ctx, dp, a, work_dev, t, entries, maps, s);
+            });
+            if (rc) return rc;
+        }
     }
     return for_row_groups(ctx, d, a.r, kRows, 1, many, [&](const SeqTable& t, int64_t entries) {
         if (dp == 64) return launch_split<64>(ctx, bf16, a, work_dev, t, entries, s);

@@ -48,6 +48,7 @@ constexpr int kRows = 2 * kRowTile;
 constexpr int kThreads = 384;  // three warpgroups, which registers are shared out by
 constexpr int kRegs = 208, kRegsRest = 88;  // 2 x 208 + 88 = 3 x 168, what the block is launched with
 constexpr int kOver = 6;       // what a block of rows costs besides its tiles, in tiles (8 or 4: a prompt of 8192 501, 519 us, not 488)
+constexpr int kLeast = 4;      // units of a thread block at least: fewer pieces to join where there is little to do
 constexpr int kMaxGrid = 148;
 constexpr int kMasks = 8;   // tiles whose masks are kept
 constexpr int kPieces = 8;  // pieces that are known ahead
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(8) uint64_t known_full[kPieces], known_empty[kPieces];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     after_previous();
-    Cut cut = cut_range<kThreads, kRows, kKeyTile, kOver, 1>(a, tab, entries, scan);
+    Cut cut = cut_range<kThreads, kRows, kKeyTile, kOver, kLeast>(a, tab, entries, scan);
     if (threadIdx.x == 0) work.split[blockIdx.x].pieces = 0;
     if (blockIdx.x >= cut.grid) return;
     const int64_t range_begin = cut.pos;

@@ -181,6 +181,60 @@ def test_many_sequences(ctx, dtype):
     Case([i % 3 for i in range(n)], past, 2, 1, 64, 16, dtype).check(ctx)
 
 
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 3), (64, 4), (100, 65), (129, 200), (1 << 40, 1)])
+def test_windows_in_tiles(ctx, window, sinks):
+    """As test_windows, with rows enough for the tiles of 128 rows, one sequence with a single tile of them."""
+    Case([1, 1, 190, 33, 430], [0, 900, 100, 1500, 64], 9, 3, 64, 16, "bf16", window, sinks).check(ctx)
+    Case([333, 20], [700, 0], 8, 2, 128, 48, "bf16", window, sinks).check(ctx)
+
+
+def test_lengths_and_pages_in_tiles(ctx):
+    n = 300
+    c = Case([n, n, n, n], [3, 0, 0, 50], 4, 2, 64, 16, "bf16")
+    c.len.copy_(torch.tensor([n // 2, 0, -5, n + 50]))
+    c.check(ctx)
+    c = Case([n, n, n], [400, 400, 300], 4, 2, 128, 16, "bf16")
+    c.table[0, 3], c.table[0, 7], c.table[0, 8] = -1, c.pages, -(2 ** 31)
+    c.table[1, :] = 2 ** 31 - 1
+    c.check(ctx)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_what_a_row_does_not_see_in_tiles(ctx, value):
+    n, past = 700, 200
+    for window, at in ((0, past + 400), (300, 20)):
+        c = Case([n], [past], 4, 2, 64, 32, "bf16", window, 3 if window else 0)
+        where = c.table[0, at // 32].long(), at % 32
+        clean_k, clean_v = c.k[where].clone(), c.v[where].clone()
+        want, tol = c.want()
+        p = torch.arange(past, past + n, device="cuda")
+        blind = (at > p) | (p - at >= window) if window else at > p
+        for pool in (c.k, c.v):
+            pool[where] = value
+            c.run(ctx)
+            torch.cuda.synchronize()
+            got = c.obuf[:n, :4 * 64].unflatten(1, (4, 64)).double()
+            assert blind.any() and ((got - want).abs() <= tol)[blind].all()
+            if pool is c.v and not blind.all():
+                assert not torch.isfinite(got[~blind]).any(-1).any()
+            c.k[where], c.v[where] = clean_k, clean_v
+    c = Case([n], [past], 4, 2, 64, 32, "bf16")
+    want, tol = c.want()
+    c.q[n - 1, 1, 5] = value
+    c.run(ctx)
+    got = c.obuf[:n].unflatten(1, (4, 64)).double()
+    others = torch.ones(n, 4, dtype=torch.bool, device="cuda")
+    others[n - 1, 1] = False
+    assert ((got - want).abs() <= tol)[others].all() and torch.isnan(got[n - 1, 1]).all()
+
+
+@pytest.mark.parametrize("lens,heads", [([512], (8, 1)), ([255], (8, 1)), ([40, 40], (32, 8)), ([17], (64, 4)), ([2100], (1, 1))], ids=str)
+def test_few_blocks_of_rows_in_many_pieces(ctx, lens, heads):
+    """One block of rows' keys cut over as many thread blocks as there are, behind long contexts."""
+    Case(lens, [9000] * len(lens), *heads, 128, 64, "bf16").check(ctx)
+    Case(lens, [3000] * len(lens), *heads, 72, 16, "bf16").check(ctx)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_many_chunks(ctx, dtype):
     """More sequences than a launch holds, each long enough for tiles of rows; and as many of one length."""
