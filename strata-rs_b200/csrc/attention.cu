@@ -561,7 +561,8 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     a.c = cache_args(c);
     a.q = q_dev, a.o = o_dev, a.q_stride = d.q_stride, a.o_stride = d.o_stride;
     a.r = (int)(d.n_head / c.n_kv_head);
-    a.window = d.window < c.max_pages * c.page_size ? (int)d.window : 0;  // a window over the whole table is none
+    // over all positions (2^31 - 1 at most) it is none; over the table's it is one for tokens behind the table
+    a.window = d.window < kMaxTokens ? (int)d.window : 0;
     a.sinks = a.window ? (int)std::min(d.sinks, kMaxTokens) : 0;
     a.scale = (float)d.scale, a.scale2 = (float)(d.scale * 1.4426950408889634);
     a.wide = ((uintptr_t)q_dev | (uintptr_t)o_dev) % 16 == 0 && (d.q_stride * size) % 16 == 0 && (d.o_stride * size) % 16 == 0;

@@ -370,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int steps = kn.piece.steps;
             const int p = kn.piece.b.p0 + min(kn.piece.b.row0 + t * kRowTile + row, kn.piece.b.row0 + kn.piece.b.rows - 1) / a.r;
             const int p_min = __shfl_sync(0xFFFFFFFFu, p, 0), p_max = __shfl_sync(0xFFFFFFFFu, p, 31);
+            const int hidden = a.window && p_max >= a.window ? p_max - a.window : -1;  // the last key that the window takes from some row
             m = -INFINITY, l = 0.0f;
             for (int j = 0; j < steps; ++j, ++tiles, ++done) {
                 live = __all_sync(0xFFFFFFFFu, bar_wait(shared_at(&s_full[t]), done & 1, err));
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) bar_arrive(shared_at(&s_free[t]));
                 const int base = kn.piece.key(j);
                 const uint32_t valid = masks[tiles % kMasks];
-                const bool masked = valid != 0xFF || base + kKeyTile - 1 > p_min || (a.window && base <= p_max - a.window);
+                const bool masked = valid != 0xFF || base + kKeyTile - 1 > p_min || base <= hidden;
                 if (masked) {
                     // bit c of the row: it sees key base + c
                     const int to = p - base, from = a.window && a.window <= to ? to - a.window + 1 : 0, sinks = a.sinks - base;
