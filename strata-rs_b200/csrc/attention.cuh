@@ -3,6 +3,7 @@
 // from the formula alone.
 #pragma once
 #include "attention_args.h"
+#include "attention_keys.h"
 #include "sequence.cuh"
 
 namespace strata {
@@ -71,29 +72,11 @@ __device__ __forceinline__ RowBlock row_block(const AttnArgs& a, const Seq& s, i
     return b;
 }
 
-// The keys that some row of a block sees: [0, sink) and [lo, hi); in tiles of
-// TILE keys, first those of the sinks, then those from lo on.
-template <int TILE>
-struct KeyRange {
-    int lo, hi, sink_tiles, tiles;
-    __device__ __forceinline__ int key(int tile) const {
-        return (tile < sink_tiles ? tile : lo / TILE + (tile - sink_tiles)) * TILE;
-    }
-};
 template <int TILE>
 __device__ __forceinline__ KeyRange<TILE> key_range(const AttnArgs& a, int p_min, int p_max) {
-    KeyRange<TILE> k;
-    const int cap = a.c.max_pages * a.c.page_size;  // below 2^31
-    k.hi = p_max < cap ? p_max + 1 : cap;
-    if (k.hi < 0) k.hi = 0;
-    k.lo = a.window && p_min >= a.window ? p_min - a.window + 1 : 0;
-    if (k.lo > k.hi) k.lo = k.hi;
-    const int sink = a.sinks < k.lo ? a.sinks : k.lo, first = k.lo / TILE;
-    k.sink_tiles = (sink + TILE - 1) / TILE;
-    if (k.sink_tiles > first) k.sink_tiles = first;  // the rest lies in lo's own tile
-    k.tiles = k.sink_tiles + (k.hi + TILE - 1) / TILE - first;
-    return k;
+    return key_range<TILE>(a.window, a.sinks, a.c.max_pages * a.c.page_size, p_min, p_max);
 }
+// The keys that some row of a block sees.
 template <int TILE>
 __device__ __forceinline__ KeyRange<TILE> key_range(const AttnArgs& a, const RowBlock& b) {
     return key_range<TILE>(a, b.p0 + b.row0 / a.r, b.p0 + (b.row0 + b.rows - 1) / a.r);

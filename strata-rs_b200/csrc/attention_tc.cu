@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int len = pc.b.p0 + pc.b.n, steps = pc.steps, head = pc.head;
                 // lane g: the page of keys 16 g .. 16 g + 15, a tile ahead
                 auto page_at = [&](int j) {
-                    const int key = j < steps ? pc.key(j) + 16 * lane : pc.kr.hi;
+                    const int key = j < steps ? pc.key(j) + 16 * (lane & 7) : pc.kr.hi;  // below 2^31: a tile ends at 2^31 at most
                     return lane < 8 && key < pc.kr.hi ? page_of(a.c, pc.b.slot, key) : -1;
                 };
                 int page = page_at(0);
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     live = __all_sync(0xFFFFFFFFu, live);
                     if (!live) break;
                     // the last tokens' page goes on behind them with whatever is there: values of zero instead
-                    const bool patch = !keys && len >= base && len < base + kKeyTile && len % box.rows;
+                    const bool patch = !keys && len >= base && len - base < kKeyTile && len % box.rows;
                     const uint32_t bar = shared_at(patch ? &landed : &full[to.slot]), dst = shared_at(ring) + to.slot * C::kTileBytes;
                     if (lane == 0) bar_expect(bar, C::kTileBytes);
                     __syncwarp();

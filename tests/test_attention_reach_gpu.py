@@ -1,7 +1,9 @@
-"""Attention (strata_cuda_attention_dev) of tokens behind the table's reach: their positions have no place, and what they see
-of the positions that have is the mask's, as everywhere. The cases, the formula in 64 bits and the tolerances are
+"""Attention (strata_cuda_attention_dev) of tokens at and behind the table's reach: positions behind it have no place, and what
+tokens there see of the positions that have is the mask's, as everywhere. The cases, the formula in 64 bits and the tolerances are
 test_attention_gpu.py's."""
 import pytest
+
+import strata_cuda as sc
 
 from test_attention_gpu import Case, ctx, torch  # noqa: F401
 
@@ -39,3 +41,21 @@ def test_the_last_positions_of_all(ctx, window, dtype):  # noqa: F811
     behind(Case([1, 20], [63, 44], 4, 2, 64, 16, dtype, window, 0, width=4), [(1 << 31) - 1] * 2).check(ctx)
     if dtype == "bf16":
         behind(Case([600, 600], [104, 104], 4, 2, 64, 16, dtype, window, 0, width=44), [(1 << 31) - 1, 5]).check(ctx)
+
+
+@pytest.mark.parametrize("lens,past,window,dtype", [([1], 639, 0, "bf16"), ([1], 639, 200, "bf16"), ([1], 634, 200, "f32"), ([30], 610, 200, "f32"), ([600], 360, 300, "bf16"),
+                                                    ([600], 355, 300, "bf16")], ids=str)
+def test_the_largest_table(ctx, lens, past, window, dtype):  # noqa: F811
+    """The largest reach there is, 2^31 - 16 positions in pages of 16, whose last pages hold the sequence (the others are none):
+    tiles that end at 2^31. What is seen is as behind `past` tokens, and so is the result."""
+    width = (1 << 27) - 1
+    c = Case(lens, [past], 4, 2, 64, 16, dtype, window)
+    want, tol = c.want()
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, width - c.width:] = c.table[0]
+    c.len.add_((width - c.width) * 16)
+    c.cache = sc.KvCache(c.k.data_ptr(), c.v.data_ptr(), table.data_ptr(), c.len.data_ptr(), n_pages=c.pages, page_size=16, n_kv_head=2, head_dim=64, max_pages=width)
+    c.run(ctx)
+    torch.cuda.synchronize()
+    got = c.obuf[: c.total].unflatten(1, (4, 64)).double()
+    assert ((got - want).abs() <= tol).all()
