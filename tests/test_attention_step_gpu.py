@@ -161,6 +161,39 @@ def test_one_chunk_or_several_give_the_same(ctx):
         assert (o - outs[0][0]).abs().max() <= 0.05 * outs[0][0].abs().max()
 
 
+def test_one_chunk_or_several_give_the_same_log_probabilities(ctx):
+    """The last token's log-probability after a prompt read whole and in pieces. With |.| element by element and the products'
+    own tolerances (1e-2 of the largest output at most, on either side): y differs by |W_out| |do| + 2e-2 max |y|, the logits x by
+    |W_head| |dy| + 2e-2 max |x|, and a log-probability by |dx| of its token and the largest |dx| (the logarithm of a mean of
+    exponentials moves by no more than they do), besides what each may be off from its own logits."""
+    rng = np.random.default_rng(5)
+    tokens = torch.from_numpy(rng.integers(0, VOCAB, 120)).cuda()
+    outs = []
+    for pieces in ([120], [64, 56], [100, 19, 1]):
+        layer, at = Layer(ctx, 1, sc.F32, 0), 0
+        for n in pieces:
+            b = layer.buffers([n])
+            part = tokens[at:at + n]
+            layer.step(b, part, part.int())
+            at += n
+        torch.cuda.synchronize()
+        outs.append({x: b[x][-1].double() for x in ("o", "y", "logits", "lp")})
+    out, head, target, first = layer.data["out"][1].abs(), layer.data["head"][1].abs(), int(tokens[-1]), outs[0]
+
+    def own(x):  # how far log p may be off from the logits it was computed from
+        lp0, _, _, _, tl, _ = lp.expected(x["logits"].float().cpu().numpy(), target, 0)
+        assert abs(float(x["lp"]) - lp0) <= tl + 2.0 ** -24 * abs(lp0)
+        return tl + 2.0 ** -24 * abs(lp0)
+
+    for x in outs[1:]:
+        dy = out @ (x["o"] - first["o"]).abs() + 2e-2 * torch.maximum(x["y"].abs().max(), first["y"].abs().max())
+        assert ((x["y"] - first["y"]).abs() <= dy).all()
+        dx = head @ (x["y"] - first["y"]).abs() + 2e-2 * torch.maximum(x["logits"].abs().max(), first["logits"].abs().max())
+        moved = (x["logits"] - first["logits"]).abs()
+        assert (moved <= dx).all()
+        assert abs(float(x["lp"] - first["lp"])) <= float(moved[target] + moved.max()) + own(x) + own(first)
+
+
 @pytest.mark.parametrize("mid", [sc.F32, sc.BF16], ids=["f32", "bf16"])
 def test_a_captured_step_gives_what_the_calls_give(ctx, mid):
     """Ten tokens of three sequences, each the last one's draw, by calls and by a captured graph that grows the lengths: the same bits."""
