@@ -71,7 +71,8 @@ typedef struct {
  * (same type and stride) where nothing else overlaps. n_head 0: there are no
  * queries, and q and q_out may be NULL. Queries of tokens without a place are
  * rotated all the same (a negative position counts as it is). No two tokens of
- * a call may have the same place. */
+ * a call may have the same place, and no key's row may share elements with a
+ * value's (pools that do are refused). */
 typedef struct {
     int64_t n_seq;
     int64_t seq_len;            /* tokens of every sequence when seq_offsets is NULL */

@@ -59,6 +59,28 @@ inline int check_kv_cache_buffers(Why& why, const strata_kv_cache& c) {
     return STRATA_OK;
 }
 
+// Whether a key's and a value's row share elements (strides resolved: rows of a pool
+// share none). The pools are apart by a number of pages, of rows of the outer stride and
+// of the inner one, each known up to one, and a rest below a row.
+inline bool pools_share(const strata_kv_cache& c) {
+    const int64_t apart = (int64_t)((uintptr_t)c.v_dev - (uintptr_t)c.k_dev) / 2;
+    const bool inside = c.token_stride >= (c.n_kv_head - 1) * c.head_stride + c.head_dim;
+    const int64_t stride[] = {c.page_stride, inside ? c.token_stride : c.head_stride, inside ? c.head_stride : c.token_stride};
+    const int64_t count[] = {c.n_pages, inside ? c.page_size : c.n_kv_head, inside ? c.n_kv_head : c.page_size};
+    for (int up = 0; up < 8; ++up) {
+        int64_t rest = apart;
+        bool near = true;
+        for (int i = 0; i < 3; ++i) {
+            int64_t n = rest / stride[i] - (rest % stride[i] < 0);  // rounded down
+            n += up >> i & 1;
+            near &= n > -count[i] && n < count[i];
+            rest -= n * stride[i];
+        }
+        if (near && rest > -c.head_dim && rest < c.head_dim) return true;
+    }
+    return false;
+}
+
 // Resolves packed strides in `d` and `c`.
 inline int check_kv_append(Why& why, strata_kv_append& d, strata_kv_cache& c, int64_t* tokens, int64_t* longest) {
     int rc;
@@ -82,6 +104,7 @@ inline int check_kv_append_buffers(Why& why, const strata_kv_append& d, const st
     const int64_t b = dtype_bytes(d.dtype), ob = dtype_bytes(d.q_dtype);
     if ((rc = check_kv_cache_buffers(why, c)) || (rc = check_aligned(why, "k", k, b)) || (rc = check_aligned(why, "v", v, b))) return rc;
     if (d.n_head && ((rc = check_aligned(why, "q", q, b)) || (rc = check_aligned(why, "q_out", q_out, ob)))) return rc;
+    if (pools_share(c)) return why.refuse(STRATA_ERR_INVALID, "the keys' pool overlaps the values' pool");
     const int64_t qr = d.n_head * c.head_dim, kvr = c.n_kv_head * c.head_dim;
     const Rows in[] = {{"k", k, kvr * b, d.k_stride * b, tokens},
                        {"v", v, kvr * b, d.v_stride * b, tokens},
