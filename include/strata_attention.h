@@ -64,7 +64,9 @@ typedef struct {
  *   a' = a cos - b sin,  b' = a sin + b cos
  * where pair i is (i, i + n_rot / 2), or (2 i, 2 i + 1) where `neighbours` is
  * set; the other elements stay (n_rot 0: all). Angles are f64, sines and
- * cosines good to 2^-23, products f32, each result rounded once.
+ * cosines good to 2^-23 at positions below 2^26 with bases of 1 and above (at the
+ * farthest, 2^31, an angle's own 53 bits leave 2^-21; bases below 1 turn faster
+ * and lose more), products f32, each result rounded once.
  * q, k and v are dtype (STRATA_QUANT_F32 or STRATA_QUANT_BF16), token rows of
  * heads side by side `*_stride` elements apart (0 = packed), so they may be
  * columns of one projection's output; q_out is q_dtype and may be q itself

@@ -10,8 +10,8 @@
 // Rows: the r query heads of a key head share its keys, so 16 rows (tokens x r
 // heads) are one tile of the tensor cores and every key is read once for them.
 // A single token's work is then its keys and values: bound by memory, 16 to 64
-// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 136 to 140 us,
-// 6.0 to 6.2 TB/s, 92 to 95% of the copy rate; one token over 4100: 16 us, launches and loads that wait on each
+// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 141 us,
+// 6.0 TB/s, 91% of the copy rate; one token over 4100: 15 us, launches and loads that wait on each
 // other (lengths, pages, keys, sums to join).
 //
 // The keys of all blocks of rows together (tiles of 64) are cut evenly over as
@@ -40,7 +40,7 @@ constexpr int kTile = kGroups * kUnit;
 // What a block of rows costs besides its tiles, in tiles (64 single tokens over 100 to 16000 keys
 // took 165, 147, 143 and 144 us with 1, 3, 4 and 6).
 constexpr int kOver = 4;
-constexpr int kLeast = 4;  // units of a thread block at least: fewer pieces to join where there is little to read
+constexpr int kLeast = 4;  // units of a thread block, or so, where there is little to read: fewer pieces to join
 
 // DP: head_dim rounded up to 64, 128 or 256. Stages and blocks side by side fill
 // the shared memory, so that about 128 KB a multiprocessor are under way.
@@ -95,7 +95,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Two floats as bf16 pairs, the largest limb first: x = limb 0 + limb 1 + ..., each
-// rounding leaves 2^-9 of what it rounds, so three limbs keep f32's 24 bits.
+// rounding leaves 2^-8 of what it rounds at most, so three limbs keep f32's 24 bits.
 template <int LIMBS>
 __device__ __forceinline__ void limbs(float x, float y, uint32_t (&out)[LIMBS]) {
 #pragma unroll
@@ -284,7 +284,10 @@ __global__ void __launch_bounds__(Cfg<DP, LIMBS>::kThreads, Cfg<DP, LIMBS>::kBlo
                             l[i] += e;
                         }
                 }
-                // weights as the left operand: its 16 keys are the two tiles' columns
+                // weights as the left operand: its 16 keys are the two tiles' columns. One limb
+                // rounds them to bf16, as exact as the values they meet (each off by 2^-8 of
+                // itself at most; their sum takes them unrounded): three, as for f32, would take
+                // three times the products for a result that is rounded to bf16 itself.
                 uint32_t wa[LIMBS][4];
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -509,11 +512,20 @@ int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, i
 
 // A sequence of kTcRows rows a key head goes to the tiles of 128 rows where the call has
 // kTcAll such rows and key heads together. Measured, tiles against 16 rows at a time (us,
-// heads of 128 behind 8000 keys, 4 query heads a key head): 16 sequences on 8 key heads
-// with 16 rows 128, 101, with 32 rows 130, 179, with 256 rows 154, 1200; one sequence
-// with 64 rows (512 in all) 65, 33, with 128 (1024) 67, 47, with 256 (2048) 72, 69; 16 sequences
-// of 8 query heads on one key head with 64 rows (1024) 58, 47, with 128 (2048) 60, 69; one
-// sequence of those with 512 rows 165, 32.
+// heads of 128; sequences x rows a key head on key heads):
+//   keys before   16x16 on 8   16x32 on 8   16x256 on 8   1x64 on 8   1x128 on 8   1x256 on 8
+//   0             18, 11       18, 12       21, 47        15, 10      16, 10       18, 11
+//   500           29, 22       31, 26       46, 106       26, 18      26, 20       30, 22
+//   8000          127, 101     131, 178     155, 1198     64, 36      65, 52       70, 75
+//   32000         388, 329     390, 633     518, 4827     121, 91     124, 152     121, 233
+//   keys before   1x1024 on 8  16x64 on 1   16x128 on 1   1x512 on 1  1x2048 on 1
+//   0             20, 28       15, 10       16, 11        18, 10      20, 19
+//   500           35, 40       26, 18       27, 22        29, 18      30, 23
+//   8000          65, 221      58, 51       59, 74        61, 34      70, 71
+//   32000         143, 781     116, 172     109, 261      171, 72     96, 210
+// What the tiles lose below is the join of many pieces (1x512 on 1 behind 8000: 155 us, not
+// 61, while a thread block could have a single unit). The keys before are not known on the
+// host; the rule is right from some thousands on, and costs up to 8 us in front of them.
 constexpr int64_t kTcRows = 32, kTcAll = 2048;
 
 bool tiles(const strata_attention& d, const strata_kv_cache& c) { return d.dtype == STRATA_QUANT_BF16 && c.head_dim <= 128; }
@@ -564,7 +576,7 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
     // over all positions (2^31 - 1 at most) it is none; over the table's it is one for tokens behind the table
     a.window = d.window < kMaxTokens ? (int)d.window : 0;
     a.sinks = a.window ? (int)std::min(d.sinks, kMaxTokens) : 0;
-    a.scale = (float)d.scale, a.scale2 = (float)(d.scale * 1.4426950408889634);
+    a.scale2 = (float)(d.scale * 1.4426950408889634);
     a.wide = ((uintptr_t)q_dev | (uintptr_t)o_dev) % 16 == 0 && (d.q_stride * size) % 16 == 0 && (d.o_stride * size) % 16 == 0;
     DeviceGuard dev(ctx->device);
     const cudaStream_t s = pick_stream(ctx, stream);

@@ -49,7 +49,7 @@ struct AttnArgs {
     int64_t q_stride, o_stride;
     int r;              // queries' heads a key head
     int window, sinks;  // window 0: none
-    float scale, scale2;  // the second in powers of two: scale * log2(e)
+    float scale2;       // in powers of two: scale * log2(e)
     int wide;           // rows of q and o can be accessed in 16-byte packs
 };
 
@@ -132,7 +132,8 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
     }
     return before + x - v;
 }
-// By all THREADS threads; blocks from c.grid on have none, the others LEAST units or more. `sh`: THREADS / 32 + 2 numbers.
+// By all THREADS threads; blocks from c.grid on have none, the others LEAST units or so (half of that at least, or all
+// there are). `sh`: THREADS / 32 + 2 numbers.
 template <int THREADS, int ROWS, int TILE, int OVER, int LEAST>
 __device__ __forceinline__ Cut cut_range(const AttnArgs& a, const SeqTable& tab, int entries, int64_t* sh) {
     Cut c;

@@ -5,7 +5,9 @@
 // A thread block takes 256 rows of one key head (tokens x query heads, token by
 // token) as two tiles of 128 and goes through its tiles of 128 keys:
 //   S = Q K^T         tcgen05.mma, both operands in shared memory, S in TMEM
-//   P = exp2(S - m)   a thread a row, from TMEM through registers and back
+//   P = exp2(S - m)   a thread a row, from TMEM through registers and back, rounded to
+//                     bf16 (2^-8 of each weight at most, as exact as the values that it
+//                     meets; their sum l takes them unrounded): the products take bf16
 //   O += P V          tcgen05.mma, P in TMEM (over S), V in shared memory
 // While the threads of one tile compute its weights, the tensor cores work for the
 // other. Exponentials (16 a clock) and products (8192 flops a clock) of a tile
@@ -48,7 +50,7 @@ constexpr int kRows = 2 * kRowTile;
 constexpr int kThreads = 384;  // three warpgroups, which registers are shared out by
 constexpr int kRegs = 208, kRegsRest = 88;  // 2 x 208 + 88 = 3 x 168, what the block is launched with
 constexpr int kOver = 6;       // what a block of rows costs besides its tiles, in tiles (8 or 4: a prompt of 8192 501, 519 us, not 488)
-constexpr int kLeast = 4;      // units of a thread block at least: fewer pieces to join where there is little to do
+constexpr int kLeast = 4;      // units of a thread block, or so, where there is little to do: fewer pieces to join
 constexpr int kMaxGrid = 148;
 constexpr int kMasks = 8;   // tiles whose masks are kept
 constexpr int kPieces = 8;  // pieces that are known ahead
