@@ -479,37 +479,6 @@ int launch_split(strata_ctx* ctx, bool bf16, const AttnArgs& a, void* work, cons
     return launch_split<DP, 3, float>(ctx, a, work, tab, entries, s);
 }
 
-// Calls launch(table, entries) for each group of the sequences of `from` tokens or
-// more but below `below`, cut into blocks of `per` rows.
-template <typename F>
-int for_row_groups(strata_ctx* ctx, const strata_attention& d, int r, int per, int64_t from, int64_t below, F launch) {
-    auto blocks = [&](int64_t n) { return (n * r + per - 1) / per; };
-    if (!d.seq_offsets) {
-        if (d.seq_len < from || d.seq_len >= below) return STRATA_OK;
-        if (d.n_seq > kMaxTokens / blocks(d.seq_len)) return fail(ctx, STRATA_ERR_INVALID, "attention: %lld sequences of %lld tokens", (long long)d.n_seq, (long long)d.seq_len);
-        SeqTable t = uniform_table(d.n_seq, 0, d.seq_len, 0, d.seq_len, 1);
-        t.tiles_all = (int)blocks(d.seq_len);
-        return launch(t, d.n_seq * t.tiles_all);
-    }
-    SeqTable t = ragged_table();
-    int64_t entries = 0;
-    for (int64_t i = 0; i < d.n_seq; ++i) {
-        const int64_t n = d.seq_offsets[i + 1] - d.seq_offsets[i];
-        if (n > 0 && n >= from && n < below) {
-            if (t.n == kSeqGroup || entries + blocks(n) > kMaxTokens) {
-                const int rc = launch(t, entries);
-                if (rc) return rc;
-                t = ragged_table();
-                entries = 0;
-            }
-            add_sequence(t, i, d.seq_offsets[i], n, 1);
-            entries += blocks(n);
-            t.tile[t.n] = (int)entries;
-        }
-    }
-    return t.n ? launch(t, entries) : STRATA_OK;
-}
-
 // A sequence of kTcRows rows a key head goes to the tiles of 128 rows where the call has
 // kTcAll such rows and key heads together. Measured, tiles against 16 rows at a time (us,
 // heads of 128; sequences x rows a key head on key heads):
@@ -591,13 +560,13 @@ extern "C" int strata_cuda_attention_dev(strata_ctx* ctx, const strata_attention
         }
         if (all * d.n_head >= kTcAll && attention_tc_maps(a.c, &maps)) {
             many = enough;
-            rc = for_row_groups(ctx, d, a.r, attention_tc_rows(), many, kMaxTokens + 1, [&](const SeqTable& t, int64_t entries) {
+            rc = for_row_groups(d, a.r, attention_tc_rows(), many, kMaxTokens + 1, [&](const SeqTable& t, int64_t entries) {
                 return launch_attention_tc(ctx, dp, a, work_dev, t, entries, maps, s);
             });
             if (rc) return rc;
         }
     }
-    return for_row_groups(ctx, d, a.r, kRows, 1, many, [&](const SeqTable& t, int64_t entries) {
+    return for_row_groups(d, a.r, kRows, 1, many, [&](const SeqTable& t, int64_t entries) {
         if (dp == 64) return launch_split<64>(ctx, bf16, a, work_dev, t, entries, s);
         if (dp == 128) return launch_split<128>(ctx, bf16, a, work_dev, t, entries, s);
         return launch_split<256>(ctx, bf16, a, work_dev, t, entries, s);

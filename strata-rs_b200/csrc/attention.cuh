@@ -3,6 +3,7 @@
 // from the formula alone.
 #pragma once
 #include "attention_args.h"
+#include "attention_groups.h"
 #include "attention_keys.h"
 #include "sequence.cuh"
 
