@@ -10,8 +10,8 @@
 // Rows: the r query heads of a key head share its keys, so 16 rows (tokens x r
 // heads) are one tile of the tensor cores and every key is read once for them.
 // A single token's work is then its keys and values: bound by memory, 16 to 64
-// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 141 us,
-// 6.0 TB/s, 91% of the copy rate; one token over 4100: 15 us, launches and loads that wait on each
+// operations a byte. 64 tokens over 100 to 16000 keys of 8 heads of 128: 140 us,
+// 6.0 TB/s, 92% of the copy rate; one token over 4100: 15 us, launches and loads that wait on each
 // other (lengths, pages, keys, sums to join).
 //
 // The keys of all blocks of rows together (tiles of 64) are cut evenly over as
@@ -38,7 +38,7 @@ constexpr int kRows = 16;  // rows of a block
 constexpr int kUnit = 16;  // keys a warp takes of a tile
 constexpr int kTile = kGroups * kUnit;
 // What a block of rows costs besides its tiles, in tiles (64 single tokens over 100 to 16000 keys
-// took 165, 147, 143 and 144 us with 1, 3, 4 and 6).
+// took 155, 142, 140 and 140 us with 1, 3, 4 and 6).
 constexpr int kOver = 4;
 constexpr int kLeast = 4;  // units of a thread block, or so, where there is little to read: fewer pieces to join
 

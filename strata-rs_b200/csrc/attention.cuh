@@ -23,7 +23,7 @@ cudaError_t launch_early(K kernel, dim3 grid, int threads, int shared, cudaStrea
 }
 // Where `next` is set, the kernel behind may then start likewise; a join does not let it:
 // its blocks' shared memory would keep blocks of the next attention kernel, which fill
-// the multiprocessors exactly, for a second round (64 tokens with heads of 64: 92, 109 us).
+// the multiprocessors exactly, for a second round (64 tokens with heads of 64: 92, 112 us).
 __device__ __forceinline__ void after_previous(bool next = true) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (next) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -26,8 +26,9 @@
 // Like attention.cu's kernel, thread blocks take equal shares of all tiles of the
 // call, and a second kernel joins the blocks of rows that were cut.
 //
-// A chunk of 1024 tokens behind 20000, 32 heads on 8 of 128: 299 us, 1.15 PFLOP/s (71% of
-// the products' measured burst rate); a prompt of 8192: 487 us, 1.13. The tensor pipe is
+// A chunk of 1024 tokens behind 20000, 32 heads on 8 of 128: 304 us, 1.13 PFLOP/s (70% of
+// the products' measured burst rate); a prompt of 8192: 500 us, 1.10. (A few calls at a
+// time: one after another for long, at the power limit, 354 and 563.) The tensor pipe is
 // busy for 67% of the cycles. What got it there from 393 and 1046 us: one region of scores
 // that the two tiles hand on, so that a tile's next scores wait for the reading of the
 // other's and not for its own weights (P has a place of its own); registers shared out by
@@ -49,7 +50,7 @@ constexpr int kRowTile = 128, kKeyTile = 128;
 constexpr int kRows = 2 * kRowTile;
 constexpr int kThreads = 384;  // three warpgroups, which registers are shared out by
 constexpr int kRegs = 208, kRegsRest = 88;  // 2 x 208 + 88 = 3 x 168, what the block is launched with
-constexpr int kOver = 6;       // what a block of rows costs besides its tiles, in tiles (8 or 4: a prompt of 8192 501, 519 us, not 488)
+constexpr int kOver = 6;       // what a block of rows costs besides its tiles, in tiles (8 or 4: a prompt of 8192 508, 532 us, not 500)
 constexpr int kLeast = 4;      // units of a thread block, or so, where there is little to do: fewer pieces to join
 constexpr int kMaxGrid = 148;
 constexpr int kMasks = 8;   // tiles whose masks are kept

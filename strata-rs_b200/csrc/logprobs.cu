@@ -13,9 +13,9 @@
 // and their logits (one in kThreads each) are read again, a warp a thread's. What
 // reaches T is ordered by counting.
 //
-// Bound by memory where rows are many (one block a row): 1024 rows of 151936 118 us,
-// 5.3 TB/s. Few rows are cut over a cluster, whose results the first block joins: 32 rows
-// 11 us, one row 14 (the pass 4, the rest steps that wait on each other). Before the
+// Bound by memory where rows are many (one block a row): 1024 rows of 151936 120 us,
+// 5.2 TB/s. Few rows are cut over a cluster, whose results the first block joins: 32 rows
+// 11 us, one row 13 (the pass 4, the rest steps that wait on each other). Before the
 // tournament each exponential went to the f64 sum by itself and maxima moved with f64
 // exponentials: 264 us for the 1024 rows.
 #include <cooperative_groups.h>
